@@ -480,6 +480,133 @@ int graft_moe_block_ep(graft_comm_t comm, const void* pool, const void* R, const
                        void* y, const GraftMoEParams* P, const GraftMoEFormat* fmt,
                        const GraftMoEScratch* scratch, graft_stream_t stream);
 
+/* ==================================================== 8-bit key/value cache ===
+ * A paged cache of attention keys and values in 8 bits, with one fp32 scale
+ * for each block of tokens and head (K and V apart):
+ *   codes  [n_blocks][kv_heads][block_tokens][head_dim]  (one byte each)
+ *   scales [n_blocks][kv_heads]                          value = code * scale
+ * Codes are signed integers in [-127, 127] (GRAFT_KV_INT8) or 8-bit floats
+ * with 4 exponent and 3 mantissa bits, largest value 448 (GRAFT_KV_E4M3).
+ * Constraints: block_tokens 16, 32, 64 or 128; head_dim a multiple of 16, at
+ * most 256; code pointers 16-byte aligned, scale pointers 4-byte aligned. */
+enum { GRAFT_KV_INT8 = 0, GRAFT_KV_E4M3 = 1 };
+/* Element types of 16- and 32-bit buffers. */
+enum { GRAFT_F16 = 0, GRAFT_BF16 = 1, GRAFT_F32 = 2 };
+
+typedef struct {
+    void* k;                 /* codes                                         */
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    uint32_t n_blocks, kv_heads, block_tokens, head_dim;
+    uint32_t format;         /* GRAFT_KV_INT8 or GRAFT_KV_E4M3                */
+} GraftKVCache;
+
+/* Consecutive tokens of each of n_seqs sequences: sequence b's tokens lie at
+ * positions start[b] .. start[b] + n_b - 1, n_b = cu_tokens[b+1] -
+ * cu_tokens[b] >= 0 (0 allowed), and are rows cu_tokens[b] .. of a buffer
+ * that holds all sequences' tokens one after the other (cu_tokens[0] = 0).
+ * Position p is in block block_table[b*table_stride + p / block_tokens].
+ * The arrays are in device memory and read when the kernels run; the host
+ * gives two upper bounds: max_tokens >= every n_b and max_len >= every
+ * start[b] + n_b.  Block numbers outside the cache and lengths beyond the
+ * bounds are skipped by the kernels and reported (graft_kv_device_errors). */
+typedef struct {
+    const int32_t* block_table;  /* [n_seqs][table_stride]                    */
+    const int32_t* start;        /* [n_seqs]                                  */
+    const int32_t* cu_tokens;    /* [n_seqs + 1]                              */
+    uint32_t n_seqs, table_stride;
+    uint32_t max_tokens, max_len;
+} GraftKVRange;
+
+/* Rows of heads: element d of head h of token t is
+ * data[t*token_stride + h*head_stride + d] (strides in elements; a slice of a
+ * joint q/k/v buffer, or a transposed one).  data 16-byte aligned, strides in
+ * bytes multiples of 16. */
+typedef struct {
+    void* data;
+    uint64_t token_stride, head_stride;
+    uint32_t tokens;             /* rows in the buffer                        */
+    uint32_t dtype;              /* GRAFT_F16, GRAFT_BF16 or GRAFT_F32        */
+} GraftHeads;
+
+/* Quantises the range's keys and values into the cache.  In each block that a
+ * sequence's new tokens touch, per head:
+ *   scale = max(amax / qmax, 2^-64, the old scale if the block already holds
+ *           earlier tokens of the sequence)         qmax = 127 or 448
+ *   code  = x / scale, rounded to nearest even;
+ * where the scale grew, the earlier tokens' codes are rounded again to it
+ * (code * old scale / new scale).  A block's first tokens start its scale
+ * afresh, whatever an earlier owner left.  amax is taken over finite values;
+ * an infinity is stored as +-qmax and a NaN as 0, so a cache holds finite
+ * numbers only.  No two sequences of a call may touch the same block. */
+int graft_kv_write(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                   const GraftKVRange* range, graft_stream_t stream);
+
+/* Reads the range back: code * scale, rounded once to the buffers' type. */
+int graft_kv_read(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                  const GraftKVRange* range, graft_stream_t stream);
+
+/* Device-side findings of the cache and attention kernels, or-ed together:
+ * GRAFT_KV_EBLOCK: a block number outside the cache; GRAFT_KV_EBOUNDS: lengths
+ * beyond max_tokens, max_len, the block table or a buffer; GRAFT_KV_EWAIT: a
+ * bounded wait gave up.  Synchronises the device; clear != 0 resets them. */
+enum { GRAFT_KV_EBLOCK = 1, GRAFT_KV_EBOUNDS = 2, GRAFT_KV_EWAIT = 4 };
+int graft_kv_device_errors(uint32_t* bits, int clear);
+
+/* ------------------------------------------------- attention over the cache */
+typedef struct {
+    uint32_t q_heads;   /* a multiple of kv_heads: q head h reads kv head h / (q_heads/kv_heads) */
+    uint32_t window;    /* keys a query sees, itself included; 0 = all        */
+    float scale;        /* of the scores, e.g. 1/sqrt(head_dim); finite       */
+} GraftAttnParams;
+
+/* Attention of the range's tokens over the cache, which holds their own keys
+ * and values already (graft_kv_write first).  Token i of a sequence, at
+ * position p = start + i, sees keys j with p - window < j <= p:
+ *   o = sum_j exp(scale q.k_j - lse) v_j,
+ *   lse = log( sum_j exp(scale q.k_j)  [+ exp(sinks[h])] ).
+ * q and out: GRAFT_F16 or GRAFT_BF16, the same type.  sinks (fp32 [q_heads], a
+ * score that takes weight but has no value) and lse (fp32 [tokens][q_heads])
+ * may be null.  ws: graft_attn_kv8_workspace bytes, 256-byte aligned, zeroed
+ * once by graft_attn_kv8_init and then kept for calls of one stream at a
+ * time. */
+size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const GraftKVRange* range,
+                                const GraftAttnParams* P);
+int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t stream);
+int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
+                   const GraftKVRange* range, const float* sinks, float* lse,
+                   const GraftAttnParams* P, void* ws, size_t ws_bytes, graft_stream_t stream);
+
+/* ======================================================== log probabilities ===
+ * From rows of logits (the lm_head's output), with z = scale * logit:
+ *   lse          = log sum_v exp(z_v)
+ *   logprob[r]   = z[targets[r]] - lse       (NaN for a target outside 0..vocab-1)
+ *   entropy[r]   = lse - sum_v p_v z_v
+ *   top_logprob, top_index [r][top_k]: the largest logits, in falling order,
+ *     equal ones by rising index.
+ * A logit of -inf is a token that cannot come: it adds nothing, and is never
+ * listed (index -1, log probability -inf fill up a row that has fewer than
+ * top_k others).  A row without any possible token gives logprob -inf and
+ * entropy 0; a row with a NaN or +inf gives NaN log probabilities and entropy. */
+typedef struct {
+    uint32_t rows, vocab;
+    uint32_t top_k;      /* 0 .. 32                                           */
+    uint32_t dtype;      /* of the logits: GRAFT_F16, GRAFT_BF16 or GRAFT_F32 */
+    uint64_t row_stride; /* elements from row to row (>= vocab, any value)    */
+    float scale;         /* 1/temperature, > 0                                */
+} GraftLogprobParams;
+
+/* logits aligned to its element; targets (int32 [rows]) and logprob may both be
+ * null, entropy may be null, top_* may be null when top_k is 0.  ws as for
+ * graft_attn_kv8: graft_logprobs_workspace bytes, 256-byte aligned, zeroed once by
+ * graft_logprobs_init and kept for calls of one stream at a time. */
+size_t graft_logprobs_workspace(const GraftLogprobParams* P);
+int graft_logprobs_init(void* ws, size_t ws_bytes, graft_stream_t stream);
+int graft_logprobs(const void* logits, const int32_t* targets, float* logprob, float* entropy,
+                   float* top_logprob, int32_t* top_index, const GraftLogprobParams* P, void* ws,
+                   size_t ws_bytes, graft_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,8 +17,9 @@ from __future__ import annotations
 
 import ctypes as C
 
-from ._lib import (ExpertParams, ExpertScratch, GemvParams, GraftError, MoEFormat, MoEParams,
-                   MoEScratch, VQParams, VQQuantParams, call, load)
+from ._lib import (AttnParams, ExpertParams, ExpertScratch, GemvParams, GraftError, Heads,
+                   KVCacheDesc, KVRangeDesc, LogprobParams, MoEFormat, MoEParams, MoEScratch,
+                   VQParams, VQQuantParams, call, load)
 
 __all__ = [
     "GemvParams", "VQParams", "MoEParams", "MoEFormat", "MoEScratch", "GraftError",
@@ -30,6 +31,9 @@ __all__ = [
     "gemv_vq_ex", "vq_decode", "vq_quantize", "moe_params", "moe_router_topk", "moe_fused_gate_up_swiglu",
     "moe_fused_down_combine", "moe_fused_gate_up_swiglu_at", "moe_fused_down_combine_at",
     "MoEWorkspace", "moe_block", "moe_block_ex", "moe_format",
+    "KVCache", "kv_range", "kv_write", "kv_read", "kv_device_errors", "AttnParams",
+    "attn_params", "AttnWorkspace", "attn_kv8", "LogprobParams", "logprob_params",
+    "LogprobWorkspace", "logprobs",
 ]
 
 
@@ -322,6 +326,189 @@ def moe_set_one_launch(on) -> int:
     whole block on one GPU, 2 a rank's share of an expert-parallel block, 3
     both, False/0 neither.  Returns the previous setting (the same bits)."""
     return int(load().graft_moe_set_one_launch(int(on)))
+
+
+# ------------------------------------------ key/value cache and attention --
+def _dtype_code(dtype) -> int:
+    import torch
+    codes = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    if dtype not in codes:
+        raise TypeError(f"unsupported element type {dtype}")
+    return codes[dtype]
+
+
+def _ints(t, name: str):
+    import torch
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, not {t.dtype}")
+    if t.stride(-1) != 1 and t.numel() > 1:
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _heads(t, heads: int, dim: int) -> Heads:
+    """A [tokens, heads, dim] tensor with any token and head strides."""
+    if t.dim() != 3 or t.shape[1:] != (heads, dim):
+        raise ValueError(f"expected a [tokens, {heads}, {dim}] tensor, not {tuple(t.shape)}")
+    if t.stride(2) != 1 and dim > 1:
+        raise ValueError("the last dimension must be contiguous")
+    return Heads(_p(t), t.stride(0), t.stride(1), t.shape[0], _dtype_code(t.dtype))
+
+
+class KVCache:
+    """A paged 8-bit key/value cache over the caller's tensors: k and v int8 or
+    float8_e4m3fn [n_blocks, kv_heads, block_tokens, head_dim], k_scale and
+    v_scale fp32 [n_blocks, kv_heads], all contiguous."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        formats = {torch.int8: 0, torch.float8_e4m3fn: 1}
+        if k.dtype not in formats or v.dtype != k.dtype:
+            raise TypeError("k and v must both be int8 or both float8_e4m3fn")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("k and v must be [n_blocks, kv_heads, block_tokens, head_dim]")
+        for s in (k_scale, v_scale):
+            if s.dtype != torch.float32 or s.shape != k.shape[:2]:
+                raise ValueError("scales must be fp32 [n_blocks, kv_heads]")
+        if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+            raise ValueError("the cache's tensors must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        n, h, bt, d = k.shape
+        self.desc = KVCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), n, h, bt, d,
+                                formats[k.dtype])
+
+    @classmethod
+    def empty(cls, n_blocks: int, kv_heads: int, head_dim: int, block_tokens: int = 64,
+              dtype=None, device="cuda"):
+        """A new cache (dtype torch.int8, the default, or torch.float8_e4m3fn)."""
+        import torch
+        shape = (n_blocks, kv_heads, block_tokens, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.int8, device=device).view(dtype or torch.int8)
+                for _ in range(2))
+        ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+
+class KVRange:
+    """Consecutive tokens of each sequence (kv_range)."""
+
+    def __init__(self, block_table, start, cu_tokens, max_tokens: int, max_len: int):
+        if block_table.dim() != 2:
+            raise ValueError("block_table must be [n_seqs, blocks]")
+        n = block_table.shape[0]
+        if tuple(start.shape) != (n,) or tuple(cu_tokens.shape) != (n + 1,):
+            raise ValueError("start must be [n_seqs] and cu_tokens [n_seqs + 1]")
+        self._keep = (_ints(block_table, "block_table"), _ints(start, "start"),
+                      _ints(cu_tokens, "cu_tokens"))
+        stride = block_table.stride(0) if n > 1 else block_table.shape[1]
+        self.desc = KVRangeDesc(_p(block_table), _p(start), _p(cu_tokens), n, stride, max_tokens,
+                                max_len)
+
+
+def kv_range(block_table, start, cu_tokens, max_tokens: int, max_len: int) -> KVRange:
+    """Tokens at positions start[b] .. of each sequence b: as many as cu_tokens
+    (int32 [n_seqs + 1], running sums from 0) says, in the blocks that
+    block_table (int32 [n_seqs, blocks]) names.  max_tokens and max_len bound a
+    sequence's tokens in the range and its last position + 1."""
+    return KVRange(block_table, start, cu_tokens, max_tokens, max_len)
+
+
+def kv_write(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
+    """Quantises K and V [tokens, kv_heads, head_dim] into the cache (graft_kv_write)."""
+    h, d = cache.desc.kv_heads, cache.desc.head_dim
+    call("graft_kv_write", C.byref(cache.desc), C.byref(_heads(K, h, d)),
+         C.byref(_heads(V, h, d)), C.byref(rng.desc), _s(stream))
+
+
+def kv_read(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
+    """Reads the range back into K and V [tokens, kv_heads, head_dim] (graft_kv_read)."""
+    h, d = cache.desc.kv_heads, cache.desc.head_dim
+    call("graft_kv_read", C.byref(cache.desc), C.byref(_heads(K, h, d)), C.byref(_heads(V, h, d)),
+         C.byref(rng.desc), _s(stream))
+
+
+def kv_device_errors(clear: bool = False) -> dict:
+    """Findings of the cache and attention kernels (graft_kv_device_errors)."""
+    b = C.c_uint32()
+    call("graft_kv_device_errors", C.byref(b), int(clear))
+    return {"block": bool(b.value & 1), "bounds": bool(b.value & 2), "wait": bool(b.value & 4)}
+
+
+def attn_params(q_heads: int, dtype=None, scale: float = 1.0, window: int = 0) -> AttnParams:
+    """dtype: the queries' type, torch.float16 or torch.bfloat16 (checked here;
+    the call goes by the tensors)."""
+    if dtype is not None and _dtype_code(dtype) > 1:
+        raise TypeError("queries are fp16 or bf16")
+    return AttnParams(q_heads, window, scale)
+
+
+class AttnWorkspace:
+    """The scratch of attn_kv8 for a cache, a range's bounds and params."""
+
+    def __init__(self, cache: KVCache, rng: KVRange, P: AttnParams, device=None):
+        import torch
+        n = load().graft_attn_kv8_workspace(C.byref(cache.desc), C.byref(rng.desc), C.byref(P))
+        if n == 0:
+            raise GraftError("graft_attn_kv8_workspace", 1,
+                             load().graft_last_error_string().decode())
+        self.buffer = torch.empty(n + 256, dtype=torch.uint8, device=device or cache.k.device)
+        self.addr, self.nbytes = (self.buffer.data_ptr() + 255) & ~255, n
+        call("graft_attn_kv8_init", self.addr, n, _s(None))
+
+
+def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorkspace, sinks=None,
+             lse=None, stream=None) -> None:
+    """Attention of the range's tokens (q and out [tokens, q_heads, head_dim])
+    over the cache (graft_attn_kv8)."""
+    import torch
+    d = cache.desc.head_dim
+    for t, shape in ((sinks, (P.q_heads,)), (lse, (q.shape[0], P.q_heads))):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape
+                              or not t.is_contiguous()):
+            raise ValueError(f"sinks and lse must be contiguous fp32, {shape}")
+    call("graft_attn_kv8", C.byref(cache.desc), C.byref(_heads(q, P.q_heads, d)),
+         C.byref(_heads(out, P.q_heads, d)), C.byref(rng.desc), _p(sinks), _p(lse), C.byref(P),
+         ws.addr, ws.nbytes, _s(stream))
+
+
+# ------------------------------------------------------ log probabilities --
+def logprob_params(rows: int, vocab: int, top_k: int, dtype, scale: float = 1.0) -> LogprobParams:
+    return LogprobParams(rows, vocab, top_k, _dtype_code(dtype), vocab, scale)
+
+
+class LogprobWorkspace:
+    """The scratch of logprobs."""
+
+    def __init__(self, P: LogprobParams, device=None):
+        import torch
+        n = load().graft_logprobs_workspace(C.byref(P))
+        if n == 0:
+            raise GraftError("graft_logprobs_workspace", 1,
+                             load().graft_last_error_string().decode())
+        self.buffer = torch.empty(n + 256, dtype=torch.uint8, device=device or "cuda")
+        self.addr, self.nbytes = (self.buffer.data_ptr() + 255) & ~255, n
+        call("graft_logprobs_init", self.addr, n, _s(None))
+
+
+def logprobs(logits, targets, logprob, entropy, top_logprob, top_index, P: LogprobParams,
+             ws: LogprobWorkspace, stream=None) -> None:
+    """Log probability of targets, entropy and top alternatives of each row of
+    logits [rows, vocab] (graft_logprobs); outputs that are None are left out."""
+    import torch
+    if tuple(logits.shape) != (P.rows, P.vocab) or _dtype_code(logits.dtype) != P.dtype:
+        raise ValueError("logits do not match the params")
+    if logits.stride(1) != 1 and P.vocab > 1:
+        raise ValueError("a row of logits must be contiguous")
+    for t, dt, shape in ((targets, torch.int32, (P.rows,)), (logprob, torch.float32, (P.rows,)),
+                         (entropy, torch.float32, (P.rows,)),
+                         (top_logprob, torch.float32, (P.rows, P.top_k)),
+                         (top_index, torch.int32, (P.rows, P.top_k))):
+        if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
+            raise ValueError(f"expected a contiguous {dt} {shape} tensor")
+    Q = LogprobParams(P.rows, P.vocab, P.top_k, P.dtype,
+                      logits.stride(0) if P.rows > 1 else P.vocab, P.scale)
+    call("graft_logprobs", _p(logits), _p(targets), _p(logprob), _p(entropy), _p(top_logprob),
+         _p(top_index), C.byref(Q), ws.addr, ws.nbytes, _s(stream))
 
 
 # ----------------------------------------------------------- multi-GPU --

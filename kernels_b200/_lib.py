@@ -68,6 +68,35 @@ class ExpertScratch(C.Structure):
                 ("h", C.c_void_p), ("xs_h", C.c_void_p)]
 
 
+class KVCacheDesc(C.Structure):
+    """GraftKVCache: codes and scales of a paged 8-bit key/value cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("n_blocks", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("block_tokens", C.c_uint32), ("head_dim", C.c_uint32), ("format", C.c_uint32)]
+
+
+class KVRangeDesc(C.Structure):
+    """GraftKVRange: consecutive tokens of each sequence, and where they are."""
+    _fields_ = [("block_table", C.c_void_p), ("start", C.c_void_p), ("cu_tokens", C.c_void_p),
+                ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32),
+                ("max_tokens", C.c_uint32), ("max_len", C.c_uint32)]
+
+
+class Heads(C.Structure):
+    """GraftHeads: a strided [tokens][heads][head_dim] buffer."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64),
+                ("tokens", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class AttnParams(C.Structure):
+    _fields_ = [("q_heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float)]
+
+
+class LogprobParams(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32), ("top_k", C.c_uint32),
+                ("dtype", C.c_uint32), ("row_stride", C.c_uint64), ("scale", C.c_float)]
+
+
 P = C.c_void_p
 U32 = C.c_uint32
 U64 = C.c_uint64
@@ -135,6 +164,19 @@ SIGNATURES: dict[str, tuple] = {
     "graft_gemm_int4_sharded": (INT, [P, P, P, P, P, U32, C.POINTER(GemvParams), P]),
     "graft_moe_block_ep": (INT, [P, P, P, P, P, C.POINTER(MoEParams), C.POINTER(MoEFormat),
                                  C.POINTER(MoEScratch), P]),
+    "graft_kv_write": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+                             C.POINTER(KVRangeDesc), P]),
+    "graft_kv_read": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+                            C.POINTER(KVRangeDesc), P]),
+    "graft_kv_device_errors": (INT, [C.POINTER(U32), INT]),
+    "graft_attn_kv8_workspace": (SIZE, [C.POINTER(KVCacheDesc), C.POINTER(KVRangeDesc),
+                                        C.POINTER(AttnParams)]),
+    "graft_attn_kv8_init": (INT, [P, SIZE, P]),
+    "graft_attn_kv8": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+                             C.POINTER(KVRangeDesc), P, P, C.POINTER(AttnParams), P, SIZE, P]),
+    "graft_logprobs_workspace": (SIZE, [C.POINTER(LogprobParams)]),
+    "graft_logprobs_init": (INT, [P, SIZE, P]),
+    "graft_logprobs": (INT, [P, P, P, P, P, P, C.POINTER(LogprobParams), P, SIZE, P]),
 }
 
 _lib: C.CDLL | None = None

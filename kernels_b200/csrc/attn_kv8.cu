@@ -1,0 +1,192 @@
+// attn_kv8.cu -- attention of new tokens over the paged 8-bit key/value cache.
+//
+//   o = sum_j exp(scale q.k_j - lse) v_j,  lse = log(sum_j exp(scale q.k_j) [+ exp(sink)])
+//   over keys j with p - window < j <= p, p the token's position
+//
+// One CTA per (token, query head): its warps take every fourth key with a
+// running maximum and sum each, and are merged at the end.
+#include "kv_common.cuh"
+
+#include <cmath>
+
+using namespace graft;
+using namespace graft::dev;
+
+namespace {
+
+__device__ unsigned g_attn_err;
+
+struct AttnArgs {
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    const int32_t *table, *start, *cu;
+    const void* q;
+    void* out;
+    const float* sinks;
+    float* lse;
+    uint64_t q_tok, q_head, o_tok, o_head;
+    uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
+    uint32_t q_heads, group, window;
+    float scale;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DT, int FMT>
+__global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant__ AttnArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ float sm[4], sl[4], so[4][256];
+    const int t = blockIdx.x, h = blockIdx.y, hk = h / a.group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int b = 0;
+    for (uint32_t s0 = 1; s0 < a.n_seqs; s0 += blockDim.x) {
+        const uint32_t s = s0 + threadIdx.x;
+        b += __syncthreads_count(s < a.n_seqs && a.cu[s] <= t);
+    }
+    const int c0 = a.cu[b], n = a.cu[b + 1] - c0, start = a.start[b];
+    if (t < c0 || t >= c0 + n) return;
+    if (n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens || start < 0 || (uint64_t)((int64_t)start + n) > a.max_len) {
+        if (threadIdx.x == 0) atomicOr(&g_attn_err, (unsigned)GRAFT_KV_EBOUNDS);
+        return;
+    }
+    const int p = start + t - c0, lo = a.window && p >= (int)a.window ? p - (int)a.window + 1 : 0;
+    const int words = a.dim / 4;       // 4-byte words of a row; lane l has words l, l + 32
+    float q[2][4], o[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int w = lane + 32 * i;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[i][e] = o[i][e] = 0.f;
+        if (w < words) {
+            const uint2 x = *reinterpret_cast<const uint2*>((const uint16_t*)a.q + t * a.q_tok +
+                                                            h * a.q_head + 4 * w);
+            const float2 y = unpack2<DT>(x.x), z = unpack2<DT>(x.y);
+            q[i][0] = y.x, q[i][1] = y.y, q[i][2] = z.x, q[i][3] = z.y;
+        }
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int j = lo + warp; j <= p; j += 4) {
+        const int blk = a.table[(size_t)b * a.table_stride + j / a.bt];
+        if ((uint32_t)blk >= a.n_blocks) {
+            if (lane == 0) atomicOr(&g_attn_err, (unsigned)GRAFT_KV_EBLOCK);
+            continue;
+        }
+        const size_t bh = (size_t)blk * a.heads + hk, at = (bh * a.bt + j % a.bt) * a.dim;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < words) {
+                float f[4];
+                kv_decode4<FMT>(*reinterpret_cast<const uint32_t*>(a.k + at + 4 * (lane + 32 * i)), f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s = fmaf(f[e], q[i][e], s);
+            }
+        s = warp_sum(s) * a.k_scale[bh] * a.scale;
+        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.f : exp2f((m - mn) * kLog2e);
+        const float w = s == -INFINITY ? 0.f : exp2f((s - mn) * kLog2e);   // (a NaN stays one)
+        m = mn;
+        l = l * c + w;
+        const float wv = w * a.v_scale[bh];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < words) {
+                float f[4];
+                kv_decode4<FMT>(*reinterpret_cast<const uint32_t*>(a.v + at + 4 * (lane + 32 * i)), f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] = fmaf(wv, f[e], o[i][e] * c);
+            }
+    }
+    if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (lane + 32 * i < words)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) so[warp][4 * (lane + 32 * i) + e] = o[i][e];
+    __syncthreads();
+    const float sink = a.sinks ? a.sinks[h] : -INFINITY;
+    float M = sink;
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w]);
+    float L = 0.f, f[4];
+    for (int w = 0; w < 4; ++w) {
+        f[w] = sl[w] == 0.f ? 0.f : exp2f((sm[w] - M) * kLog2e);
+        L += f[w] * sl[w];
+    }
+    if (sink != -INFINITY) L += exp2f((sink - M) * kLog2e);
+    for (int d = threadIdx.x; d < (int)a.dim; d += 128) {
+        float v = 0.f;
+        for (int w = 0; w < 4; ++w) v += f[w] * so[w][d];
+        v = L != 0.f ? v / L : 0.f;
+        uint16_t* y = (uint16_t*)a.out + t * a.o_tok + h * a.o_head + d;
+        *y = (uint16_t)pack2<DT>(v, 0.f);
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[(size_t)t * a.q_heads + h] = L != 0.f ? M + logf(L) : -INFINITY;
+}
+
+int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const GraftAttnParams* P) {
+    int rc;
+    if ((rc = kv_check_cache(cache)) || (rc = kv_check_range(cache, range))) return rc;
+    GRAFT_REQUIRE(P, "params pointer is null");
+    GRAFT_REQUIRE(P->q_heads >= 1 && P->q_heads <= 32767 && P->q_heads % cache->kv_heads == 0,
+                  "q_heads %u must be a multiple of kv_heads %u", P->q_heads, cache->kv_heads);
+    GRAFT_REQUIRE(std::isfinite(P->scale), "scale must be finite");
+    GRAFT_REQUIRE(P->window <= 0x7FFFFFFFu, "window %u out of range", P->window);
+    return GRAFT_OK;
+}
+
+}  // namespace
+
+namespace graft {
+unsigned attn_device_errors(bool clear) { return read_device_errors(g_attn_err, clear); }
+}  // namespace graft
+
+extern "C" size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const GraftKVRange* range,
+                                           const GraftAttnParams* P) {
+    return check_attn(cache, range, P) ? 0 : 256;
+}
+
+extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t stream) {
+    clear_error();
+    GRAFT_REQUIRE(ws && aligned(ws, 256), "the workspace must be 256-byte aligned");
+    GRAFT_CUDA(cudaMemsetAsync(ws, 0, ws_bytes, stream));
+    return GRAFT_OK;
+}
+
+extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
+                              const GraftKVRange* range, const float* sinks, float* lse,
+                              const GraftAttnParams* P, void* ws, size_t ws_bytes,
+                              graft_stream_t stream) {
+    int rc;
+    if ((rc = check_attn(cache, range, P)) || (rc = kv_check_heads("q", q, cache->head_dim)) ||
+        (rc = kv_check_heads("out", out, cache->head_dim)))
+        return rc;
+    GRAFT_REQUIRE(q->dtype == out->dtype && q->dtype != GRAFT_F32,
+                  "q and out must both be fp16 or both bf16");
+    GRAFT_REQUIRE(q->tokens == out->tokens, "q and out must have the same number of tokens");
+    GRAFT_REQUIRE(aligned(sinks, 4) && aligned(lse, 4), "sinks and lse must be 4-byte aligned");
+    const size_t need = graft_attn_kv8_workspace(cache, range, P);
+    GRAFT_REQUIRE(ws && aligned(ws, 256) && ws_bytes >= need,
+                  "the workspace must be 256-byte aligned and hold %zu bytes", need);
+    if (range->n_seqs == 0 || q->tokens == 0) return GRAFT_OK;
+    AttnArgs a = {};
+    a.k = (const uint8_t*)cache->k, a.v = (const uint8_t*)cache->v;
+    a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+    a.table = range->block_table, a.start = range->start, a.cu = range->cu_tokens;
+    a.q = q->data, a.out = out->data, a.sinks = sinks, a.lse = lse;
+    a.q_tok = q->token_stride, a.q_head = q->head_stride;
+    a.o_tok = out->token_stride, a.o_head = out->head_stride;
+    a.n_blocks = cache->n_blocks, a.heads = cache->kv_heads, a.bt = cache->block_tokens;
+    a.dim = cache->head_dim, a.n_seqs = range->n_seqs, a.table_stride = range->table_stride;
+    a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = q->tokens;
+    a.q_heads = P->q_heads, a.group = P->q_heads / cache->kv_heads, a.window = P->window;
+    a.scale = P->scale;
+    void (*kern)(const AttnArgs);
+    if (q->dtype == GRAFT_F16)
+        kern = cache->format == GRAFT_KV_INT8 ? attn_simple_kernel<GRAFT_F16, GRAFT_KV_INT8>
+                                              : attn_simple_kernel<GRAFT_F16, GRAFT_KV_E4M3>;
+    else
+        kern = cache->format == GRAFT_KV_INT8 ? attn_simple_kernel<GRAFT_BF16, GRAFT_KV_INT8>
+                                              : attn_simple_kernel<GRAFT_BF16, GRAFT_KV_E4M3>;
+    return launch_pdl("attn_kv8", kern, dim3(q->tokens, P->q_heads), 128, 0, stream, a);
+}

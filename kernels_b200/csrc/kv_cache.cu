@@ -1,0 +1,348 @@
+// kv_cache.cu -- the paged 8-bit key/value cache: quantising tokens as they
+// are written, and reading them back.
+//
+//   scale(block, head) = max(amax / qmax, 2^-64 [, old scale]),  code = round(x / scale)
+//   value = code * scale
+//
+// Both kernels move each byte once and compute a few operations per element,
+// so HBM bounds the long calls and launch plus load latency the short ones.
+// Work items are (block that a sequence touches, head, K or V): a block's
+// amax, and the rounding again of its earlier codes when the scale grows,
+// concern one item alone, so an item is one CTA, its elements stay in
+// registers between the maximum and the rounding, and nothing is atomic.
+// The item of a CTA follows from cu_tokens in closed form: sequence b's items
+// start at cu_tokens[b] / block_tokens + 2 b, which leaves room for every
+// block it can touch whatever its start, so no prefix sum of block counts is
+// needed (a CTA past its sequence's blocks returns).
+#include "kv_common.cuh"
+
+using namespace graft;
+using namespace graft::dev;
+
+namespace {
+
+__device__ unsigned g_kv_err;
+
+constexpr int kChunk = 8;        // elements a thread moves at once
+constexpr int kMaxChunks = 8;    // chunks a thread holds (128 tokens x 256 / 512 threads)
+
+struct KVArgs {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t *table, *start, *cu;
+    const void *x_k, *x_v;                 // rows (read by write, written by read)
+    uint64_t tok_k, head_k, tok_v, head_v; // strides in elements
+    uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
+};
+
+// One item: `count` tokens of one sequence in one block.
+struct Item {
+    int block;      // block number in the cache
+    int slot;       // first slot in it
+    int row;        // row of the first token
+    int count;
+};
+
+// The item of flat index x (false: none).  Every thread of the CTA calls it.
+__device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it) {
+    const uint32_t bt = a.bt;
+    int b = 0;   // the last sequence whose items start at or before x
+    for (uint32_t s0 = 1; s0 < a.n_seqs; s0 += blockDim.x) {
+        const uint32_t s = s0 + threadIdx.x;
+        const bool p = s < a.n_seqs && (uint32_t)a.cu[s] / bt + 2 * s <= x;
+        const int c = __syncthreads_count(p);
+        b += c;
+        if (c < (int)blockDim.x) break;
+    }
+    const int c0 = a.cu[b];
+    int n = a.cu[b + 1] - c0;
+    const int64_t start = a.start[b];
+    const bool first = threadIdx.x == 0 && blockIdx.y == 0;
+    if (c0 < 0 || n < 0 || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens ||
+        start < 0 || (uint64_t)(start + n) > a.max_len) {
+        if (first) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
+        return false;
+    }
+    if (n == 0) return false;
+    const uint32_t j = x - ((uint32_t)c0 / bt + 2 * b);
+    const int64_t base = (start / bt + j) * bt;      // first position of the block
+    if (base >= start + n) return false;
+    const int64_t lo = base > start ? base : start;
+    it.slot = (int)(lo - base);
+    it.row = c0 + (int)(lo - start);
+    it.count = min((int)bt - it.slot, (int)(start + n - lo));
+    it.block = a.table[(size_t)b * a.table_stride + (size_t)(base / bt)];
+    if ((uint32_t)it.block >= a.n_blocks) {
+        if (first) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBLOCK);
+        return false;
+    }
+    return true;
+}
+
+// |x| of a finite element, 0 of another
+__device__ __forceinline__ float fin_abs(float x) {
+    const float a = fabsf(x);
+    return a < __int_as_float(0x7f800000) ? a : 0.f;
+}
+
+template <int DT>
+struct Raw {
+    uint4 w[DT == GRAFT_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const void* base, uint64_t elem) {
+    Raw<DT> r;
+    const char* p = (const char*)base + elem * (DT == GRAFT_F32 ? 4 : 2);
+    r.w[0] = ld_stream(p);
+    if constexpr (DT == GRAFT_F32) r.w[1] = ld_stream(p + 16);
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void to_floats(const Raw<DT>& r, float (&f)[8]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == GRAFT_F32) {
+            f[2 * i] = __uint_as_float(w[2 * i]);
+            f[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+        } else {
+            const float2 p = unpack2<DT>(w[i]);
+            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+        }
+    }
+}
+
+template <int DT, int FMT>
+__global__ void kv_write_kernel(const __grid_constant__ KVArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ float red[16];
+    Item it;
+    if (!find_item(a, blockIdx.x, it)) return;
+    const int head = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    const void* x = is_v ? a.x_v : a.x_k;
+    const uint64_t ts = is_v ? a.tok_v : a.tok_k, hs = is_v ? a.head_v : a.head_k;
+    const size_t bh = (size_t)it.block * a.heads + head;
+    uint8_t* codes = (is_v ? a.v : a.k) + bh * a.bt * a.dim;
+    float* scale = (is_v ? a.v_scale : a.k_scale) + bh;
+    const int tid = threadIdx.x, T = blockDim.x;
+    const int cpt = a.dim / kChunk, n = it.count * cpt;   // chunks a token, chunks of the item
+    const float old = it.slot ? *scale : 0.f;
+
+    Raw<DT> r[kMaxChunks];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxChunks; ++i) {
+        const int c = tid + i * T;
+        if (c < n) {
+            const int t = c / cpt;
+            r[i] = load_raw<DT>(x, (it.row + t) * ts + head * hs + (c - t * cpt) * kChunk);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxChunks; ++i)
+        if (tid + i * T < n) {
+            float f[8];
+            to_floats<DT>(r[i], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fin_abs(f[e]));
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+    if ((tid & 31) == 0) red[tid >> 5] = amax;
+    __syncthreads();
+    for (int w = 0; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
+    const float s = fmaxf(fmaxf(__fdiv_rn(amax, kKVQmax<FMT>), kKVScaleFloor), old);
+    if (tid == 0) *scale = s;
+
+    if (it.slot && s > old) {   // the earlier tokens' codes, to the grown scale
+        const float ratio = __fdiv_rn(old, s);
+        for (int c = tid; c < it.slot * (int)a.dim / 4; c += T) {
+            uint32_t* p = reinterpret_cast<uint32_t*>(codes) + c;
+            float f[4];
+            kv_decode4<FMT>(*p, f);
+            uint32_t o = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o |= kv_code<FMT>(f[e] * ratio) << (8 * e);
+            *p = o;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxChunks; ++i) {
+        const int c = tid + i * T;
+        if (c < n) {
+            float f[8];
+            to_floats<DT>(r[i], f);
+            uint2 o = make_uint2(0u, 0u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o.x |= kv_code<FMT>(__fdiv_rn(f[e], s)) << (8 * e);
+                o.y |= kv_code<FMT>(__fdiv_rn(f[e + 4], s)) << (8 * e);
+            }
+            *reinterpret_cast<uint2*>(codes + (size_t)it.slot * a.dim + (size_t)c * kChunk) = o;
+        }
+    }
+}
+
+template <int DT, int FMT>
+__global__ void kv_read_kernel(const __grid_constant__ KVArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    Item it;
+    if (!find_item(a, blockIdx.x, it)) return;
+    const int head = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    void* y = const_cast<void*>(is_v ? a.x_v : a.x_k);
+    const uint64_t ts = is_v ? a.tok_v : a.tok_k, hs = is_v ? a.head_v : a.head_k;
+    const size_t bh = (size_t)it.block * a.heads + head;
+    const uint8_t* codes = (is_v ? a.v : a.k) + (bh * a.bt + it.slot) * a.dim;
+    const float s = (is_v ? a.v_scale : a.k_scale)[bh];
+    const int cpt = a.dim / 16, n = it.count * cpt;   // 16 codes at a time
+    for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        const int t = c / cpt;
+        const uint4 w = ld_stream(codes + (size_t)c * 16);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        const uint64_t e = (it.row + t) * ts + head * hs + (c - t * cpt) * 16;
+        if constexpr (DT == GRAFT_F32) {
+            float4* o = reinterpret_cast<float4*>((float*)y + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f[4];
+                kv_decode4<FMT>(ws[i], f);
+                o[i] = make_float4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
+            }
+        } else {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float f[4];
+                kv_decode4<FMT>(ws[i], f);
+                o[2 * i] = pack2<DT>(f[0] * s, f[1] * s);
+                o[2 * i + 1] = pack2<DT>(f[2] * s, f[3] * s);
+            }
+            uint4* p = reinterpret_cast<uint4*>((uint16_t*)y + e);
+            p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+    }
+}
+
+using KVKernel = void (*)(const KVArgs);
+template <int DT>
+KVKernel pick(bool write, uint32_t fmt) {
+    if (write)
+        return fmt == GRAFT_KV_INT8 ? kv_write_kernel<DT, GRAFT_KV_INT8>
+                                    : kv_write_kernel<DT, GRAFT_KV_E4M3>;
+    return fmt == GRAFT_KV_INT8 ? kv_read_kernel<DT, GRAFT_KV_INT8>
+                                : kv_read_kernel<DT, GRAFT_KV_E4M3>;
+}
+
+int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+            const GraftKVRange* range, cudaStream_t st) {
+    int rc;
+    if ((rc = kv_check_cache(cache)) || (rc = kv_check_range(cache, range)) ||
+        (rc = kv_check_heads("K", K, cache->head_dim)) ||
+        (rc = kv_check_heads("V", V, cache->head_dim)))
+        return rc;
+    GRAFT_REQUIRE(K->dtype == V->dtype && K->tokens == V->tokens,
+                  "K and V must have the same type and number of tokens");
+    if (range->n_seqs == 0 || K->tokens == 0) return GRAFT_OK;
+    KVArgs a = {};
+    a.k = (uint8_t*)cache->k, a.v = (uint8_t*)cache->v;
+    a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+    a.table = range->block_table, a.start = range->start, a.cu = range->cu_tokens;
+    a.x_k = K->data, a.x_v = V->data;
+    a.tok_k = K->token_stride, a.head_k = K->head_stride;
+    a.tok_v = V->token_stride, a.head_v = V->head_stride;
+    a.n_blocks = cache->n_blocks, a.heads = cache->kv_heads, a.bt = cache->block_tokens;
+    a.dim = cache->head_dim, a.n_seqs = range->n_seqs, a.table_stride = range->table_stride;
+    a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = K->tokens;
+    const uint64_t items = (uint64_t)K->tokens / a.bt + 2ull * a.n_seqs;
+    GRAFT_REQUIRE(items < (1ull << 31), "too many tokens in one call");
+    // 4 chunks of 8 elements a thread, up to 512 threads (then 8 chunks)
+    const int chunks = (int)(a.bt * a.dim) / (write ? kChunk : 16);
+    int threads = (chunks / 4 + 31) / 32 * 32;
+    threads = threads < 64 ? 64 : threads > 512 ? 512 : threads;
+    const KVKernel kern = K->dtype == GRAFT_F16    ? pick<GRAFT_F16>(write, cache->format)
+                          : K->dtype == GRAFT_BF16 ? pick<GRAFT_BF16>(write, cache->format)
+                                                   : pick<GRAFT_F32>(write, cache->format);
+    return launch_pdl(write ? "kv_write" : "kv_read", kern,
+                      dim3((unsigned)items, 2 * a.heads), threads, 0, st, a);
+}
+
+}  // namespace
+
+namespace graft {
+
+int kv_check_cache(const GraftKVCache* c) {
+    clear_error();
+    GRAFT_REQUIRE(c, "cache is null");
+    GRAFT_REQUIRE(c->k && c->v && c->k_scale && c->v_scale, "the cache has a null buffer");
+    GRAFT_REQUIRE(aligned(c->k, 16) && aligned(c->v, 16), "cache codes must be 16-byte aligned");
+    GRAFT_REQUIRE(aligned(c->k_scale, 4) && aligned(c->v_scale, 4),
+                  "cache scales must be 4-byte aligned");
+    GRAFT_REQUIRE(c->format == GRAFT_KV_INT8 || c->format == GRAFT_KV_E4M3,
+                  "unknown cache format %u", c->format);
+    const uint32_t bt = c->block_tokens;
+    GRAFT_REQUIRE(bt == 16 || bt == 32 || bt == 64 || bt == 128,
+                  "block_tokens must be 16, 32, 64 or 128, not %u", bt);
+    GRAFT_REQUIRE(c->head_dim >= 16 && c->head_dim <= 256 && c->head_dim % 16 == 0,
+                  "head_dim must be a multiple of 16 up to 256, not %u", c->head_dim);
+    GRAFT_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 32767, "kv_heads %u out of range",
+                  c->kv_heads);
+    GRAFT_REQUIRE(c->n_blocks >= 1 && c->n_blocks <= 0x7FFFFFFFu, "n_blocks %u out of range",
+                  c->n_blocks);
+    return GRAFT_OK;
+}
+
+int kv_check_range(const GraftKVCache* c, const GraftKVRange* r) {
+    GRAFT_REQUIRE(r, "range is null");
+    if (r->n_seqs == 0) return GRAFT_OK;
+    GRAFT_REQUIRE(r->block_table && r->start && r->cu_tokens, "the range has a null array");
+    GRAFT_REQUIRE(aligned(r->block_table, 4) && aligned(r->start, 4) && aligned(r->cu_tokens, 4),
+                  "the range's arrays must be 4-byte aligned");
+    GRAFT_REQUIRE(r->n_seqs < (1u << 28), "n_seqs %u out of range", r->n_seqs);
+    GRAFT_REQUIRE(r->max_len <= 0x7FFFFFFFu && r->max_tokens <= r->max_len,
+                  "max_tokens %u must not exceed max_len %u", r->max_tokens, r->max_len);
+    GRAFT_REQUIRE((uint64_t)r->table_stride * c->block_tokens >= r->max_len,
+                  "a block table row of %u blocks of %u tokens does not hold max_len %u",
+                  r->table_stride, c->block_tokens, r->max_len);
+    return GRAFT_OK;
+}
+
+int kv_check_heads(const char* name, const GraftHeads* h, uint32_t dim) {
+    GRAFT_REQUIRE(h, "%s is null", name);
+    GRAFT_REQUIRE(h->dtype == GRAFT_F16 || h->dtype == GRAFT_BF16 || h->dtype == GRAFT_F32,
+                  "%s: unknown element type %u", name, h->dtype);
+    if (h->tokens == 0) return GRAFT_OK;
+    const uint64_t es = h->dtype == GRAFT_F32 ? 4 : 2;
+    GRAFT_REQUIRE(h->data && aligned(h->data, 16), "%s must be a 16-byte aligned buffer", name);
+    GRAFT_REQUIRE(h->token_stride * es % 16 == 0 && h->head_stride * es % 16 == 0,
+                  "%s: strides must be multiples of 16 bytes", name);
+    GRAFT_REQUIRE(h->tokens <= 0x7FFFFFFFu, "%s: too many tokens", name);
+    (void)dim;
+    return GRAFT_OK;
+}
+
+unsigned kv_cache_device_errors(bool clear) { return read_device_errors(g_kv_err, clear); }
+
+}  // namespace graft
+
+extern "C" int graft_kv_write(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                              const GraftKVRange* range, graft_stream_t stream) {
+    return kv_move(true, cache, K, V, range, stream);
+}
+
+extern "C" int graft_kv_read(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                             const GraftKVRange* range, graft_stream_t stream) {
+    return kv_move(false, cache, K, V, range, stream);
+}
+
+extern "C" int graft_kv_device_errors(uint32_t* bits, int clear) {
+    clear_error();
+    GRAFT_REQUIRE(bits, "bits pointer is null");
+    GRAFT_CUDA(cudaDeviceSynchronize());
+    *bits = kv_cache_device_errors(clear != 0) | attn_device_errors(clear != 0);
+    return GRAFT_OK;
+}
