@@ -1,0 +1,157 @@
+// attn_common.cuh -- what the attention kernels over the 8-bit cache share:
+// arguments, code conversions to fp16 pairs, matrix instructions, the split of
+// the work over the grid and the joining of partial results.
+#pragma once
+#include "kv_common.cuh"
+
+namespace graft {
+namespace dev {
+
+struct AttnArgs {
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    const int32_t *table, *start, *cu;
+    const void* q;
+    void* out;
+    const float* sinks;
+    float* lse;
+    uint64_t q_tok, q_head, o_tok, o_head;
+    uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
+    uint32_t q_heads, group, window;
+    float scale;
+    int bf16;             // q and out: 1 bf16, 0 fp16
+    unsigned* counters;   // one per CTA, zero between calls
+    float* partials;      // two slots per CTA
+    int min_units;        // smallest piece that a pair is cut into
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The running maximum of a row without a key yet: finite, so that a masked
+// score (-inf) minus it is -inf and never NaN.
+constexpr float kNoMax = -1e30f;
+// Weights are held as 2^(t - max + kPShift): fp16 then keeps 11 bits of a
+// weight down to 2^-24 of the row's largest.
+constexpr float kPShift = 10.f;
+
+// Limit of every wait for a kernel's own copies or products.
+constexpr uint64_t kAttnWaitNs = 2000000000ull;
+// Most CTAs of an attention grid: one counter and two partial slots each.
+constexpr int kAttnMaxGrid = 512;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A sequence of the range as the attention kernels see it (n = 0: skip it).
+struct Seq {
+    int c0, n, start;
+};
+__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b, unsigned* err) {
+    Seq s;
+    s.c0 = a.cu[b];
+    s.n = a.cu[b + 1] - s.c0;
+    s.start = a.start[b];
+    if (s.c0 < 0 || s.n < 0 || s.n > (int)a.max_tokens ||
+        (uint64_t)s.c0 + (uint64_t)s.n > a.tokens || s.start < 0 ||
+        (uint64_t)((int64_t)s.start + s.n) > a.max_len) {
+        atomicOr(err, (unsigned)GRAFT_KV_EBOUNDS);
+        s.n = 0;
+    }
+    return s;
+}
+// First key that token i (position p) sees.
+__device__ __forceinline__ int first_key(const AttnArgs& a, int p) {
+    return a.window && p >= (int)a.window ? p - (int)a.window + 1 : 0;
+}
+
+// ---- codes to fp16 pairs
+// int8: with the sign bit flipped a code is code + 128 in 0..255; as the low
+// byte of 0x64xx it is the fp16 number 1024 + 128 + code, and one exact
+// subtraction of 1152 leaves the code.
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
+    return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// bytes 0,1 of w as an fp16 pair in lo, bytes 2,3 in hi
+template <int FMT>
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (FMT == GRAFT_KV_INT8) {
+        w ^= 0x80808080u;
+        lo = hsub2(prmt(w, 0x64646464u, 0x4140), 0x64806480u);
+        hi = hsub2(prmt(w, 0x64646464u, 0x4342), 0x64806480u);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\t"
+            "mov.b32 {a, b}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+// D += A (16 x 16, fp16, row) B (16 x 8, fp16, col), fp32 sums
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8 x 8 transpose of 16-bit elements across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Sixteen consecutive query elements as eight fp16 pairs.  bf16 queries become
+// fp16 through a power of two per row that brings the row's largest magnitude
+// to [2^14, 2^15): every element keeps its 8 bits unless it is under 2^-28 of
+// the row's largest.  `up` multiplies the scores to undo it.
+__device__ __forceinline__ float bf16_row_exponent(float amax) {
+    if (!(amax > 0.f) || amax > 3.4e38f) return 0.f;   // zeros; NaN, infinity: as they are
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127 - 14;
+    return (float)max(e, -126);
+}
+
+// ---- the split of the work
+// Units (fixed numbers of keys) of all (sequence, tile, head) "pairs" lie in
+// one row; CTA c of G takes those from x_c to x_{c+1}, x_c = floor(c U / G),
+// each bound moved to the pair's edge if that is nearer than `snap` units.
+// A pair that is cut has as its first piece the CTA before the first cut, and
+// each CTA holds at most one first piece and one later piece, so two partial
+// slots and one counter per CTA are enough.
+struct Split {
+    long long U;
+    int G, snap;
+    __device__ __forceinline__ long long bound(int c) const { return (long long)c * U / G; }
+    __device__ __forceinline__ long long snapped(long long x, long long p0, long long p1) const {
+        if (x - p0 < snap && x - p0 <= p1 - x) return p0;
+        if (p1 - x < snap) return p1;
+        return x;
+    }
+    // cuts inside [p0, p1): CTAs ca..cb start there (none if cb < ca)
+    __device__ __forceinline__ void cuts(long long p0, long long p1, int& ca, int& cb) const {
+        const long long lo = p0 + snap, hi = p1 - snap;
+        ca = 0, cb = -1;
+        if (lo > hi) return;
+        ca = (int)((lo * G + U - 1) / U);
+        cb = (int)(((hi + 1) * G + U - 1) / U) - 1;
+    }
+};
+
+}  // namespace dev
+}  // namespace graft

@@ -5,8 +5,9 @@
 //
 // One CTA per (token, query head): its warps take every fourth key with a
 // running maximum and sum each, and are merged at the end.
-#include "kv_common.cuh"
+#include "attn_few.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 using namespace graft;
@@ -15,22 +16,6 @@ using namespace graft::dev;
 namespace {
 
 __device__ unsigned g_attn_err;
-
-struct AttnArgs {
-    const uint8_t *k, *v;
-    const float *k_scale, *v_scale;
-    const int32_t *table, *start, *cu;
-    const void* q;
-    void* out;
-    const float* sinks;
-    float* lse;
-    uint64_t q_tok, q_head, o_tok, o_head;
-    uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
-    uint32_t q_heads, group, window;
-    float scale;
-};
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DT, int FMT>
 __global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant__ AttnArgs a) {
@@ -124,6 +109,38 @@ __global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant_
         a.lse[(size_t)t * a.q_heads + h] = L != 0.f ? M + logf(L) : -INFINITY;
 }
 
+// ---- few query rows
+template <int DP, int NT, int FMT>
+int launch_few(AttnArgs a, cudaStream_t st) {
+    DeviceInfo di;
+    int rc = current_device_info(&di);
+    if (rc) return rc;
+    constexpr int smem = kFewSmem<DP, NT>;
+    const void* kern = (const void*)attn_few_kernel<DP, NT, FMT>;
+    int per_sm = 1;
+    if ((rc = ensure_smem(kern, smem)) || (rc = occupancy(kern, kFewThreads, smem, &per_sm)))
+        return rc;
+    unsigned* err = nullptr;
+    GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
+    // no more CTAs than the longest possible range has pieces
+    const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
+                                   : a.max_len;
+    const uint64_t units = keys / kFewUnit<DP> + 2, pairs = (uint64_t)a.n_seqs * a.heads;
+    a.min_units = 2 * kFewWarps;
+    const uint64_t want = std::max(pairs, pairs * units / a.min_units + 1);
+    const int grid = (int)std::min<uint64_t>(std::min(di.sm_count * per_sm, kAttnMaxGrid), want);
+    return launch_pdl("attn_kv8", attn_few_kernel<DP, NT, FMT>, dim3(grid), kFewThreads, smem, st,
+                      a, err);
+}
+template <int DP, int NT>
+int launch_few(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
+    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8>(a, st)
+                                : launch_few<DP, NT, GRAFT_KV_E4M3>(a, st);
+}
+
+// Query rows that the few-row kernel takes for a head_dim (registers).
+int few_rows(uint32_t dim) { return dim <= 64 ? 32 : dim <= 128 ? 16 : 8; }
+
 int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const GraftAttnParams* P) {
     int rc;
     if ((rc = kv_check_cache(cache)) || (rc = kv_check_range(cache, range))) return rc;
@@ -143,7 +160,11 @@ unsigned attn_device_errors(bool clear) { return read_device_errors(g_attn_err, 
 
 extern "C" size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const GraftKVRange* range,
                                            const GraftAttnParams* P) {
-    return check_attn(cache, range, P) ? 0 : 256;
+    if (check_attn(cache, range, P)) return 0;
+    const uint32_t d = cache->head_dim;
+    const size_t slot = d <= 64 ? kFewPartial<64, 4> : d <= 128 ? kFewPartial<128, 2>
+                                                                : kFewPartial<256, 1>;
+    return kAttnMaxGrid * (4 + 2 * 4 * slot);
 }
 
 extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t stream) {
@@ -181,6 +202,21 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
     a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = q->tokens;
     a.q_heads = P->q_heads, a.group = P->q_heads / cache->kv_heads, a.window = P->window;
     a.scale = P->scale;
+    a.bf16 = q->dtype == GRAFT_BF16;
+    a.counters = (unsigned*)ws;
+    a.partials = (float*)((char*)ws + kAttnMaxGrid * 4);
+    const uint64_t rows = (uint64_t)range->max_tokens * a.group;
+    if (range->max_tokens == 0) return GRAFT_OK;
+    if (rows <= (uint64_t)few_rows(a.dim)) {
+        if (a.dim <= 64)
+            return rows <= 8    ? launch_few<64, 1>(a, cache->format, stream)
+                   : rows <= 16 ? launch_few<64, 2>(a, cache->format, stream)
+                                : launch_few<64, 4>(a, cache->format, stream);
+        if (a.dim <= 128)
+            return rows <= 8 ? launch_few<128, 1>(a, cache->format, stream)
+                             : launch_few<128, 2>(a, cache->format, stream);
+        return launch_few<256, 1>(a, cache->format, stream);
+    }
     void (*kern)(const AttnArgs);
     if (q->dtype == GRAFT_F16)
         kern = cache->format == GRAFT_KV_INT8 ? attn_simple_kernel<GRAFT_F16, GRAFT_KV_INT8>
