@@ -19,10 +19,12 @@ struct AttnArgs {
     uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
     uint32_t q_heads, group, window;
     float scale;
+    int bt_log2;          // block_tokens = 1 << bt_log2
     int bf16;             // q and out: 1 bf16, 0 fp16
     unsigned* counters;   // one per CTA, zero between calls
     float* partials;      // two slots per CTA
-    int min_units;        // smallest piece that a pair is cut into
+    int min_units;        // smallest share of a CTA that is worth one
+    int pad_units;        // units that a pair costs besides its own
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -30,9 +32,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum of a row without a key yet: finite, so that a masked
 // score (-inf) minus it is -inf and never NaN.
 constexpr float kNoMax = -1e30f;
-// Weights are held as 2^(t - max + kPShift): fp16 then keeps 11 bits of a
-// weight down to 2^-24 of the row's largest.
-constexpr float kPShift = 10.f;
+// Weights are held as 2^(t - m + kPShift) for a reference m that no t passes
+// by more than kPSlack: at most 2^14 in fp16, which keeps its 11 bits down to
+// 2^-28 of that.
+constexpr float kPShift = 10.f, kPSlack = 4.f;
 
 // Limit of every wait for a kernel's own copies or products.
 constexpr uint64_t kAttnWaitNs = 2000000000ull;
@@ -43,6 +46,16 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // A sequence of the range as the attention kernels see it (n = 0: skip it).
@@ -68,9 +81,6 @@ __device__ __forceinline__ int first_key(const AttnArgs& a, int p) {
 }
 
 // ---- codes to fp16 pairs
-// int8: with the sign bit flipped a code is code + 128 in 0..255; as the low
-// byte of 0x64xx it is the fp16 number 1024 + 128 + code, and one exact
-// subtraction of 1152 leaves the code.
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
     uint32_t r;
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
@@ -81,7 +91,9 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// bytes 0,1 of w as an fp16 pair in lo, bytes 2,3 in hi
+// The four codes of a word as fp16 pairs, codes 0,1 and 2,3.  An int8 code with
+// its sign bit flipped is code + 128; as the low byte of 0x64xx that is the fp16
+// number 1024 + 128 + code, and one exact subtraction of 1152 leaves the code.
 template <int FMT>
 __device__ __forceinline__ void codes_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
     if constexpr (FMT == GRAFT_KV_INT8) {
@@ -129,27 +141,37 @@ __device__ __forceinline__ float bf16_row_exponent(float amax) {
 
 // ---- the split of the work
 // Units (fixed numbers of keys) of all (sequence, tile, head) "pairs" lie in
-// one row; CTA c of G takes those from x_c to x_{c+1}, x_c = floor(c U / G),
-// each bound moved to the pair's edge if that is nearer than `snap` units.
-// A pair that is cut has as its first piece the CTA before the first cut, and
-// each CTA holds at most one first piece and one later piece, so two partial
-// slots and one counter per CTA are enough.
+// one row, each pair preceded by `pad` empty ones that stand for what a pair
+// costs besides its units (queries, joining the warps, output).  CTA c of G
+// takes those from x_c to x_{c+1}, where the x_c cut the row evenly (the first
+// U % G shares are one longer), each moved to its pair's edge if it would
+// leave a piece of less than `snap` units.  A pair that is cut has as its first
+// piece the CTA before the first cut, and each CTA holds at most one first
+// piece and one later piece, so two partial slots and one counter per CTA are
+// enough.  U < 2^31 (the host's check).
 struct Split {
-    long long U;
-    int G, snap;
-    __device__ __forceinline__ long long bound(int c) const { return (long long)c * U / G; }
-    __device__ __forceinline__ long long snapped(long long x, long long p0, long long p1) const {
-        if (x - p0 < snap && x - p0 <= p1 - x) return p0;
-        if (p1 - x < snap) return p1;
-        return x;
+    int U, G, pad, snap, share, longer;   // share = U / G, longer = U % G
+    __device__ __forceinline__ void set(int units, int ctas, int pad_units, int snap_units) {
+        U = units, G = ctas, pad = pad_units, snap = snap_units;
+        share = U / G, longer = U - share * G;
+    }
+    __device__ __forceinline__ int bound(int c) const { return c * share + min(c, longer); }
+    // the first CTA whose bound is x or more
+    __device__ __forceinline__ int at_least(int x) const {
+        const int head = longer * (share + 1);
+        return x <= head ? (x + share) / (share + 1) : longer + (x - head + share - 1) / share;
+    }
+    __device__ __forceinline__ int snapped(int x, int p0, int p1) const {
+        const bool head = x < p0 + pad + snap, tail = x > p1 - snap;
+        return !head && !tail ? x : !tail || (head && x - p0 <= p1 - x) ? p0 : p1;
     }
     // cuts inside [p0, p1): CTAs ca..cb start there (none if cb < ca)
-    __device__ __forceinline__ void cuts(long long p0, long long p1, int& ca, int& cb) const {
-        const long long lo = p0 + snap, hi = p1 - snap;
+    __device__ __forceinline__ void cuts(int p0, int p1, int& ca, int& cb) const {
+        const int lo = p0 + pad + snap, hi = p1 - snap;
         ca = 0, cb = -1;
         if (lo > hi) return;
-        ca = (int)((lo * G + U - 1) / U);
-        cb = (int)(((hi + 1) * G + U - 1) / U) - 1;
+        ca = at_least(lo);
+        cb = at_least(hi + 1) - 1;
     }
 };
 

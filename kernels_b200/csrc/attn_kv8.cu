@@ -110,32 +110,39 @@ __global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant_
 }
 
 // ---- few query rows
-template <int DP, int NT, int FMT>
+template <int DP, int NT, int FMT, bool FULL>
 int launch_few(AttnArgs a, cudaStream_t st) {
     DeviceInfo di;
     int rc = current_device_info(&di);
     if (rc) return rc;
     constexpr int smem = kFewSmem<DP, NT>;
-    const void* kern = (const void*)attn_few_kernel<DP, NT, FMT>;
+    const auto kern = attn_few_kernel<DP, NT, FMT, FULL>;
     int per_sm = 1;
-    if ((rc = ensure_smem(kern, smem)) || (rc = occupancy(kern, kFewThreads, smem, &per_sm)))
+    if ((rc = ensure_smem((const void*)kern, smem)) ||
+        (rc = occupancy((const void*)kern, kFewThreads, smem, &per_sm)))
         return rc;
     unsigned* err = nullptr;
     GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
     // no more CTAs than the longest possible range has pieces
     const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
                                    : a.max_len;
-    const uint64_t units = keys / kFewUnit<DP> + 2, pairs = (uint64_t)a.n_seqs * a.heads;
     a.min_units = 2 * kFewWarps;
+    a.pad_units = 2 * kFewWarps;
+    const uint64_t units = keys / kFewUnit<DP> + 2 + a.pad_units;
+    const uint64_t pairs = (uint64_t)a.n_seqs * a.heads;
+    GRAFT_REQUIRE(pairs * units < (1ull << 31), "max_len %u of %u sequences is too long", a.max_len,
+                  a.n_seqs);
     const uint64_t want = std::max(pairs, pairs * units / a.min_units + 1);
     const int grid = (int)std::min<uint64_t>(std::min(di.sm_count * per_sm, kAttnMaxGrid), want);
-    return launch_pdl("attn_kv8", attn_few_kernel<DP, NT, FMT>, dim3(grid), kFewThreads, smem, st,
-                      a, err);
+    return launch_pdl("attn_kv8", kern, dim3(grid), kFewThreads, smem, st, a, err);
 }
 template <int DP, int NT>
 int launch_few(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
-    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8>(a, st)
-                                : launch_few<DP, NT, GRAFT_KV_E4M3>(a, st);
+    if (a.dim == DP)
+        return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, true>(a, st)
+                                    : launch_few<DP, NT, GRAFT_KV_E4M3, true>(a, st);
+    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, false>(a, st)
+                                : launch_few<DP, NT, GRAFT_KV_E4M3, false>(a, st);
 }
 
 // Query rows that the few-row kernel takes for a head_dim (registers).
@@ -202,6 +209,7 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
     a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = q->tokens;
     a.q_heads = P->q_heads, a.group = P->q_heads / cache->kv_heads, a.window = P->window;
     a.scale = P->scale;
+    a.bt_log2 = a.bt == 16 ? 4 : a.bt == 32 ? 5 : a.bt == 64 ? 6 : 7;
     a.bf16 = q->dtype == GRAFT_BF16;
     a.counters = (unsigned*)ws;
     a.partials = (float*)((char*)ws + kAttnMaxGrid * 4);
