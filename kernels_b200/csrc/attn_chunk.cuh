@@ -1,0 +1,739 @@
+// attn_chunk.cuh -- attention over the 8-bit cache for many query rows a head
+// (chunks of a prompt), on the fifth-generation tensor cores.
+//
+// Rows are (token, query head of the key/value head) pairs.  A CTA (one per SM)
+// works on RT tiles of 128 rows against units of KT keys, with O and the scores
+// in tensor memory and these roles:
+//   softmax     (4 warps a row tile)  thread = row = TMEM lane: reads its KT scores,
+//               takes the weights and writes them back as fp16 (the A operand
+//               of the second product) over the scores;
+//   converters  (4 warps)  read a unit's codes from the cache and store them as
+//               fp16 in shared memory, 128-byte swizzled rows of 64 dims: the
+//               K-major B operand of q K^T and, unchanged in layout, the
+//               MN-major B operand of P V;
+//   MMA         (one lane)  per row tile: P V of unit j, then q K^T of unit j + 1,
+//               so that one tile's products run under the other's softmax.
+// The scales enter the exponents as in the few-row kernel (attn_few.cuh).  The
+// reference of the exponents follows the row's maximum only when it is passed by
+// more than kPSlack, so that O is seldom rescaled in tensor memory.
+// Work is split evenly over the CTAs by (row tile, head, unit), and the pieces of
+// a cut pair meet in the workspace (Split in attn_common.cuh).
+#pragma once
+#include "attn_common.cuh"
+
+#include <type_traits>
+
+namespace graft {
+namespace dev {
+
+template <int DP>
+struct Chunk {
+    static constexpr int RT = DP <= 128 ? 2 : 1;     // row tiles
+    static constexpr int KT = DP <= 128 ? 128 : 64;  // keys of a unit
+    static constexpr int ST = DP <= 64 ? 3 : 2;      // stages of K and V
+    static constexpr int ROWS = 128 * RT;
+    static constexpr int SOFT = 4 * RT;              // softmax warps
+    static constexpr int THREADS = 32 * (SOFT + 4 + 1);
+    static constexpr int DB = DP / 64;               // blocks of 64 dims
+    static constexpr int Q_BYTES = RT * DB * 128 * 128;
+    static constexpr int KV_BYTES = DB * KT * 128;   // K or V of a unit
+    static constexpr int SMEM = 1024 + Q_BYTES + 2 * ST * KV_BYTES;
+    static constexpr int O_COL = 256;                // TMEM: scores of tile i at i*128, O at 256 + i*DP
+    static constexpr int SC = 4;                     // slots of a unit's scales
+    // floats of a partial result: O column by column, maximum and sum of each row
+    static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
+};
+
+// ---- tcgen05 (inline PTX)
+__device__ __forceinline__ void tc5_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc5_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc5_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tc5_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc5_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Shared-memory descriptor of 128-byte swizzled rows: start, leading and stride
+// byte offsets (>> 4), version 1, layout SWIZZLE_128B.  K-major: 8-row groups
+// `stride` apart.  MN-major: groups of 8 along K `stride` apart, blocks of 64
+// along MN `lead` apart.
+__device__ __forceinline__ uint64_t tc5_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
+           ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 instruction descriptor: f32 sums, fp16 operands, M = 128, N; bit 16: B is MN-major.
+__device__ __forceinline__ constexpr uint32_t tc5_idesc(int n, bool mn_major) {
+    return (1u << 4) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+          "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31, %32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// sum of floor((a i + b) / m) over i < n, for a, b >= 0 (the Euclid-like recursion)
+__device__ __forceinline__ int floor_sum(int n, int m, int a, int b) {
+    long long s = 0, nn = n, mm = m, aa = a, bb = b;
+    while (nn > 0) {
+        s += (nn - 1) * nn / 2 * (aa / mm) + nn * (bb / mm);
+        aa %= mm, bb %= mm;
+        const long long y = aa * nn + bb;
+        if (y < mm) break;
+        nn = y / mm, bb = y % mm;
+        const long long t = mm;
+        mm = aa, aa = t;
+    }
+    return (int)s;
+}
+
+template <int DP, int FMT>
+__global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
+    attn_chunk_kernel(const __grid_constant__ AttnArgs a, unsigned* err) {
+    using C = Chunk<DP>;
+    constexpr int RT = C::RT, KT = C::KT, ST = C::ST, SC = C::SC, DB = C::DB, ROWS = C::ROWS;
+    struct Walk {
+        int at, prefix;   // next unit; units (of all heads) before the row tile
+        Seq s;
+        int b, rt, tiles; // sequence, row tile, row tiles of the sequence
+        int nu, u0;       // units of the row tile a head with the pad, its first unit
+        int h, lo, hi;    // the piece: head, units [lo, hi)
+        int p0;           // first unit of the pair
+    };
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ Walk sh_edge[2];
+    __shared__ uint64_t kfull[ST], kfree[ST], vfull[ST], vfree[ST], scfull[SC], sfull[RT], pfull[RT],
+        ofull[RT], qfull[RT], done;
+    __shared__ float4 scales[SC][KT / 16];   // k_scale, log2(v_scale), 1 / v_scale
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int dead;            // a wait gave up: every role stops
+    __shared__ int sh_scan[C::THREADS / 32], sh_last[RT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int D = a.dim, H = a.heads, G = a.group, TT = ROWS / G;   // tokens of a row tile
+    uint8_t* base = smem + ((1024 - (smem_u32(smem) & 1023)) & 1023);
+    uint8_t *sq = base, *sk = base + C::Q_BYTES, *sv = sk + ST * C::KV_BYTES;
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(smem_u32(&kfull[i]), 4), mbar_init(smem_u32(&vfull[i]), 4);   // converter warps
+            mbar_init(smem_u32(&kfree[i]), 1), mbar_init(smem_u32(&vfree[i]), 1);   // commits
+        }
+        for (int i = 0; i < SC; ++i) mbar_init(smem_u32(&scfull[i]), 4);
+        for (int i = 0; i < RT; ++i) {
+            mbar_init(smem_u32(&sfull[i]), 1), mbar_init(smem_u32(&ofull[i]), 1);
+            mbar_init(smem_u32(&pfull[i]), 4), mbar_init(smem_u32(&qfull[i]), 4);   // softmax warps
+        }
+        mbar_init(smem_u32(&done), 1);
+        dead = 0;
+    }
+    fence_mbar_init();
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- units of a row tile and of the row tiles before it
+    auto open_tile = [&](Walk& w) {
+        const int i0 = w.rt * TT, i1 = min(w.s.n - 1, i0 + TT - 1);
+        w.u0 = first_key(a, w.s.start + i0) / KT;
+        w.nu = (w.s.start + i1) / KT + 1 - w.u0 + a.pad_units;
+    };
+    auto open_seq = [&](Walk& w) {
+        w.s = load_seq(a, w.b, err);
+        w.tiles = (w.s.n + TT - 1) / TT;
+    };
+    auto units_before = [&](const Walk& w, int rt) {   // rt <= tiles
+        int full = min(rt, w.s.n / TT);                // (the last tile may have fewer tokens)
+        int u = floor_sum(full, KT, TT, w.s.start + TT - 1) + rt * (1 + a.pad_units);
+        if (full < rt) u += (w.s.start + w.s.n - 1) / KT;
+        if (a.window) {   // first units: floor((start - window + 1 + TT i) / KT) where that is positive
+            const int c = w.s.start - (int)a.window + 1;
+            const int skip = c >= 0 ? 0 : min(rt, (-c + TT - 1) / TT);
+            u -= floor_sum(rt - skip, KT, TT, c + skip * TT);
+        }
+        return u;
+    };
+    Split sp;
+    Walk cw;
+    int fe;
+    {
+        int U = 0, pairs = 0, prefix = 0, base_u = 0;
+        auto scan = [&](int v, int& before) {   // over the CTA's threads; returns the total
+            int x = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) sh_scan[warp] = x;
+            __syncthreads();
+            before = x - v;
+            int total = 0;
+            for (int w = 0; w < C::THREADS / 32; ++w) {
+                const int y = sh_scan[w];
+                if (w < warp) before += y;
+                total += y;
+            }
+            return total;
+        };
+        for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += C::THREADS) {
+            cw.b = b0 + tid, cw.tiles = 0;
+            if (cw.b < (int)a.n_seqs) open_seq(cw);
+            int skip;
+            pairs += scan(cw.tiles, skip);
+            U += scan(cw.tiles ? units_before(cw, cw.tiles) : 0, prefix);
+        }
+        U *= H, pairs *= H;
+        if (U == 0) return;
+        const int grid = min((int)gridDim.x, max(pairs, (U - pairs * a.pad_units) / a.min_units));
+        if ((int)blockIdx.x >= grid) return;
+        sp.set(U, grid, a.pad_units, max(1, a.min_units / 2));
+        const int x0 = sp.bound(blockIdx.x), x1 = sp.bound(blockIdx.x + 1);
+        for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += C::THREADS) {   // the bounds' sequences
+            int mine = 0;
+            if (a.n_seqs > C::THREADS) {
+                cw.b = b0 + tid, cw.tiles = 0;
+                if (cw.b < (int)a.n_seqs) open_seq(cw);
+            }
+            if (cw.tiles) mine = units_before(cw, cw.tiles);
+            const int total = scan(mine, prefix);
+            cw.prefix = (base_u + prefix) * H;
+            const int e = cw.prefix + mine * H;
+            if (cw.prefix <= x0 && x0 < e) sh_edge[0] = cw;
+            if (cw.prefix <= x1 && x1 < e) sh_edge[1] = cw;
+            base_u += total;
+        }
+        __syncthreads();
+        // their row tiles: the CTA's threads test every step-th row tile, then the ones between
+        auto find_tile = [&](int k, int x) {
+            Walk w = sh_edge[k];
+            const int seq_at = w.prefix;
+            int lo = 0, n = w.tiles;   // the row tile is one of [lo, lo + n)
+            while (n > 0) {
+                const int step = (n + C::THREADS - 1) / C::THREADS, rt = lo + tid * step;
+                __syncthreads();
+                if (tid * step < n && rt < w.tiles) {
+                    const int end = min(min(rt + step, lo + n), w.tiles);
+                    const int p = seq_at + units_before(w, rt) * H;
+                    if (p <= x && x < seq_at + units_before(w, end) * H) {
+                        w.rt = rt;
+                        w.prefix = p;
+                        sh_edge[k] = w;
+                    }
+                }
+                __syncthreads();
+                if (step == 1) break;
+                const int end = lo + n;
+                lo = sh_edge[k].rt;
+                n = min(step, end - lo);
+            }
+            w = sh_edge[k];
+            open_tile(w);
+            return w;
+        };
+        auto edge = [&](const Walk& w, int x) {
+            const int p0 = w.prefix + (x - w.prefix) / w.nu * w.nu;
+            return sp.snapped(x, p0, p0 + w.nu);
+        };
+        fe = U;
+        if (x1 < U) fe = edge(find_tile(1, x1), x1);
+        cw = find_tile(0, x0);
+        cw.at = edge(cw, x0);
+        if (cw.at >= fe) return;
+    }
+    auto next_piece = [&](Walk& w) {   // false: no more
+        if (w.at >= fe) return false;
+        while (w.at >= w.prefix + w.nu * H) {
+            w.prefix += w.nu * H;
+            if (++w.rt >= w.tiles) {
+                w.rt = 0;
+                do {
+                    ++w.b;
+                    open_seq(w);
+                } while (w.tiles == 0);
+            }
+            open_tile(w);
+        }
+        w.h = (w.at - w.prefix) / w.nu;
+        w.p0 = w.prefix + w.h * w.nu;
+        const int e = min(fe, w.p0 + w.nu);
+        w.lo = w.u0 + max(0, w.at - w.p0 - a.pad_units);
+        w.hi = w.u0 + e - w.p0 - a.pad_units;
+        w.at = e;
+        return true;
+    };
+    // false: this or another wait gave up
+    auto wait_lane = [&](uint64_t* bar, uint32_t phase) {
+        uint64_t t0 = 0;
+        while (!mbar_try_wait(smem_u32(bar), phase & 1)) {
+            if (dead) return false;
+            const uint64_t now = global_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kAttnWaitNs) {
+                atomicOr(err, (unsigned)GRAFT_KV_EWAIT);
+                dead = 1;
+                return false;
+            }
+        }
+        return true;
+    };
+    auto wait = [&](uint64_t* bar, uint32_t phase) {   // by a whole warp
+        return (bool)__all_sync(~0u, wait_lane(bar, phase));
+    };
+    if (warp == C::SOFT + 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_at)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp < C::SOFT) {
+        // =========================================================== softmax
+        const int tile = warp >> 2, row = (warp & 3) * 32 + lane;   // row of the tile = TMEM lane
+        const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t ts = tlane + tile * 128, to = tlane + C::O_COL + tile * DP;
+        int it = 0, pc = 0;   // units and pieces done
+        bool live = true;
+        while (live && next_piece(cw)) {
+            const int r = tile * 128 + row, tok = cw.rt * TT + r / G, hq = cw.h * G + r % G;
+            const bool on = r < TT * G && tok < cw.s.n;
+            // ---- the row's queries, as fp16 (the sign of the scale goes with them)
+            float cr;
+            {
+                const uint16_t* src = (const uint16_t*)a.q + (size_t)(cw.s.c0 + (on ? tok : 0)) * a.q_tok +
+                                      (size_t)(on ? hq : 0) * a.q_head;
+                float down = 1.f, up = 1.f;
+                if (a.bf16) {
+                    float amax = 0.f;
+                    for (int d = 0; d < D && on; d += 8) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(src + d);
+                        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 p = unpack2<GRAFT_BF16>(w[e]);
+                            amax = (p.x == p.x) ? fmaxf(amax, fabsf(p.x)) : INFINITY;
+                            amax = (p.y == p.y) ? fmaxf(amax, fabsf(p.y)) : INFINITY;
+                        }
+                    }
+                    const float e = bf16_row_exponent(amax);
+                    down = exp2f(-e), up = exp2f(e);
+                }
+                const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+                cr = fabsf(a.scale) * kLog2e * up;
+#pragma unroll 2
+                for (int c = 0; c < DP / 8; ++c) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (on && 8 * c < D) x = *reinterpret_cast<const uint4*>(src + 8 * c);
+                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (a.bf16) {
+                            const float2 p = unpack2<GRAFT_BF16>(w[e]);
+                            w[e] = pack_h2(p.x * down, p.y * down);
+                        }
+                        w[e] ^= flip;
+                    }
+                    *reinterpret_cast<uint4*>(sq + ((tile * DB + c / 8) * 128 + row) * 128 +
+                                              (((c & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&qfull[tile]));
+            }
+            const int p = on ? cw.s.start + tok : -1, lo = on ? first_key(a, p) : 0;
+            float m = kNoMax, l = 0.f;
+            for (int u = cw.lo; u < cw.hi; ++u, ++it) {
+                if (!(live = wait(&sfull[tile], it)) || !(live = wait(&scfull[it % SC], it / SC))) break;
+                tc5_fence_after();
+                const float4* sc = scales[it % SC];
+                const int c_lo = lo - u * KT, c_hi = p - u * KT;   // columns that the row sees
+                const bool edge_unit = __any_sync(~0u, c_lo > 0 || c_hi < KT - 1);
+                // ---- the row's maximum
+                float mx = kNoMax;
+                auto take_max = [&](auto masked) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(ts + 32 * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float4 f = sc[2 * c + q];
+                            float x = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                float y = __uint_as_float(v[16 * q + e]);
+                                const int col = 32 * c + 16 * q + e;
+                                if (decltype(masked)::value) y = col >= c_lo && col <= c_hi ? y : -INFINITY;
+                                x = fmaxf(x, y);
+                            }
+                            x = x == -INFINITY ? x : fmaf(x, f.x * cr, f.y);
+                            mx = fmaxf(mx, x);
+                        }
+                    }
+                };
+                if (edge_unit) take_max(std::true_type{});
+                else take_max(std::false_type{});
+                if (__any_sync(~0u, mx > m + kPSlack)) {
+                    const float nm = fmaxf(m, mx), f = ex2(m - nm);
+                    l *= f;
+                    m = nm;
+                    if (u > cw.lo) {   // (the scores' arrival says that the product before is done)
+#pragma unroll
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t v[32];
+                            tmem_ld32(to + 32 * c, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tmem_st32(to + 32 * c, v);
+                        }
+                    }
+                }
+                // ---- the weights, over the scores that have been read
+                auto weigh = [&](auto masked) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t v[32], w[16];
+                        tmem_ld32(ts + 32 * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float4 f = sc[2 * c + q];
+                            const float fa = f.x * cr, fb = f.y - (m - kPShift);
+                            float sum[2] = {0.f, 0.f};
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                float y[2];
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    y[k] = fmaf(__uint_as_float(v[16 * q + e + k]), fa, fb);
+                                    const int col = 32 * c + 16 * q + e + k;
+                                    if (decltype(masked)::value)
+                                        y[k] = col >= c_lo && col <= c_hi ? y[k] : -INFINITY;
+                                    y[k] = ex2(y[k]);
+                                    sum[k] += y[k];
+                                }
+                                w[8 * q + e / 2] = pack_h2(y[0], y[1]);
+                            }
+                            l = fmaf(sum[0] + sum[1], f.z, l);
+                        }
+                        tmem_st16(ts + 16 * c, w);
+                    }
+                };
+                if (edge_unit) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                tmem_wait_st();
+                tc5_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&pfull[tile]));
+            }
+            if (!live || !(live = wait(&ofull[tile], pc))) break;
+            ++pc;
+            tc5_fence_after();
+            // ---- output: the row itself, or its part of a cut pair
+            int ca, cb;
+            sp.cuts(cw.p0, cw.p0 + cw.nu, ca, cb);
+            const bool cut = cb >= ca;
+            const int first = ca - 1, pieces = cb - ca + 2;
+            if (cut) {
+                float* part = a.partials + ((size_t)blockIdx.x * 2 + (cw.lo == cw.u0)) * C::PARTIAL + r;
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(to + 32 * c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        __stcg(part + (32 * c + e) * ROWS, __uint_as_float(v[e]));
+                }
+                __stcg(part + DP * ROWS, m);
+                __stcg(part + DP * ROWS + ROWS, l);
+                // the row tile's 4 warps; each row tile has its own count
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
+                if ((tid & 127) == 0) {
+                    unsigned was;
+                    unsigned* count = a.counters + first * RT + tile;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                                 : "=r"(was) : "l"(count) : "memory");
+                    sh_last[tile] = was + 1 == (unsigned)pieces;
+                    if (sh_last[tile]) *count = 0;
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
+                if (!sh_last[tile]) continue;
+            }
+            const float* parts = a.partials + (size_t)first * 2 * C::PARTIAL + r;   // piece k: CTA first + k
+            auto piece = [&](int k) { return parts + (size_t)(2 * k + (k == 0)) * C::PARTIAL; };
+            if (cut) {
+                m = kNoMax, l = 0.f;
+                for (int k = 0; k < pieces; ++k) m = fmaxf(m, __ldcg(piece(k) + DP * ROWS));
+                for (int k = 0; k < pieces; ++k)
+                    l = fmaf(__ldcg(piece(k) + DP * ROWS + ROWS), ex2(__ldcg(piece(k) + DP * ROWS) - m), l);
+            }
+            float ref = m - kPShift, fo = 1.f;
+            if (a.sinks) {
+                const float s = a.sinks[on ? hq : 0] * kLog2e;
+                if (s > ref) {
+                    fo = ex2(ref - s);
+                    l = l * fo + 1.f;
+                    ref = s;
+                } else if (s != -INFINITY) {
+                    l += ex2(s - ref);
+                }
+            }
+            fo = l != 0.f ? __fdividef(fo, l) : 0.f;
+            uint16_t* y = (uint16_t*)a.out + (size_t)(cw.s.c0 + (on ? tok : 0)) * a.o_tok +
+                          (size_t)(on ? hq : 0) * a.o_head;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+                float o[32];
+                if (!cut) {
+                    tmem_ld32(to + 32 * c, reinterpret_cast<uint32_t(&)[32]>(o));
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    for (int k = 0; k < pieces; ++k) {
+                        const float* q = piece(k);
+                        const float f = ex2(__ldcg(q + DP * ROWS) - m);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = fmaf(__ldcg(q + (32 * c + e) * ROWS), f, o[e]);
+                    }
+                }
+                if (!on) continue;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int d = 32 * c + 8 * k;
+                    if (d >= D) break;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x0 = o[8 * k + 2 * e] * fo, x1 = o[8 * k + 2 * e + 1] * fo;
+                        w[e] = a.bf16 ? pack2<GRAFT_BF16>(x0, x1) : pack2<GRAFT_F16>(x0, x1);
+                    }
+                    *reinterpret_cast<uint4*>(y + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (a.lse && on)
+                a.lse[(size_t)(cw.s.c0 + tok) * a.q_heads + hq] = l != 0.f ? (ref + lg2(l)) * kLn2 : -INFINITY;
+        }
+    } else if (warp < C::SOFT + 4) {
+        // ======================================================== converters
+        constexpr int SEG = KT * DB / 128;   // segments (a key's 64 dims) of a thread, K and V each
+        const int ct = tid - 32 * C::SOFT;
+        Walk w = cw;
+        w.hi = 0;
+        int u = 0, blk[SEG];
+        bool more = true;
+        auto lookup = [&]() {   // the next unit, and the numbers of its blocks
+            if (more && ++u >= w.hi) {
+                more = next_piece(w);
+                u = w.lo;
+            }
+            if (!more) return;
+#pragma unroll
+            for (int k = 0; k < SEG; ++k) {
+                const int key = u * KT + (ct + 128 * k) % KT;
+                blk[k] = key < w.s.start + w.s.n
+                             ? a.table[(size_t)w.b * a.table_stride + (key >> a.bt_log2)] : 0;
+            }
+        };
+        uint4 kc[SEG][4], vc[SEG][4];
+        float ks = 0.f, vs = 1.f;
+        auto fetch = [&]() {    // its codes, and the scales of every 16 keys
+#pragma unroll
+            for (int k = 0; k < SEG; ++k) {
+                const int key = u * KT + (ct + 128 * k) % KT, db = (ct + 128 * k) / KT;
+                const bool in = key < w.s.start + w.s.n;
+                if (in && (uint32_t)blk[k] >= a.n_blocks) {
+                    atomicOr(err, (unsigned)GRAFT_KV_EBLOCK);
+                    blk[k] = 0;
+                }
+                const size_t bh = (size_t)blk[k] * H + w.h;
+                const size_t off = ((bh << a.bt_log2) + (key & ((1 << a.bt_log2) - 1))) * D + 64 * db;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const bool ok = in && 64 * db + 16 * c < D;
+                    kc[k][c] = ok ? ld_ro(a.k + off + 16 * c) : make_uint4(0, 0, 0, 0);
+                    vc[k][c] = ok ? ld_ro(a.v + off + 16 * c) : make_uint4(0, 0, 0, 0);
+                }
+                if (k == 0) {
+                    ks = in ? a.k_scale[bh] : 0.f;
+                    vs = in ? fmaxf(a.v_scale[bh], kKVScaleFloor) : 1.f;
+                }
+            }
+        };
+        auto store = [&](uint8_t* to, const uint4 (&x)[SEG][4]) {
+#pragma unroll
+            for (int k = 0; k < SEG; ++k) {
+                const int row = (ct + 128 * k) % KT, db = (ct + 128 * k) / KT;
+                uint8_t* line = to + (db * KT + row) * 128;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[8];
+                    codes_h2<FMT>(x[k][c].x, o[0], o[1]);
+                    codes_h2<FMT>(x[k][c].y, o[2], o[3]);
+                    codes_h2<FMT>(x[k][c].z, o[4], o[5]);
+                    codes_h2<FMT>(x[k][c].w, o[6], o[7]);
+                    *reinterpret_cast<uint4*>(line + (((2 * c) ^ (row & 7)) << 4)) =
+                        make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(line + (((2 * c + 1) ^ (row & 7)) << 4)) =
+                        make_uint4(o[4], o[5], o[6], o[7]);
+                }
+            }
+        };
+        lookup();
+        if (more) fetch();
+        bool have = more;
+        lookup();
+        for (int it = 0; have; ++it) {
+            const int st = it % ST, round = it / ST;
+            if (round && !wait(&kfree[st], round - 1)) break;
+            store(sk + st * C::KV_BYTES, kc);
+            if (ct < KT && ct % 16 == 0) {
+                const float lv = lg2(vs);
+                scales[it % SC][ct / 16] = make_float4(ks, lv, ex2(-lv), 0.f);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&kfull[st])), mbar_arrive(smem_u32(&scfull[it % SC]));
+            if (round && !wait(&vfree[st], round - 1)) break;
+            store(sv + st * C::KV_BYTES, vc);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&vfull[st]));
+            have = more;
+            if (more) fetch();
+            lookup();
+        }
+    } else if (lane == 0) {
+        // =============================================================== MMA
+        constexpr uint32_t iqk = tc5_idesc(KT, false), ipv = tc5_idesc(DP, true);
+        const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk), v0 = smem_u32(sv);
+        auto scores = [&](int tile, int st) {   // S = q K^T
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+                tc5_mma_ss(tmem + tile * 128,
+                           tc5_desc(q0 + (tile * DB + s / 4) * 128 * 128 + (s & 3) * 32, 16, 1024),
+                           tc5_desc(k0 + st * C::KV_BYTES + (s / 4) * KT * 128 + (s & 3) * 32, 16, 1024),
+                           iqk, s > 0);
+            tc5_commit(smem_u32(&sfull[tile]));
+        };
+        int it = 0, pc = 0;
+        bool live = true;
+        while (live && next_piece(cw)) {
+            const int n = cw.hi - cw.lo;
+            for (int i = 0; i < RT && live; ++i) {
+                if (!(live = wait_lane(&qfull[i], pc))) break;
+                if (i == 0 && !(live = wait_lane(&kfull[it % ST], it / ST))) break;
+                tc5_fence_after();
+                scores(i, it % ST);
+            }
+            if (!live) break;
+            tc5_commit(smem_u32(&kfree[it % ST]));
+            for (int j = 0; j < n && live; ++j, ++it) {
+                const int st = it % ST, nx = (it + 1) % ST;
+                for (int i = 0; i < RT; ++i) {
+                    if (i == 0 && !(live = wait_lane(&vfull[st], it / ST))) break;
+                    if (!(live = wait_lane(&pfull[i], it))) break;
+                    tc5_fence_after();
+#pragma unroll
+                    for (int s = 0; s < KT / 16; ++s)   // O += P V
+                        tc5_mma_ts(tmem + C::O_COL + i * DP, tmem + i * 128 + 8 * s,
+                                   tc5_desc(v0 + st * C::KV_BYTES + s * 2048, KT * 128, 1024), ipv,
+                                   j > 0 || s > 0);
+                    if (j + 1 == n) tc5_commit(smem_u32(&ofull[i]));
+                    if (i == RT - 1) tc5_commit(smem_u32(&vfree[st]));
+                    if (j + 1 < n) {
+                        if (i == 0) {
+                            if (!(live = wait_lane(&kfull[nx], (it + 1) / ST))) break;
+                            tc5_fence_after();
+                        }
+                        scores(i, nx);
+                        if (i == RT - 1) tc5_commit(smem_u32(&kfree[nx]));
+                    }
+                }
+            }
+            ++pc;
+        }
+        tc5_commit(smem_u32(&done));   // arrives once every product has completed
+    }
+    __syncthreads();
+    if (warp == C::SOFT + 4) {
+        uint64_t t0 = 0;   // (bounded like the other waits, also after one of them gave up)
+        while (!mbar_try_wait(smem_u32(&done), 0)) {
+            const uint64_t now = global_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kAttnWaitNs) {
+                atomicOr(err, (unsigned)GRAFT_KV_EWAIT);
+                break;
+            }
+        }
+        __syncwarp();
+        tc5_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                     : "memory");
+    }
+}
+
+}  // namespace dev
+}  // namespace graft

@@ -41,6 +41,7 @@ constexpr float kPShift = 10.f, kPSlack = 4.f;
 constexpr uint64_t kAttnWaitNs = 2000000000ull;
 // Most CTAs of an attention grid: one counter and two partial slots each.
 constexpr int kAttnMaxGrid = 512;
+constexpr int kChunkMaxGrid = 192;   // of the kernel for many rows (two counters a CTA)
 
 __device__ __forceinline__ float ex2(float x) {
     float y;

@@ -3,8 +3,11 @@
 //   o = sum_j exp(scale q.k_j - lse) v_j,  lse = log(sum_j exp(scale q.k_j) [+ exp(sink)])
 //   over keys j with p - window < j <= p, p the token's position
 //
-// One CTA per (token, query head): its warps take every fourth key with a
-// running maximum and sum each, and are merged at the end.
+// Up to few_rows() query rows (tokens of a sequence x query heads of a key/value
+// head) go to the kernel of attn_few.cuh, whose registers hold all of them: one
+// pass over the keys at the rate of HBM.  More rows go to the kernel of
+// attn_chunk.cuh (tcgen05).
+#include "attn_chunk.cuh"
 #include "attn_few.cuh"
 
 #include <algorithm>
@@ -16,98 +19,6 @@ using namespace graft::dev;
 namespace {
 
 __device__ unsigned g_attn_err;
-
-template <int DT, int FMT>
-__global__ void __launch_bounds__(128) attn_simple_kernel(const __grid_constant__ AttnArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    __shared__ float sm[4], sl[4], so[4][256];
-    const int t = blockIdx.x, h = blockIdx.y, hk = h / a.group;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int b = 0;
-    for (uint32_t s0 = 1; s0 < a.n_seqs; s0 += blockDim.x) {
-        const uint32_t s = s0 + threadIdx.x;
-        b += __syncthreads_count(s < a.n_seqs && a.cu[s] <= t);
-    }
-    const int c0 = a.cu[b], n = a.cu[b + 1] - c0, start = a.start[b];
-    if (t < c0 || t >= c0 + n) return;
-    if (n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens || start < 0 || (uint64_t)((int64_t)start + n) > a.max_len) {
-        if (threadIdx.x == 0) atomicOr(&g_attn_err, (unsigned)GRAFT_KV_EBOUNDS);
-        return;
-    }
-    const int p = start + t - c0, lo = a.window && p >= (int)a.window ? p - (int)a.window + 1 : 0;
-    const int words = a.dim / 4;       // 4-byte words of a row; lane l has words l, l + 32
-    float q[2][4], o[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int w = lane + 32 * i;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[i][e] = o[i][e] = 0.f;
-        if (w < words) {
-            const uint2 x = *reinterpret_cast<const uint2*>((const uint16_t*)a.q + t * a.q_tok +
-                                                            h * a.q_head + 4 * w);
-            const float2 y = unpack2<DT>(x.x), z = unpack2<DT>(x.y);
-            q[i][0] = y.x, q[i][1] = y.y, q[i][2] = z.x, q[i][3] = z.y;
-        }
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int j = lo + warp; j <= p; j += 4) {
-        const int blk = a.table[(size_t)b * a.table_stride + j / a.bt];
-        if ((uint32_t)blk >= a.n_blocks) {
-            if (lane == 0) atomicOr(&g_attn_err, (unsigned)GRAFT_KV_EBLOCK);
-            continue;
-        }
-        const size_t bh = (size_t)blk * a.heads + hk, at = (bh * a.bt + j % a.bt) * a.dim;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 32 * i < words) {
-                float f[4];
-                kv_decode4<FMT>(*reinterpret_cast<const uint32_t*>(a.k + at + 4 * (lane + 32 * i)), f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s = fmaf(f[e], q[i][e], s);
-            }
-        s = warp_sum(s) * a.k_scale[bh] * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.f : exp2f((m - mn) * kLog2e);
-        const float w = s == -INFINITY ? 0.f : exp2f((s - mn) * kLog2e);   // (a NaN stays one)
-        m = mn;
-        l = l * c + w;
-        const float wv = w * a.v_scale[bh];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 32 * i < words) {
-                float f[4];
-                kv_decode4<FMT>(*reinterpret_cast<const uint32_t*>(a.v + at + 4 * (lane + 32 * i)), f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] = fmaf(wv, f[e], o[i][e] * c);
-            }
-    }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lane + 32 * i < words)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) so[warp][4 * (lane + 32 * i) + e] = o[i][e];
-    __syncthreads();
-    const float sink = a.sinks ? a.sinks[h] : -INFINITY;
-    float M = sink;
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w]);
-    float L = 0.f, f[4];
-    for (int w = 0; w < 4; ++w) {
-        f[w] = sl[w] == 0.f ? 0.f : exp2f((sm[w] - M) * kLog2e);
-        L += f[w] * sl[w];
-    }
-    if (sink != -INFINITY) L += exp2f((sink - M) * kLog2e);
-    for (int d = threadIdx.x; d < (int)a.dim; d += 128) {
-        float v = 0.f;
-        for (int w = 0; w < 4; ++w) v += f[w] * so[w][d];
-        v = L != 0.f ? v / L : 0.f;
-        uint16_t* y = (uint16_t*)a.out + t * a.o_tok + h * a.o_head + d;
-        *y = (uint16_t)pack2<DT>(v, 0.f);
-    }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[(size_t)t * a.q_heads + h] = L != 0.f ? M + logf(L) : -INFINITY;
-}
 
 // ---- few query rows
 template <int DP, int NT, int FMT, bool FULL>
@@ -145,8 +56,39 @@ int launch_few(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
                                 : launch_few<DP, NT, GRAFT_KV_E4M3, false>(a, st);
 }
 
+// ---- many query rows
+template <int DP, int FMT>
+int launch_chunk(AttnArgs a, cudaStream_t st) {
+    using C = Chunk<DP>;
+    DeviceInfo di;
+    int rc = current_device_info(&di);
+    if (rc) return rc;
+    const auto kern = attn_chunk_kernel<DP, FMT>;
+    if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
+    unsigned* err = nullptr;
+    GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
+    // a piece costs about as much besides its units as 3 units (queries in, output)
+    a.min_units = 4;
+    a.pad_units = 3;
+    const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
+                                   : a.max_len;
+    const uint64_t units = keys / C::KT + 2 + a.pad_units;
+    const uint64_t tokens = C::ROWS / a.group;
+    const uint64_t pairs = (a.tokens / tokens + a.n_seqs) * a.heads;
+    GRAFT_REQUIRE(pairs * units < (1ull << 31), "max_len %u of %u tokens is too long for one call",
+                  a.max_len, a.tokens);
+    const uint64_t want = std::max(pairs, pairs * units / a.min_units + 1);
+    const int grid = (int)std::min<uint64_t>(std::min(di.sm_count, kChunkMaxGrid), want);
+    return launch_pdl("attn_kv8", kern, dim3(grid), C::THREADS, C::SMEM, st, a, err);
+}
+template <int DP>
+int launch_chunk(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
+    return fmt == GRAFT_KV_INT8 ? launch_chunk<DP, GRAFT_KV_INT8>(a, st)
+                                : launch_chunk<DP, GRAFT_KV_E4M3>(a, st);
+}
+
 // Query rows that the few-row kernel takes for a head_dim (registers).
-int few_rows(uint32_t dim) { return dim <= 64 ? 32 : dim <= 128 ? 16 : 8; }
+uint32_t few_rows(uint32_t dim) { return dim <= 64 ? 32 : dim <= 128 ? 16 : 8; }
 
 int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const GraftAttnParams* P) {
     int rc;
@@ -154,7 +96,11 @@ int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const Graft
     GRAFT_REQUIRE(P, "params pointer is null");
     GRAFT_REQUIRE(P->q_heads >= 1 && P->q_heads <= 32767 && P->q_heads % cache->kv_heads == 0,
                   "q_heads %u must be a multiple of kv_heads %u", P->q_heads, cache->kv_heads);
+    GRAFT_REQUIRE(P->q_heads / cache->kv_heads <= (cache->head_dim <= 128 ? 256u : 128u),
+                  "%u query heads a key/value head are too many", P->q_heads / cache->kv_heads);
     GRAFT_REQUIRE(std::isfinite(P->scale), "scale must be finite");
+    GRAFT_REQUIRE(range->n_seqs == 0 || range->max_len <= (1u << 30), "max_len %u out of range",
+                  range->max_len);
     GRAFT_REQUIRE(P->window <= 0x7FFFFFFFu, "window %u out of range", P->window);
     return GRAFT_OK;
 }
@@ -169,9 +115,13 @@ extern "C" size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const Graf
                                            const GraftAttnParams* P) {
     if (check_attn(cache, range, P)) return 0;
     const uint32_t d = cache->head_dim;
-    const size_t slot = d <= 64 ? kFewPartial<64, 4> : d <= 128 ? kFewPartial<128, 2>
-                                                                : kFewPartial<256, 1>;
-    return kAttnMaxGrid * (4 + 2 * 4 * slot);
+    const bool few = (uint64_t)range->max_tokens * (P->q_heads / cache->kv_heads) <= few_rows(d);
+    const size_t floats =
+        few ? kAttnMaxGrid * (size_t)(d <= 64    ? kFewPartial<64, 4>
+                                      : d <= 128 ? kFewPartial<128, 2> : kFewPartial<256, 1>)
+            : kChunkMaxGrid * (size_t)(d <= 64    ? Chunk<64>::PARTIAL
+                                       : d <= 128 ? Chunk<128>::PARTIAL : Chunk<256>::PARTIAL);
+    return kAttnMaxGrid * 4 + 2 * 4 * floats;
 }
 
 extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t stream) {
@@ -215,7 +165,7 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
     a.partials = (float*)((char*)ws + kAttnMaxGrid * 4);
     const uint64_t rows = (uint64_t)range->max_tokens * a.group;
     if (range->max_tokens == 0) return GRAFT_OK;
-    if (rows <= (uint64_t)few_rows(a.dim)) {
+    if (rows <= few_rows(a.dim)) {
         if (a.dim <= 64)
             return rows <= 8    ? launch_few<64, 1>(a, cache->format, stream)
                    : rows <= 16 ? launch_few<64, 2>(a, cache->format, stream)
@@ -225,12 +175,7 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
                              : launch_few<128, 2>(a, cache->format, stream);
         return launch_few<256, 1>(a, cache->format, stream);
     }
-    void (*kern)(const AttnArgs);
-    if (q->dtype == GRAFT_F16)
-        kern = cache->format == GRAFT_KV_INT8 ? attn_simple_kernel<GRAFT_F16, GRAFT_KV_INT8>
-                                              : attn_simple_kernel<GRAFT_F16, GRAFT_KV_E4M3>;
-    else
-        kern = cache->format == GRAFT_KV_INT8 ? attn_simple_kernel<GRAFT_BF16, GRAFT_KV_INT8>
-                                              : attn_simple_kernel<GRAFT_BF16, GRAFT_KV_E4M3>;
-    return launch_pdl("attn_kv8", kern, dim3(q->tokens, P->q_heads), 128, 0, stream, a);
+    return a.dim <= 64    ? launch_chunk<64>(a, cache->format, stream)
+           : a.dim <= 128 ? launch_chunk<128>(a, cache->format, stream)
+                          : launch_chunk<256>(a, cache->format, stream);
 }
