@@ -38,7 +38,11 @@ struct Chunk {
     static constexpr int Q_BYTES = RT * DB * 128 * 128;
     static constexpr int KV_BYTES = DB * KT * 128;   // K or V of a unit
     static constexpr int SMEM = 1024 + Q_BYTES + 2 * ST * KV_BYTES;
-    static constexpr int O_COL = 256;                // TMEM: scores of tile i at i*128, O at 256 + i*DP
+    // TMEM columns: scores of tile i at i*128; its weights (two fp16 a column) over the
+    // scores, or where there is room beside them; its output.
+    static constexpr bool BESIDE = DP != 128;
+    static constexpr int P_COL = DP <= 64 ? 256 : DP <= 128 ? 0 : 64, P_STEP = DP <= 64 ? 64 : 128;
+    static constexpr int O_COL = DP <= 64 ? 384 : 256;
     static constexpr int SC = 4;                     // slots of a unit's scales
     // floats of a partial result: O column by column, maximum and sum of each row
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
@@ -56,31 +60,42 @@ __device__ __forceinline__ void tc5_commit(uint32_t bar) {
                      bar)
                  : "memory");
 }
-__device__ __forceinline__ void tc5_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+// D (+)= A B: A from shared memory or from tensor memory, B from shared memory.
+// Descriptors of 128-byte swizzled rows as two words: low, start address >> 4 and
+// leading byte offset >> 4; high, the constant part (stride byte offset 1024 >> 4,
+// version 1, SWIZZLE_128B).  K-major: groups of 8 rows are 1024 bytes apart.
+// MN-major: groups of 8 along K are 1024 bytes, blocks of 64 along MN `lead` apart.
+constexpr uint32_t kTc5High = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tc5_low(uint32_t addr, uint32_t lead) {
+    return (addr >> 4) | ((lead >> 4) << 16);
+}
+__device__ __forceinline__ void tc5_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kTc5High)
         : "memory");
 }
-__device__ __forceinline__ void tc5_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void tc5_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                            uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kTc5High)
         : "memory");
 }
-// Shared-memory descriptor of 128-byte swizzled rows: start, leading and stride
-// byte offsets (>> 4), version 1, layout SWIZZLE_128B.  K-major: 8-row groups
-// `stride` apart.  MN-major: groups of 8 along K `stride` apart, blocks of 64
-// along MN `lead` apart.
-__device__ __forceinline__ uint64_t tc5_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
-           ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
 }
 // kind::f16 instruction descriptor: f32 sums, fp16 operands, M = 128, N; bit 16: B is MN-major.
 __device__ __forceinline__ constexpr uint32_t tc5_idesc(int n, bool mn_major) {
@@ -127,42 +142,28 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// sum of floor((a i + b) / m) over i < n, for a, b >= 0 (the Euclid-like recursion)
-__device__ __forceinline__ int floor_sum(int n, int m, int a, int b) {
-    long long s = 0, nn = n, mm = m, aa = a, bb = b;
-    while (nn > 0) {
-        s += (nn - 1) * nn / 2 * (aa / mm) + nn * (bb / mm);
-        aa %= mm, bb %= mm;
-        const long long y = aa * nn + bb;
-        if (y < mm) break;
-        nn = y / mm, bb = y % mm;
-        const long long t = mm;
-        mm = aa, aa = t;
-    }
-    return (int)s;
-}
-
 template <int DP, int FMT>
 __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     attn_chunk_kernel(const __grid_constant__ AttnArgs a, unsigned* err) {
     using C = Chunk<DP>;
     constexpr int RT = C::RT, KT = C::KT, ST = C::ST, SC = C::SC, DB = C::DB, ROWS = C::ROWS;
     struct Walk {
-        int at, prefix;   // next unit; units (of all heads) before the row tile
+        long long at, prefix;   // next key; keys (with the pads, of all heads) before the row tile
+        long long p0;           // first key of the pair
         Seq s;
-        int b, rt, tiles; // sequence, row tile, row tiles of the sequence
-        int nu, u0;       // units of the row tile a head with the pad, its first unit
-        int h, lo, hi;    // the piece: head, units [lo, hi)
-        int p0;           // first unit of the pair
+        int b, rt, tiles;       // sequence, row tile, row tiles of the sequence
+        int nk, k0, k1;         // keys of the row tile a head with the pad; first key, last + 1
+        int h, lo, hi;          // the piece: head, units [lo, hi)
     };
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Walk sh_edge[2];
     __shared__ uint64_t kfull[ST], kfree[ST], vfull[ST], vfree[ST], scfull[SC], sfull[RT], pfull[RT],
-        ofull[RT], qfull[RT], done;
+        pdone[RT], qfull[RT], done;
     __shared__ float4 scales[SC][KT / 16];   // k_scale, log2(v_scale), 1 / v_scale
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;            // a wait gave up: every role stops
-    __shared__ int sh_scan[C::THREADS / 32], sh_last[RT];
+    __shared__ long long sh_scan[C::THREADS / 32];
+    __shared__ int sh_last[RT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = a.dim, H = a.heads, G = a.group, TT = ROWS / G;   // tokens of a row tile
     uint8_t* base = smem + ((1024 - (smem_u32(smem) & 1023)) & 1023);
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         }
         for (int i = 0; i < SC; ++i) mbar_init(smem_u32(&scfull[i]), 4);
         for (int i = 0; i < RT; ++i) {
-            mbar_init(smem_u32(&sfull[i]), 1), mbar_init(smem_u32(&ofull[i]), 1);
+            mbar_init(smem_u32(&sfull[i]), 1), mbar_init(smem_u32(&pdone[i]), 1);
             mbar_init(smem_u32(&pfull[i]), 4), mbar_init(smem_u32(&qfull[i]), 4);   // softmax warps
         }
         mbar_init(smem_u32(&done), 1);
@@ -184,91 +185,100 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- units of a row tile and of the row tiles before it
+    // ---- keys of a row tile and of the row tiles before it
     auto open_tile = [&](Walk& w) {
-        const int i0 = w.rt * TT, i1 = min(w.s.n - 1, i0 + TT - 1);
-        w.u0 = first_key(a, w.s.start + i0) / KT;
-        w.nu = (w.s.start + i1) / KT + 1 - w.u0 + a.pad_units;
+        const int i0 = w.rt * TT, i1 = min(w.s.n, i0 + TT);
+        w.k0 = first_key(a, w.s.start + i0), w.k1 = w.s.start + i1;
+        w.nk = w.k1 - w.k0 + a.pad_units;
     };
     auto open_seq = [&](Walk& w) {
         w.s = load_seq(a, w.b, err);
         w.tiles = (w.s.n + TT - 1) / TT;
     };
-    auto units_before = [&](const Walk& w, int rt) {   // rt <= tiles
-        int full = min(rt, w.s.n / TT);                // (the last tile may have fewer tokens)
-        int u = floor_sum(full, KT, TT, w.s.start + TT - 1) + rt * (1 + a.pad_units);
-        if (full < rt) u += (w.s.start + w.s.n - 1) / KT;
-        if (a.window) {   // first units: floor((start - window + 1 + TT i) / KT) where that is positive
+    auto keys_before = [&](const Walk& w, int rt) {   // rt <= tiles
+        const long long n = rt;
+        long long k = n * (w.s.start + a.pad_units) + n * (n + 1) / 2 * TT;
+        if (rt == w.tiles) k -= n * TT - w.s.n;   // (the last tile may have fewer tokens)
+        if (a.window) {   // first keys: start - window + 1 + TT i where that is positive
             const int c = w.s.start - (int)a.window + 1;
             const int skip = c >= 0 ? 0 : min(rt, (-c + TT - 1) / TT);
-            u -= floor_sum(rt - skip, KT, TT, c + skip * TT);
+            const long long r = rt - skip;
+            k -= r * (c + (long long)skip * TT) + (r - 1) * r / 2 * TT;
         }
-        return u;
+        return k;
     };
-    Split sp;
+    Split<long long> sp;
     Walk cw;
-    int fe;
+    long long fe;
     {
-        int U = 0, pairs = 0, prefix = 0, base_u = 0;
-        auto scan = [&](int v, int& before) {   // over the CTA's threads; returns the total
-            int x = v;
+        long long U = 0, prefix = 0, base = 0;
+        int pairs = 0;
+        auto scan = [&](long long v, long long& before) {   // over the CTA's threads; the total
+            long long x = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(~0u, x, o);
+                const long long y = __shfl_up_sync(~0u, x, o);
                 if (lane >= o) x += y;
             }
             __syncthreads();
             if (lane == 31) sh_scan[warp] = x;
             __syncthreads();
             before = x - v;
-            int total = 0;
+            long long total = 0;
             for (int w = 0; w < C::THREADS / 32; ++w) {
-                const int y = sh_scan[w];
+                const long long y = sh_scan[w];
                 if (w < warp) before += y;
                 total += y;
             }
             return total;
         };
+        long long mine = 0;
         for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += C::THREADS) {
             cw.b = b0 + tid, cw.tiles = 0;
             if (cw.b < (int)a.n_seqs) open_seq(cw);
-            int skip;
-            pairs += scan(cw.tiles, skip);
-            U += scan(cw.tiles ? units_before(cw, cw.tiles) : 0, prefix);
+            mine = cw.tiles ? keys_before(cw, cw.tiles) : 0;
+            U += scan(mine, prefix);
+            pairs += __reduce_add_sync(~0u, cw.tiles);   // (this warp's; summed below)
         }
-        U *= H, pairs *= H;
         if (U == 0) return;
-        const int grid = min((int)gridDim.x, max(pairs, (U - pairs * a.pad_units) / a.min_units));
+        {
+            long long skip;
+            pairs = (int)scan(lane == 0 ? pairs : 0, skip) * H;
+        }
+        U *= H;
+        const int grid = (int)min((long long)gridDim.x,
+                                  max((long long)pairs, (U - (long long)pairs * a.pad_units) /
+                                                            (a.min_units * KT)));
         if ((int)blockIdx.x >= grid) return;
-        sp.set(U, grid, a.pad_units, max(1, a.min_units / 2));
-        const int x0 = sp.bound(blockIdx.x), x1 = sp.bound(blockIdx.x + 1);
+        sp.set(U, grid, a.pad_units, a.min_units / 2 * KT);
+        const long long x0 = sp.bound(blockIdx.x), x1 = sp.bound(blockIdx.x + 1);
         for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += C::THREADS) {   // the bounds' sequences
-            int mine = 0;
-            if (a.n_seqs > C::THREADS) {
+            if (a.n_seqs > C::THREADS) {   // (else all is still at hand)
                 cw.b = b0 + tid, cw.tiles = 0;
                 if (cw.b < (int)a.n_seqs) open_seq(cw);
+                mine = cw.tiles ? keys_before(cw, cw.tiles) : 0;
+                const long long total = scan(mine, prefix);
+                prefix += base;
+                base += total;
             }
-            if (cw.tiles) mine = units_before(cw, cw.tiles);
-            const int total = scan(mine, prefix);
-            cw.prefix = (base_u + prefix) * H;
-            const int e = cw.prefix + mine * H;
+            cw.prefix = prefix * H;
+            const long long e = cw.prefix + mine * H;
             if (cw.prefix <= x0 && x0 < e) sh_edge[0] = cw;
             if (cw.prefix <= x1 && x1 < e) sh_edge[1] = cw;
-            base_u += total;
         }
         __syncthreads();
         // their row tiles: the CTA's threads test every step-th row tile, then the ones between
-        auto find_tile = [&](int k, int x) {
+        auto find_tile = [&](int k, long long x) {
             Walk w = sh_edge[k];
-            const int seq_at = w.prefix;
+            const long long seq_at = w.prefix;
             int lo = 0, n = w.tiles;   // the row tile is one of [lo, lo + n)
             while (n > 0) {
                 const int step = (n + C::THREADS - 1) / C::THREADS, rt = lo + tid * step;
                 __syncthreads();
-                if (tid * step < n && rt < w.tiles) {
-                    const int end = min(min(rt + step, lo + n), w.tiles);
-                    const int p = seq_at + units_before(w, rt) * H;
-                    if (p <= x && x < seq_at + units_before(w, end) * H) {
+                if (tid * step < n) {
+                    const int end = min(rt + step, lo + n);
+                    const long long p = seq_at + keys_before(w, rt) * H;
+                    if (p <= x && x < seq_at + keys_before(w, end) * H) {
                         w.rt = rt;
                         w.prefix = p;
                         sh_edge[k] = w;
@@ -284,9 +294,9 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             open_tile(w);
             return w;
         };
-        auto edge = [&](const Walk& w, int x) {
-            const int p0 = w.prefix + (x - w.prefix) / w.nu * w.nu;
-            return sp.snapped(x, p0, p0 + w.nu);
+        auto edge = [&](const Walk& w, long long x) {
+            const long long p0 = w.prefix + (int)(x - w.prefix) / w.nk * w.nk;
+            return sp.snapped(x, p0, p0 + w.nk);
         };
         fe = U;
         if (x1 < U) fe = edge(find_tile(1, x1), x1);
@@ -296,8 +306,8 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     }
     auto next_piece = [&](Walk& w) {   // false: no more
         if (w.at >= fe) return false;
-        while (w.at >= w.prefix + w.nu * H) {
-            w.prefix += w.nu * H;
+        while (w.at >= w.prefix + (long long)w.nk * H) {
+            w.prefix += (long long)w.nk * H;
             if (++w.rt >= w.tiles) {
                 w.rt = 0;
                 do {
@@ -307,12 +317,12 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             }
             open_tile(w);
         }
-        w.h = (w.at - w.prefix) / w.nu;
-        w.p0 = w.prefix + w.h * w.nu;
-        const int e = min(fe, w.p0 + w.nu);
-        w.lo = w.u0 + max(0, w.at - w.p0 - a.pad_units);
-        w.hi = w.u0 + e - w.p0 - a.pad_units;
-        w.at = e;
+        w.h = (int)(w.at - w.prefix) / w.nk;
+        w.p0 = w.prefix + (long long)w.h * w.nk;
+        const int from = (int)(w.at - w.p0), to = (int)(min(fe, w.p0 + w.nk) - w.p0);
+        w.lo = (w.k0 + max(0, from - a.pad_units)) / KT;
+        w.hi = to == w.nk ? (w.k1 - 1) / KT + 1 : (w.k0 + to - a.pad_units) / KT;
+        w.at = w.p0 + to;
         return true;
     };
     // false: this or another wait gave up
@@ -349,8 +359,9 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         // =========================================================== softmax
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;   // row of the tile = TMEM lane
         const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t ts = tlane + tile * 128, to = tlane + C::O_COL + tile * DP;
-        int it = 0, pc = 0;   // units and pieces done
+        const uint32_t ts = tlane + tile * 128, tp = tlane + C::P_COL + tile * C::P_STEP;
+        const uint32_t to = tlane + C::O_COL + tile * DP;
+        int it = 0;   // units done
         bool live = true;
         while (live && next_piece(cw)) {
             const int r = tile * 128 + row, tok = cw.rt * TT + r / G, hq = cw.h * G + r % G;
@@ -399,7 +410,8 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&qfull[tile]));
             }
-            const int p = on ? cw.s.start + tok : -1, lo = on ? first_key(a, p) : 0;
+            // (rows without a token need no mask: nothing of theirs is kept)
+            const int p = on ? cw.s.start + tok : 1 << 30, lo = on ? first_key(a, p) : 0;
             float m = kNoMax, l = 0.f;
             for (int u = cw.lo; u < cw.hi; ++u, ++it) {
                 if (!(live = wait(&sfull[tile], it)) || !(live = wait(&scfull[it % SC], it / SC))) break;
@@ -433,11 +445,14 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 };
                 if (edge_unit) take_max(std::true_type{});
                 else take_max(std::false_type{});
+                // (the product before has read its weights and written O)
+                if (u > cw.lo && !(live = wait(&pdone[tile], it - 1))) break;
+                tc5_fence_after();
                 if (__any_sync(~0u, mx > m + kPSlack)) {
                     const float nm = fmaxf(m, mx), f = ex2(m - nm);
                     l *= f;
                     m = nm;
-                    if (u > cw.lo) {   // (the scores' arrival says that the product before is done)
+                    if (u > cw.lo) {
 #pragma unroll
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t v[32];
@@ -449,7 +464,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                         }
                     }
                 }
-                // ---- the weights, over the scores that have been read
+                // ---- the weights
                 auto weigh = [&](auto masked) {
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
@@ -477,7 +492,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                             }
                             l = fmaf(sum[0] + sum[1], f.z, l);
                         }
-                        tmem_st16(ts + 16 * c, w);
+                        tmem_st16(tp + 16 * c, w);
                     }
                 };
                 if (edge_unit) weigh(std::true_type{});
@@ -487,16 +502,15 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&pfull[tile]));
             }
-            if (!live || !(live = wait(&ofull[tile], pc))) break;
-            ++pc;
+            if (!live || !(live = wait(&pdone[tile], it - 1))) break;
             tc5_fence_after();
             // ---- output: the row itself, or its part of a cut pair
             int ca, cb;
-            sp.cuts(cw.p0, cw.p0 + cw.nu, ca, cb);
+            sp.cuts(cw.p0, cw.p0 + cw.nk, ca, cb);
             const bool cut = cb >= ca;
             const int first = ca - 1, pieces = cb - ca + 2;
             if (cut) {
-                float* part = a.partials + ((size_t)blockIdx.x * 2 + (cw.lo == cw.u0)) * C::PARTIAL + r;
+                float* part = a.partials + ((size_t)blockIdx.x * 2 + (cw.lo == cw.k0 / KT)) * C::PARTIAL + r;
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     uint32_t v[32];
@@ -665,57 +679,63 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             if (more) fetch();
             lookup();
         }
-    } else if (lane == 0) {
+    } else {
         // =============================================================== MMA
+        // (the whole warp walks and waits; one lane issues)
         constexpr uint32_t iqk = tc5_idesc(KT, false), ipv = tc5_idesc(DP, true);
-        const uint32_t q0 = smem_u32(sq), k0 = smem_u32(sk), v0 = smem_u32(sv);
+        const bool leader = elect_one();
+        const uint32_t q0 = tc5_low(smem_u32(sq), 16), k0 = tc5_low(smem_u32(sk), 16);
+        const uint32_t v0 = tc5_low(smem_u32(sv), KT * 128);
         auto scores = [&](int tile, int st) {   // S = q K^T
+            if (leader) {
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-                tc5_mma_ss(tmem + tile * 128,
-                           tc5_desc(q0 + (tile * DB + s / 4) * 128 * 128 + (s & 3) * 32, 16, 1024),
-                           tc5_desc(k0 + st * C::KV_BYTES + (s / 4) * KT * 128 + (s & 3) * 32, 16, 1024),
-                           iqk, s > 0);
-            tc5_commit(smem_u32(&sfull[tile]));
+                for (int s = 0; s < DP / 16; ++s)
+                    tc5_mma_ss(tmem + tile * 128,
+                               q0 + ((tile * DB + s / 4) * 128 * 128 + (s & 3) * 32) / 16,
+                               k0 + (st * C::KV_BYTES + (s / 4) * KT * 128 + (s & 3) * 32) / 16, iqk, s > 0);
+                tc5_commit(smem_u32(&sfull[tile]));
+                if (tile == RT - 1) tc5_commit(smem_u32(&kfree[st]));
+            }
+        };
+        auto product = [&](int tile, int st, bool accumulate) {   // O += P V
+            if (leader) {
+#pragma unroll
+                for (int s = 0; s < KT / 16; ++s)
+                    tc5_mma_ts(tmem + C::O_COL + tile * DP, tmem + C::P_COL + tile * C::P_STEP + 8 * s,
+                               v0 + (st * C::KV_BYTES + s * 2048) / 16, ipv, accumulate || s > 0);
+                tc5_commit(smem_u32(&pdone[tile]));
+                if (tile == RT - 1) tc5_commit(smem_u32(&vfree[st]));
+            }
         };
         int it = 0, pc = 0;
         bool live = true;
         while (live && next_piece(cw)) {
             const int n = cw.hi - cw.lo;
-            for (int i = 0; i < RT && live; ++i) {
-                if (!(live = wait_lane(&qfull[i], pc))) break;
-                if (i == 0 && !(live = wait_lane(&kfull[it % ST], it / ST))) break;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                live = live && wait(&qfull[i], pc) && (i || wait(&kfull[it % ST], it / ST));
+                if (!live) break;
                 tc5_fence_after();
                 scores(i, it % ST);
             }
-            if (!live) break;
-            tc5_commit(smem_u32(&kfree[it % ST]));
             for (int j = 0; j < n && live; ++j, ++it) {
                 const int st = it % ST, nx = (it + 1) % ST;
-                for (int i = 0; i < RT; ++i) {
-                    if (i == 0 && !(live = wait_lane(&vfull[st], it / ST))) break;
-                    if (!(live = wait_lane(&pfull[i], it))) break;
-                    tc5_fence_after();
 #pragma unroll
-                    for (int s = 0; s < KT / 16; ++s)   // O += P V
-                        tc5_mma_ts(tmem + C::O_COL + i * DP, tmem + i * 128 + 8 * s,
-                                   tc5_desc(v0 + st * C::KV_BYTES + s * 2048, KT * 128, 1024), ipv,
-                                   j > 0 || s > 0);
-                    if (j + 1 == n) tc5_commit(smem_u32(&ofull[i]));
-                    if (i == RT - 1) tc5_commit(smem_u32(&vfree[st]));
-                    if (j + 1 < n) {
-                        if (i == 0) {
-                            if (!(live = wait_lane(&kfull[nx], (it + 1) / ST))) break;
-                            tc5_fence_after();
-                        }
-                        scores(i, nx);
-                        if (i == RT - 1) tc5_commit(smem_u32(&kfree[nx]));
-                    }
+                for (int i = 0; i < RT; ++i) {
+                    live = live && wait(&pfull[i], it) && (i || wait(&vfull[st], it / ST)) &&
+                           (i || j + 1 == n || wait(&kfull[nx], (it + 1) / ST));
+                    if (!live) break;
+                    tc5_fence_after();
+                    // where the weights lie beside the scores the next scores go first: they
+                    // are waited for, the product runs under their softmax
+                    if (C::BESIDE && j + 1 < n) scores(i, nx);
+                    product(i, st, j > 0);
+                    if (!C::BESIDE && j + 1 < n) scores(i, nx);
                 }
             }
             ++pc;
         }
-        tc5_commit(smem_u32(&done));   // arrives once every product has completed
+        if (leader) tc5_commit(smem_u32(&done));   // arrives once every product has completed
     }
     __syncthreads();
     if (warp == C::SOFT + 4) {

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         w.u0 = first_key(a, w.s.start) / UK;
         w.nu = w.s.n ? (w.s.start + w.s.n + UK - 1) / UK - w.u0 + a.pad_units : 0;
     };
-    Split sp;
+    Split<int> sp;
     Walk cw;
     int fe;   // this CTA's units: [cw.at, fe)
     {

@@ -67,16 +67,16 @@ int launch_chunk(AttnArgs a, cudaStream_t st) {
     if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
     unsigned* err = nullptr;
     GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
-    // a piece costs about as much besides its units as 3 units (queries in, output)
+    // a piece costs about as much besides its units as 3 units (queries in, output);
+    // the pad is counted in keys
     a.min_units = 4;
-    a.pad_units = 3;
+    a.pad_units = 3 * C::KT;
     const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
                                    : a.max_len;
-    const uint64_t units = keys / C::KT + 2 + a.pad_units;
-    const uint64_t tokens = C::ROWS / a.group;
-    const uint64_t pairs = (a.tokens / tokens + a.n_seqs) * a.heads;
-    GRAFT_REQUIRE(pairs * units < (1ull << 31), "max_len %u of %u tokens is too long for one call",
-                  a.max_len, a.tokens);
+    const uint64_t units = keys / C::KT + 2;
+    const uint64_t pairs = ((uint64_t)a.tokens / (C::ROWS / a.group) + a.n_seqs) * a.heads;
+    GRAFT_REQUIRE(pairs < (1ull << 31) && (keys + a.pad_units) * a.heads < (1ull << 31),
+                  "%u tokens, max_len %u are too many for one call", a.tokens, a.max_len);
     const uint64_t want = std::max(pairs, pairs * units / a.min_units + 1);
     const int grid = (int)std::min<uint64_t>(std::min(di.sm_count, kChunkMaxGrid), want);
     return launch_pdl("attn_kv8", kern, dim3(grid), C::THREADS, C::SMEM, st, a, err);
