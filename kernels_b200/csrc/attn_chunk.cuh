@@ -43,6 +43,9 @@ struct Chunk {
     static constexpr bool BESIDE = DP != 128;
     static constexpr int P_COL = DP <= 64 ? 256 : DP <= 128 ? 0 : 64, P_STEP = DP <= 64 ? 64 : 128;
     static constexpr int O_COL = DP <= 64 ? 384 : 256;
+    // weights are 2^(t - m + SHIFT): where a unit is weighed before its maximum is known
+    // there is room for 2^11 more in fp16, and full precision down to 2^-18
+    static constexpr float SHIFT = BESIDE ? 4.f : kPShift;
     static constexpr int SC = 4;                     // slots of a unit's scales
     // floats of a partial result: O column by column, maximum and sum of each row
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
@@ -126,14 +129,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16};" ::"r"(addr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-        "r"(v[15])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15])
+        : "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
+                     addr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -325,10 +336,12 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         w.at = w.p0 + to;
         return true;
     };
-    // false: this or another wait gave up
+    // A wait for a barrier's phase; false: this or another wait gave up.  It spins on
+    // probes that do not suspend: a suspended one wakes up to half a microsecond late.
     auto wait_lane = [&](uint64_t* bar, uint32_t phase) {
         uint64_t t0 = 0;
-        while (!mbar_try_wait(smem_u32(bar), phase & 1)) {
+        for (uint32_t i = 1; !mbar_test(smem_u32(bar), phase & 1); ++i) {
+            if (i & 255) continue;
             if (dead) return false;
             const uint64_t now = global_ns();
             if (t0 == 0) t0 = now;
@@ -413,16 +426,38 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             // (rows without a token need no mask: nothing of theirs is kept)
             const int p = on ? cw.s.start + tok : 1 << 30, lo = on ? first_key(a, p) : 0;
             float m = kNoMax, l = 0.f;
+            int raise = 0;   // of the reference, before the next unit
             for (int u = cw.lo; u < cw.hi; ++u, ++it) {
                 if (!(live = wait(&sfull[tile], it)) || !(live = wait(&scfull[it % SC], it / SC))) break;
                 tc5_fence_after();
                 const float4* sc = scales[it % SC];
                 const int c_lo = lo - u * KT, c_hi = p - u * KT;   // columns that the row sees
                 const bool edge_unit = __any_sync(~0u, c_lo > 0 || c_hi < KT - 1);
-                // ---- the row's maximum
-                float mx = kNoMax;
-                auto take_max = [&](auto masked) {
+                // The product before has read its weights and written O (waited for where
+                // that first matters).
+                bool after = u == cw.lo;
+                auto wait_product = [&]() {
+                    if (after) return;
+                    after = true;
+                    live = wait(&pdone[tile], it - 1);
+                    tc5_fence_after();
+                };
+                auto rescale = [&](float f) {   // O
+                    wait_product();
+#pragma unroll 1
+                    for (int c = 0; c < DP / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * c, v);
+                        tmem_wait_ld();
 #pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                        tmem_st32(to + 32 * c, v);
+                    }
+                };
+                // ---- the row's maximum becomes the reference of the exponents
+                auto follow = [&](auto masked) {
+                    float mx = m;
+#pragma unroll 1
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t v[32];
                         tmem_ld32(ts + 32 * c, v);
@@ -442,61 +477,75 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                             mx = fmaxf(mx, x);
                         }
                     }
-                };
-                if (edge_unit) take_max(std::true_type{});
-                else take_max(std::false_type{});
-                // (the product before has read its weights and written O)
-                if (u > cw.lo && !(live = wait(&pdone[tile], it - 1))) break;
-                tc5_fence_after();
-                if (__any_sync(~0u, mx > m + kPSlack)) {
-                    const float nm = fmaxf(m, mx), f = ex2(m - nm);
+                    if (!__any_sync(~0u, mx > m + (C::BESIDE ? 0.f : kPSlack))) return;
+                    const float f = ex2(m - mx);
                     l *= f;
-                    m = nm;
-                    if (u > cw.lo) {
-#pragma unroll
-                        for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t v[32];
-                            tmem_ld32(to + 32 * c, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tmem_st32(to + 32 * c, v);
-                        }
-                    }
-                }
-                // ---- the weights
-                auto weigh = [&](auto masked) {
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t v[32], w[16];
-                        tmem_ld32(ts + 32 * c, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const float4 f = sc[2 * c + q];
-                            const float fa = f.x * cr, fb = f.y - (m - kPShift);
-                            float sum[2] = {0.f, 0.f};
-#pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                float y[2];
-#pragma unroll
-                                for (int k = 0; k < 2; ++k) {
-                                    y[k] = fmaf(__uint_as_float(v[16 * q + e + k]), fa, fb);
-                                    const int col = 32 * c + 16 * q + e + k;
-                                    if (decltype(masked)::value)
-                                        y[k] = col >= c_lo && col <= c_hi ? y[k] : -INFINITY;
-                                    y[k] = ex2(y[k]);
-                                    sum[k] += y[k];
-                                }
-                                w[8 * q + e / 2] = pack_h2(y[0], y[1]);
-                            }
-                            l = fmaf(sum[0] + sum[1], f.z, l);
-                        }
-                        tmem_st16(tp + 16 * c, w);
-                    }
+                    m = mx;
+                    if (u > cw.lo) rescale(f);
                 };
-                if (edge_unit) weigh(std::true_type{});
-                else weigh(std::false_type{});
+                // ---- the weights; the largest sum of 16 of them
+                float dl;
+                auto weigh = [&](auto masked) {
+                    float top = 0.f;
+                    dl = 0.f;
+                    uint32_t v[2][16];
+                    tmem_ld16(ts, v[0]);
+#pragma unroll
+                    for (int c = 0; c < KT / 16; ++c) {
+                        uint32_t w[8];
+                        tmem_wait_ld();
+                        if (c + 1 < KT / 16) tmem_ld16(ts + 16 * (c + 1), v[(c + 1) & 1]);
+                        const float4 f = sc[c];
+                        const float fa = f.x * cr, fb = f.y - (m - C::SHIFT);
+                        float sum[2] = {0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float y[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                y[k] = fmaf(__uint_as_float(v[c & 1][e + k]), fa, fb);
+                                const int col = 16 * c + e + k;
+                                if (decltype(masked)::value)
+                                    y[k] = col >= c_lo && col <= c_hi ? y[k] : -INFINITY;
+                                y[k] = ex2(y[k]);
+                                sum[k] += y[k];
+                            }
+                            w[e / 2] = pack_h2(y[0], y[1]);
+                        }
+                        sum[0] += sum[1];
+                        top = fmaxf(top, sum[0]);
+                        dl = fmaf(sum[0], f.z, dl);
+                        if (c == 0) wait_product();
+                        tmem_st8(tp + 8 * c, w);
+                    }
+                    return top;
+                };
+                // Where the weights lie beside the scores, a unit is weighed with the reference
+                // that the units before left, and weighed again in the rare case that a row
+                // reached fp16's limit (no weight reaches 2^15 unless a sum of 16 does).
+                if (!C::BESIDE || u == cw.lo) {
+                    if (edge_unit) follow(std::true_type{});
+                    else follow(std::false_type{});
+                } else if (__any_sync(~0u, raise > 0)) {
+                    // by a power of two: the rows' sums and O keep their bits
+                    const float f = ex2((float)-raise);
+                    l *= f;
+                    m += (float)raise;
+                    rescale(f);
+                }
+                float top;
+                while (true) {
+                    top = edge_unit ? weigh(std::true_type{}) : weigh(std::false_type{});
+                    if (!C::BESIDE || !__any_sync(~0u, top > 32768.f)) break;
+                    if (edge_unit) follow(std::true_type{});
+                    else follow(std::false_type{});
+                    if (__all_sync(~0u, !(top > 32768.f) || !(m < INFINITY))) break;
+                }
+                // the next unit's reference: up once the weights pass 2^(SHIFT + kPSlack)
+                constexpr float kRaise = 256.f;
+                raise = C::BESIDE && top > kRaise ? (int)(__float_as_uint(top) >> 23) - 127 - (int)C::SHIFT : 0;
+                if (!live) break;
+                l += dl;
                 tmem_wait_st();
                 tc5_fence_before();
                 __syncwarp();
@@ -543,7 +592,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 for (int k = 0; k < pieces; ++k)
                     l = fmaf(__ldcg(piece(k) + DP * ROWS + ROWS), ex2(__ldcg(piece(k) + DP * ROWS) - m), l);
             }
-            float ref = m - kPShift, fo = 1.f;
+            float ref = m - C::SHIFT, fo = 1.f;
             if (a.sinks) {
                 const float s = a.sinks[on ? hq : 0] * kLog2e;
                 if (s > ref) {
