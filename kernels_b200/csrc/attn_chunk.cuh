@@ -11,8 +11,11 @@
 //               fp16 in shared memory, 128-byte swizzled rows of 64 dims: the
 //               K-major B operand of q K^T and, unchanged in layout, the
 //               MN-major B operand of P V;
-//   MMA         (one lane)  per row tile: P V of unit j, then q K^T of unit j + 1,
-//               so that one tile's products run under the other's softmax.
+//   MMA         (one lane)  per row tile and half unit of 64 keys: q K^T of half
+//               j + 2 and P V of half j.
+// Scores and weights are double-buffered by the half's parity, so a tile's softmax
+// finds the next half's scores ready when it ends one: its chain is not
+// lengthened by the products.
 // The scales enter the exponents as in the few-row kernel (attn_few.cuh).  The
 // reference of the exponents follows the row's maximum only when it is passed by
 // more than kPSlack, so that O is seldom rescaled in tensor memory.
@@ -29,8 +32,9 @@ namespace dev {
 template <int DP>
 struct Chunk {
     static constexpr int RT = DP <= 128 ? 2 : 1;     // row tiles
-    static constexpr int KT = DP <= 128 ? 128 : 64;  // keys of a unit
-    static constexpr int ST = DP <= 64 ? 3 : 2;      // stages of K and V
+    static constexpr int KT = DP <= 128 ? 128 : 64;  // keys of a unit (one stage of K and V)
+    static constexpr int HN = KT / 64;               // its halves of 64 keys (one product each)
+    static constexpr int ST = DP <= 64 ? 3 : 2;      // stages
     static constexpr int ROWS = 128 * RT;
     static constexpr int SOFT = 4 * RT;              // softmax warps
     static constexpr int THREADS = 32 * (SOFT + 4 + 1);
@@ -38,15 +42,18 @@ struct Chunk {
     static constexpr int Q_BYTES = RT * DB * 128 * 128;
     static constexpr int KV_BYTES = DB * KT * 128;   // K or V of a unit
     static constexpr int SMEM = 1024 + Q_BYTES + 2 * ST * KV_BYTES;
-    // TMEM columns: scores of tile i at i*128; its weights (two fp16 a column) over the
-    // scores, or where there is room beside them; its output.
+    // TMEM columns: scores of tile i, half of parity b at i*128 + b*64; its weights (two fp16 a
+    // column) over the scores, or where there is room beside them; its output.
     static constexpr bool BESIDE = DP != 128;
-    static constexpr int P_COL = DP <= 64 ? 256 : DP <= 128 ? 0 : 64, P_STEP = DP <= 64 ? 64 : 128;
+    static constexpr int P_COL = DP <= 64 ? 256 : DP <= 128 ? 0 : 128;
+    static constexpr int P_TILE = DP <= 64 ? 64 : 128, P_STEP = DP == 128 ? 64 : 32;
     static constexpr int O_COL = DP <= 64 ? 384 : 256;
-    // weights are 2^(t - m + SHIFT): where a unit is weighed before its maximum is known
-    // there is room for 2^11 more in fp16, and full precision down to 2^-18
-    static constexpr float SHIFT = BESIDE ? 4.f : kPShift;
-    static constexpr int SC = 4;                     // slots of a unit's scales
+    // Weights are 2^(t - m + SHIFT).  Where a half is weighed before its maximum is known,
+    // fp16 leaves room for scores up to 12 (in log2) above the reference, and keeps its 11
+    // bits down to 17 below it; the reference goes up only near that limit, because O's
+    // rescaling waits for the product before.
+    static constexpr float SHIFT = BESIDE ? 3.f : kPShift;
+    static constexpr int SC = 8;                     // slots of a unit's scales (up to ST + 2 in use)
     // floats of a partial result: O column by column, maximum and sum of each row
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
 };
@@ -92,6 +99,25 @@ __device__ __forceinline__ void tc5_mma_ts(uint32_t d, uint32_t a, uint32_t b, u
         "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kTc5High)
         : "memory");
 }
+// Pairs of fp32 numbers (sm_100's two-wide operations).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // One lane of a converged warp, always the same.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -129,23 +155,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-          "=r"(v[14]), "=r"(v[15])
-        : "r"(addr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
-                     addr),
-                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-                 "r"(v[7])
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -168,8 +177,8 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     };
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Walk sh_edge[2];
-    __shared__ uint64_t kfull[ST], kfree[ST], vfull[ST], vfree[ST], scfull[SC], sfull[RT], pfull[RT],
-        pdone[RT], qfull[RT], done;
+    __shared__ uint64_t kfull[ST], kfree[ST], vfull[ST], vfree[ST], scfull[SC], qfull[RT], done;
+    __shared__ uint64_t sfull[RT][2], pfull[RT][2], pdone[RT][2];   // by the half's parity
     __shared__ float4 scales[SC][KT / 16];   // k_scale, log2(v_scale), 1 / v_scale
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;            // a wait gave up: every role stops
@@ -186,8 +195,11 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         }
         for (int i = 0; i < SC; ++i) mbar_init(smem_u32(&scfull[i]), 4);
         for (int i = 0; i < RT; ++i) {
-            mbar_init(smem_u32(&sfull[i]), 1), mbar_init(smem_u32(&pdone[i]), 1);
-            mbar_init(smem_u32(&pfull[i]), 4), mbar_init(smem_u32(&qfull[i]), 4);   // softmax warps
+            mbar_init(smem_u32(&qfull[i]), 4);             // softmax warps
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(smem_u32(&pfull[i][b]), 4);
+                mbar_init(smem_u32(&sfull[i][b]), 1), mbar_init(smem_u32(&pdone[i][b]), 1);   // commits
+            }
         }
         mbar_init(smem_u32(&done), 1);
         dead = 0;
@@ -336,25 +348,29 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         w.at = w.p0 + to;
         return true;
     };
-    // A wait for a barrier's phase; false: this or another wait gave up.  It spins on
-    // probes that do not suspend: a suspended one wakes up to half a microsecond late.
-    auto wait_lane = [&](uint64_t* bar, uint32_t phase) {
-        uint64_t t0 = 0;
-        for (uint32_t i = 1; !mbar_test(smem_u32(bar), phase & 1); ++i) {
-            if (i & 255) continue;
-            if (dead) return false;
-            const uint64_t now = global_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > kAttnWaitNs) {
-                atomicOr(err, (unsigned)GRAFT_KV_EWAIT);
-                dead = 1;
-                return false;
-            }
-        }
+    // A wait for a barrier's phase.  When it gives up it sets an error bit and `dead`, after
+    // which no wait waits: every role runs through its (bounded) loops and the call ends with
+    // undefined outputs.  The MMA warp, whose lateness all others feel, spins on probes that
+    // do not suspend (a suspended one wakes up to half a microsecond late).
+    auto late = [&](uint64_t& t0) {
+        if (dead) return true;
+        const uint64_t now = global_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 <= kAttnWaitNs) return false;
+        atomicOr(err, (unsigned)GRAFT_KV_EWAIT);
+        dead = 1;
         return true;
     };
-    auto wait = [&](uint64_t* bar, uint32_t phase) {   // by a whole warp
-        return (bool)__all_sync(~0u, wait_lane(bar, phase));
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+        if (mbar_test(smem_u32(bar), phase & 1)) return;   // (the usual case)
+        uint64_t t0 = 0;
+        while (!mbar_try_wait(smem_u32(bar), phase & 1))
+            if (late(t0)) break;
+    };
+    auto spin = [&](uint64_t* bar, uint32_t phase) {
+        uint64_t t0 = 0;
+        for (uint32_t i = 1; !mbar_test(smem_u32(bar), phase & 1); ++i)
+            if ((i & 255) == 0 && late(t0)) break;
     };
     if (warp == C::SOFT + 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -370,13 +386,15 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
 
     if (warp < C::SOFT) {
         // =========================================================== softmax
+        // (registers move from the converters: 8 x 152 + 4 x 80, or 8 x 136 + 4 x 112, = 12 x 128)
+        if constexpr (DP <= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        else if constexpr (DP <= 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;   // row of the tile = TMEM lane
         const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t ts = tlane + tile * 128, tp = tlane + C::P_COL + tile * C::P_STEP;
+        const uint32_t ts0 = tlane + tile * 128, tp0 = tlane + C::P_COL + tile * C::P_TILE;
         const uint32_t to = tlane + C::O_COL + tile * DP;
-        int it = 0;   // units done
-        bool live = true;
-        while (live && next_piece(cw)) {
+        int it = 0, hc = 0;   // units and halves done
+        while (next_piece(cw)) {
             const int r = tile * 128 + row, tok = cw.rt * TT + r / G, hq = cw.h * G + r % G;
             const bool on = r < TT * G && tok < cw.s.n;
             // ---- the row's queries, as fp16 (the sign of the scale goes with them)
@@ -402,22 +420,29 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 }
                 const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
                 cr = fabsf(a.scale) * kLog2e * up;
-#pragma unroll 2
-                for (int c = 0; c < DP / 8; ++c) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (on && 8 * c < D) x = *reinterpret_cast<const uint4*>(src + 8 * c);
-                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (a.bf16) {
-                            const float2 p = unpack2<GRAFT_BF16>(w[e]);
-                            w[e] = pack_h2(p.x * down, p.y * down);
-                        }
-                        w[e] ^= flip;
+                for (int c0 = 0; c0 < DP / 8; c0 += 8) {   // eight loads in flight
+                    uint4 x[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        x[c] = make_uint4(0, 0, 0, 0);
+                        if (on && 8 * (c0 + c) < D) x[c] = *reinterpret_cast<const uint4*>(src + 8 * (c0 + c));
                     }
-                    *reinterpret_cast<uint4*>(sq + ((tile * DB + c / 8) * 128 + row) * 128 +
-                                              (((c & 7) ^ (row & 7)) << 4)) =
-                        make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (a.bf16) {
+                                const float2 p = unpack2<GRAFT_BF16>(w[e]);
+                                w[e] = pack_h2(p.x * down, p.y * down);
+                            }
+                            w[e] ^= flip;
+                        }
+                        *reinterpret_cast<uint4*>(sq + ((tile * DB + c0 / 8) * 128 + row) * 128 +
+                                                  ((c ^ (row & 7)) << 4)) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -428,22 +453,21 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             float m = kNoMax, l = 0.f;
             int raise = 0;   // of the reference, before the next unit
             for (int u = cw.lo; u < cw.hi; ++u, ++it) {
-                if (!(live = wait(&sfull[tile], it)) || !(live = wait(&scfull[it % SC], it / SC))) break;
-                tc5_fence_after();
-                const float4* sc = scales[it % SC];
+                const bool first_unit = u == cw.lo;
                 const int c_lo = lo - u * KT, c_hi = p - u * KT;   // columns that the row sees
                 const bool edge_unit = __any_sync(~0u, c_lo > 0 || c_hi < KT - 1);
-                // The product before has read its weights and written O (waited for where
-                // that first matters).
-                bool after = u == cw.lo;
-                auto wait_product = [&]() {
-                    if (after) return;
-                    after = true;
-                    live = wait(&pdone[tile], it - 1);
+                wait(&scfull[it % SC], it / SC);
+                float top = 0.f;
+#pragma unroll
+                for (int hh = 0; hh < C::HN; ++hh, ++hc) {   // its halves
+                const int b = C::HN == 1 ? hc & 1 : hh;
+                const uint32_t ts = ts0 + b * 64, tp = tp0 + b * C::P_STEP;
+                const float4* sc = scales[it % SC] + hh * 4;
+                wait(&sfull[tile][b], hc >> 1);
+                tc5_fence_after();
+                auto rescale = [&](float f) {   // O, once the half before has been added
+                    wait(&pdone[tile][b ^ 1], (hc - 1) >> 1);
                     tc5_fence_after();
-                };
-                auto rescale = [&](float f) {   // O
-                    wait_product();
 #pragma unroll 1
                     for (int c = 0; c < DP / 32; ++c) {
                         uint32_t v[32];
@@ -458,7 +482,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 auto follow = [&](auto masked) {
                     float mx = m;
 #pragma unroll 1
-                    for (int c = 0; c < KT / 32; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t v[32];
                         tmem_ld32(ts + 32 * c, v);
                         tmem_wait_ld();
@@ -469,7 +493,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 float y = __uint_as_float(v[16 * q + e]);
-                                const int col = 32 * c + 16 * q + e;
+                                const int col = 64 * hh + 32 * c + 16 * q + e;
                                 if (decltype(masked)::value) y = col >= c_lo && col <= c_hi ? y : -INFINITY;
                                 x = fmaxf(x, y);
                             }
@@ -481,77 +505,80 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                     const float f = ex2(m - mx);
                     l *= f;
                     m = mx;
-                    if (u > cw.lo) rescale(f);
+                    if (!first_unit || hh) rescale(f);
                 };
                 // ---- the weights; the largest sum of 16 of them
                 float dl;
                 auto weigh = [&](auto masked) {
-                    float top = 0.f;
+                    // (all 64 scores at once: straight code that keeps the MUFU fed, two
+                    // fp32 operations an instruction where there are such)
+                    float most = 0.f;
                     dl = 0.f;
-                    uint32_t v[2][16];
-                    tmem_ld16(ts, v[0]);
+                    uint32_t v[64];
+                    tmem_ld32(ts, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                    tmem_ld32(ts + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < KT / 16; ++c) {
-                        uint32_t w[8];
-                        tmem_wait_ld();
-                        if (c + 1 < KT / 16) tmem_ld16(ts + 16 * (c + 1), v[(c + 1) & 1]);
+                    for (int c = 0; c < 4; ++c) {
                         const float4 f = sc[c];
                         const float fa = f.x * cr, fb = f.y - (m - C::SHIFT);
-                        float sum[2] = {0.f, 0.f};
+                        const uint64_t fa2 = pair(fa, fa), fb2 = pair(fb, fb);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            float y[2];
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                y[k] = fmaf(__uint_as_float(v[c & 1][e + k]), fa, fb);
-                                const int col = 16 * c + e + k;
-                                if (decltype(masked)::value)
-                                    y[k] = col >= c_lo && col <= c_hi ? y[k] : -INFINITY;
-                                y[k] = ex2(y[k]);
-                                sum[k] += y[k];
+                            const int col = 16 * c + e;
+                            float x, y;
+                            unpair(fma2(pair(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), fa2, fb2), x, y);
+                            if (decltype(masked)::value) {
+                                const int at = 64 * hh + col;
+                                x = at >= c_lo && at <= c_hi ? x : -INFINITY;
+                                y = at + 1 >= c_lo && at + 1 <= c_hi ? y : -INFINITY;
                             }
-                            w[e / 2] = pack_h2(y[0], y[1]);
+                            x = ex2(x), y = ex2(y);
+                            sum = add2(sum, pair(x, y));
+                            v[8 * c + e / 2] = pack_h2(x, y);
                         }
-                        sum[0] += sum[1];
-                        top = fmaxf(top, sum[0]);
-                        dl = fmaf(sum[0], f.z, dl);
-                        if (c == 0) wait_product();
-                        tmem_st8(tp + 8 * c, w);
+                        float s0, s1;
+                        unpair(sum, s0, s1);
+                        s0 += s1;
+                        most = fmaxf(most, s0);
+                        dl = fmaf(s0, f.z, dl);
                     }
-                    return top;
+                    tmem_st32(tp, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                    return most;
                 };
-                // Where the weights lie beside the scores, a unit is weighed with the reference
-                // that the units before left, and weighed again in the rare case that a row
+                // Where the weights lie beside the scores, a half is weighed with the reference
+                // that the halves before left, and weighed again in the rare case that a row
                 // reached fp16's limit (no weight reaches 2^15 unless a sum of 16 does).
-                if (!C::BESIDE || u == cw.lo) {
+                if (!C::BESIDE || (first_unit && hh == 0)) {
                     if (edge_unit) follow(std::true_type{});
                     else follow(std::false_type{});
-                } else if (__any_sync(~0u, raise > 0)) {
+                } else if (hh == 0 && __any_sync(~0u, raise > 0)) {
                     // by a power of two: the rows' sums and O keep their bits
                     const float f = ex2((float)-raise);
                     l *= f;
                     m += (float)raise;
                     rescale(f);
                 }
-                float top;
+                float most;
                 while (true) {
-                    top = edge_unit ? weigh(std::true_type{}) : weigh(std::false_type{});
-                    if (!C::BESIDE || !__any_sync(~0u, top > 32768.f)) break;
+                    most = edge_unit ? weigh(std::true_type{}) : weigh(std::false_type{});
+                    if (!C::BESIDE || !__any_sync(~0u, most > 32768.f)) break;
                     if (edge_unit) follow(std::true_type{});
                     else follow(std::false_type{});
-                    if (__all_sync(~0u, !(top > 32768.f) || !(m < INFINITY))) break;
+                    if (__all_sync(~0u, !(most > 32768.f) || !(m < INFINITY))) break;
                 }
-                // the next unit's reference: up once the weights pass 2^(SHIFT + kPSlack)
-                constexpr float kRaise = 256.f;
-                raise = C::BESIDE && top > kRaise ? (int)(__float_as_uint(top) >> 23) - 127 - (int)C::SHIFT : 0;
-                if (!live) break;
+                top = fmaxf(top, most);
                 l += dl;
                 tmem_wait_st();
                 tc5_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&pfull[tile]));
+                if (lane == 0) mbar_arrive(smem_u32(&pfull[tile][b]));
+                }
+                // the next unit's reference goes up once the weights come near the limit
+                raise = C::BESIDE && top > 16384.f ? (int)(__float_as_uint(top) >> 23) - 127 - (int)C::SHIFT : 0;
             }
-            if (!live || !(live = wait(&pdone[tile], it - 1))) break;
+            wait(&pdone[tile][(hc - 1) & 1], (hc - 1) >> 1);
             tc5_fence_after();
             // ---- output: the row itself, or its part of a cut pair
             int ca, cb;
@@ -641,67 +668,58 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         }
     } else if (warp < C::SOFT + 4) {
         // ======================================================== converters
-        constexpr int SEG = KT * DB / 128;   // segments (a key's 64 dims) of a thread, K and V each
-        const int ct = tid - 32 * C::SOFT;
+        if constexpr (DP <= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else if constexpr (DP <= 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        constexpr int NC = DP * KT / (16 * 128);   // chunks of 16 codes of a thread, K and V each
+        const int ct = tid - 32 * C::SOFT, row = ct % KT, c0 = ct / KT * NC;
         Walk w = cw;
         w.hi = 0;
-        int u = 0, blk[SEG];
+        int u = 0, blk = 0;
         bool more = true;
-        auto lookup = [&]() {   // the next unit, and the numbers of its blocks
+        auto lookup = [&]() {   // the next unit, and the number of its key's block
             if (more && ++u >= w.hi) {
                 more = next_piece(w);
                 u = w.lo;
             }
             if (!more) return;
-#pragma unroll
-            for (int k = 0; k < SEG; ++k) {
-                const int key = u * KT + (ct + 128 * k) % KT;
-                blk[k] = key < w.s.start + w.s.n
-                             ? a.table[(size_t)w.b * a.table_stride + (key >> a.bt_log2)] : 0;
-            }
+            const int key = u * KT + row;
+            blk = key < w.s.start + w.s.n
+                      ? a.table[(size_t)w.b * a.table_stride + (key >> a.bt_log2)] : 0;
         };
-        uint4 kc[SEG][4], vc[SEG][4];
+        uint4 kc[NC], vc[NC];
         float ks = 0.f, vs = 1.f;
-        auto fetch = [&]() {    // its codes, and the scales of every 16 keys
-#pragma unroll
-            for (int k = 0; k < SEG; ++k) {
-                const int key = u * KT + (ct + 128 * k) % KT, db = (ct + 128 * k) / KT;
-                const bool in = key < w.s.start + w.s.n;
-                if (in && (uint32_t)blk[k] >= a.n_blocks) {
-                    atomicOr(err, (unsigned)GRAFT_KV_EBLOCK);
-                    blk[k] = 0;
-                }
-                const size_t bh = (size_t)blk[k] * H + w.h;
-                const size_t off = ((bh << a.bt_log2) + (key & ((1 << a.bt_log2) - 1))) * D + 64 * db;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const bool ok = in && 64 * db + 16 * c < D;
-                    kc[k][c] = ok ? ld_ro(a.k + off + 16 * c) : make_uint4(0, 0, 0, 0);
-                    vc[k][c] = ok ? ld_ro(a.v + off + 16 * c) : make_uint4(0, 0, 0, 0);
-                }
-                if (k == 0) {
-                    ks = in ? a.k_scale[bh] : 0.f;
-                    vs = in ? fmaxf(a.v_scale[bh], kKVScaleFloor) : 1.f;
-                }
+        auto fetch = [&]() {    // its codes, and the block's scales
+            const int key = u * KT + row;
+            const bool in = key < w.s.start + w.s.n;
+            if (in && (uint32_t)blk >= a.n_blocks) {
+                atomicOr(err, (unsigned)GRAFT_KV_EBLOCK);
+                blk = 0;
             }
+            const size_t bh = (size_t)blk * H + w.h;
+            const size_t off = ((bh << a.bt_log2) + (key & ((1 << a.bt_log2) - 1))) * D + 16 * c0;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const bool ok = in && 16 * (c0 + c) < D;
+                kc[c] = ok ? ld_ro(a.k + off + 16 * c) : make_uint4(0, 0, 0, 0);
+                vc[c] = ok ? ld_ro(a.v + off + 16 * c) : make_uint4(0, 0, 0, 0);
+            }
+            ks = in ? a.k_scale[bh] : 0.f;
+            vs = in ? fmaxf(a.v_scale[bh], kKVScaleFloor) : 1.f;
         };
-        auto store = [&](uint8_t* to, const uint4 (&x)[SEG][4]) {
+        auto store = [&](uint8_t* to, const uint4 (&x)[NC]) {
 #pragma unroll
-            for (int k = 0; k < SEG; ++k) {
-                const int row = (ct + 128 * k) % KT, db = (ct + 128 * k) / KT;
-                uint8_t* line = to + (db * KT + row) * 128;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[8];
-                    codes_h2<FMT>(x[k][c].x, o[0], o[1]);
-                    codes_h2<FMT>(x[k][c].y, o[2], o[3]);
-                    codes_h2<FMT>(x[k][c].z, o[4], o[5]);
-                    codes_h2<FMT>(x[k][c].w, o[6], o[7]);
-                    *reinterpret_cast<uint4*>(line + (((2 * c) ^ (row & 7)) << 4)) =
-                        make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(line + (((2 * c + 1) ^ (row & 7)) << 4)) =
-                        make_uint4(o[4], o[5], o[6], o[7]);
-                }
+            for (int c = 0; c < NC; ++c) {
+                const int at = c0 + c;   // 16 dims: chunks 2 (at & 3), + 1 of a 128-byte row
+                uint8_t* line = to + ((at >> 2) * KT + row) * 128;
+                uint32_t o[8];
+                codes_h2<FMT>(x[c].x, o[0], o[1]);
+                codes_h2<FMT>(x[c].y, o[2], o[3]);
+                codes_h2<FMT>(x[c].z, o[4], o[5]);
+                codes_h2<FMT>(x[c].w, o[6], o[7]);
+                *reinterpret_cast<uint4*>(line + (((2 * (at & 3)) ^ (row & 7)) << 4)) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(line + (((2 * (at & 3) + 1) ^ (row & 7)) << 4)) =
+                    make_uint4(o[4], o[5], o[6], o[7]);
             }
         };
         lookup();
@@ -710,16 +728,16 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         lookup();
         for (int it = 0; have; ++it) {
             const int st = it % ST, round = it / ST;
-            if (round && !wait(&kfree[st], round - 1)) break;
+            if (round) wait(&kfree[st], round - 1);
             store(sk + st * C::KV_BYTES, kc);
-            if (ct < KT && ct % 16 == 0) {
+            if (ct < KT && ct % 16 == 0) {   // (16 keys lie in one block)
                 const float lv = lg2(vs);
                 scales[it % SC][ct / 16] = make_float4(ks, lv, ex2(-lv), 0.f);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&kfull[st])), mbar_arrive(smem_u32(&scfull[it % SC]));
-            if (round && !wait(&vfree[st], round - 1)) break;
+            if (round) wait(&vfree[st], round - 1);
             store(sv + st * C::KV_BYTES, vc);
             fence_proxy_async_smem();
             __syncwarp();
@@ -731,55 +749,62 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     } else {
         // =============================================================== MMA
         // (the whole warp walks and waits; one lane issues)
-        constexpr uint32_t iqk = tc5_idesc(KT, false), ipv = tc5_idesc(DP, true);
+        constexpr uint32_t iqk = tc5_idesc(64, false), ipv = tc5_idesc(DP, true);
         const bool leader = elect_one();
         const uint32_t q0 = tc5_low(smem_u32(sq), 16), k0 = tc5_low(smem_u32(sk), 16);
         const uint32_t v0 = tc5_low(smem_u32(sv), KT * 128);
-        auto scores = [&](int tile, int st) {   // S = q K^T
+        auto scores = [&](int tile, int hc) {   // S = q K^T of half hc
+            const int st = hc / C::HN % ST;
             if (leader) {
 #pragma unroll
                 for (int s = 0; s < DP / 16; ++s)
-                    tc5_mma_ss(tmem + tile * 128,
+                    tc5_mma_ss(tmem + tile * 128 + (hc & 1) * 64,
                                q0 + ((tile * DB + s / 4) * 128 * 128 + (s & 3) * 32) / 16,
-                               k0 + (st * C::KV_BYTES + (s / 4) * KT * 128 + (s & 3) * 32) / 16, iqk, s > 0);
-                tc5_commit(smem_u32(&sfull[tile]));
-                if (tile == RT - 1) tc5_commit(smem_u32(&kfree[st]));
+                               k0 + (st * C::KV_BYTES + hc % C::HN * 64 * 128 +
+                                     (s / 4) * KT * 128 + (s & 3) * 32) / 16, iqk, s > 0);
+                tc5_commit(smem_u32(&sfull[tile][hc & 1]));
+                if (tile == RT - 1 && hc % C::HN == C::HN - 1) tc5_commit(smem_u32(&kfree[st]));
             }
         };
-        auto product = [&](int tile, int st, bool accumulate) {   // O += P V
+        auto product = [&](int tile, int hc, bool accumulate) {   // O += P V
+            const int st = hc / C::HN % ST;
             if (leader) {
 #pragma unroll
-                for (int s = 0; s < KT / 16; ++s)
-                    tc5_mma_ts(tmem + C::O_COL + tile * DP, tmem + C::P_COL + tile * C::P_STEP + 8 * s,
-                               v0 + (st * C::KV_BYTES + s * 2048) / 16, ipv, accumulate || s > 0);
-                tc5_commit(smem_u32(&pdone[tile]));
-                if (tile == RT - 1) tc5_commit(smem_u32(&vfree[st]));
+                for (int s = 0; s < 4; ++s)
+                    tc5_mma_ts(tmem + C::O_COL + tile * DP,
+                               tmem + C::P_COL + tile * C::P_TILE + (hc & 1) * C::P_STEP + 8 * s,
+                               v0 + (st * C::KV_BYTES + hc % C::HN * 64 * 128 + s * 2048) / 16, ipv,
+                               accumulate || s > 0);
+                tc5_commit(smem_u32(&pdone[tile][hc & 1]));
+                if (tile == RT - 1 && hc % C::HN == C::HN - 1) tc5_commit(smem_u32(&vfree[st]));
             }
         };
-        int it = 0, pc = 0;
-        bool live = true;
-        while (live && next_piece(cw)) {
-            const int n = cw.hi - cw.lo;
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                live = live && wait(&qfull[i], pc) && (i || wait(&kfull[it % ST], it / ST));
-                if (!live) break;
-                tc5_fence_after();
-                scores(i, it % ST);
-            }
-            for (int j = 0; j < n && live; ++j, ++it) {
-                const int st = it % ST, nx = (it + 1) % ST;
+        auto wait_stage = [&](uint64_t* bars, int hc) {   // before a unit's first half
+            if (hc % C::HN == 0) spin(&bars[hc / C::HN % ST], hc / C::HN / ST);
+        };
+        int hc = 0, pc = 0;
+        while (next_piece(cw)) {
+            const int n = (cw.hi - cw.lo) * C::HN;
+            for (int j = 0; j < 2 && j < n; ++j) {   // the first two halves' scores
+                wait_stage(kfull, hc + j);
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    live = live && wait(&pfull[i], it) && (i || wait(&vfull[st], it / ST)) &&
-                           (i || j + 1 == n || wait(&kfull[nx], (it + 1) / ST));
-                    if (!live) break;
+                    if (j == 0) spin(&qfull[i], pc);
                     tc5_fence_after();
-                    // where the weights lie beside the scores the next scores go first: they
-                    // are waited for, the product runs under their softmax
-                    if (C::BESIDE && j + 1 < n) scores(i, nx);
-                    product(i, st, j > 0);
-                    if (!C::BESIDE && j + 1 < n) scores(i, nx);
+                    scores(i, hc + j);
+                }
+            }
+            for (int j = 0; j < n; ++j, ++hc) {
+                wait_stage(vfull, hc);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    spin(&pfull[i][hc & 1], hc >> 1);
+                    if (i == 0 && j + 2 < n) wait_stage(kfull, hc + 2);
+                    tc5_fence_after();
+                    // (in this order the scores' arrival says that the weights of the same
+                    // parity have been read)
+                    product(i, hc, j > 0);
+                    if (j + 2 < n) scores(i, hc + 2);
                 }
             }
             ++pc;
