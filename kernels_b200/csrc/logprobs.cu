@@ -13,11 +13,11 @@
 // 70% at that rate for 16-bit logits).
 //
 // The top k come from the threads' own maxima, which the pass finds on the
-// way: the k-th largest of them bounds the k-th largest logit from below, so only
-// the k threads whose maximum reaches it can hold one of the top k.  Their
-// chunks (k / 256 of the segment) are read again, from L2, what reaches the
-// bound is collected and ranked by counting.  Ties go to the lowest index: keys
-// are (value, index) pairs, all different.  Segments meet in the workspace, and a
+// way: the k-th largest of the warps' eight best each bounds the k-th largest logit
+// from below, so only threads whose maximum reaches it can hold one of the top
+// k.  Their chunks (little more than k / 128 of the segment) are read again, from
+// L2, and what reaches the bound is collected and ranked.  Ties go to the lowest
+// index: keys are (value, chunk or index) pairs, all different.  Segments meet in the workspace, and a
 // row's last CTA joins them.
 #include "kv_common.cuh"
 
@@ -29,12 +29,13 @@ using namespace graft::dev;
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxTop = 32, kMaxSegs = 16;
-constexpr int kCap = 512;            // collected keys; more take the slow selection
-constexpr int kMinSeg = 8192;        // elements of a segment, at least
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kBest = 32 / kWarps;   // of each warp's thread maxima
+constexpr int kMaxTop = 32, kMaxSegs = 32;
+constexpr int kCap = 2048;           // collected keys; more are selected from the logits one by one
+constexpr int kMinSeg = 4096;        // elements of a segment, at least
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 4 x 4)
+constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 8 x 2)
 constexpr size_t kCounterBytes = (kRounds * 4 + 255) / 256 * 256;   // a row is cut only if rows < kRounds
 constexpr uint64_t kNoKey = 0;       // below every key of a logit that is not -inf
 
@@ -124,6 +125,23 @@ __device__ __forceinline__ void floats_of(const uint4& v, float (&x)[kPer<DT>]) 
     }
 }
 
+// Two 16-bit logits minus ref in fp32: fma.rn.f32.f16 with a factor of one, so
+// that no conversion is needed.
+template <int DT>
+__device__ __forceinline__ void minus(uint32_t w, float ref, float& d0, float& d1) {
+    if constexpr (DT == GRAFT_F16) {
+        asm("{\n\t.reg .f16 a, b, one;\n\t"
+            "mov.b32 {a, b}, %2;\n\tmov.b16 one, 0x3C00;\n\t"
+            "fma.rn.f32.f16 %0, a, one, %3;\n\tfma.rn.f32.f16 %1, b, one, %3;\n\t}"
+            : "=f"(d0), "=f"(d1) : "r"(w), "f"(-ref));
+    } else {
+        asm("{\n\t.reg .b16 a, b, one;\n\t"
+            "mov.b32 {a, b}, %2;\n\tmov.b16 one, 0x3F80;\n\t"
+            "fma.rn.f32.bf16 %0, a, one, %3;\n\tfma.rn.f32.bf16 %1, b, one, %3;\n\t}"
+            : "=f"(d0), "=f"(d1) : "r"(w), "f"(-ref));
+    }
+}
+
 // (ref, L, E) of two parts; ref = -inf marks an empty one.  L and E are
 // relative to their part's ref, c = scale log2(e).
 __device__ __forceinline__ void join(float& ref, float& L, float& E, float r2, float L2, float E2,
@@ -142,12 +160,12 @@ struct Shared {
     float ref[kWarps], L[kWarps], E[kWarps];
     uint64_t key[kCap];
     uint64_t best[kMaxTop];
+    uint64_t top[32];   // the warps' best thread maxima
     uint64_t red[kWarps];
-    int list[kMaxTop];
-    int n, listed, last, count[2];
+    int list[kThreads];
+    int n, listed, last;
 };
 
-// Largest key below `limit` that `mine` yields over the CTA.
 __device__ __forceinline__ uint64_t block_max(Shared& sh, uint64_t v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -161,67 +179,94 @@ __device__ __forceinline__ uint64_t block_max(Shared& sh, uint64_t v) {
     return v;
 }
 
-// Ranks the n different keys sh.key[0..n): sh.best[r] = the r-th largest, r < k.
+// The k largest of the n different keys sh.key[0..n) into sh.best: a few by
+// counting for each key those above it, many one after the other.
 __device__ __forceinline__ void rank_keys(Shared& sh, int n, int k) {
-    for (int i = threadIdx.x; i < k; i += kThreads) sh.best[i] = kNoKey;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t v = sh.key[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += sh.key[j] > v;
-        if (r < k) sh.best[r] = v;
+    const int tid = threadIdx.x;
+    if (n <= kThreads) {
+        if (tid < k) sh.best[tid] = kNoKey;
+        __syncthreads();
+        if (tid < n) {
+            const uint64_t v = sh.key[tid];
+            int r = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) r += sh.key[j] > v;
+            if (r < k) sh.best[r] = v;
+        }
+    } else {
+        uint64_t before = ~0ull;
+        for (int r = 0; r < k; ++r) {
+            uint64_t v = kNoKey;
+            for (int i = tid; i < n; i += kThreads) {
+                const uint64_t w = sh.key[i];
+                if (w < before && w > v) v = w;
+            }
+            before = block_max(sh, v);
+            if (tid == 0) sh.best[r] = before;
+        }
     }
     __syncthreads();
 }
 
-// The top k keys of the segment's chunks [c0, c1) into sh.best.  tmax, tchunk: the
-// thread's largest logit (-inf: none) and the first chunk that holds it.
+// A segment's chunks: those wholly in the row are [i0, i1), chunk i0 + t + j*kThreads
+// is thread t's j-th; a row's first chunk belongs to thread 0 and its last to
+// thread 1 where they lie partly outside (first, last: -1 if not).
+struct Span {
+    int i0, i1, first, last;
+};
+
+// The top k keys of the segment into sh.best.  tmax, tchunk: the thread's largest
+// logit (-inf: none) and the first chunk that holds it.
 template <int DT>
 __device__ __forceinline__ void select_top(Shared& sh, const void* row, int off, uint32_t vocab,
-                                           int c0, int c1, float tmax, int tchunk, int k) {
+                                           const Span& sp, float tmax, int tchunk, int k) {
     constexpr int N = kPer<DT>;
-    const int tid = threadIdx.x;
-    // ---- the k-th largest thread maximum, bit by bit (16-bit logits as fp32 differ in
-    // their upper 16 or 19 bits only)
-    constexpr int kLow = DT == GRAFT_F32 ? 0 : DT == GRAFT_BF16 ? 16 : 13;
-    const bool some = tmax > -INFINITY;
-    const uint32_t mine = some ? order(tmax) >> kLow : 0;
-    uint32_t bound = 0;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // ---- the best of each warp
+    const uint32_t mine = tmax > -INFINITY ? order(tmax) : 0;
+    const uint32_t inv = 0xFFFFFFFFu - (uint32_t)tchunk;
+    uint32_t left = mine;
+#pragma unroll
+    for (int r = 0; r < kBest; ++r) {
+        const uint32_t v = __reduce_max_sync(~0u, left);
+        const uint32_t c = __reduce_max_sync(~0u, left == v ? inv : 0u);
+        if (lane == 0) sh.top[warp * kBest + r] = v ? ((uint64_t)v << 32) | c : kNoKey;
+        if (left == v && inv == c) left = 0;
+    }
     if (tid == 0) sh.n = sh.listed = 0;
-    if (__syncthreads_count(some) > k) {
-#pragma unroll 1
-        for (int b = 31 - kLow; b >= 0; --b) {
-            const uint32_t t = bound | (1u << b);
-            if (__syncthreads_count(mine >= t) >= k) bound = t;
-        }
-    }
-    bound = max(bound, 1u);
-    // ---- equal maxima: the first chunks go first
-    int last_chunk = 0x7FFFFFFF;
-    const int above = __syncthreads_count(mine > bound);
-    if (__syncthreads_count(mine >= bound) > k) {
-        last_chunk = 0;
-#pragma unroll 1
-        for (int b = 30; b >= 0; --b) {   // the least t with k threads at or before it, minus 1
-            const int t = last_chunk | (1 << b);
-            if (above + __syncthreads_count(mine == bound && tchunk < t) < k) last_chunk = t;
-        }
-    }
-    if (mine > bound || (mine == bound && tchunk <= last_chunk)) sh.list[atomicAdd(&sh.listed, 1)] = tid;
+    __syncthreads();
+    // ---- the k-th largest of them (every warp for itself): the bound
+    // (keys are all different but for the empty ones, which come last)
+    const uint64_t own = sh.top[lane];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) rank += sh.top[j] > own;
+    const uint32_t at = __ballot_sync(~0u, rank == k - 1 && own != kNoKey);
+    uint64_t bound = __shfl_sync(~0u, own, at ? __ffs(at) - 1 : 0);
+    if (!at) bound = 1ull << 32;   // fewer than k: whatever is not -inf
+    if (mine && (((uint64_t)mine << 32) | inv) >= bound) sh.list[atomicAdd(&sh.listed, 1)] = tid;
     __syncthreads();
     // ---- what reaches the bound in those threads' chunks
-    const int listed = sh.listed, per = (c1 - c0 + kThreads - 1) / kThreads;
+    const uint32_t bv = (uint32_t)(bound >> 32);
+    const int bc = (int)(0xFFFFFFFFu - (uint32_t)bound);   // (negative: any chunk)
+    const int listed = sh.listed, per = (max(sp.i1 - sp.i0, 0) + kThreads - 1) / kThreads + 1;
+    auto chunk_of = [&](int i) {   // the i-th to look at, -1: none
+        const int q = i / per, j = i - q * per, t = sh.list[q];
+        if (j == per - 1) return t == 0 ? sp.first : t == 1 ? sp.last : -1;
+        const int c = sp.i0 + t + j * kThreads;
+        return c < sp.i1 ? c : -1;
+    };
     for (int i = tid; i < listed * per; i += kThreads) {
-        const int q = i / per, c = c0 + sh.list[q] + (i - q * per) * kThreads;
-        if (c >= c1) continue;
+        const int c = chunk_of(i);
+        if (c < 0) continue;
         float x[N];
         floats_of<DT>(load_chunk<DT>(row, off, vocab, c), x);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t o = x[e] > -INFINITY ? order(x[e]) >> kLow : 0;
-            if (o > bound || (o == bound && c <= last_chunk)) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kCap) sh.key[at] = key_of(x[e], c * N - off + e);
+            const uint32_t o = x[e] > -INFINITY ? order(x[e]) : 0;
+            if (o > bv || (o == bv && (uint32_t)c <= (uint32_t)bc)) {
+                const int to = atomicAdd(&sh.n, 1);
+                if (to < kCap) sh.key[to] = key_of(x[e], c * N - off + e);
             }
         }
     }
@@ -236,8 +281,8 @@ __device__ __forceinline__ void select_top(Shared& sh, const void* row, int off,
     for (int r = 0; r < k; ++r) {
         uint64_t v = kNoKey;
         for (int i = tid; i < listed * per; i += kThreads) {
-            const int q = i / per, c = c0 + sh.list[q] + (i - q * per) * kThreads;
-            if (c >= c1) continue;
+            const int c = chunk_of(i);
+            if (c < 0) continue;
             float x[N];
             floats_of<DT>(load_chunk<DT>(row, off, vocab, c), x);
 #pragma unroll
@@ -253,8 +298,26 @@ __device__ __forceinline__ void select_top(Shared& sh, const void* row, int off,
     __syncthreads();
 }
 
+// Largest element of a chunk (NaN is passed over).
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_constant__ LpArgs a) {
+__device__ __forceinline__ float chunk_max(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (DT == GRAFT_F32) {
+        return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                     fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    } else {
+        uint32_t m = w[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            if constexpr (DT == GRAFT_F16) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+            else asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+        }
+        const float2 p = unpack2<DT>(m);
+        return fmaxf(p.x, p.y);
+    }
+}
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const __grid_constant__ LpArgs a) {
     constexpr int N = kPer<DT>, UN = 4;   // elements of a chunk, chunks in flight
     __shared__ Shared sh;
     pdl_wait();
@@ -266,59 +329,115 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
     const int off = (int)(((uintptr_t)base & 15) / (16 / N));
     const int chunks = (int)(((uint64_t)off + a.vocab + N - 1) / N);
     const int per_seg = (chunks + a.segs - 1) / a.segs;
-    const int c0 = seg * per_seg, c1 = min(c0 + per_seg, chunks);
+    const int c0 = min(seg * per_seg, chunks), c1 = min(c0 + per_seg, chunks);
+    Span sp;
+    sp.first = c0 == 0 && c1 > 0 && (off || (int)a.vocab < N) ? 0 : -1;
+    sp.last = c1 == chunks && c1 - 1 > sp.first && c1 > c0 && (off + a.vocab) % N ? c1 - 1 : -1;
+    sp.i0 = c0 + (sp.first >= 0), sp.i1 = c1 - (sp.last >= 0);
     const float c = a.scale * kLog2e, reach = 64.f / c;
 
     // ---- the pass: sums against the thread's reference, its maximum and where that is first
-    float ref = 0.f, lim = -INFINITY, L = 0.f, E = 0.f, tmax = -INFINITY;
+    float ref = 0.f, lim = -INFINITY, tmax = -INFINITY;
+    float L2[2] = {0.f, 0.f}, E2[2] = {0.f, 0.f};   // two partial sums each
     int tchunk = 0;
-    auto take = [&](const uint4& v, int ch) {
-        float x[N];
-        floats_of<DT>(v, x);
-        float cm = x[0];
+    auto take = [&](const auto& v, int ch) {   // chunks ch, ch + kThreads, ..
+        constexpr int U = sizeof(v) / sizeof(uint4);
+        float cm[U], gm;
 #pragma unroll
-        for (int e = 1; e < N; ++e) cm = fmaxf(cm, x[e]);
-        if (cm > tmax) tmax = cm, tchunk = ch;
-        if (cm > lim) {
-            const float f = lim == -INFINITY ? 0.f : ex2((ref - cm) * c);
-            E = lim == -INFINITY ? E : f * fmaf(L, max_nan((ref - cm) * c, -256.f), E);
-            L = lim == -INFINITY ? L : f * L;
-            ref = cm;
-            lim = cm + reach;
+        for (int u = 0; u < U; ++u) {
+            cm[u] = chunk_max<DT>(v[u]);
+            gm = u ? fmaxf(gm, cm[u]) : cm[u];
         }
-        float l2[2] = {0.f, 0.f}, e2[2] = {0.f, 0.f};
+        if (gm > tmax) {   // (lim is never below tmax)
+            tmax = gm;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float d = max_nan((x[e] - ref) * c, -256.f);   // (-inf: weight 0, and not 0 * inf)
-            const float w = ex2(d);
-            l2[e & 1] += w;
-            e2[e & 1] = fmaf(w, d, e2[e & 1]);
+            for (int u = U - 1; u >= 0; --u)
+                if (cm[u] == gm) tchunk = ch + u * kThreads;
+            if (gm > lim) {
+                if (lim > -INFINITY) {
+                    const float a = (ref - gm) * c, f = ex2(a), b = max_nan(a, -256.f);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) E2[i] = f * fmaf(L2[i], b, E2[i]), L2[i] *= f;
+                }
+                ref = gm;
+                lim = gm + reach;
+            }
         }
-        L += l2[0] + l2[1];
-        E += e2[0] + e2[1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t w4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                float d0, d1;
+                if constexpr (DT == GRAFT_F32) {
+                    d0 = __uint_as_float(w4[e]) - ref, d1 = __uint_as_float(w4[e + 1]) - ref;
+                } else {
+                    minus<DT>(w4[e / 2], ref, d0, d1);
+                }
+                // (a weight of -inf is 0, and must not be 0 * inf)
+                d0 = max_nan(d0 * c, -256.f), d1 = max_nan(d1 * c, -256.f);
+                const float w0 = ex2(d0), w1 = ex2(d1);
+                L2[0] += w0, L2[1] += w1;
+                E2[0] = fmaf(w0, d0, E2[0]), E2[1] = fmaf(w1, d1, E2[1]);
+            }
+        }
     };
-    int ch = c0 + tid;
-    for (; ch + (UN - 1) * kThreads < c1; ch += UN * kThreads) {
-        uint4 v[UN];
+    auto take_edge = [&](int ch) {
+        const uint4 v[1] = {load_chunk<DT>(base, off, a.vocab, ch)};
+        take(v, ch);
+    };
+    {
+        int ch = sp.i0 + tid;
+        const char* at = base + ((int64_t)ch * N - off) * (16 / N);
+        if (tid == 0 && sp.first >= 0) take_edge(sp.first);   // (each thread's chunks in rising order)
+#pragma unroll 1
+        for (; ch + (UN - 1) * kThreads < sp.i1; ch += UN * kThreads, at += UN * kThreads * 16) {
+            uint4 v[UN];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) v[u] = load_chunk<DT>(base, off, a.vocab, ch + u * kThreads);
+            for (int u = 0; u < UN; ++u) v[u] = ld_stream(at + u * kThreads * 16);
+            take(v, ch);
+        }
+        if (ch < sp.i1) {   // what is left, as one more round with empty chunks
+            constexpr uint32_t none = DT == GRAFT_F32 ? 0xFF800000u : DT == GRAFT_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+            uint4 v[UN];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) take(v[u], ch + u * kThreads);
+            for (int u = 0; u < UN; ++u)
+                v[u] = ch + u * kThreads < sp.i1 ? ld_stream(at + u * kThreads * 16)
+                                                 : make_uint4(none, none, none, none);
+            take(v, ch);
+        }
+        if (tid == 1 && sp.last >= 0) take_edge(sp.last);
     }
-    for (; ch < c1; ch += kThreads) take(load_chunk<DT>(base, off, a.vocab, ch), ch);
 
-    // ---- the CTA's sums
-    float r = lim == -INFINITY ? -INFINITY : ref;
+    // ---- the CTA's sums: against the warp's largest reference, then the warps'
+    float L, E, r = lim == -INFINITY ? -INFINITY : ref;
+    {
+        L = L2[0] + L2[1], E = E2[0] + E2[1];
+        float m = r;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float r2 = __shfl_xor_sync(~0u, r, o), L2 = __shfl_xor_sync(~0u, L, o);
-        join(r, L, E, r2, L2, __shfl_xor_sync(~0u, E, o), c);
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        const float b = r == -INFINITY ? 0.f : (r - m) * c, f = r == -INFINITY ? 0.f : ex2(b);
+        E = f * fmaf(L, max_nan(b, -256.f), E);
+        L *= f;
+        r = m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            L += __shfl_xor_sync(~0u, L, o);
+            E += __shfl_xor_sync(~0u, E, o);
+        }
     }
     if (lane == 0) sh.ref[warp] = r, sh.L[warp] = L, sh.E[warp] = E;
-    if (k) select_top<DT>(sh, base, off, a.vocab, c0, c1, tmax, tchunk, k);
+    if (k) select_top<DT>(sh, base, off, a.vocab, sp, tmax, tchunk, k);
     else __syncthreads();
-    r = sh.ref[0], L = sh.L[0], E = sh.E[0];
-    for (int w = 1; w < kWarps; ++w) join(r, L, E, sh.ref[w], sh.L[w], sh.E[w], c);
+    if (warp == 0) {   // (the others' stay their own: the first warp writes the results)
+        r = -INFINITY, L = E = 0.f;
+        if (lane < kWarps) r = sh.ref[lane], L = sh.L[lane], E = sh.E[lane];
+#pragma unroll
+        for (int o = kWarps / 2; o; o >>= 1) {
+            const float r2 = __shfl_xor_sync(~0u, r, o), m2 = __shfl_xor_sync(~0u, L, o);
+            join(r, L, E, r2, m2, __shfl_xor_sync(~0u, E, o), c);
+        }
+    }
 
     // ---- segments meet in the workspace; the row's last CTA goes on
     if (a.segs > 1) {
@@ -341,25 +460,34 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
             const float4 v = __ldcg(reinterpret_cast<const float4*>(&p[lane]));
             r = v.x, L = v.y, E = v.z;
         }
-        uint64_t low = kNoKey;   // the best k-th key of a segment: nothing below it counts
-        if (k && lane < a.segs) low = __ldcg((const unsigned long long*)&p[lane].key[k - 1]);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {   // (in the same order in every warp)
+        for (int o = 16; o; o >>= 1) {
             const float r2 = __shfl_xor_sync(~0u, r, o), L2 = __shfl_xor_sync(~0u, L, o);
             join(r, L, E, r2, L2, __shfl_xor_sync(~0u, E, o), c);
-            const uint64_t w = __shfl_xor_sync(~0u, low, o);
-            low = w > low ? w : low;
         }
         if (k) {
+            // the k-th largest of the segments' first ceil(k / segs) keys bounds the k-th of all
+            const int J = (k + a.segs - 1) / a.segs, m = a.segs * J;   // k <= m < k + segs
+            const uint64_t own = tid < m ? __ldcg((const unsigned long long*)&p[tid / J].key[tid % J]) : kNoKey;
+            if (tid < m) sh.key[tid] = own;
+            if (tid == 0) sh.red[0] = kNoKey + 1;
+            __syncthreads();
+            int rank = 0;
+            for (int j = 0; j < m; ++j) rank += sh.key[j] > own;
+            if (own != kNoKey && rank == k - 1) sh.red[0] = own;   // (valid keys are all different)
+            __syncthreads();
+            const uint64_t low = sh.red[0];
             for (int i = tid; i < a.segs * k; i += kThreads) {
                 const uint64_t v = __ldcg((const unsigned long long*)&p[i / k].key[i % k]);
-                if (v != kNoKey && v >= low) sh.key[atomicAdd(&sh.n, 1)] = v;
+                if (v >= low) sh.key[atomicAdd(&sh.n, 1)] = v;
             }
             __syncthreads();
             rank_keys(sh, sh.n, k);
         }
     }
-    // ---- the row's results: lse = scale*r + ln L
+    // ---- the row's results, by the first warp: lse = scale*r + ln L
+    if (warp) return;
+    r = __shfl_sync(~0u, r, 0), L = __shfl_sync(~0u, L, 0), E = __shfl_sync(~0u, E, 0);
     const bool none = r == -INFINITY && L == L;   // no token is possible (and no NaN)
     const float lnL = none ? 0.f : logf(L);
     const float at = r == -INFINITY ? 0.f : r;
