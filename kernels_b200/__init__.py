@@ -329,12 +329,37 @@ def moe_set_one_launch(on) -> int:
 
 
 # ------------------------------------------ key/value cache and attention --
+# (these calls take a few microseconds on the GPU in a decode step, so the host
+# side keeps to what each call needs)
+_DTYPES: dict = {}
+
+
 def _dtype_code(dtype) -> int:
-    import torch
-    codes = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-    if dtype not in codes:
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise TypeError(f"unsupported element type {dtype}")
-    return codes[dtype]
+    return code
+
+
+_RAW_STREAM: list = []
+
+
+def _raw_stream(stream) -> int:
+    """_s() without a Stream object for the usual case, the current stream."""
+    if stream is not None:
+        return stream if isinstance(stream, int) else stream.cuda_stream
+    if not _RAW_STREAM:
+        import torch
+        torch.cuda.current_stream()      # (CUDA is initialised from here on)
+        try:
+            _RAW_STREAM.extend((torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice))
+        except AttributeError:
+            _RAW_STREAM.extend((lambda d: torch.cuda.current_stream(d).cuda_stream,
+                                torch.cuda.current_device))
+    return _RAW_STREAM[0](_RAW_STREAM[1]())
 
 
 def _ints(t, name: str):
@@ -348,11 +373,21 @@ def _ints(t, name: str):
 
 def _heads(t, heads: int, dim: int) -> Heads:
     """A [tokens, heads, dim] tensor with any token and head strides."""
-    if t.dim() != 3 or t.shape[1:] != (heads, dim):
-        raise ValueError(f"expected a [tokens, {heads}, {dim}] tensor, not {tuple(t.shape)}")
-    if t.stride(2) != 1 and dim > 1:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"expected a [tokens, {heads}, {dim}] tensor, not {tuple(shape)}")
+    if stride[2] != 1 and dim > 1:
         raise ValueError("the last dimension must be contiguous")
-    return Heads(_p(t), t.stride(0), t.stride(1), t.shape[0], _dtype_code(t.dtype))
+    return Heads(t.data_ptr(), stride[0], stride[1], shape[0], _dtype_code(t.dtype))
+
+
+def _dense(t, dtype, shape) -> int | None:
+    """The address of a contiguous tensor of that type and shape; None for None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"expected a contiguous {dtype} {tuple(shape)} tensor")
+    return t.data_ptr()
 
 
 class KVCache:
@@ -376,6 +411,7 @@ class KVCache:
         n, h, bt, d = k.shape
         self.desc = KVCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), n, h, bt, d,
                                 formats[k.dtype])
+        self.ref, self.heads, self.dim = C.byref(self.desc), h, d
 
     @classmethod
     def empty(cls, n_blocks: int, kv_heads: int, head_dim: int, block_tokens: int = 64,
@@ -403,6 +439,7 @@ class KVRange:
         stride = block_table.stride(0) if n > 1 else block_table.shape[1]
         self.desc = KVRangeDesc(_p(block_table), _p(start), _p(cu_tokens), n, stride, max_tokens,
                                 max_len)
+        self.ref = C.byref(self.desc)
 
 
 def kv_range(block_table, start, cu_tokens, max_tokens: int, max_len: int) -> KVRange:
@@ -413,18 +450,20 @@ def kv_range(block_table, start, cu_tokens, max_tokens: int, max_len: int) -> KV
     return KVRange(block_table, start, cu_tokens, max_tokens, max_len)
 
 
+def _kv_move(name: str, cache: KVCache, K, V, rng: KVRange, stream) -> None:
+    h, d = cache.heads, cache.dim
+    call(name, cache.ref, C.byref(_heads(K, h, d)), C.byref(_heads(V, h, d)), rng.ref,
+         _raw_stream(stream))
+
+
 def kv_write(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
     """Quantises K and V [tokens, kv_heads, head_dim] into the cache (graft_kv_write)."""
-    h, d = cache.desc.kv_heads, cache.desc.head_dim
-    call("graft_kv_write", C.byref(cache.desc), C.byref(_heads(K, h, d)),
-         C.byref(_heads(V, h, d)), C.byref(rng.desc), _s(stream))
+    _kv_move("graft_kv_write", cache, K, V, rng, stream)
 
 
 def kv_read(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
     """Reads the range back into K and V [tokens, kv_heads, head_dim] (graft_kv_read)."""
-    h, d = cache.desc.kv_heads, cache.desc.head_dim
-    call("graft_kv_read", C.byref(cache.desc), C.byref(_heads(K, h, d)), C.byref(_heads(V, h, d)),
-         C.byref(rng.desc), _s(stream))
+    _kv_move("graft_kv_read", cache, K, V, rng, stream)
 
 
 def kv_device_errors(clear: bool = False) -> dict:
@@ -460,15 +499,12 @@ def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorksp
              lse=None, stream=None) -> None:
     """Attention of the range's tokens (q and out [tokens, q_heads, head_dim])
     over the cache (graft_attn_kv8)."""
-    import torch
-    d = cache.desc.head_dim
-    for t, shape in ((sinks, (P.q_heads,)), (lse, (q.shape[0], P.q_heads))):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape
-                              or not t.is_contiguous()):
-            raise ValueError(f"sinks and lse must be contiguous fp32, {shape}")
-    call("graft_attn_kv8", C.byref(cache.desc), C.byref(_heads(q, P.q_heads, d)),
-         C.byref(_heads(out, P.q_heads, d)), C.byref(rng.desc), _p(sinks), _p(lse), C.byref(P),
-         ws.addr, ws.nbytes, _s(stream))
+    d, hq = cache.dim, P.q_heads
+    if sinks is not None or lse is not None:
+        from torch import float32
+        sinks, lse = _dense(sinks, float32, (hq,)), _dense(lse, float32, (q.shape[0], hq))
+    call("graft_attn_kv8", cache.ref, C.byref(_heads(q, hq, d)), C.byref(_heads(out, hq, d)),
+         rng.ref, sinks, lse, C.byref(P), ws.addr, ws.nbytes, _raw_stream(stream))
 
 
 # ------------------------------------------------------ log probabilities --
@@ -494,21 +530,19 @@ def logprobs(logits, targets, logprob, entropy, top_logprob, top_index, P: Logpr
              ws: LogprobWorkspace, stream=None) -> None:
     """Log probability of targets, entropy and top alternatives of each row of
     logits [rows, vocab] (graft_logprobs); outputs that are None are left out."""
-    import torch
-    if tuple(logits.shape) != (P.rows, P.vocab) or _dtype_code(logits.dtype) != P.dtype:
+    from torch import float32, int32
+    rows, vocab, k = P.rows, P.vocab, P.top_k
+    if logits.shape != (rows, vocab) or _dtype_code(logits.dtype) != P.dtype:
         raise ValueError("logits do not match the params")
-    if logits.stride(1) != 1 and P.vocab > 1:
+    stride = logits.stride()
+    if stride[1] != 1 and vocab > 1:
         raise ValueError("a row of logits must be contiguous")
-    for t, dt, shape in ((targets, torch.int32, (P.rows,)), (logprob, torch.float32, (P.rows,)),
-                         (entropy, torch.float32, (P.rows,)),
-                         (top_logprob, torch.float32, (P.rows, P.top_k)),
-                         (top_index, torch.int32, (P.rows, P.top_k))):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
-            raise ValueError(f"expected a contiguous {dt} {shape} tensor")
-    Q = LogprobParams(P.rows, P.vocab, P.top_k, P.dtype,
-                      logits.stride(0) if P.rows > 1 else P.vocab, P.scale)
-    call("graft_logprobs", _p(logits), _p(targets), _p(logprob), _p(entropy), _p(top_logprob),
-         _p(top_index), C.byref(Q), ws.addr, ws.nbytes, _s(stream))
+    args = (_dense(targets, int32, (rows,)), _dense(logprob, float32, (rows,)),
+            _dense(entropy, float32, (rows,)), _dense(top_logprob, float32, (rows, k)),
+            _dense(top_index, int32, (rows, k)))
+    Q = LogprobParams(rows, vocab, k, P.dtype, stride[0] if rows > 1 else vocab, P.scale)
+    call("graft_logprobs", logits.data_ptr(), *args, C.byref(Q), ws.addr, ws.nbytes,
+         _raw_stream(stream))
 
 
 # ----------------------------------------------------------- multi-GPU --

@@ -207,7 +207,7 @@ class GraftError(RuntimeError):
 
 
 def call(name: str, *args):
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != GRAFT_OK:
         raise GraftError(name, rc, lib.graft_last_error_string().decode())

@@ -11,6 +11,7 @@
 #include "attn_few.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 using namespace graft;
@@ -19,6 +20,18 @@ using namespace graft::dev;
 namespace {
 
 __device__ unsigned g_attn_err;
+
+// The error word's address on a device (asked for once).
+int error_word(int device, unsigned** out) {
+    static std::atomic<unsigned*> known[64];
+    unsigned* p = device < 64 ? known[device].load(std::memory_order_relaxed) : nullptr;
+    if (!p) {
+        GRAFT_CUDA(cudaGetSymbolAddress((void**)&p, g_attn_err));
+        if (device < 64) known[device].store(p, std::memory_order_relaxed);
+    }
+    *out = p;
+    return GRAFT_OK;
+}
 
 // ---- few query rows
 template <int DP, int NT, int FMT, bool FULL>
@@ -33,7 +46,7 @@ int launch_few(AttnArgs a, cudaStream_t st) {
         (rc = occupancy((const void*)kern, kFewThreads, smem, &per_sm)))
         return rc;
     unsigned* err = nullptr;
-    GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
+    if ((rc = error_word(di.device, &err))) return rc;
     // no more CTAs than the longest possible range has pieces
     const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
                                    : a.max_len;
@@ -66,7 +79,7 @@ int launch_chunk(AttnArgs a, cudaStream_t st) {
     const auto kern = attn_chunk_kernel<DP, FMT>;
     if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
     unsigned* err = nullptr;
-    GRAFT_CUDA(cudaGetSymbolAddress((void**)&err, g_attn_err));
+    if ((rc = error_word(di.device, &err))) return rc;
     // a piece costs about as much besides its units as 3 units (queries in, output);
     // the pad is counted in keys
     a.min_units = 4;
