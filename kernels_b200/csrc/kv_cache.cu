@@ -6,15 +6,18 @@
 //
 // Both kernels move each byte once and compute a few operations per element,
 // so HBM bounds the long calls and launch plus load latency the short ones.
-// Work items are (block that a sequence touches, head, K or V): a block's
-// amax, and the rounding again of its earlier codes when the scale grows,
-// concern one item alone, so an item is one CTA, its elements stay in
-// registers between the maximum and the rounding, and nothing is atomic.
+// Work items are the blocks that a sequence touches.  Writing gives each (item,
+// head, K or V) a CTA: a block's amax, and the rounding again of its earlier codes
+// when the scale grows, concern that CTA alone, so its elements stay in registers
+// between the maximum and the rounding, and nothing is atomic.  Reading gives a
+// CTA as many heads of an item as make 32 KB of codes.
 // The item of a CTA follows from cu_tokens in closed form: sequence b's items
 // start at cu_tokens[b] / block_tokens + 2 b, which leaves room for every
 // block it can touch whatever its start, so no prefix sum of block counts is
 // needed (a CTA past its sequence's blocks returns).
 #include "kv_common.cuh"
+
+#include <algorithm>
 
 using namespace graft;
 using namespace graft::dev;
@@ -24,7 +27,7 @@ namespace {
 __device__ unsigned g_kv_err;
 
 constexpr int kChunk = 8;        // elements a thread moves at once
-constexpr int kMaxChunks = 8;    // chunks a thread holds (128 tokens x 256 / 512 threads)
+constexpr int kWarpChunks = 256; // an item of up to so many chunks a head is a warp's (8 a lane)
 
 struct KVArgs {
     uint8_t *k, *v;
@@ -33,50 +36,62 @@ struct KVArgs {
     const void *x_k, *x_v;                 // rows (read by write, written by read)
     uint64_t tok_k, head_k, tok_v, head_v; // strides in elements
     uint32_t n_blocks, heads, bt, dim, n_seqs, table_stride, max_tokens, max_len, tokens;
+    uint32_t bt_log2;
+    uint32_t cpt, cpt_magic;   // chunks of a row; c / cpt = c cpt_magic >> 20 (c < 128 cpt <= 4096)
+    uint32_t cta_heads;        // heads of a CTA (read)
+    uint32_t wide;             // rows are 32-byte aligned (16-bit types; read)
 };
 
 // One item: `count` tokens of one sequence in one block.
 struct Item {
-    int block;      // block number in the cache
-    int slot;       // first slot in it
-    int row;        // row of the first token
+    const int32_t* block;   // where the block's number stands
+    int slot;               // first slot in it
+    int row;                // row of the first token
     int count;
 };
 
-// The item of flat index x (false: none).  Every thread of the CTA calls it.
+// The item of flat index x (false: none).  Every thread of the CTA calls it.  The
+// lengths of a sequence are read by the thread that looks at it, so that only one
+// round trip to memory comes before the rows' and the block number's.
 __device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it) {
-    const uint32_t bt = a.bt;
-    int b = 0;   // the last sequence whose items start at or before x
-    for (uint32_t s0 = 1; s0 < a.n_seqs; s0 += blockDim.x) {
+    __shared__ int sh_seq[4];   // sequence, its first row, one past its last, its start
+    const uint32_t bt = 1u << a.bt_log2;
+    for (uint32_t s0 = 0;; s0 += blockDim.x) {
         const uint32_t s = s0 + threadIdx.x;
-        const bool p = s < a.n_seqs && (uint32_t)a.cu[s] / bt + 2 * s <= x;
-        const int c = __syncthreads_count(p);
-        b += c;
-        if (c < (int)blockDim.x) break;
+        bool here = false;   // x is one of its items: they start at or before x, the next one's after
+        if (s < a.n_seqs) {
+            const int c = a.cu[s], e = a.cu[s + 1], st = a.start[s];
+            here = (s == 0 || ((uint32_t)c >> a.bt_log2) + 2 * s <= x) &&
+                   (s + 1 == a.n_seqs || ((uint32_t)e >> a.bt_log2) + 2 * (s + 1) > x);
+            if (here) sh_seq[0] = s, sh_seq[1] = c, sh_seq[2] = e, sh_seq[3] = st;
+        }
+        const int found = __syncthreads_count(here);
+        if (found == 1) break;
+        // (none, or with cu_tokens that do not rise several: nothing to do here)
+        if (found > 1 || s0 + blockDim.x >= a.n_seqs) return false;
     }
-    const int c0 = a.cu[b];
-    int n = a.cu[b + 1] - c0;
-    const int64_t start = a.start[b];
-    const bool first = threadIdx.x == 0 && blockIdx.y == 0;
+    const int b = sh_seq[0], c0 = sh_seq[1], n = sh_seq[2] - c0;
+    const int64_t start = sh_seq[3];
     if (c0 < 0 || n < 0 || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens ||
         start < 0 || (uint64_t)(start + n) > a.max_len) {
-        if (first) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
+        if (threadIdx.x == 0) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
         return false;
     }
     if (n == 0) return false;
-    const uint32_t j = x - ((uint32_t)c0 / bt + 2 * b);
-    const int64_t base = (start / bt + j) * bt;      // first position of the block
+    const uint32_t j = x - (((uint32_t)c0 >> a.bt_log2) + 2 * b);
+    const int64_t page = (start >> a.bt_log2) + j, base = page << a.bt_log2;
     if (base >= start + n) return false;
     const int64_t lo = base > start ? base : start;
     it.slot = (int)(lo - base);
     it.row = c0 + (int)(lo - start);
     it.count = min((int)bt - it.slot, (int)(start + n - lo));
-    it.block = a.table[(size_t)b * a.table_stride + (size_t)(base / bt)];
-    if ((uint32_t)it.block >= a.n_blocks) {
-        if (first) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBLOCK);
-        return false;
-    }
+    it.block = a.table + (size_t)b * a.table_stride + (size_t)page;
     return true;
+}
+__device__ __forceinline__ bool good_block(const KVArgs& a, int block) {
+    if ((uint32_t)block < a.n_blocks) return true;
+    if (threadIdx.x == 0) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBLOCK);
+    return false;
 }
 
 // |x| of a finite element, 0 of another
@@ -112,36 +127,42 @@ __device__ __forceinline__ void to_floats(const Raw<DT>& r, float (&f)[8]) {
     }
 }
 
-template <int DT, int FMT>
-__global__ void kv_write_kernel(const __grid_constant__ KVArgs a) {
+// CH: chunks a thread holds.  WARP: each warp takes a (head, K or V) of the item,
+// else the CTA takes one.
+template <int DT, int FMT, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_kernel(const __grid_constant__ KVArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float red[16];
     Item it;
     if (!find_item(a, blockIdx.x, it)) return;
-    const int head = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
+    const int block = *it.block;   // (not needed before the scale)
+    const int unit = WARP ? blockIdx.y * 8 + (threadIdx.x >> 5) : blockIdx.y;
+    if (WARP && unit >= 2 * (int)a.heads) return;
+    const int head = unit >> 1;
+    const bool is_v = unit & 1;
     const void* x = is_v ? a.x_v : a.x_k;
     const uint64_t ts = is_v ? a.tok_v : a.tok_k, hs = is_v ? a.head_v : a.head_k;
-    const size_t bh = (size_t)it.block * a.heads + head;
-    uint8_t* codes = (is_v ? a.v : a.k) + bh * a.bt * a.dim;
-    float* scale = (is_v ? a.v_scale : a.k_scale) + bh;
-    const int tid = threadIdx.x, T = blockDim.x;
-    const int cpt = a.dim / kChunk, n = it.count * cpt;   // chunks a token, chunks of the item
-    const float old = it.slot ? *scale : 0.f;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
+    const int n = it.count * (int)a.cpt;   // chunks of the item
 
-    Raw<DT> r[kMaxChunks];
-    float amax = 0.f;
+    Raw<DT> r[CH];
 #pragma unroll
-    for (int i = 0; i < kMaxChunks; ++i) {
+    for (int i = 0; i < CH; ++i) {
         const int c = tid + i * T;
         if (c < n) {
-            const int t = c / cpt;
-            r[i] = load_raw<DT>(x, (it.row + t) * ts + head * hs + (c - t * cpt) * kChunk);
+            const int t = (c * a.cpt_magic) >> 20;
+            r[i] = load_raw<DT>(x, (it.row + t) * ts + head * hs + (c - t * (int)a.cpt) * kChunk);
         }
     }
+    if (!good_block(a, block)) return;
+    const size_t bh = (size_t)block * a.heads + head;
+    uint8_t* codes = (is_v ? a.v : a.k) + bh * a.bt * a.dim;
+    float* scale = (is_v ? a.v_scale : a.k_scale) + bh;
+    const float old = it.slot ? *scale : 0.f;
+    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < kMaxChunks; ++i)
+    for (int i = 0; i < CH; ++i)
         if (tid + i * T < n) {
             float f[8];
             to_floats<DT>(r[i], f);
@@ -150,26 +171,37 @@ __global__ void kv_write_kernel(const __grid_constant__ KVArgs a) {
         }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-    if ((tid & 31) == 0) red[tid >> 5] = amax;
-    __syncthreads();
-    for (int w = 0; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
+    if constexpr (!WARP) {
+        if ((tid & 31) == 0) red[tid >> 5] = amax;
+        __syncthreads();
+        for (int w = 0; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
+    }
     const float s = fmaxf(fmaxf(__fdiv_rn(amax, kKVQmax<FMT>), kKVScaleFloor), old);
+    if constexpr (WARP) __syncwarp();   // (all lanes have read the old scale)
     if (tid == 0) *scale = s;
 
     if (it.slot && s > old) {   // the earlier tokens' codes, to the grown scale
         const float ratio = __fdiv_rn(old, s);
-        for (int c = tid; c < it.slot * (int)a.dim / 4; c += T) {
-            uint32_t* p = reinterpret_cast<uint32_t*>(codes) + c;
-            float f[4];
-            kv_decode4<FMT>(*p, f);
-            uint32_t o = 0;
+        uint4* p = reinterpret_cast<uint4*>(codes);
+        const int m = it.slot * (int)a.dim / 16;
+#pragma unroll 4
+        for (int c = tid; c < m; c += T) {
+            uint4 w = p[c];
+            uint32_t* v = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o |= kv_code<FMT>(f[e] * ratio) << (8 * e);
-            *p = o;
+            for (int q = 0; q < 4; ++q) {
+                float f[4];
+                kv_decode4<FMT>(v[q], f);
+                uint32_t o = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o |= kv_code<FMT>(f[e] * ratio) << (8 * e);
+                v[q] = o;
+            }
+            p[c] = w;
         }
     }
 #pragma unroll
-    for (int i = 0; i < kMaxChunks; ++i) {
+    for (int i = 0; i < CH; ++i) {
         const int c = tid + i * T;
         if (c < n) {
             float f[8];
@@ -185,57 +217,87 @@ __global__ void kv_write_kernel(const __grid_constant__ KVArgs a) {
     }
 }
 
+constexpr int kReadThreads = 256, kReadUnroll = 4;   // (kReadThreads: also the launch's)
+
 template <int DT, int FMT>
-__global__ void kv_read_kernel(const __grid_constant__ KVArgs a) {
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_constant__ KVArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     Item it;
     if (!find_item(a, blockIdx.x, it)) return;
-    const int head = blockIdx.y >> 1;
+    const int block = *it.block;
+    const int h0 = (blockIdx.y >> 1) * a.cta_heads, h1 = min(h0 + a.cta_heads, a.heads);
     const bool is_v = blockIdx.y & 1;
     void* y = const_cast<void*>(is_v ? a.x_v : a.x_k);
     const uint64_t ts = is_v ? a.tok_v : a.tok_k, hs = is_v ? a.head_v : a.head_k;
-    const size_t bh = (size_t)it.block * a.heads + head;
-    const uint8_t* codes = (is_v ? a.v : a.k) + (bh * a.bt + it.slot) * a.dim;
-    const float s = (is_v ? a.v_scale : a.k_scale)[bh];
-    const int cpt = a.dim / 16, n = it.count * cpt;   // 16 codes at a time
-    for (int c = threadIdx.x; c < n; c += blockDim.x) {
-        const int t = c / cpt;
-        const uint4 w = ld_stream(codes + (size_t)c * 16);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-        const uint64_t e = (it.row + t) * ts + head * hs + (c - t * cpt) * 16;
-        if constexpr (DT == GRAFT_F32) {
-            float4* o = reinterpret_cast<float4*>((float*)y + e);
+    const uint8_t* codes = is_v ? a.v : a.k;
+    const float* scales = is_v ? a.v_scale : a.k_scale;
+    if (!good_block(a, block)) return;
+    const int per = it.count * (int)a.cpt, n = (h1 - h0) * per;   // chunks of 16 codes: a head's, all
+    for (int c0 = threadIdx.x; c0 < n; c0 += kReadThreads * kReadUnroll) {
+        uint4 w[kReadUnroll];
+        float s[kReadUnroll];
+        uint64_t to[kReadUnroll];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float f[4];
-                kv_decode4<FMT>(ws[i], f);
-                o[i] = make_float4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
-            }
-        } else {
-            uint32_t o[8];
+        for (int u = 0; u < kReadUnroll; ++u) {
+            const int c = c0 + u * kReadThreads;
+            if (c >= n) break;
+            const int h = c / per, r = c - h * per, t = (r * a.cpt_magic) >> 20;
+            const size_t bh = (size_t)block * a.heads + h0 + h;
+            w[u] = ld_stream(codes + (bh * a.bt + it.slot) * a.dim + (size_t)r * 16);
+            s[u] = scales[bh];
+            to[u] = (it.row + t) * ts + (h0 + h) * hs + (r - t * (int)a.cpt) * 16;
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float f[4];
-                kv_decode4<FMT>(ws[i], f);
-                o[2 * i] = pack2<DT>(f[0] * s, f[1] * s);
-                o[2 * i + 1] = pack2<DT>(f[2] * s, f[3] * s);
+        for (int u = 0; u < kReadUnroll; ++u) {
+            if (c0 + u * kReadThreads >= n) break;
+            const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            if constexpr (DT == GRAFT_F32) {
+                float4* o = reinterpret_cast<float4*>((float*)y + to[u]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f[4];
+                    kv_decode4<FMT>(ws[i], f);
+                    o[i] = make_float4(f[0] * s[u], f[1] * s[u], f[2] * s[u], f[3] * s[u]);
+                }
+            } else {
+                uint32_t o[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f[4];
+                    kv_decode4<FMT>(ws[i], f);
+                    o[2 * i] = pack2<DT>(f[0] * s[u], f[1] * s[u]);
+                    o[2 * i + 1] = pack2<DT>(f[2] * s[u], f[3] * s[u]);
+                }
+                uint4* p = reinterpret_cast<uint4*>((uint16_t*)y + to[u]);
+                if (a.wide) {   // whole 32-byte sectors
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
+                                 "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]),
+                                 "r"(o[6]), "r"(o[7])
+                                 : "memory");
+                } else {
+                    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                }
             }
-            uint4* p = reinterpret_cast<uint4*>((uint16_t*)y + e);
-            p[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            p[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
     }
 }
 
 using KVKernel = void (*)(const KVArgs);
+enum Form { kRead, kWriteOne, kWriteWarp, kWriteCta };   // kWriteOne: a chunk a lane
+template <int DT, int FMT>
+KVKernel pick(Form form, int chunks) {
+    return form == kRead       ? kv_read_kernel<DT, FMT>
+           : form == kWriteOne ? kv_write_kernel<DT, FMT, 1, true>
+           : form == kWriteWarp ? kv_write_kernel<DT, FMT, 8, true>
+           : chunks <= 4       ? kv_write_kernel<DT, FMT, 4, false>
+                               : kv_write_kernel<DT, FMT, 8, false>;
+}
 template <int DT>
-KVKernel pick(bool write, uint32_t fmt) {
-    if (write)
-        return fmt == GRAFT_KV_INT8 ? kv_write_kernel<DT, GRAFT_KV_INT8>
-                                    : kv_write_kernel<DT, GRAFT_KV_E4M3>;
-    return fmt == GRAFT_KV_INT8 ? kv_read_kernel<DT, GRAFT_KV_INT8>
-                                : kv_read_kernel<DT, GRAFT_KV_E4M3>;
+KVKernel pick(Form form, int chunks, uint32_t fmt) {
+    return fmt == GRAFT_KV_INT8 ? pick<DT, GRAFT_KV_INT8>(form, chunks)
+                                : pick<DT, GRAFT_KV_E4M3>(form, chunks);
 }
 
 int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
@@ -258,17 +320,30 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     a.n_blocks = cache->n_blocks, a.heads = cache->kv_heads, a.bt = cache->block_tokens;
     a.dim = cache->head_dim, a.n_seqs = range->n_seqs, a.table_stride = range->table_stride;
     a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = K->tokens;
+    const uint64_t bits = ((uint64_t)(uintptr_t)K->data | (uintptr_t)V->data |
+                           2 * (K->token_stride | K->head_stride | V->token_stride | V->head_stride));
+    a.wide = bits % 32 == 0;
     const uint64_t items = (uint64_t)K->tokens / a.bt + 2ull * a.n_seqs;
     GRAFT_REQUIRE(items < (1ull << 31), "too many tokens in one call");
-    // 4 chunks of 8 elements a thread, up to 512 threads (then 8 chunks)
-    const int chunks = (int)(a.bt * a.dim) / (write ? kChunk : 16);
-    int threads = (chunks / 4 + 31) / 32 * 32;
-    threads = threads < 64 ? 64 : threads > 512 ? 512 : threads;
-    const KVKernel kern = K->dtype == GRAFT_F16    ? pick<GRAFT_F16>(write, cache->format)
-                          : K->dtype == GRAFT_BF16 ? pick<GRAFT_BF16>(write, cache->format)
-                                                   : pick<GRAFT_F32>(write, cache->format);
+    a.bt_log2 = a.bt == 16 ? 4 : a.bt == 32 ? 5 : a.bt == 64 ? 6 : 7;
+    a.cpt = a.dim / (write ? kChunk : 16);
+    a.cpt_magic = ((1u << 20) + a.cpt - 1) / a.cpt;
+    a.cta_heads = std::min(a.heads, std::max(1u, 32768u / (a.bt * a.dim)));
+    // Writing, a CTA a (head, K or V): 4 chunks of 8 elements a thread, up to 512 threads (then
+    // 8 chunks).  Short items (decode steps) take a warp each, eight to a CTA: a step of 64
+    // sequences with one CTA each spent 10 us on launching and emptying 2080 CTAs.
+    const uint32_t most = std::min(range->max_tokens, a.bt) * a.cpt;   // chunks of an item
+    const Form form = !write ? kRead : most <= 32 ? kWriteOne : most <= kWarpChunks ? kWriteWarp : kWriteCta;
+    int threads = ((int)(a.bt * a.cpt) / 4 + 31) / 32 * 32;
+    threads = form != kWriteCta ? 256 : threads < 64 ? 64 : threads > 512 ? 512 : threads;
+    const int chunks = (int)(a.bt * a.cpt + threads - 1) / threads;
+    const uint32_t ny = form == kRead      ? 2 * ((a.heads + a.cta_heads - 1) / a.cta_heads)
+                        : form == kWriteCta ? 2 * a.heads : (2 * a.heads + 7) / 8;
+    const KVKernel kern = K->dtype == GRAFT_F16    ? pick<GRAFT_F16>(form, chunks, cache->format)
+                          : K->dtype == GRAFT_BF16 ? pick<GRAFT_BF16>(form, chunks, cache->format)
+                                                   : pick<GRAFT_F32>(form, chunks, cache->format);
     return launch_pdl(write ? "kv_write" : "kv_read", kern,
-                      dim3((unsigned)items, 2 * a.heads), threads, 0, st, a);
+                      dim3((unsigned)items, ny), threads, 0, st, a);
 }
 
 }  // namespace
