@@ -9,6 +9,9 @@ the counterpart of the reference harness binaries' flags (int4gemv --M --K --G
     python -m kernels_b200.run batch --M 128256 --K 4096 --B 8 [--tcgen05]
     python -m kernels_b200.run vqquant --M 4096 --K 4096
     python -m kernels_b200.run expert [--copies 4]     # one gpt-oss expert (bf16 format)
+    python -m kernels_b200.run attn [--ctx 131071] [--B 1] [--new 1] [--heads 64,8,64] [--e4m3]
+    python -m kernels_b200.run kvwrite|kvread [--ctx 65536] [--heads 64,8,64] [--e4m3]
+    python -m kernels_b200.run logprobs [--B 1] [--M 201088] [--top-k 20]   # B rows of M logits
 
 Each iteration is one launch on a rotating weight copy, timed with CUDA events;
 use it for small profiler captures (a few launches, a few GB).  --graph N
@@ -25,7 +28,7 @@ import json
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["int4", "vq", "moe", "stream", "batch", "vqquant",
-                                       "expert"])
+                                       "expert", "attn", "kvwrite", "kvread", "logprobs"])
     ap.add_argument("--M", type=int, default=4096)
     ap.add_argument("--K", type=int, default=4096)
     ap.add_argument("--G", type=int, default=64)
@@ -35,6 +38,12 @@ def main() -> None:
     ap.add_argument("--top-k", type=int, default=4)
     ap.add_argument("--mbytes", type=int, default=1024)
     ap.add_argument("--B", type=int, default=8, help="batch: tokens per call")
+    ap.add_argument("--ctx", type=int, default=131071, help="attn, kv*: tokens in the cache")
+    ap.add_argument("--new", type=int, default=1, help="attn: new tokens of each of B sequences")
+    ap.add_argument("--heads", default="64,8,64", help="attn, kv*: query heads, kv heads, head_dim")
+    ap.add_argument("--block", type=int, default=64, help="attn, kv*: tokens of a cache block")
+    ap.add_argument("--window", type=int, default=0, help="attn: sliding window")
+    ap.add_argument("--e4m3", action="store_true", help="attn, kv*: 8-bit floats instead of int8")
     ap.add_argument("--f32out", action="store_true")
     ap.add_argument("--s32", action="store_true", help="vq: per-32 scales (the reference's form)")
     ap.add_argument("--tcgen05", action="store_true",
@@ -110,6 +119,46 @@ def main() -> None:
         nbytes = a.top_k * 3 * (2880 * 1440 + 2 * 2 * 2880 * 45) + a.experts * 2880 * 2 + 6 * 2880 \
             + 4 * a.top_k * 2880
         f = lambda i: kb.moe_block_ex(pool, R, xs_[i % 8], y, P, fmt, wsp)  # noqa
+    elif a.kernel in ("attn", "kvwrite", "kvread"):
+        Hq, H, D = (int(x) for x in a.heads.split(","))
+        B = a.B if a.kernel == "attn" else 1
+        per = -(-a.ctx // a.block)
+        g = torch.Generator(device="cuda").manual_seed(0)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        table = torch.randperm(B * per, device="cuda", generator=g).to(torch.int32).view(B, per)
+        cache = kb.KVCache.empty(B * per, H, D, a.block,
+                                 torch.float8_e4m3fn if a.e4m3 else torch.int8)
+        x = torch.randn(a.ctx, H, D, device="cuda", generator=g).half()
+        for b in range(B):
+            whole = kb.kv_range(table[b:b + 1], torch.zeros(1, **i32),
+                                torch.tensor([0, a.ctx], **i32), a.ctx, a.ctx)
+            kb.kv_write(cache, x, x, whole)
+        if a.kernel == "attn":
+            rng = kb.kv_range(table, torch.full((B,), a.ctx - a.new, **i32),
+                              torch.arange(B + 1, **i32) * a.new, a.new, a.ctx)
+            P = kb.attn_params(Hq, torch.float16, scale=D ** -0.5, window=a.window)
+            wsa = kb.AttnWorkspace(cache, rng, P)
+            q = torch.randn(B * a.new, Hq, D, device="cuda", generator=g).half()
+            o = torch.empty_like(q)
+            nbytes = 2 * B * (min(a.ctx, a.window + a.new) if a.window else a.ctx) * H * D
+            f = lambda i: kb.attn_kv8(cache, q, o, rng, P, wsa)  # noqa
+        elif a.kernel == "kvwrite":
+            nbytes = 6 * a.ctx * H * D
+            f = lambda i: kb.kv_write(cache, x, x, whole)  # noqa
+        else:
+            k, v = torch.empty_like(x), torch.empty_like(x)
+            nbytes = 6 * a.ctx * H * D
+            f = lambda i: kb.kv_read(cache, k, v, whole)  # noqa
+    elif a.kernel == "logprobs":
+        z = [torch.randn(a.B, a.M, device="cuda").mul_(3).half() for _ in range(a.copies)]
+        P = kb.logprob_params(a.B, a.M, a.top_k, torch.float16)
+        wsl = kb.LogprobWorkspace(P)
+        t = torch.zeros(a.B, dtype=torch.int32, device="cuda")
+        o = (torch.empty(a.B, device="cuda"), torch.empty(a.B, device="cuda"),
+             torch.empty(a.B, a.top_k, device="cuda"),
+             torch.empty(a.B, a.top_k, dtype=torch.int32, device="cuda"))
+        nbytes = 2 * a.B * a.M
+        f = lambda i: kb.logprobs(z[i % a.copies], t, *o, P, wsl)  # noqa
     else:
         n = a.mbytes << 20
         bufs = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in range(a.copies)]
