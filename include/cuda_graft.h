@@ -486,7 +486,8 @@ int graft_moe_block_ep(graft_comm_t comm, const void* pool, const void* R, const
  *   codes  [n_blocks][kv_heads][block_tokens][head_dim]  (one byte each)
  *   scales [n_blocks][kv_heads]                          value = code * scale
  * Codes are signed integers in [-127, 127] (GRAFT_KV_INT8) or 8-bit floats
- * with 4 exponent and 3 mantissa bits, largest value 448 (GRAFT_KV_E4M3).
+ * with 4 exponent and 3 mantissa bits, largest value 448 (GRAFT_KV_E4M3);
+ * scales are not negative (one below 2^-64 counts as 2^-64 for values).
  * Constraints: block_tokens 16, 32, 64 or 128; head_dim a multiple of 16, at
  * most 256; code pointers 16-byte aligned, scale pointers 4-byte aligned. */
 enum { GRAFT_KV_INT8 = 0, GRAFT_KV_E4M3 = 1 };
@@ -556,7 +557,8 @@ int graft_kv_device_errors(uint32_t* bits, int clear);
 
 /* ------------------------------------------------- attention over the cache */
 typedef struct {
-    uint32_t q_heads;   /* a multiple of kv_heads: q head h reads kv head h / (q_heads/kv_heads) */
+    uint32_t q_heads;   /* a multiple of kv_heads: q head h reads kv head h / (q_heads/kv_heads);
+                           at most 256 times kv_heads (128 times above head_dim 128)  */
     uint32_t window;    /* keys a query sees, itself included; 0 = all        */
     float scale;        /* of the scores, e.g. 1/sqrt(head_dim); finite       */
 } GraftAttnParams;
@@ -568,8 +570,11 @@ typedef struct {
  *   lse = log( sum_j exp(scale q.k_j)  [+ exp(sinks[h])] ).
  * q and out: GRAFT_F16 or GRAFT_BF16, the same type.  sinks (fp32 [q_heads], a
  * score that takes weight but has no value) and lse (fp32 [tokens][q_heads])
- * may be null.  ws: graft_attn_kv8_workspace bytes, 256-byte aligned, zeroed
- * once by graft_attn_kv8_init and then kept for calls of one stream at a
+ * may be null.  Few rows a key/value head (max_tokens * q_heads/kv_heads up to
+ * 32, 16 or 8 for head_dim up to 64, 128 or 256) take one pass over the keys at
+ * the rate of HBM; more take tcgen05 tiles of 256 rows.  ws:
+ * graft_attn_kv8_workspace bytes, 256-byte aligned, zeroed once by
+ * graft_attn_kv8_init; it serves any call that it is large enough for, one at a
  * time. */
 size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const GraftKVRange* range,
                                 const GraftAttnParams* P);
@@ -594,7 +599,7 @@ typedef struct {
     uint32_t top_k;      /* 0 .. 32                                           */
     uint32_t dtype;      /* of the logits: GRAFT_F16, GRAFT_BF16 or GRAFT_F32 */
     uint64_t row_stride; /* elements from row to row (>= vocab, any value)    */
-    float scale;         /* 1/temperature, > 0                                */
+    float scale;         /* 1/temperature, 2^-100 to 2^100                    */
 } GraftLogprobParams;
 
 /* logits aligned to its element; targets (int32 [rows]) and logprob may both be
