@@ -125,9 +125,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         }
         U *= H, pairs *= H;
         if (U == 0) return;
-        const int G = min((int)gridDim.x, max(pairs, (U - pairs * a.pad_units) / a.min_units));
+        // (more than pairs, while shares stay above a pad and a unit: few CTAs get two pairs)
+        const int G = min((int)gridDim.x, max(max(pairs, (U - pairs * a.pad_units) / a.min_units),
+                                              min(2 * pairs, U / (a.pad_units + 1))));
         if ((int)blockIdx.x >= G) return;
-        sp.set(U, G, a.pad_units, max(1, a.min_units / 2));
+        sp.set(U, G, a.pad_units, a.min_units);
         const int x0 = sp.bound(blockIdx.x), x1 = sp.bound(blockIdx.x + 1);
         int base = 0;
         for (uint32_t b0 = 0; b0 < a.n_seqs; b0 += kFewThreads) {

@@ -35,7 +35,7 @@ constexpr int kMaxTop = 32, kMaxSegs = 32;
 constexpr int kCap = 2048;           // collected keys; more are selected from the logits one by one
 constexpr int kMinSeg = 4096;        // elements of a segment, at least
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 8 x 2)
+constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 16)
 constexpr size_t kCounterBytes = (kRounds * 4 + 255) / 256 * 256;   // a row is cut only if rows < kRounds
 constexpr uint64_t kNoKey = 0;       // below every key of a logit that is not -inf
 
@@ -317,7 +317,7 @@ __device__ __forceinline__ float chunk_max(const uint4& v) {
     }
 }
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const __grid_constant__ LpArgs a) {
+__global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_constant__ LpArgs a) {
     constexpr int N = kPer<DT>, UN = 4;   // elements of a chunk, chunks in flight
     __shared__ Shared sh;
     pdl_wait();
