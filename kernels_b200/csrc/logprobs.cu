@@ -12,13 +12,14 @@
 // and HBM bounds a long call (one exponential an element keeps the MUFU at about
 // 70% at that rate for 16-bit logits).
 //
-// The top k come from the threads' own maxima, which the pass finds on the
-// way: the k-th largest of the warps' eight best each bounds the k-th largest logit
-// from below, so only threads whose maximum reaches it can hold one of the top
-// k.  Their chunks (little more than k / 128 of the segment) are read again, from
-// L2, and what reaches the bound is collected and ranked.  Ties go to the lowest
-// index: keys are (value, chunk or index) pairs, all different.  Segments meet in the workspace, and a
-// row's last CTA joins them.
+// The top k come from the threads' own maxima, which the pass finds on the way: each
+// thread keeps its largest logit, the round of chunks where that is first, and the
+// largest of its other rounds.  A row's last CTA takes every thread's largest over the
+// segments; the k-th largest of these bounds the k-th largest logit from below, so only
+// rounds that reach it can hold one of the top k.  Those (little more than k) are read
+// again, and what reaches the bound is collected and ranked.  Ties go to the lowest
+// index: keys are (value, index) pairs, all different.  Segments meet in the workspace,
+// and the row's last CTA joins them.
 #include "kv_common.cuh"
 
 #include <algorithm>
@@ -30,18 +31,24 @@ using namespace graft::dev;
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kBest = 32 / kWarps;   // of each warp's thread maxima
 constexpr int kMaxTop = 32, kMaxSegs = 32;
-constexpr int kCap = 2048;           // collected keys; more are selected from the logits one by one
+constexpr int kUnroll = 4;           // chunks of a thread's round
+constexpr int kCap = 2048;           // keys that are collected at most
+constexpr int kList = 1024;          // chunks that are read again at most
 constexpr int kMinSeg = 4096;        // elements of a segment, at least
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 16)
 constexpr size_t kCounterBytes = (kRounds * 4 + 255) / 256 * 256;   // a row is cut only if rows < kRounds
 constexpr uint64_t kNoKey = 0;       // below every key of a logit that is not -inf
 
+struct Seen {                        // of a thread: besides its largest logit
+    int chunk;                       // the first chunk of the first round with it
+    uint32_t other;                  // largest of its other rounds, as order()
+};
 struct Partial {                     // of a segment
     float ref, L, E, pad;
-    uint64_t key[kMaxTop];
+    uint32_t value[kThreads];        // the threads' largest logits as order() (0: none), if k
+    Seen seen[kThreads];
 };
 
 struct LpArgs {
@@ -88,14 +95,10 @@ __device__ __forceinline__ float logit(const void* row, uint32_t i) {
 template <int DT>
 constexpr int kPer = DT == GRAFT_F32 ? 4 : 8;   // elements of a chunk
 
-// Chunk c of a row whose first element is `off` elements into the row's first
-// 16-byte chunk; elements outside the row are -inf and are not read.
+// A chunk that begins `first` elements into a row and lies partly outside it; elements
+// outside are -inf and are not read.
 template <int DT>
-__device__ __forceinline__ uint4 load_chunk(const void* row, int off, uint32_t vocab, int c) {
-    constexpr int N = kPer<DT>;
-    const int first = c * N - off;
-    if (first >= 0 && first + N <= (int)vocab)
-        return ld_stream((const char*)row + (int64_t)first * (16 / N));
+__device__ __noinline__ uint4 edge_chunk(const void* row, int first, uint32_t vocab) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -110,6 +113,15 @@ __device__ __forceinline__ uint4 load_chunk(const void* row, int off, uint32_t v
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Chunk c of a row whose first element is `off` elements into the row's first 16-byte chunk.
+template <int DT>
+__device__ __forceinline__ uint4 load_chunk(const void* row, int off, uint32_t vocab, int c) {
+    constexpr int N = kPer<DT>;
+    const int first = c * N - off;
+    if (first >= 0 && first + N <= (int)vocab)
+        return ld_stream((const char*)row + (int64_t)first * (16 / N));
+    return edge_chunk<DT>(row, first, vocab);
 }
 template <int DT>
 __device__ __forceinline__ void floats_of(const uint4& v, float (&x)[kPer<DT>]) {
@@ -158,15 +170,19 @@ __device__ __forceinline__ void join(float& ref, float& L, float& E, float r2, f
 
 struct Shared {
     float ref[kWarps], L[kWarps], E[kWarps];
-    uint64_t key[kCap];
+    union {
+        uint64_t key[kCap];
+        uint32_t value[kMaxSegs][kThreads];   // the threads' maxima, before keys are collected
+    };
     uint64_t best[kMaxTop];
-    uint64_t top[32];   // the warps' best thread maxima
     uint64_t red[kWarps];
-    int list[kThreads];
+    uint32_t most[kThreads];   // the threads' maxima over the segments
+    int list[kList];           // chunks
     int n, listed, last;
 };
+static_assert(kMaxSegs * kThreads * 4 <= kCap * 8, "the maxima fit where the keys go");
 
-__device__ __forceinline__ uint64_t block_max(Shared& sh, uint64_t v) {
+__device__ __noinline__ uint64_t block_max(Shared& sh, uint64_t v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const uint64_t w = __shfl_xor_sync(~0u, v, o);
@@ -208,88 +224,165 @@ __device__ __forceinline__ void rank_keys(Shared& sh, int n, int k) {
     __syncthreads();
 }
 
+// A row and its cut.
+struct Row {
+    const char* base;
+    int off;          // elements between a 16-byte boundary and the row
+    uint32_t vocab;
+    int chunks, per_seg, segs;
+};
+
 // A segment's chunks: those wholly in the row are [i0, i1), chunk i0 + t + j*kThreads
 // is thread t's j-th; a row's first chunk belongs to thread 0 and its last to
 // thread 1 where they lie partly outside (first, last: -1 if not).
 struct Span {
     int i0, i1, first, last;
 };
+template <int N>
+__device__ __forceinline__ Span span_of(const Row& w, int seg) {
+    const int c0 = min(seg * w.per_seg, w.chunks), c1 = min(c0 + w.per_seg, w.chunks);
+    Span sp;
+    sp.first = c0 == 0 && c1 > 0 && (w.off || (int)w.vocab < N) ? 0 : -1;
+    sp.last = c1 == w.chunks && c1 - 1 > sp.first && c1 > c0 && (w.off + w.vocab) % N ? c1 - 1 : -1;
+    sp.i0 = c0 + (sp.first >= 0), sp.i1 = c1 - (sp.last >= 0);
+    return sp;
+}
 
-// The top k keys of the segment into sh.best.  tmax, tchunk: the thread's largest
-// logit (-inf: none) and the first chunk that holds it.
+__device__ __forceinline__ uint32_t order_or_none(float x) { return x > -INFINITY ? order(x) : 0; }
+
+// The top k keys of a row into sh.best.  own, seen: the thread's largest logit and where it
+// is, if the row has one segment; else they stand in `parts`.
 template <int DT>
-__device__ __forceinline__ void select_top(Shared& sh, const void* row, int off, uint32_t vocab,
-                                           const Span& sp, float tmax, int tchunk, int k) {
+__device__ __forceinline__ void select_top(Shared& sh, const Row& w, const Partial* parts,
+                                           uint32_t own, Seen seen, int k) {
     constexpr int N = kPer<DT>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // ---- the best of each warp
-    const uint32_t mine = tmax > -INFINITY ? order(tmax) : 0;
-    const uint32_t inv = 0xFFFFFFFFu - (uint32_t)tchunk;
-    uint32_t left = mine;
-#pragma unroll
-    for (int r = 0; r < kBest; ++r) {
-        const uint32_t v = __reduce_max_sync(~0u, left);
-        const uint32_t c = __reduce_max_sync(~0u, left == v ? inv : 0u);
-        if (lane == 0) sh.top[warp * kBest + r] = v ? ((uint64_t)v << 32) | c : kNoKey;
-        if (left == v && inv == c) left = 0;
+    // ---- each thread's largest over the segments
+    if (parts) {
+        for (int i = tid; i < w.segs * (kThreads / 4); i += kThreads)
+            cp_async16(smem_u32(&sh.value[i / (kThreads / 4)][i % (kThreads / 4) * 4]),
+                       &parts[i / (kThreads / 4)].value[i % (kThreads / 4) * 4]);
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        own = 0;
+#pragma unroll 4
+        for (int s = 0; s < w.segs; ++s) own = max(own, sh.value[s][tid]);
     }
+    sh.most[tid] = own;
+    __syncthreads();
+    // ---- the k-th largest of these: the bound (1 if there are fewer: whatever is not -inf)
+    int above[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int j = 0; j < kThreads; j += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(&sh.most[j]);
+        above[0] += v.x > own, above[1] += v.y > own, above[2] += v.z > own, above[3] += v.w > own;
+    }
+    const bool high = above[0] + above[1] + above[2] + above[3] < k;
+    const uint32_t low = __reduce_min_sync(~0u, high ? own : 0xFFFFFFFFu);
+    if (lane == 0) sh.red[warp] = low;
     if (tid == 0) sh.n = sh.listed = 0;
     __syncthreads();
-    // ---- the k-th largest of them (every warp for itself): the bound
-    // (keys are all different but for the empty ones, which come last)
-    const uint64_t own = sh.top[lane];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) rank += sh.top[j] > own;
-    const uint32_t at = __ballot_sync(~0u, rank == k - 1 && own != kNoKey);
-    uint64_t bound = __shfl_sync(~0u, own, at ? __ffs(at) - 1 : 0);
-    if (!at) bound = 1ull << 32;   // fewer than k: whatever is not -inf
-    if (mine && (((uint64_t)mine << 32) | inv) >= bound) sh.list[atomicAdd(&sh.listed, 1)] = tid;
-    __syncthreads();
-    // ---- what reaches the bound in those threads' chunks
-    const uint32_t bv = (uint32_t)(bound >> 32);
-    const int bc = (int)(0xFFFFFFFFu - (uint32_t)bound);   // (negative: any chunk)
-    const int listed = sh.listed, per = (max(sp.i1 - sp.i0, 0) + kThreads - 1) / kThreads + 1;
-    auto chunk_of = [&](int i) {   // the i-th to look at, -1: none
-        const int q = i / per, j = i - q * per, t = sh.list[q];
-        if (j == per - 1) return t == 0 ? sp.first : t == 1 ? sp.last : -1;
-        const int c = sp.i0 + t + j * kThreads;
-        return c < sp.i1 ? c : -1;
+    uint32_t bound = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) bound = min(bound, (uint32_t)sh.red[i]);
+    bound = max(bound, 1u);
+
+    // ---- the keys of at least `least`, from the rounds that hold such (false: too many)
+    auto list = [&](int s, Seen at, uint32_t least) {
+        const Span sp = span_of<N>(w, s);
+        const bool all = at.other >= least, edge = at.chunk < sp.i0 || at.chunk >= sp.i1;
+        const int i0 = all ? sp.i0 + tid : at.chunk;
+        const int i1 = all ? sp.i1 : edge ? at.chunk + 1 : min(at.chunk + kUnroll * kThreads, sp.i1);
+        const int more = all ? (tid == 0 ? sp.first : tid == 1 ? sp.last : -1) : -1;
+        const int count = (max(i1 - i0, 0) + kThreads - 1) / kThreads + (more >= 0);
+        int to = atomicAdd(&sh.listed, count);
+        if (to + count > kList) return;
+        for (int c = i0; c < i1; c += kThreads) sh.list[to++] = c;
+        if (more >= 0) sh.list[to] = more;
     };
-    for (int i = tid; i < listed * per; i += kThreads) {
-        const int c = chunk_of(i);
-        if (c < 0) continue;
+    auto collect = [&](int c, uint32_t least, uint32_t most) {
         float x[N];
-        floats_of<DT>(load_chunk<DT>(row, off, vocab, c), x);
+        floats_of<DT>(load_chunk<DT>(w.base, w.off, w.vocab, c), x);
+        uint32_t hits = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t o = x[e] > -INFINITY ? order(x[e]) : 0;
-            if (o > bv || (o == bv && (uint32_t)c <= (uint32_t)bc)) {
-                const int to = atomicAdd(&sh.n, 1);
-                if (to < kCap) sh.key[to] = key_of(x[e], c * N - off + e);
+            const uint32_t o = order_or_none(x[e]);
+            hits |= (uint32_t)(o >= least && o <= most) << e;
+        }
+        if (!hits) return;
+        int to = atomicAdd(&sh.n, __popc(hits));
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (hits >> e & 1) {
+                if (to < kCap) sh.key[to] = key_of(x[e], c * N - w.off + e);
+                ++to;
             }
+    };
+    bool done = false;
+    uint32_t least = bound;
+#pragma unroll 1
+    for (int pass = 0; pass < 2 && !done; ++pass, ++least) {
+        // (many equal to the bound, in a row of which all but a few tokens have one lowest
+        // value, say, are passed over by the second pass: those above it)
+        if (pass) {
+            __syncthreads();
+            if (tid == 0) sh.n = sh.listed = 0;
+            __syncthreads();
+        }
+        if (own >= least) {
+            uint32_t segs = 1;
+            if (parts) {
+                segs = 0;
+                if (pass == 0) {
+#pragma unroll 4
+                    for (int s = 0; s < w.segs; ++s) segs |= (uint32_t)(sh.value[s][tid] >= least) << s;
+                } else {   // (keys lie there now)
+#pragma unroll 4
+                    for (int s = 0; s < w.segs; ++s)
+                        segs |= (uint32_t)(__ldcg(&parts[s].value[tid]) >= least) << s;
+                }
+            }
+            for (; segs; segs &= segs - 1) {
+                const int s = __ffs(segs) - 1;
+                if (parts) {
+                    const uint2 v = __ldcg(reinterpret_cast<const uint2*>(&parts[s].seen[tid]));
+                    seen = Seen{(int)v.x, v.y};
+                }
+                list(s, seen, least);
+            }
+        }
+        __syncthreads();
+        if (sh.listed > kList) continue;
+        for (int i = tid; i < sh.listed; i += kThreads) collect(sh.list[i], least, ~0u);
+        __syncthreads();
+        done = sh.n <= (pass ? kCap - kThreads * N : kCap);
+    }
+    if (done && least > bound + 1) {   // .. and the first of the equal ones in their order
+        const int want = sh.n + k;
+        for (int c = 0; c < w.chunks && sh.n < want; c += kThreads) {
+            __syncthreads();   // (sh.n has been read)
+            if (c + tid < w.chunks) collect(c + tid, bound, bound);
+            __syncthreads();
         }
     }
     __syncthreads();
-    const int n = sh.n;
-    if (n <= kCap) {
-        rank_keys(sh, n, k);
+    if (done) {
+        rank_keys(sh, sh.n, k);
         return;
     }
-    // ---- too many (a few threads hold most of the large logits): one by one
+    // ---- a few threads hold most of the large logits: one by one
     uint64_t before = ~0ull;
     for (int r = 0; r < k; ++r) {
         uint64_t v = kNoKey;
-        for (int i = tid; i < listed * per; i += kThreads) {
-            const int c = chunk_of(i);
-            if (c < 0) continue;
+        for (int c = tid; c < w.chunks; c += kThreads) {
             float x[N];
-            floats_of<DT>(load_chunk<DT>(row, off, vocab, c), x);
+            floats_of<DT>(load_chunk<DT>(w.base, w.off, w.vocab, c), x);
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 if (x[e] > -INFINITY) {
-                    const uint64_t w = key_of(x[e], c * N - off + e);
-                    if (w < before && w > v) v = w;
+                    const uint64_t y = key_of(x[e], c * N - w.off + e);
+                    if (y < before && y > v) v = y;
                 }
         }
         before = block_max(sh, v);
@@ -318,7 +411,7 @@ __device__ __forceinline__ float chunk_max(const uint4& v) {
 }
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_constant__ LpArgs a) {
-    constexpr int N = kPer<DT>, UN = 4;   // elements of a chunk, chunks in flight
+    constexpr int N = kPer<DT>, UN = kUnroll;
     __shared__ Shared sh;
     pdl_wait();
     pdl_launch_dependents();
@@ -328,43 +421,35 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
     const char* base = (const char*)a.logits + (uint64_t)row * a.row_stride * (16 / N);
     const int off = (int)(((uintptr_t)base & 15) / (16 / N));
     const int chunks = (int)(((uint64_t)off + a.vocab + N - 1) / N);
-    const int per_seg = (chunks + a.segs - 1) / a.segs;
-    const int c0 = min(seg * per_seg, chunks), c1 = min(c0 + per_seg, chunks);
-    Span sp;
-    sp.first = c0 == 0 && c1 > 0 && (off || (int)a.vocab < N) ? 0 : -1;
-    sp.last = c1 == chunks && c1 - 1 > sp.first && c1 > c0 && (off + a.vocab) % N ? c1 - 1 : -1;
-    sp.i0 = c0 + (sp.first >= 0), sp.i1 = c1 - (sp.last >= 0);
+    const Row w{base, off, a.vocab, chunks, (chunks + a.segs - 1) / a.segs, a.segs};
+    const Span sp = span_of<N>(w, seg);
     const float c = a.scale * kLog2e, reach = 64.f / c;
 
     // ---- the pass: sums against the thread's reference, its maximum and where that is first
-    float ref = 0.f, lim = -INFINITY, tmax = -INFINITY;
+    float ref = 0.f, lim = -INFINITY, tmax = -INFINITY, other = -INFINITY;
     float L2[2] = {0.f, 0.f}, E2[2] = {0.f, 0.f};   // two partial sums each
-    int tchunk = 0;
-    auto take = [&](const auto& v, int ch) {   // chunks ch, ch + kThreads, ..
-        constexpr int U = sizeof(v) / sizeof(uint4);
-        float cm[U], gm;
+    int round = 0;
+    auto take = [&](const uint4 (&v)[UN], int ch) {   // chunks ch, ch + kThreads, ..
+        float gm;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            cm[u] = chunk_max<DT>(v[u]);
-            gm = u ? fmaxf(gm, cm[u]) : cm[u];
+        for (int u = 0; u < UN; ++u) {
+            const float m = chunk_max<DT>(v[u]);
+            gm = u ? fmaxf(gm, m) : m;
         }
-        if (gm > tmax) {   // (lim is never below tmax)
-            tmax = gm;
+        other = fmaxf(other, fminf(gm, tmax));
+        round = gm > tmax ? ch : round;
+        tmax = fmaxf(tmax, gm);
+        if (gm > lim) {
+            if (lim > -INFINITY) {
+                const float a = (ref - gm) * c, f = ex2(a), b = max_nan(a, -256.f);
 #pragma unroll
-            for (int u = U - 1; u >= 0; --u)
-                if (cm[u] == gm) tchunk = ch + u * kThreads;
-            if (gm > lim) {
-                if (lim > -INFINITY) {
-                    const float a = (ref - gm) * c, f = ex2(a), b = max_nan(a, -256.f);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) E2[i] = f * fmaf(L2[i], b, E2[i]), L2[i] *= f;
-                }
-                ref = gm;
-                lim = gm + reach;
+                for (int i = 0; i < 2; ++i) E2[i] = f * fmaf(L2[i], b, E2[i]), L2[i] *= f;
             }
+            ref = gm;
+            lim = gm + reach;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < UN; ++u) {
             const uint32_t w4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
@@ -382,31 +467,32 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
             }
         }
     };
-    auto take_edge = [&](int ch) {
-        const uint4 v[1] = {load_chunk<DT>(base, off, a.vocab, ch)};
-        take(v, ch);
-    };
-    {
-        int ch = sp.i0 + tid;
-        const char* at = base + ((int64_t)ch * N - off) * (16 / N);
-        if (tid == 0 && sp.first >= 0) take_edge(sp.first);   // (each thread's chunks in rising order)
+    int ch = sp.i0 + tid;
+    const char* from = base + ((int64_t)ch * N - off) * (16 / N);
 #pragma unroll 1
-        for (; ch + (UN - 1) * kThreads < sp.i1; ch += UN * kThreads, at += UN * kThreads * 16) {
-            uint4 v[UN];
+    for (; ch + (UN - 1) * kThreads < sp.i1; ch += UN * kThreads, from += UN * kThreads * 16) {
+        uint4 v[UN];
 #pragma unroll
-            for (int u = 0; u < UN; ++u) v[u] = ld_stream(at + u * kThreads * 16);
-            take(v, ch);
-        }
-        if (ch < sp.i1) {   // what is left, as one more round with empty chunks
-            constexpr uint32_t none = DT == GRAFT_F32 ? 0xFF800000u : DT == GRAFT_F16 ? 0xFC00FC00u : 0xFF80FF80u;
-            uint4 v[UN];
+        for (int u = 0; u < UN; ++u) v[u] = ld_stream(from + u * kThreads * 16);
+        take(v, ch);
+    }
+    // what is left, and the row's edge, as rounds with empty chunks
+    const int edge = tid == 0 ? sp.first : tid == 1 ? sp.last : -1;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        if (part ? edge < 0 : ch >= sp.i1) continue;
+        constexpr uint32_t none = DT == GRAFT_F32 ? 0xFF800000u : DT == GRAFT_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+        uint4 v[UN];
 #pragma unroll
-            for (int u = 0; u < UN; ++u)
-                v[u] = ch + u * kThreads < sp.i1 ? ld_stream(at + u * kThreads * 16)
-                                                 : make_uint4(none, none, none, none);
-            take(v, ch);
+        for (int u = 0; u < UN; ++u) {
+            v[u] = make_uint4(none, none, none, none);
+            if (part) {
+                if (u == 0) v[u] = load_chunk<DT>(base, off, a.vocab, edge);
+            } else if (ch + u * kThreads < sp.i1) {
+                v[u] = ld_stream(from + u * kThreads * 16);
+            }
         }
-        if (tid == 1 && sp.last >= 0) take_edge(sp.last);
+        take(v, part ? edge : ch);
     }
 
     // ---- the CTA's sums: against the warp's largest reference, then the warps'
@@ -427,8 +513,7 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
         }
     }
     if (lane == 0) sh.ref[warp] = r, sh.L[warp] = L, sh.E[warp] = E;
-    if (k) select_top<DT>(sh, base, off, a.vocab, sp, tmax, tchunk, k);
-    else __syncthreads();
+    __syncthreads();
     if (warp == 0) {   // (the others' stay their own: the first warp writes the results)
         r = -INFINITY, L = E = 0.f;
         if (lane < kWarps) r = sh.ref[lane], L = sh.L[lane], E = sh.E[lane];
@@ -439,10 +524,15 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
         }
     }
 
+    const uint32_t mine = order_or_none(tmax);
+    const Seen seen{round, order_or_none(other)};
     // ---- segments meet in the workspace; the row's last CTA goes on
     if (a.segs > 1) {
         Partial* p = a.partials + (size_t)row * a.segs;
-        if (tid < k) __stcg((unsigned long long*)&p[seg].key[tid], sh.best[tid]);
+        if (k) {
+            __stcg(&p[seg].value[tid], mine);
+            __stcg(reinterpret_cast<uint2*>(&p[seg].seen[tid]), make_uint2(seen.chunk, seen.other));
+        }
         if (tid == 0) __stcg(reinterpret_cast<float4*>(&p[seg]), make_float4(r, L, E, 0.f));
         __syncthreads();
         if (tid == 0) {
@@ -451,7 +541,6 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
                          : "=r"(was) : "l"(a.counters + row) : "memory");
             sh.last = was + 1 == (unsigned)a.segs;
             if (sh.last) a.counters[row] = 0;
-            sh.n = 0;
         }
         __syncthreads();
         if (!sh.last) return;
@@ -465,26 +554,9 @@ __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_con
             const float r2 = __shfl_xor_sync(~0u, r, o), L2 = __shfl_xor_sync(~0u, L, o);
             join(r, L, E, r2, L2, __shfl_xor_sync(~0u, E, o), c);
         }
-        if (k) {
-            // the k-th largest of the segments' first ceil(k / segs) keys bounds the k-th of all
-            const int J = (k + a.segs - 1) / a.segs, m = a.segs * J;   // k <= m < k + segs
-            const uint64_t own = tid < m ? __ldcg((const unsigned long long*)&p[tid / J].key[tid % J]) : kNoKey;
-            if (tid < m) sh.key[tid] = own;
-            if (tid == 0) sh.red[0] = kNoKey + 1;
-            __syncthreads();
-            int rank = 0;
-            for (int j = 0; j < m; ++j) rank += sh.key[j] > own;
-            if (own != kNoKey && rank == k - 1) sh.red[0] = own;   // (valid keys are all different)
-            __syncthreads();
-            const uint64_t low = sh.red[0];
-            for (int i = tid; i < a.segs * k; i += kThreads) {
-                const uint64_t v = __ldcg((const unsigned long long*)&p[i / k].key[i % k]);
-                if (v >= low) sh.key[atomicAdd(&sh.n, 1)] = v;
-            }
-            __syncthreads();
-            rank_keys(sh, sh.n, k);
-        }
     }
+    if (k) select_top<DT>(sh, w, a.segs > 1 ? a.partials + (size_t)row * a.segs : nullptr,
+                          mine, seen, k);
     // ---- the row's results, by the first warp: lse = scale*r + ln L
     if (warp) return;
     r = __shfl_sync(~0u, r, 0), L = __shfl_sync(~0u, L, 0), E = __shfl_sync(~0u, E, 0);
