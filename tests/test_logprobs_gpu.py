@@ -205,3 +205,23 @@ def test_graph_and_other_stream(lib):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("rest", [0.0, -1e4, float(torch.finfo(torch.float16).min)])
+@pytest.mark.parametrize("V,k", [(5000, 5), (128256, 32)])
+def test_most_tokens_share_one_value(lib, V, k, rest):
+    z = torch.full((4, V), rest, dtype=torch.float16, device="cuda")
+    z[1, V - 1], z[1, 4097], z[1, 11] = 2.0, 1.0, 3.0      # three above the rest
+    z[2, ::7] = -float("inf")                              # the first is no token
+    z[3, V // 2:] = 1.0                                    # two shared values
+    check(z, k)
+
+
+def test_large_logits_lie_together(lib):
+    # every 786 chunks of 8 hold all large logits in their first 31, so that the
+    # threads' maxima say little about the k-th largest
+    V = 201088
+    z = normal(1, V, "f16", sd=1.0)
+    z[:, (torch.arange(V, device="cuda") // 8 % 786 % 128) < 31] += 50.0
+    check(z, 32)
+    check(z.float()[:, :100001], 32)
