@@ -395,10 +395,20 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     a.cpt_magic = ((1u << 20) + a.cpt - 1) / a.cpt;
     a.cta_heads = std::min(a.heads, std::max(1u, 32768u / (a.bt * a.dim)));
     // Writing, a CTA a (head, K or V): 4 chunks of 8 elements a thread, up to 512 threads (then
-    // 8 chunks).  Short items (decode steps) take a warp each, eight to a CTA: a step of 64
-    // sequences with one CTA each spent 10 us on launching and emptying 2080 CTAs.
+    // 8 chunks).  Where most CTAs would be nearly empty and many, a warp each, eight to a CTA:
+    //   one token of 64 sequences (8 heads of 128)      a chunk a lane 7.8 us, a CTA 10
+    //   8 tokens of 256 sequences (8 heads of 64)       a warp 16.3 us, a CTA 22.0
+    //   8 tokens of 64                                  a warp 10.3 us, a CTA 10.4
+    //   32 tokens of one                                a warp 7.0 us, a CTA 5.8
+    //   7687 tokens of 4, whole blocks of 16 (of 128)   a warp 22.6 us, a CTA 21.1
     const uint32_t most = std::min(range->max_tokens, a.bt) * a.cpt;   // chunks of an item
-    const Form form = !write ? kRead : most <= 32 ? kWriteOne : most <= kWarpChunks ? kWriteWarp : kWriteCta;
+    DeviceInfo di;
+    if (const int rc = current_device_info(&di)) return rc;
+    const bool sparse = 2 * (uint64_t)range->max_tokens <= a.bt && items * 2 * a.heads > 16ull * di.sm_count;
+    const Form form = !write                                ? kRead
+                      : most <= 32                          ? kWriteOne
+                      : most <= kWarpChunks && sparse       ? kWriteWarp
+                                                            : kWriteCta;
     int threads = ((int)(a.bt * a.cpt) / 4 + 31) / 32 * 32;
     threads = form != kWriteCta ? 256 : threads < 64 ? 64 : threads > 512 ? 512 : threads;
     const int chunks = (int)(a.bt * a.cpt + threads - 1) / threads;

@@ -42,6 +42,7 @@ CASES = [
     ([127], [2], 1, 256, 128),
     ([0, 128], [300, 128], 2, 256, 128),
     (list(range(0, 140, 2)), [1 + i % 3 for i in range(70)], 2, 80, 16),
+    (list(range(160)), [1 + i % 8 for i in range(160)], 8, 64, 64),
 ]
 
 
