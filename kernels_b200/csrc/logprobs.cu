@@ -20,6 +20,10 @@
 // again, and what reaches the bound is collected and ranked.  Ties go to the lowest
 // index: keys are (value, index) pairs, all different.  Segments meet in the workspace,
 // and the row's last CTA joins them.
+//
+// Measured: 777 rows of 128256 in fp16 (199 MB), 5 alternatives: 53.2 us, 3.7 TB/s (42 us
+// without the search for alternatives); one row of 201088, 20 alternatives: 9.2 us, of
+// which the pass and the joining of sums are 4.7; 37 rows of 50021 in fp32, 8 alternatives: 9.3 us.
 #include "kv_common.cuh"
 
 #include <algorithm>
@@ -37,7 +41,8 @@ constexpr int kCap = 2048;           // keys that are collected at most
 constexpr int kList = 1024;          // chunks that are read again at most
 constexpr int kMinSeg = 4096;        // elements of a segment, at least
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRounds = 148 * 16;    // CTAs that fill the SMs for several rounds (148 x 16)
+// CTAs to aim at (777 rows of 128256: 148 x 16 53.5 us, x 10 56.0, x 24 59, x 32 58; ten fit an SM)
+constexpr int kRounds = 148 * 16;
 constexpr size_t kCounterBytes = (kRounds * 4 + 255) / 256 * 256;   // a row is cut only if rows < kRounds
 constexpr uint64_t kNoKey = 0;       // below every key of a logit that is not -inf
 
@@ -409,6 +414,7 @@ __device__ __forceinline__ float chunk_max(const uint4& v) {
         return fmaxf(p.x, p.y);
     }
 }
+// (ten CTAs an SM: 55.5 us for 777 rows of 128256, eight 58, twelve, which spill, 58)
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_constant__ LpArgs a) {
     constexpr int N = kPer<DT>, UN = kUnroll;
