@@ -106,25 +106,6 @@ __device__ __forceinline__ void tc5_mma_ts(uint32_t d, uint32_t a, uint32_t b, u
         "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kTc5High)
         : "memory");
 }
-// Pairs of fp32 numbers (sm_100's two-wide operations).
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // One lane of a converged warp, always the same.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;

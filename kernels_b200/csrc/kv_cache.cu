@@ -17,8 +17,9 @@
 // needed (a CTA past its sequence's blocks returns).
 //
 // Measured: reading 65521 tokens of 8 heads of 128 back in fp16 70.5 us, 5.7 TB/s; writing
-// 7687 tokens of 8 heads of 64 and reading them back 14.5 us; one token of 64 sequences
-// (8 heads of 128), written and its block read back, 7.8 us.
+// them 84 us, 4.8 TB/s (instruction issue: rounding a code costs about seven instructions);
+// writing 7687 tokens of 8 heads of 64 and reading them back 14.1 us; one token of 64
+// sequences (8 heads of 128), written and its block read back, 7.8 us.
 #include "kv_common.cuh"
 
 #include <algorithm>
@@ -104,25 +105,29 @@ __device__ __forceinline__ float fin_abs(float x) {
     return a < __int_as_float(0x7f800000) ? a : 0.f;
 }
 
-// x / s for a finite x: the product with 1/s (correctly rounded) and one correction by the
+// x / s for two finite x: the product with 1/s (correctly rounded) and one correction by the
 // exact remainder, which gives the correctly rounded quotient (Markstein, 1990) in three
 // operations instead of the general division's ten.
-__device__ __forceinline__ float quotient(float x, float s, float inv) {
-    const float q = x * inv;
-    return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
+__device__ __forceinline__ uint64_t quotient2(uint64_t x, uint64_t minus_s, uint64_t inv) {
+    const uint64_t q = mul2(x, inv);
+    return fma2(fma2(q, minus_s, x), inv, q);
 }
 
 // Four quotients of finite elements as codes.  None is beyond qmax by more than its
 // rounding, so an int8 code needs no clamp: the sum with 1.5 2^23 rounds to nearest even
 // and holds the integer in its low bits.
 template <int FMT>
-__device__ __forceinline__ uint32_t finite_codes(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t finite_codes(uint64_t ab, uint64_t cd) {
+    float a, b, c, d;
     if constexpr (FMT == GRAFT_KV_INT8) {
-        constexpr float k = 12582912.f;
-        const uint32_t ab = __byte_perm(__float_as_uint(a + k), __float_as_uint(b + k), 0x0040);
-        const uint32_t cd = __byte_perm(__float_as_uint(c + k), __float_as_uint(d + k), 0x0040);
-        return __byte_perm(ab, cd, 0x5410);
+        const uint64_t k = pair(12582912.f, 12582912.f);
+        unpair(add2(ab, k), a, b);
+        unpair(add2(cd, k), c, d);
+        return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                           __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
     } else {
+        unpair(ab, a, b);
+        unpair(cd, c, d);
         uint16_t lo, hi;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_kernel(const __grid
     const float s = fmaxf(fmaxf(__fdiv_rn(amax, kKVQmax<FMT>), kKVScaleFloor), old);
     if constexpr (WARP) __syncwarp();   // (all lanes have read the old scale)
     if (tid == 0) *scale = s;
-    const float inv = __frcp_rn(s);
+    const uint64_t inv = pair(__frcp_rn(s), __frcp_rn(s)), minus_s = pair(-s, -s);
 
     if (it.slot && s > old) {   // the earlier tokens' codes, to the grown scale
         const float ratio = __fdiv_rn(old, s);
@@ -276,10 +281,11 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_kernel(const __grid
                     o.y |= kv_code<FMT>(__fdiv_rn(f[e + 4], s)) << (8 * e);
                 }
             } else {
+                uint64_t q[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = quotient(f[e], s, inv);
-                o.x = finite_codes<FMT>(f[0], f[1], f[2], f[3]);
-                o.y = finite_codes<FMT>(f[4], f[5], f[6], f[7]);
+                for (int e = 0; e < 4; ++e) q[e] = quotient2(pair(f[2 * e], f[2 * e + 1]), minus_s, inv);
+                o.x = finite_codes<FMT>(q[0], q[1]);
+                o.y = finite_codes<FMT>(q[2], q[3]);
             }
             *reinterpret_cast<uint2*>(codes + (size_t)it.slot * a.dim + (size_t)c * kChunk) = o;
         }
@@ -398,8 +404,10 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     a.cpt = a.dim / (write ? kChunk : 16);
     a.cpt_magic = ((1u << 20) + a.cpt - 1) / a.cpt;
     a.cta_heads = std::min(a.heads, std::max(1u, 32768u / (a.bt * a.dim)));
-    // Writing, a CTA a (head, K or V): 4 chunks of 8 elements a thread, up to 512 threads (then
-    // 8 chunks).  Where most CTAs would be nearly empty and many, a warp each, eight to a CTA:
+    // Writing, a CTA a (head, K or V): 8 chunks of 8 elements a thread (what every thread does
+    // once costs as much as two chunks), or 4 where that makes fewer than 128 threads.
+    // 65521 tokens, blocks of 64, written and read back: 8 heads of 128 154 us so and 166 with
+    // 4 chunks; 8 heads of 64 76 with 4 chunks (128 threads) and 78 with 8.  Where most CTAs would be nearly empty and many, a warp each, eight to a CTA:
     //   one token of 64 sequences (8 heads of 128)      a chunk a lane 7.8 us, a CTA 10
     //   8 tokens of 256 sequences (8 heads of 64)       a warp 16.3 us, a CTA 22.0
     //   8 tokens of 64                                  a warp 10.3 us, a CTA 10.4
@@ -413,8 +421,8 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
                       : most <= 32                          ? kWriteOne
                       : most <= kWarpChunks && sparse       ? kWriteWarp
                                                             : kWriteCta;
-    int threads = ((int)(a.bt * a.cpt) / 4 + 31) / 32 * 32;
-    threads = form != kWriteCta ? 256 : threads < 64 ? 64 : threads > 512 ? 512 : threads;
+    const int whole = (int)(a.bt * a.cpt), fourth = (whole / 4 + 31) / 32 * 32, eighth = (whole / 8 + 31) / 32 * 32;
+    const int threads = form != kWriteCta ? 256 : std::min(512, std::max({64, eighth, std::min(fourth, 128)}));
     const int chunks = (int)(a.bt * a.cpt + threads - 1) / threads;
     const uint32_t ny = form == kRead      ? 2 * ((a.heads + a.cta_heads - 1) / a.cta_heads)
                         : form == kWriteCta ? 2 * a.heads : (2 * a.heads + 7) / 8;
