@@ -21,9 +21,9 @@
 // index: keys are (value, index) pairs, all different.  Segments meet in the workspace,
 // and the row's last CTA joins them.
 //
-// Measured: 777 rows of 128256 in fp16 (199 MB), 5 alternatives: 53.2 us, 3.7 TB/s (42 us
-// without the search for alternatives); one row of 201088, 20 alternatives: 9.2 us, of
-// which the pass and the joining of sums are 4.7; 37 rows of 50021 in fp32, 8 alternatives: 9.3 us.
+// Measured: 777 rows of 128256 in fp16 (199 MB), 5 alternatives: 52.3 us, 3.8 TB/s (46 us
+// without alternatives); one row of 201088, 20 alternatives: 9.3 us, without them 4.5;
+// 37 rows of 50021 in fp32, 8 alternatives: 9.1 us, without them 5.6.
 #include "kv_common.cuh"
 
 #include <algorithm>
@@ -41,7 +41,7 @@ constexpr int kCap = 2048;           // keys that are collected at most
 constexpr int kList = 1024;          // chunks that are read again at most
 constexpr int kMinSeg = 4096;        // elements of a segment, at least
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// CTAs to aim at (777 rows of 128256: 148 x 16 53.5 us, x 10 56.0, x 24 59, x 32 58; ten fit an SM)
+// CTAs to aim at (777 rows of 128256: 148 x 16 53.5 us, x 10 56.0, x 24 59, x 32 58)
 constexpr int kRounds = 148 * 16;
 constexpr size_t kCounterBytes = (kRounds * 4 + 255) / 256 * 256;   // a row is cut only if rows < kRounds
 constexpr uint64_t kNoKey = 0;       // below every key of a logit that is not -inf
@@ -414,9 +414,9 @@ __device__ __forceinline__ float chunk_max(const uint4& v) {
         return fmaxf(p.x, p.y);
     }
 }
-// (ten CTAs an SM: 55.5 us for 777 rows of 128256, eight 58, twelve, which spill, 58)
+// (nine CTAs an SM, 56 registers: 52.3 us for 777 rows of 128256; ten 53.3)
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 10) logprobs_kernel(const __grid_constant__ LpArgs a) {
+__global__ void __launch_bounds__(kThreads, 9) logprobs_kernel(const __grid_constant__ LpArgs a) {
     constexpr int N = kPer<DT>, UN = kUnroll;
     __shared__ Shared sh;
     pdl_wait();
