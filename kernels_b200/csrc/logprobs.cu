@@ -361,7 +361,8 @@ __device__ __forceinline__ void select_top(Shared& sh, const Row& w, const Parti
         if (sh.listed > kList) continue;
         for (int i = tid; i < sh.listed; i += kThreads) collect(sh.list[i], least, ~0u);
         __syncthreads();
-        done = sh.n <= (pass ? kCap - kThreads * N : kCap);
+        // (room for the equal ones: fewer than k, and one more round of the CTA's chunks)
+        done = sh.n <= (pass ? kCap - kThreads * N - kMaxTop : kCap);
     }
     if (done && least > bound + 1) {   // .. and the first of the equal ones in their order
         const int want = sh.n + k;

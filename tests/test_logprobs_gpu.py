@@ -225,3 +225,16 @@ def test_large_logits_lie_together(lib):
     z[:, (torch.arange(V, device="cuda") // 8 % 786 % 128) < 31] += 50.0
     check(z, 32)
     check(z.float()[:, :100001], 32)
+
+
+@pytest.mark.parametrize("above", [960, 1000, 1024, 1100])
+def test_many_above_and_many_equal(lib, above):
+    # one token's neighbours above a value that all others share: about as many as the
+    # collected keys leave room for
+    V = 201088
+    z = torch.zeros(1, V, dtype=torch.float16, device="cuda")
+    at = torch.arange(V, device="cuda")
+    few = at[at // 8 % 786 % 128 < 20][:above]
+    z[0, few] = 1.0 + torch.arange(above, device="cuda", dtype=torch.float16) / 1024
+    check(z, 32)
+    check(-z, 32)
