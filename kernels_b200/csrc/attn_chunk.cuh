@@ -207,16 +207,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         w.tiles = (w.s.n + TT - 1) / TT;
     };
     auto keys_before = [&](const Walk& w, int rt) {   // rt <= tiles
-        const long long n = rt;
-        long long k = n * (w.s.start + a.pad_units) + n * (n + 1) / 2 * TT;
-        if (rt == w.tiles) k -= n * TT - w.s.n;   // (the last tile may have fewer tokens)
-        if (a.window) {   // first keys: start - window + 1 + TT i where that is positive
-            const int c = w.s.start - (int)a.window + 1;
-            const int skip = c >= 0 ? 0 : min(rt, (-c + TT - 1) / TT);
-            const long long r = rt - skip;
-            k -= r * (c + (long long)skip * TT) + (r - 1) * r / 2 * TT;
-        }
-        return k;
+        return tile_keys(w.s.start, w.s.n, TT, w.tiles, rt, (int)a.window, a.pad_units);
     };
     Split<long long> sp;
     Walk cw;

@@ -2,6 +2,7 @@
 // arguments, code conversions to fp16 pairs, matrix instructions, the split of
 // the work over the grid and the joining of partial results.
 #pragma once
+#include "attn_split.cuh"
 #include "kv_common.cuh"
 
 namespace graft {

@@ -177,7 +177,9 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
     a.n_blocks = cache->n_blocks, a.heads = cache->kv_heads, a.bt = cache->block_tokens;
     a.dim = cache->head_dim, a.n_seqs = range->n_seqs, a.table_stride = range->table_stride;
     a.max_tokens = range->max_tokens, a.max_len = range->max_len, a.tokens = q->tokens;
-    a.q_heads = P->q_heads, a.group = P->q_heads / cache->kv_heads, a.window = P->window;
+    a.q_heads = P->q_heads, a.group = P->q_heads / cache->kv_heads;
+    // (a window that reaches beyond every sequence, the largest int say, is none)
+    a.window = P->window < range->max_len ? P->window : 0;
     a.scale = P->scale;
     a.bt_log2 = a.bt == 16 ? 4 : a.bt == 32 ? 5 : a.bt == 64 ? 6 : 7;
     a.bf16 = q->dtype == GRAFT_BF16;
