@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                         for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
                         tmem_st32(to + 32 * c, v);
                     }
+                    tmem_wait_st();   // (a second rescaling reads what this one stored)
                 };
                 // ---- the row's maximum becomes the reference of the exponents
                 auto follow = [&](auto masked) {
@@ -544,6 +545,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 while (true) {
                     most = edge_unit ? weigh(std::true_type{}) : weigh(std::false_type{});
                     if (!C::BESIDE || !__any_sync(~0u, most > 32768.f)) break;
+                    tmem_wait_st();   // (the weights are stored again where these lie)
                     if (edge_unit) follow(std::true_type{});
                     else follow(std::false_type{});
                     if (__all_sync(~0u, !(most > 32768.f) || !(m < INFINITY))) break;

@@ -34,3 +34,75 @@ def test_windows_beyond_every_sequence(lib, window):
 def test_windows_beyond_the_sequences_of_a_longer_bound(lib):
     """A window that is within max_len and beyond what the sequences hold."""
     run_case([0, 700, 5], [129, 64, 300], 8, 1, 64, 16, "int8", "f16", 1200, False)
+
+
+def raw_cache(kc, vc, ks, vs, bt):
+    """A cache of one sequence from int8 code values kc, vc [T, H, D] and scales ks, vs
+    [ceil(T / bt), H]; block 0 belongs to nobody."""
+    T, H, D = kc.shape
+    nb = -(-T // bt)
+    dev = kb.KVCache.empty(nb + 1, H, D, bt)
+    for codes, x in ((dev.k, kc), (dev.v, vc)):
+        pad = torch.zeros(nb * bt, H, D, dtype=torch.int8)
+        pad[:T] = x.to(torch.int8)
+        codes[1:] = pad.view(nb, bt, H, D).transpose(1, 2).cuda()
+    dev.k_scale[1:], dev.v_scale[1:] = ks.cuda(), vs.cuda()
+    return dev, torch.arange(1, nb + 1, dtype=torch.int32, device="cuda")[None]
+
+
+def check_against_formula(dev, table, q, T, scale, window=0):
+    """Output and lse of the sequence's last tokens against the formula in 64 bits, with
+    the tolerances of test_attn_kv8_gpu.py."""
+    n, Hq, D = q.shape
+    P = kb.attn_params(Hq, scale=scale, window=window)
+    lse = torch.empty(n, Hq, device="cuda")
+    out = attend(dev, q, one_range(table, T - n, n), P, lse=lse)
+    k, v = (torch.empty(T, dev.heads, D, device="cuda") for _ in "kv")
+    kb.kv_read(dev, k, v, one_range(table, 0, T))
+    o, l, a, mag = attention(f64(q), f64(k), f64(v), T - n, np.float64(np.float32(scale)), window, None)
+    d = (D + 8) * 2.0 ** -24 * mag + 2.0 ** -20
+    tol = ROUND["f16" if q.dtype == torch.float16 else "bf16"] * abs(o) * 1.01 + a * (2.0 ** -11 + 2 * d) + 1e-7
+    assert (abs(f64(out) - o) <= tol).all(), (abs(f64(out) - o) / tol).max()
+    assert (abs(lse.cpu().double().numpy() - l) <= d + 2.0 ** -20 * (1 + abs(l))).all()
+    assert not any(kb.kv_device_errors().values())
+
+
+@pytest.mark.parametrize("D", [64, 48, 128, 256])
+@pytest.mark.parametrize("step", [2.0, 5.0, 9.0, 11.0, 12.0, 13.0, 14.0, 17.0])
+@pytest.mark.parametrize("keys", [32, 64, 128])
+def test_scores_that_rise(lib, keys, step, D):
+    """Scores that rise by `step` (log2) every `keys` keys, so that references follow in
+    every unit, go up before one and follow within it, and outputs are rescaled twice in
+    a row.  Rows of a tile differ in how steep theirs are, down to falling ones."""
+    g = torch.Generator().manual_seed(int(step) + keys + D)
+    T, Hq, n = 900, 8, 60
+    runs = -(-T // keys)
+    kc = torch.randint(-2, 3, (T, 1, D), generator=g).float()
+    kc[:, 0, 0] = (torch.arange(T) // keys).float() * 4       # up to 112
+    vc = torch.randint(-127, 128, (T, 1, D), generator=g).float()
+    nb = -(-T // 16)
+    ks = torch.full((nb, 1), 0.25)
+    vs = 2.0 ** torch.randint(-2, 3, (nb, 1), generator=g).float()
+    dev, table = raw_cache(kc, vc, ks, vs, 16)
+    q = 0.05 * torch.randn(n, Hq, D, generator=g)
+    steep = torch.tensor([1.0, 1.0, 0.9, 0.5, 0.1, 0.0, -0.5, -1.0])
+    q[:, :, 0] = steep * (1 + 0.01 * torch.arange(n))[:, None]
+    check_against_formula(dev, table, q.half().cuda(), T, step / 1.4426950408889634)
+    assert runs * 4 <= 127
+
+
+@pytest.mark.parametrize("n", [3, 60])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scales_far_apart_many_rows_too(lib, n, D):
+    """Blocks whose scales differ by many orders, blocks of zeros among them."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T, H = 320, 1
+    K = torch.randn(T, H, D, device="cuda", generator=g)
+    V = torch.randn(T, H, D, device="cuda", generator=g)
+    factors = [1.0, 0.0, 1e-8, 1e6, 1e-3, 0.0, 1.0, 1e-12, 30.0, 1e-15]
+    for j in range(T // 16):
+        V[16 * j:16 * j + 16] *= factors[j % 10]
+    V[48:64, :, ::2] = 0
+    dev, table = cache_of(K, V)
+    q = torch.randn(n, 8, D, device="cuda", generator=g).to(torch.bfloat16)
+    check_against_formula(dev, table, q, T, D ** -0.5)
