@@ -55,10 +55,10 @@ struct Chunk {
     static constexpr int P_COL = DP <= 64 ? 256 : DP <= 128 ? 0 : 128;
     static constexpr int P_TILE = DP <= 64 ? 64 : 128, P_STEP = DP == 128 ? 64 : 32;
     static constexpr int O_COL = DP <= 64 ? 384 : 256;
-    // Weights are 2^(t - m + SHIFT).  Where a half is weighed before its maximum is known,
-    // fp16 leaves room for scores up to 12 (in log2) above the reference, and keeps its 11
-    // bits down to 17 below it; the reference goes up only near that limit, because O's
-    // rescaling waits for the product before.
+    // Weights are 2^(t - m), the reference m SHIFT below the largest t that it was taken
+    // from.  Where a half is weighed before its maximum is known, fp16 leaves room for scores
+    // up to 12 (in log2) above that, and keeps its 11 bits down to 17 below it; the reference
+    // goes up only near that limit, because O's rescaling waits for the product before.
     static constexpr float SHIFT = BESIDE ? 3.f : kPShift;
     static constexpr int SC = 8;                     // slots of a unit's scales (up to ST + 2 in use)
     // floats of a partial result: O column by column, maximum and sum of each row
@@ -430,12 +430,21 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             }
             // (rows without a token need no mask: nothing of theirs is kept)
             const int p = on ? cw.s.start + tok : 1 << 30, lo = on ? first_key(a, p) : 0;
-            float m = kNoMax, l = 0.f;
-            int raise = 0;   // of the reference, before the next unit
+            float m = kNoMax, l = 0.f;   // reference, sum of the weights
+            int raise = 0;               // of the reference, before the next unit
+            // A reference beyond 2^20 (of any row of the warp): what is below is then worked out
+            // as rounded scores, whose differences are exact.  The shorter form's sum of a scale
+            // and the reference would be off by whole steps, and 2^(t - m) beyond fp16.
+            // (Rows without a key yet and infinite ones do not count.)
+            bool wide = false, careful;   // (careful: a unit that needs masks, or exact differences)
+            auto widen = [&]() {
+                wide = __any_sync(~0u, fabsf(m) > 0x1p20f && m != kNoMax && m < INFINITY);
+                careful |= wide;
+            };
             for (int u = cw.lo; u < cw.hi; ++u, ++it) {
                 const bool first_unit = u == cw.lo;
                 const int c_lo = lo - u * KT, c_hi = p - u * KT;   // columns that the row sees
-                const bool edge_unit = __any_sync(~0u, c_lo > 0 || c_hi < KT - 1);
+                careful = wide || __any_sync(~0u, c_lo > 0 || c_hi < KT - 1);
                 wait(&scfull[it % SC], it / SC);
                 float top = 0.f;
 #pragma unroll
@@ -459,9 +468,9 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                     }
                     tmem_wait_st();   // (a second rescaling reads what this one stored)
                 };
-                // ---- the row's maximum becomes the reference of the exponents
+                // ---- the row's maximum leads the reference of the exponents
                 auto follow = [&](auto masked) {
-                    float mx = m;
+                    float mx = -INFINITY;
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
                         uint32_t v[32];
@@ -482,15 +491,16 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                             mx = fmaxf(mx, x);
                         }
                     }
-                    if (!__any_sync(~0u, mx > m + (C::BESIDE ? 0.f : kPSlack))) return;
-                    const float f = ex2(m - mx);
+                    if (!__any_sync(~0u, mx - m > C::SHIFT + (C::BESIDE ? 0.f : kPSlack))) return;
+                    const float up = fmaxf(m, reference(mx, C::SHIFT)), f = ex2(m - up);
                     l *= f;
-                    m = mx;
+                    m = up;
+                    widen();
                     if (!first_unit || hh) rescale(f);
                 };
                 // ---- the weights; the largest sum of 16 of them
                 float dl;
-                auto weigh = [&](auto masked) {
+                auto weigh = [&](auto masked) {   // (masked: with exact differences too)
                     // (all 64 scores at once: straight code that keeps the MUFU fed, two
                     // fp32 operations an instruction where there are such)
                     float most = 0.f;
@@ -502,14 +512,15 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const float4 f = sc[c];
-                        const float fa = f.x * cr, fb = f.y - (m - C::SHIFT);
+                        const float fa = f.x * cr, fb = decltype(masked)::value ? f.y : f.y - m;
                         const uint64_t fa2 = pair(fa, fa), fb2 = pair(fb, fb);
                         uint64_t sum = 0;
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             const int col = 16 * c + e;
                             float x, y;
-                            unpair(fma2(pair(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), fa2, fb2), x, y);
+                            const uint64_t t2 = fma2(pair(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), fa2, fb2);
+                            unpair(decltype(masked)::value ? add2(t2, pair(-m, -m)) : t2, x, y);
                             if (decltype(masked)::value) {
                                 const int at = 64 * hh + col;
                                 x = at >= c_lo && at <= c_hi ? x : -INFINITY;
@@ -532,23 +543,24 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 // that the halves before left, and weighed again in the rare case that a row
                 // reached fp16's limit (no weight reaches 2^15 unless a sum of 16 does).
                 if (!C::BESIDE || (first_unit && hh == 0)) {
-                    if (edge_unit) follow(std::true_type{});
+                    if (careful) follow(std::true_type{});
                     else follow(std::false_type{});
                 } else if (hh == 0 && __any_sync(~0u, raise > 0)) {
                     // by a power of two: the rows' sums and O keep their bits
-                    const float f = ex2((float)-raise);
+                    const float up = m + (float)raise, f = ex2(m - up);
                     l *= f;
-                    m += (float)raise;
+                    m = up;
+                    widen();
                     rescale(f);
                 }
+                // (Once: no score lies more than SHIFT above the reference that follows it.)
                 float most;
-                while (true) {
-                    most = edge_unit ? weigh(std::true_type{}) : weigh(std::false_type{});
-                    if (!C::BESIDE || !__any_sync(~0u, most > 32768.f)) break;
+                for (bool again = false;; again = true) {
+                    most = careful ? weigh(std::true_type{}) : weigh(std::false_type{});
+                    if (!C::BESIDE || again || !__any_sync(~0u, most > 32768.f)) break;
                     tmem_wait_st();   // (the weights are stored again where these lie)
-                    if (edge_unit) follow(std::true_type{});
+                    if (careful) follow(std::true_type{});
                     else follow(std::false_type{});
-                    if (__all_sync(~0u, !(most > 32768.f) || !(m < INFINITY))) break;
                 }
                 top = fmaxf(top, most);
                 l += dl;
@@ -601,7 +613,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 for (int k = 0; k < pieces; ++k)
                     l = fmaf(__ldcg(piece(k) + DP * ROWS + ROWS), ex2(__ldcg(piece(k) + DP * ROWS) - m), l);
             }
-            float ref = m - C::SHIFT, fo = 1.f;
+            float ref = m, fo = 1.f;
             if (a.sinks) {
                 const float s = a.sinks[on ? hq : 0] * kLog2e;
                 if (s > ref) {

@@ -37,6 +37,13 @@ constexpr float kNoMax = -1e30f;
 // by more than kPSlack: at most 2^14 in fp16, which keeps its 11 bits down to
 // 2^-28 of that.
 constexpr float kPShift = 10.f, kPSlack = 4.f;
+// The reference `shift` below a score t.  Above 2^25 steps of fp32 are as large as the
+// shift: where the difference would be rounded to more than shift + kPSlack, which fp16
+// might not hold as an exponent, it is t itself.
+__device__ __forceinline__ float reference(float t, float shift) {
+    const float r = t - shift;
+    return t - r > shift + kPSlack ? t : r;
+}
 
 // Limit of every wait for a kernel's own copies or products.
 constexpr uint64_t kAttnWaitNs = 2000000000ull;

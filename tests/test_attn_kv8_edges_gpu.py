@@ -106,3 +106,61 @@ def test_scales_far_apart_many_rows_too(lib, n, D):
     dev, table = cache_of(K, V)
     q = torch.randn(n, 8, D, device="cuda", generator=g).to(torch.bfloat16)
     check_against_formula(dev, table, q, T, D ** -0.5)
+
+
+def check_huge(n, D, exponent):
+    """Scores of about 2^exponent (log2 units) whose neighbours are one step of fp32 apart
+    from 2^25 on: S, S + 1 and S + 2 in three runs of 256 keys, S about 1.66e7 < 2^24 (sums
+    of products are exact in fp32) and of every parity, times 2^(exponent - 24)."""
+    g = torch.Generator().manual_seed(0)
+    T = 768
+    kc = torch.zeros(T, 1, D)
+    kc[:, 0, :2] = 127
+    kc[:, 0, 2] = torch.arange(T) // 256
+    kc[:, 0, 3] = 1
+    vc = torch.randint(-127, 128, (T, 1, D), generator=g).float()
+    dev, table = raw_cache(kc, vc, torch.ones(T // 16, 1), torch.ones(T // 16, 1), 16)
+    q = torch.zeros(n, 8, D)
+    q[:, :, :2] = 65504
+    q[:, :, 2] = 1
+    q[:, :, 3] = torch.arange(8)
+    q = q.half().cuda()
+    P = kb.attn_params(8, scale=2.0 ** (exponent - 24) / 1.4426950408889634)
+    lse = torch.empty(n, 8, device="cuda")
+    out = attend(dev, q, one_range(table, T - n, n), P, lse=lse)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    # the weights are what rounded scores make of them, but weights: an average of values
+    # (each weight is off by 2^-11, the output by 2^-11 more)
+    assert (out.float().cpu() <= vc.amax(0) * (1 + 2.0 ** -10)).all()
+    assert (out.float().cpu() >= vc.amin(0) * (1 + 2.0 ** -10)).all()
+    # lse is the largest score, off by a few roundings, and at most log T above
+    top = (f64(q) @ kc[:, 0].double().numpy().T * np.float64(np.float32(P.scale))).max(-1)
+    assert (abs(lse.cpu().double().numpy() - top) <= 2.0 ** -20 * abs(top) + np.log(T)).all()
+    assert not any(kb.kv_device_errors().values())
+
+
+@pytest.mark.parametrize("D", [64, 48, 128, 256])
+@pytest.mark.parametrize("exponent", [18, 20, 22, 24, 25, 26, 27, 28, 29, 30, 34, 40])
+def test_huge_scores_many_rows(lib, exponent, D):
+    check_huge(60, D, exponent)
+
+
+@pytest.mark.parametrize("scale", [-1.0, float("inf"), float("nan")])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_sequence_of_bad_scales_keeps_to_itself(lib, scale, D):
+    """Key scales that no cache should hold: the call ends, other sequences are right."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    T, n, nb = 300, 60, 19
+    dev = kb.KVCache.empty(2 * nb, 1, D, 16)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.arange(2 * nb, **i32).view(2, nb)
+    K, V = (torch.randn(2 * T, 1, D, device="cuda", generator=g) for _ in "kv")
+    kb.kv_write(dev, K, V, kb.kv_range(table, torch.zeros(2, **i32), torch.tensor([0, T, 2 * T], **i32), T, T))
+    dev.k_scale[3:nb:2] = scale
+    q = (40 * torch.randn(2 * n, 8, D, device="cuda", generator=g)).to(torch.float16)
+    P = kb.attn_params(8, scale=D ** -0.5)
+    want = attend(dev, q[n:], one_range(table[1:], T - n, n), P)
+    r = kb.kv_range(table, torch.tensor([T - n] * 2, **i32), torch.tensor([0, n, 2 * n], **i32), n, T)
+    got = attend(dev, q, r, P)[n:]
+    assert (got.float() - want.float()).abs().max() <= 2.0 ** -9 * want.abs().max()
+    assert not any(kb.kv_device_errors().values())
