@@ -61,7 +61,7 @@ struct Chunk {
     // goes up only near that limit, because O's rescaling waits for the product before.
     static constexpr float SHIFT = BESIDE ? 3.f : kPShift;
     static constexpr int SC = 8;                     // slots of a unit's scales (up to ST + 2 in use)
-    // floats of a partial result: O column by column, maximum and sum of each row
+    // floats of a partial result: O column by column, reference and sum of each row
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
 };
 

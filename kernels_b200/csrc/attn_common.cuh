@@ -30,12 +30,12 @@ struct AttnArgs {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// The running maximum of a row without a key yet: finite, so that a masked
-// score (-inf) minus it is -inf and never NaN.
+// The reference of a row without a key yet: finite, so that a masked score
+// (-inf) minus it is -inf and never NaN.
 constexpr float kNoMax = -1e30f;
-// Weights are held as 2^(t - m + kPShift) for a reference m that no t passes
-// by more than kPSlack: at most 2^14 in fp16, which keeps its 11 bits down to
-// 2^-28 of that.
+// Weights are held as 2^(t - m) for a reference m that lies kPShift below the largest
+// t that it was taken from, and that no t passes by more than kPShift + kPSlack: at most
+// 2^14 in fp16, which keeps its 11 bits down to 2^-28 of that.
 constexpr float kPShift = 10.f, kPSlack = 4.f;
 // The reference `shift` below a score t.  Above 2^25 steps of fp32 are as large as the
 // shift: where the difference would be rounded to more than shift + kPSlack, which fp16

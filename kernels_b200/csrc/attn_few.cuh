@@ -48,11 +48,11 @@ template <int DP, int NT>
 constexpr int kFewOut = (DP / 16) * NT * 4;    // accumulators of a lane
 template <int DP, int NT>
 constexpr int kFewSmem = kFewWarps * (kFewRing<DP, NT> * kFewSlot<DP> + kFewOut<DP, NT> * 32 * 4);
-// floats of a partial result: O, and the maximum and sum of each row
+// floats of a partial result: O, and the reference and sum of each row
 template <int DP, int NT>
 constexpr int kFewPartial = kFewOut<DP, NT> * 32 + 2 * 8 * NT;
 
-// The state of one warp: O^T and the running maximum and sum of its columns.
+// The state of one warp: O^T and its columns' references and sums of weights.
 template <int DP, int NT>
 struct FewState {
     float o[DP / 16][NT][4];
@@ -231,14 +231,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     float cn[NT][2];    // scale log2(e) of the columns' rows
     int pn[NT][2];      // positions of the columns' tokens
 
-    // ---- two elements of a row of a finished pair, L relative to 2^(M - kPShift)
+    // ---- two elements of a row of a finished pair, L relative to 2^M
     const int je = warp & 3, ce = (warp >> 2) & 1;   // the thread's accumulators: tile 4i + je, column ce
     auto finish = [&](int n, int i, float x0, float x1, float M, float L) {
         const int r = 8 * n + 2 * t + ce, d = 64 * i + 8 * g + 2 * je;
         const int tok = cw.s.n == 1 ? 0 : r / (int)a.group, head = r - tok * (int)a.group;
         if (tok >= cw.s.n || head >= (int)a.group || (!FULL && d >= D)) return;
         const int hq = cw.h * (int)a.group + head;
-        float ref = M - kPShift, fo = 1.f;
+        float ref = M, fo = 1.f;
         if (a.sinks) {
             const float sk = a.sinks[hq] * kLog2e;
             if (sk > ref) {
@@ -385,9 +385,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                     }
             }
             // ---- reference for the exponents, weights, their sum.  The reference
-            // follows the row's maximum only when a score passes it by more than
-            // kPSlack, which after the first units is rare: no reduction across
-            // the lanes is needed for a unit that stays below.
+            // (kPShift below the maximum it was taken from) follows only when a score
+            // passes that maximum by more than kPSlack, which after the first units is
+            // rare: no reduction across the lanes is needed for a unit that stays below.
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float mx[2];
@@ -398,24 +398,25 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                     for (int kt = 1; kt < KT; ++kt)
                         mx[c] = fmaxf(mx[c], fmaxf(s[kt][n][c], s[kt][n][c + 2]));
                 }
-                if (__any_sync(~0u, mx[0] > st.m[n][0] + kPSlack || mx[1] > st.m[n][1] + kPSlack)) {
+                constexpr float limit = kPShift + kPSlack;
+                if (__any_sync(~0u, mx[0] - st.m[n][0] > limit || mx[1] - st.m[n][1] > limit)) {
                     float f[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1)
                             mx[c] = fmaxf(mx[c], __shfl_xor_sync(~0u, mx[c], o));
-                        mx[c] = fmaxf(mx[c], st.m[n][c]);
-                        f[c] = ex2(st.m[n][c] - mx[c]);
+                        const float up = fmaxf(st.m[n][c], reference(mx[c], kPShift));
+                        f[c] = ex2(st.m[n][c] - up);
                         st.l[n][c] *= f[c];
-                        st.m[n][c] = mx[c];
+                        st.m[n][c] = up;
                     }
 #pragma unroll
                     for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) st.o[i][n][e] *= f[e & 1];
                 }
-                const float b0 = st.m[n][0] - kPShift, b1 = st.m[n][1] - kPShift;
+                const float b0 = st.m[n][0], b1 = st.m[n][1];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     float* x = s[kt][n];

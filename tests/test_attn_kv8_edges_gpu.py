@@ -145,6 +145,12 @@ def test_huge_scores_many_rows(lib, exponent, D):
     check_huge(60, D, exponent)
 
 
+@pytest.mark.parametrize("n,D", [(1, 64), (2, 64), (4, 64), (1, 48), (1, 128), (2, 128), (1, 256)])
+@pytest.mark.parametrize("exponent", [18, 20, 22, 24, 25, 26, 27, 28, 29, 30, 34, 40])
+def test_huge_scores_few_rows(lib, exponent, n, D):
+    check_huge(n, D, exponent)
+
+
 @pytest.mark.parametrize("scale", [-1.0, float("inf"), float("nan")])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_a_sequence_of_bad_scales_keeps_to_itself(lib, scale, D):
