@@ -568,6 +568,8 @@ typedef struct {
  * position p = start + i, sees keys j with p - window < j <= p:
  *   o = sum_j exp(scale q.k_j - lse) v_j,
  *   lse = log( sum_j exp(scale q.k_j)  [+ exp(sinks[h])] ).
+ * Blocks wholly before the window of a sequence's first new token are not
+ * read, nor are their entries in the block table.
  * q and out: GRAFT_F16 or GRAFT_BF16, the same type.  sinks (fp32 [q_heads], a
  * score that takes weight but has no value) and lse (fp32 [tokens][q_heads])
  * may be null.  Few rows a key/value head (max_tokens * q_heads/kv_heads up to

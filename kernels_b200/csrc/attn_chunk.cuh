@@ -670,6 +670,9 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         w.hi = 0;
         int u = 0, blk = 0;
         bool more = true;
+        // Keys that a row of the tile sees, and those that share 16 with one: a block before the
+        // window may be gone.  (16 keys lie in one block.)
+        auto inside = [&](int key) { return (key | 15) >= w.k0 && key < w.s.start + w.s.n; };
         auto lookup = [&]() {   // the next unit, and the number of its key's block
             if (more && ++u >= w.hi) {
                 more = next_piece(w);
@@ -677,14 +680,13 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
             }
             if (!more) return;
             const int key = u * KT + row;
-            blk = key < w.s.start + w.s.n
-                      ? a.table[(size_t)w.b * a.table_stride + (key >> a.bt_log2)] : 0;
+            blk = inside(key) ? a.table[(size_t)w.b * a.table_stride + (key >> a.bt_log2)] : 0;
         };
         uint4 kc[NC], vc[NC];
         float ks = 0.f, vs = 1.f;
         auto fetch = [&]() {    // its codes, and the block's scales
             const int key = u * KT + row;
-            const bool in = key < w.s.start + w.s.n;
+            const bool in = inside(key);
             if (in && (uint32_t)blk >= a.n_blocks) {
                 atomicOr(err, (unsigned)GRAFT_KV_EBLOCK);
                 blk = 0;

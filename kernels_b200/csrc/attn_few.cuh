@@ -191,9 +191,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         }
         if (!more) return;
         const int32_t* row = a.table + (size_t)iw.b * a.table_stride + (iu * UK >> a.bt_log2);
+        // (a unit of two blocks may end in its first, and its first may lie before the window:
+        // such a block may be gone, and the other's codes come in its place)
 #pragma unroll
-        for (int i = 0; i < NB; ++i)   // (a unit of two blocks may end in its first)
-            blk[i] = row[split && iu * UK + i * 16 < iw.s.start + iw.s.n ? i : 0];
+        for (int i = 0; i < NB; ++i)
+            blk[i] = row[!split || iu * UK + i * 16 >= iw.s.start + iw.s.n ? 0
+                         : iu * UK + i * 16 + 16 <= first_key(a, iw.s.start) ? 1 : i];
     };
     auto copy = [&](int to) {   // always closes a group, maybe an empty one
         if (more) {
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         st.reset();
         const int len = cw.s.start + cw.s.n;
         const int free_lo = first_key(a, len - 1);   // keys [free_lo, start] are seen by every row
+        const int first = first_key(a, cw.s.start);  // keys before it by none
 #pragma unroll 1
         for (int u = cw.lo + warp; u < cw.hi; u += W) {
             if (u < cw.lo + W) load_queries();
@@ -334,6 +338,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                 uint8_t* vr = sl + UK * DP;
                 for (int i = valid * D / 16 + lane; i < UK * D / 16; i += 32)
                     reinterpret_cast<uint4*>(vr)[i] = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
+            if (NB > 1 && FMT == GRAFT_KV_E4M3 && split && key0 + 16 <= first) {
+                // .. and so may the codes that stand for a block before the window
+                for (int i = lane; i < D; i += 32)
+                    reinterpret_cast<uint4*>(sl + UK * DP)[i] = make_uint4(0, 0, 0, 0);
                 __syncwarp();
             }
             // ---- scores

@@ -170,3 +170,37 @@ def test_a_sequence_of_bad_scales_keeps_to_itself(lib, scale, D):
     got = attend(dev, q, r, P)[n:]
     assert (got.float() - want.float()).abs().max() <= 2.0 ** -9 * want.abs().max()
     assert not any(kb.kv_device_errors().values())
+
+
+@pytest.mark.parametrize("left", ["minus one", "another's block"])
+@pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("bt", [16, 32, 64, 128])
+@pytest.mark.parametrize("H,D", [(2, 64), (1, 128), (1, 256), (1, 48)])
+def test_blocks_before_the_window_are_not_needed(lib, H, D, bt, fmt, left):
+    """A host that frees the blocks which a window has left behind puts anything into
+    their table entries: the same bits come out, and nothing is reported."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T, G = 700, 4
+    nb = -(-T // bt)
+    dev = kb.KVCache.empty(nb + 1, H, D, bt, dtype=fmt)
+    for c, s in ((dev.k, dev.k_scale), (dev.v, dev.v_scale)):   # block 0: what nobody wrote
+        c.view(torch.uint8)[0] = 0x7F
+        s[0] = float("nan")
+    table = torch.arange(nb, 0, -1, dtype=torch.int32, device="cuda")[None]
+    K, V = (torch.randn(T, H, D, device="cuda", generator=g) for _ in "kv")
+    kb.kv_write(dev, K, V, one_range(table, 0, T))
+    for c in (dev.k, dev.v):          # nor the last block's rest
+        if T % bt:
+            c.view(torch.uint8)[1, :, T % bt:] = 0x7F
+    kb.kv_device_errors(clear=True)
+    for n in (1, 2, 70, 300):
+        for window in (1, 5, 12, 16, 17, 40, 130):
+            q = torch.randn(n, H * G, D, device="cuda", generator=g).to(torch.float16)
+            P = kb.attn_params(H * G, scale=D ** -0.5, window=window)
+            want = attend(dev, q, one_range(table, T - n, n), P)
+            assert torch.isfinite(want).all()
+            freed = table.clone()
+            freed[0, :max(0, T - n - window + 1) // bt] = -1 if left == "minus one" else 0
+            got = attend(dev, q, one_range(freed, T - n, n), P)
+            assert not any(kb.kv_device_errors(clear=True).values()), (n, window)
+            assert torch.equal(got, want), (n, window)
