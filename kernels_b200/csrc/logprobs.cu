@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 9) logprobs_kernel(const __grid_cons
                 for (int i = 0; i < 2; ++i) E2[i] = f * fmaf(L2[i], b, E2[i]), L2[i] *= f;
             }
             ref = gm;
-            lim = gm + reach;
+            lim = __fadd_rd(gm, reach);   // (rounded up, it might let 2^128 through)
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
