@@ -66,6 +66,9 @@ __device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it)
         bool here = false;   // x is one of its items: they start at or before x, the next one's after
         if (s < a.n_seqs) {
             const int c = a.cu[s], e = a.cu[s + 1], st = a.start[s];
+            // (a sequence of fewer than no tokens may have no items that would tell; the last
+            // CTA looks at every sequence up to the last or to one that it finds too long)
+            if (e < c) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
             here = (s == 0 || ((uint32_t)c >> a.bt_log2) + 2 * s <= x) &&
                    (s + 1 == a.n_seqs || ((uint32_t)e >> a.bt_log2) + 2 * (s + 1) > x);
             if (here) sh_seq[0] = s, sh_seq[1] = c, sh_seq[2] = e, sh_seq[3] = st;
