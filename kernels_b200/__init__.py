@@ -347,10 +347,11 @@ def _dtype_code(dtype) -> int:
 _RAW_STREAM: list = []
 
 
-def _raw_stream(stream) -> int:
-    """_s() without a Stream object for the usual case, the current stream."""
-    if stream is not None:
-        return stream if isinstance(stream, int) else stream.cuda_stream
+def _raw_stream(stream, dev: int) -> int:
+    """_s() without a Stream object for the usual case, the current stream; the
+    tensors' device must be the current one."""
+    if dev < 0:
+        raise ValueError("the tensors must be on a GPU")
     if not _RAW_STREAM:
         import torch
         torch.cuda.current_stream()      # (CUDA is initialised from here on)
@@ -359,7 +360,12 @@ def _raw_stream(stream) -> int:
         except AttributeError:
             _RAW_STREAM.extend((lambda d: torch.cuda.current_stream(d).cuda_stream,
                                 torch.cuda.current_device))
-    return _RAW_STREAM[0](_RAW_STREAM[1]())
+    now = _RAW_STREAM[1]()
+    if now != dev:
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{now}")
+    if stream is not None:
+        return stream if isinstance(stream, int) else stream.cuda_stream
+    return _RAW_STREAM[0](now)
 
 
 def _ints(t, name: str):
@@ -371,22 +377,41 @@ def _ints(t, name: str):
     return t
 
 
-def _heads(t, heads: int, dim: int) -> Heads:
+def _elsewhere(t, dev: int):
+    raise ValueError(f"expected a tensor on {f'cuda:{dev}' if dev >= 0 else 'the CPU'}, "
+                     f"not on {t.device}")
+
+
+def _one_device(*tensors) -> int:
+    """The GPU that all of them are on; -1 for the CPU (calls refuse it)."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev:
+            _elsewhere(t, dev)
+    return dev
+
+
+def _heads(t, heads: int, dim: int, dev: int) -> Heads:
     """A [tokens, heads, dim] tensor with any token and head strides."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
         raise ValueError(f"expected a [tokens, {heads}, {dim}] tensor, not {tuple(shape)}")
     if stride[2] != 1 and dim > 1:
         raise ValueError("the last dimension must be contiguous")
-    return Heads(t.data_ptr(), stride[0], stride[1], shape[0], _dtype_code(t.dtype))
+    code = _dtype_code(t.dtype)
+    if t.get_device() != dev:
+        _elsewhere(t, dev)
+    return Heads(t.data_ptr(), stride[0], stride[1], shape[0], code)
 
 
-def _dense(t, dtype, shape) -> int | None:
+def _dense(t, dtype, shape, dev: int) -> int | None:
     """The address of a contiguous tensor of that type and shape; None for None."""
     if t is None:
         return None
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"expected a contiguous {dtype} {tuple(shape)} tensor")
+    if t.get_device() != dev:
+        _elsewhere(t, dev)
     return t.data_ptr()
 
 
@@ -407,6 +432,7 @@ class KVCache:
                 raise ValueError("scales must be fp32 [n_blocks, kv_heads]")
         if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
             raise ValueError("the cache's tensors must be contiguous")
+        self.dev = _one_device(k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         n, h, bt, d = k.shape
         self.desc = KVCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), n, h, bt, d,
@@ -436,6 +462,7 @@ class KVRange:
             raise ValueError("start must be [n_seqs] and cu_tokens [n_seqs + 1]")
         self._keep = (_ints(block_table, "block_table"), _ints(start, "start"),
                       _ints(cu_tokens, "cu_tokens"))
+        self.dev = _one_device(block_table, start, cu_tokens)
         stride = block_table.stride(0) if n > 1 else block_table.shape[1]
         self.desc = KVRangeDesc(_p(block_table), _p(start), _p(cu_tokens), n, stride, max_tokens,
                                 max_len)
@@ -451,9 +478,11 @@ def kv_range(block_table, start, cu_tokens, max_tokens: int, max_len: int) -> KV
 
 
 def _kv_move(name: str, cache: KVCache, K, V, rng: KVRange, stream) -> None:
-    h, d = cache.heads, cache.dim
-    call(name, cache.ref, C.byref(_heads(K, h, d)), C.byref(_heads(V, h, d)), rng.ref,
-         _raw_stream(stream))
+    h, d, dev = cache.heads, cache.dim, cache.dev
+    K, V = _heads(K, h, d, dev), _heads(V, h, d, dev)
+    if rng.dev != dev:
+        raise ValueError("the cache and the range are on different devices")
+    call(name, cache.ref, C.byref(K), C.byref(V), rng.ref, _raw_stream(stream, dev))
 
 
 def kv_write(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
@@ -481,30 +510,43 @@ def attn_params(q_heads: int, dtype=None, scale: float = 1.0, window: int = 0) -
     return AttnParams(q_heads, window, scale)
 
 
+def _scratch(n: int, init: str, device):
+    """A zeroed workspace of n bytes: buffer, 256-byte aligned address, device."""
+    import torch
+    buffer = torch.empty(n + 256, dtype=torch.uint8, device=device)
+    addr, dev = (buffer.data_ptr() + 255) & ~255, buffer.get_device()
+    call(init, addr, n, _raw_stream(None, dev))
+    return buffer, addr, dev
+
+
 class AttnWorkspace:
     """The scratch of attn_kv8 for a cache, a range's bounds and params."""
 
     def __init__(self, cache: KVCache, rng: KVRange, P: AttnParams, device=None):
-        import torch
         n = load().graft_attn_kv8_workspace(C.byref(cache.desc), C.byref(rng.desc), C.byref(P))
         if n == 0:
             raise GraftError("graft_attn_kv8_workspace", 1,
                              load().graft_last_error_string().decode())
-        self.buffer = torch.empty(n + 256, dtype=torch.uint8, device=device or cache.k.device)
-        self.addr, self.nbytes = (self.buffer.data_ptr() + 255) & ~255, n
-        call("graft_attn_kv8_init", self.addr, n, _s(None))
+        self.buffer, self.addr, self.dev = _scratch(n, "graft_attn_kv8_init", device or cache.k.device)
+        self.nbytes = n
 
 
 def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorkspace, sinks=None,
              lse=None, stream=None) -> None:
     """Attention of the range's tokens (q and out [tokens, q_heads, head_dim])
     over the cache (graft_attn_kv8)."""
-    d, hq = cache.dim, P.q_heads
+    d, hq, dev = cache.dim, P.q_heads, cache.dev
     if sinks is not None or lse is not None:
         from torch import float32
-        sinks, lse = _dense(sinks, float32, (hq,)), _dense(lse, float32, (q.shape[0], hq))
-    call("graft_attn_kv8", cache.ref, C.byref(_heads(q, hq, d)), C.byref(_heads(out, hq, d)),
-         rng.ref, sinks, lse, C.byref(P), ws.addr, ws.nbytes, _raw_stream(stream))
+        sinks, lse = (_dense(sinks, float32, (hq,), dev),
+                      _dense(lse, float32, (q.shape[0], hq), dev))
+    q, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
+    if rng.dev != dev:
+        raise ValueError("the cache and the range are on different devices")
+    if ws.dev != dev:
+        raise ValueError("the workspace is on another device than the tensors")
+    call("graft_attn_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, sinks, lse, C.byref(P),
+         ws.addr, ws.nbytes, _raw_stream(stream, dev))
 
 
 # ------------------------------------------------------ log probabilities --
@@ -516,14 +558,12 @@ class LogprobWorkspace:
     """The scratch of logprobs."""
 
     def __init__(self, P: LogprobParams, device=None):
-        import torch
         n = load().graft_logprobs_workspace(C.byref(P))
         if n == 0:
             raise GraftError("graft_logprobs_workspace", 1,
                              load().graft_last_error_string().decode())
-        self.buffer = torch.empty(n + 256, dtype=torch.uint8, device=device or "cuda")
-        self.addr, self.nbytes = (self.buffer.data_ptr() + 255) & ~255, n
-        call("graft_logprobs_init", self.addr, n, _s(None))
+        self.buffer, self.addr, self.dev = _scratch(n, "graft_logprobs_init", device or "cuda")
+        self.nbytes = n
 
 
 def logprobs(logits, targets, logprob, entropy, top_logprob, top_index, P: LogprobParams,
@@ -537,12 +577,15 @@ def logprobs(logits, targets, logprob, entropy, top_logprob, top_index, P: Logpr
     stride = logits.stride()
     if stride[1] != 1 and vocab > 1:
         raise ValueError("a row of logits must be contiguous")
-    args = (_dense(targets, int32, (rows,)), _dense(logprob, float32, (rows,)),
-            _dense(entropy, float32, (rows,)), _dense(top_logprob, float32, (rows, k)),
-            _dense(top_index, int32, (rows, k)))
+    dev = logits.get_device()
+    args = (_dense(targets, int32, (rows,), dev), _dense(logprob, float32, (rows,), dev),
+            _dense(entropy, float32, (rows,), dev), _dense(top_logprob, float32, (rows, k), dev),
+            _dense(top_index, int32, (rows, k), dev))
     Q = LogprobParams(rows, vocab, k, P.dtype, stride[0] if rows > 1 else vocab, P.scale)
-    call("graft_logprobs", logits.data_ptr(), *args, C.byref(Q), ws.addr, ws.nbytes,
-         _raw_stream(stream))
+    raw = _raw_stream(stream, dev)
+    if ws.dev != dev:
+        raise ValueError("the workspace is on another device than the tensors")
+    call("graft_logprobs", logits.data_ptr(), *args, C.byref(Q), ws.addr, ws.nbytes, raw)
 
 
 # ----------------------------------------------------------- multi-GPU --
