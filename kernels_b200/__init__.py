@@ -437,7 +437,7 @@ class KVCache:
         n, h, bt, d = k.shape
         self.desc = KVCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), n, h, bt, d,
                                 formats[k.dtype])
-        self.ref, self.heads, self.dim = C.byref(self.desc), h, d
+        self.ref, self.heads, self.dim, self.block_tokens = C.byref(self.desc), h, d, bt
 
     @classmethod
     def empty(cls, n_blocks: int, kv_heads: int, head_dim: int, block_tokens: int = 64,
@@ -466,6 +466,8 @@ class KVRange:
         stride = block_table.stride(0) if n > 1 else block_table.shape[1]
         self.desc = KVRangeDesc(_p(block_table), _p(start), _p(cu_tokens), n, stride, max_tokens,
                                 max_len)
+        # (a row may be a slice of a wider table: the library sees only its stride)
+        self.blocks, self.max_len = block_table.shape[1] if n else 1 << 31, max_len
         self.ref = C.byref(self.desc)
 
 
@@ -477,11 +479,18 @@ def kv_range(block_table, start, cu_tokens, max_tokens: int, max_len: int) -> KV
     return KVRange(block_table, start, cu_tokens, max_tokens, max_len)
 
 
+def _bad_range(cache: KVCache, rng: KVRange):
+    if rng.dev != cache.dev:
+        raise ValueError("the cache and the range are on different devices")
+    raise ValueError(f"a block table of {rng.blocks} blocks of {cache.block_tokens} tokens a "
+                     f"sequence does not hold max_len {rng.max_len}")
+
+
 def _kv_move(name: str, cache: KVCache, K, V, rng: KVRange, stream) -> None:
     h, d, dev = cache.heads, cache.dim, cache.dev
     K, V = _heads(K, h, d, dev), _heads(V, h, d, dev)
-    if rng.dev != dev:
-        raise ValueError("the cache and the range are on different devices")
+    if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
+        _bad_range(cache, rng)
     call(name, cache.ref, C.byref(K), C.byref(V), rng.ref, _raw_stream(stream, dev))
 
 
@@ -541,8 +550,8 @@ def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorksp
         sinks, lse = (_dense(sinks, float32, (hq,), dev),
                       _dense(lse, float32, (q.shape[0], hq), dev))
     q, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
-    if rng.dev != dev:
-        raise ValueError("the cache and the range are on different devices")
+    if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
+        _bad_range(cache, rng)
     if ws.dev != dev:
         raise ValueError("the workspace is on another device than the tensors")
     call("graft_attn_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, sinks, lse, C.byref(P),
