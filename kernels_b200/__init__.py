@@ -372,7 +372,7 @@ def _ints(t, name: str):
     import torch
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, not {t.dtype}")
-    if t.stride(-1) != 1 and t.numel() > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous")
     return t
 
@@ -401,7 +401,9 @@ def _heads(t, heads: int, dim: int, dev: int) -> Heads:
     code = _dtype_code(t.dtype)
     if t.get_device() != dev:
         _elsewhere(t, dev)
-    return Heads(t.data_ptr(), stride[0], stride[1], shape[0], code)
+    # (the stride of a single token or head is any number)
+    return Heads(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0,
+                 shape[0], code)
 
 
 def _dense(t, dtype, shape, dev: int) -> int | None:
