@@ -160,44 +160,5 @@ __device__ __forceinline__ float bf16_row_exponent(float amax) {
     return (float)max(e, -126);
 }
 
-// ---- the split of the work
-// Units (fixed numbers of keys) of all (sequence, tile, head) "pairs" lie in
-// one row, each pair preceded by `pad` empty ones that stand for what a pair
-// costs besides its units (queries, joining the warps, output).  CTA c of G
-// takes those from x_c to x_{c+1}, where the x_c cut the row evenly (the first
-// U % G shares are one longer), each moved to its pair's edge if it would
-// leave a piece of less than `snap` units.  A pair that is cut has as its first
-// piece the CTA before the first cut, and each CTA holds at most one first
-// piece and one later piece, so two partial slots and one counter per CTA are
-// enough.  The few-row kernel counts in its units (U < 2^31, the host's check),
-// the kernel for many rows in keys, whose sums over row tiles have a closed form.
-template <typename T>
-struct Split {
-    T U, share;              // share = U / G, longer = U % G
-    int G, pad, snap, longer;
-    __device__ __forceinline__ void set(T units, int ctas, int pad_units, int snap_units) {
-        U = units, G = ctas, pad = pad_units, snap = snap_units;
-        share = U / G, longer = (int)(U - share * G);
-    }
-    __device__ __forceinline__ T bound(int c) const { return c * share + min(c, longer); }
-    // the first CTA whose bound is x or more
-    __device__ __forceinline__ int at_least(T x) const {
-        const T head = longer * (share + 1);
-        return (int)(x <= head ? (x + share) / (share + 1) : longer + (x - head + share - 1) / share);
-    }
-    __device__ __forceinline__ T snapped(T x, T p0, T p1) const {
-        const bool head = x < p0 + pad + snap, tail = x > p1 - snap;
-        return !head && !tail ? x : !tail || (head && x - p0 <= p1 - x) ? p0 : p1;
-    }
-    // cuts inside [p0, p1): CTAs ca..cb start there (none if cb < ca)
-    __device__ __forceinline__ void cuts(T p0, T p1, int& ca, int& cb) const {
-        const T lo = p0 + pad + snap, hi = p1 - snap;
-        ca = 0, cb = -1;
-        if (lo > hi) return;
-        ca = at_least(lo);
-        cb = at_least(hi + 1) - 1;
-    }
-};
-
 }  // namespace dev
 }  // namespace graft

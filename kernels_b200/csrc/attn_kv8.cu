@@ -61,8 +61,9 @@ int launch_few(AttnArgs a, cudaStream_t st) {
     a.pad_units = 3 * kFewWarps;
     const uint64_t units = keys / kFewUnit<DP> + 2 + a.pad_units;
     const uint64_t pairs = (uint64_t)a.n_seqs * a.heads;
-    GRAFT_REQUIRE(pairs * units < (1ull << 31), "max_len %u of %u sequences is too long", a.max_len,
-                  a.n_seqs);
+    // (units and a piece's edge beyond them are counted in 31 bits)
+    GRAFT_REQUIRE(pairs * units < (1ull << 31) - a.pad_units - a.min_units,
+                  "max_len %u of %u sequences is too long", a.max_len, a.n_seqs);
     const uint64_t want = std::max(2 * pairs, pairs * units / a.min_units + 1);
     const int grid = (int)std::min<uint64_t>(std::min(di.sm_count * per_sm, kAttnMaxGrid), want);
     return launch_pdl("attn_kv8", kern, dim3(grid), kFewThreads, smem, st, a, err);
