@@ -1,5 +1,6 @@
-"""Attention over the 8-bit cache where it can go wrong at the edges: windows
-without a limit."""
+"""Attention over the 8-bit cache where it can go wrong at the edges: windows without a
+limit and blocks they have left behind, scores that rise from unit to unit, huge and far
+apart ones, scales that are zero, negative or no numbers."""
 from __future__ import annotations
 
 import numpy as np
@@ -204,3 +205,38 @@ def test_blocks_before_the_window_are_not_needed(lib, H, D, bt, fmt, left):
             got = attend(dev, q, one_range(freed, T - n, n), P)
             assert not any(kb.kv_device_errors(clear=True).values()), (n, window)
             assert torch.equal(got, want), (n, window)
+
+
+@pytest.mark.parametrize("n,D,below", [(n, D, b) for n, D in ((1, 64), (4, 64), (1, 128), (1, 256), (60, 128))
+                                       for b in (10.3, 16.3, 23.3)] +
+                         [(60, D, b) for D in (64, 48, 256) for b in (10.3, 16.3)])
+@pytest.mark.parametrize("alike", [False, True])
+def test_many_keys_far_below_the_largest(lib, alike, n, D, below):
+    """One key of value zero takes the weight; the output is what thousands of others add,
+    each `below` (log2) under it: down to 2^-17 of the largest (2^-24 where the reference is
+    found first) their weights keep fp16's 11 bits, also where all are rounded alike."""
+    g = torch.Generator().manual_seed(0)
+    T, bt = 4000, 64
+    kc = torch.zeros(T, 1, D)
+    kc[7, 0, 0] = 100
+    if not alike:
+        kc[:, 0, 1:] = torch.randint(-1, 2, (T, D - 1), generator=g).float()
+    vc = torch.randint(20, 128, (T, 1, D), generator=g).float()
+    vc[7] = 0
+    nb = -(-T // bt)
+    dev, table = raw_cache(kc, vc, torch.ones(nb, 1), torch.full((nb, 1), 0.01), bt)
+    q = torch.zeros(n, 8, D)
+    q[:, :, 0] = 1 - 0.005 * torch.arange(8)
+    q[:, :, 1:] = 0.01 * torch.randn(n, 8, D - 1, generator=g)
+    check_against_formula(dev, table, q.half().cuda(), T, below / 100 / 1.4426950408889634)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+@pytest.mark.parametrize("n,D", [(1, 64), (4, 64), (60, 64), (60, 128), (60, 256)])
+def test_scales_that_are_not_positive(lib, n, D, scale):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    T = 500
+    K, V = (torch.randn(T, 1, D, device="cuda", generator=g) for _ in "kv")
+    dev, table = cache_of(K, V)
+    q = torch.randn(n, 8, D, device="cuda", generator=g).half()
+    check_against_formula(dev, table, q, T, scale)
