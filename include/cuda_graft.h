@@ -487,7 +487,8 @@ int graft_moe_block_ep(graft_comm_t comm, const void* pool, const void* R, const
  *   scales [n_blocks][kv_heads]                          value = code * scale
  * Codes are signed integers in [-127, 127] (GRAFT_KV_INT8) or 8-bit floats
  * with 4 exponent and 3 mantissa bits, largest value 448 (GRAFT_KV_E4M3);
- * scales are not negative (one below 2^-64 counts as 2^-64 for values).
+ * scales are finite and not negative.  graft_kv_write stores none below 2^-64;
+ * attention takes a smaller one of V for 2^-64.
  * Constraints: block_tokens 16, 32, 64 or 128; head_dim a multiple of 16, at
  * most 256; code pointers 16-byte aligned, scale pointers 4-byte aligned. */
 enum { GRAFT_KV_INT8 = 0, GRAFT_KV_E4M3 = 1 };
@@ -570,6 +571,13 @@ typedef struct {
  *   lse = log( sum_j exp(scale q.k_j)  [+ exp(sinks[h])] ).
  * Blocks wholly before the window of a sequence's first new token are not
  * read, nor are their entries in the block table.
+ * Scores, maxima and sums are fp32; the weights of the second product are
+ * rounded to fp16: with all its 11 bits down to 2^-13 of a row's largest at
+ * least, and as 0 from 2^-25 on at the earliest (2^-24 and 2^-35 where few rows
+ * are taken or head_dim is 65 to 128).  In lse and in the sum that the output is
+ * divided by they count in full.
+ * A value's scale counts as part of its weight here.  exp2, log2 and the last
+ * division are the device's approximate ones (about 2^-22).
  * q and out: GRAFT_F16 or GRAFT_BF16, the same type.  sinks (fp32 [q_heads], a
  * score that takes weight but has no value) and lse (fp32 [tokens][q_heads])
  * may be null.  Few rows a key/value head (max_tokens * q_heads/kv_heads up to

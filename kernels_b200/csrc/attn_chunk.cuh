@@ -23,11 +23,12 @@
 // a cut pair meet in the workspace (Split in attn_common.cuh).
 //
 // What bounds it: the softmax warps.  Chunks of 1024, 777 and 57 tokens behind 1024 to
-// 4001 cached ones, 64 query heads on 8 of 64: 169 us, 430 TFLOP/s; tensor pipe 18%,
-// MUFU 38%, 0.46 instructions a cycle.  A half of 64 keys takes a tile's warps about
-// 1450 cycles, of which 512 are the exponentials of two tiles on one scheduler's MUFU; without
-// the exponentials the call takes 143 us, without any softmax 119, without the
-// conversion 170, without P V 175.
+// 4001 cached ones, 64 query heads on 8 of 64: 172 us, 423 TFLOP/s; 2048 last tokens of
+// 5120: issue 39%, tensor pipe 23% (281 us cold).  An SM ends a half of 64 keys every 1400 cycles
+// (at 1.9 GHz), so each of its two tiles' warps take about 2800 for one: a chain of waiting,
+// loading, exponentials and storing, in which the exponentials of both tiles keep the MUFU busy
+// for 1024.  When the call took 169 us, it took 143 without the exponentials, 119 without any
+// softmax, 170 without the conversion and 175 without P V.
 #pragma once
 #include "attn_common.cuh"
 
@@ -57,8 +58,10 @@ struct Chunk {
     static constexpr int O_COL = DP <= 64 ? 384 : 256;
     // Weights are 2^(t - m), the reference m SHIFT below the largest t that it was taken
     // from.  Where a half is weighed before its maximum is known, fp16 leaves room for scores
-    // up to 12 (in log2) above that, and keeps its 11 bits down to 17 below it; the reference
-    // goes up only near that limit, because O's rescaling waits for the product before.
+    // up to 12 (in log2) above that, and keeps its 11 bits down to 17 below it (nothing is left
+    // 28 below); the reference goes up only near that limit, because O's rescaling waits for
+    // the product before.  (Shifts of 5 and 8, which keep more, make it go up more often:
+    // the chunks above 177 and 187 us, 172 with 3.)
     static constexpr float SHIFT = BESIDE ? 3.f : kPShift;
     static constexpr int SC = 8;                     // slots of a unit's scales (up to ST + 2 in use)
     // floats of a partial result: O column by column, reference and sum of each row

@@ -21,12 +21,15 @@
 // of weights is that of 2^(t - max t) / v_scale, in fp32.
 //
 // What bounds it: HBM in long calls of wide heads (64 sequences of up to 8192 keys,
-// 8 heads of 128, 4 query heads each, e4m3: 101 us, 5.3 TB/s; 32 of up to 8192, 8
+// 8 heads of 128, 4 query heads each, e4m3: 102 us, 5.3 TB/s; 32 of up to 8192, 8
 // heads of 256: 101 us, 5.3 TB/s); with heads of 64 instruction issue as much (430 to
-// 500 warp instructions a unit of 4 KB, 55% of the issue slots).  One sequence of 131071 keys, 8 heads of 64, 64
-// query heads: 38.4 us, of which the stream is 21, the start (lengths, block numbers,
-// first copies) 3.5 and the joins 7.  Short calls are a chain of latencies: 517 keys 7.7 us,
-// 32 sequences with a window of 128 and two tokens each 13.4 us.
+// 500 warp instructions a unit of 4 KB, 48% of the issue slots).  One sequence of 131071
+// keys, 8 heads of 64, 64 query heads: 38.2 us, of which the stream is 21, the start (lengths,
+// block numbers, first copies) 3.5 and the joins 7; where the other 7 go has not been found.
+// Short calls are a chain of latencies: 517 keys 7.5 us, 32 sequences with a window of 128 and
+// two tokens each 9.8 us.  17 to 32 rows take one CTA an SM (registers), whose 8 warps hide
+// little: 32 sequences of up to 8192 keys 76 us, with 8 rows 41.
+// Spills: instances for 16 rows of 64 dims 56 to 104 bytes, for 8 rows 28 to 40.
 #pragma once
 #include "attn_common.cuh"
 

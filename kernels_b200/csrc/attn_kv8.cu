@@ -8,9 +8,9 @@
 // pass over the keys at the rate of HBM.  More rows go to the kernel of
 // attn_chunk.cuh (tcgen05), whose tiles have 128 rows whether they are full or not.
 // Both sides of the rule, in us (64 query heads on 8 of 64; 32 on 8 of 128; 16 on 8 of 256):
-//   131071 keys, 8 rows 38 | 148, 32 rows 67 | 150
-//   32 sequences of up to 8192 keys, 8 rows 41 | 143, 16 rows 59 | 143, 32 rows 76 | 144
-//   the same, heads of 128: 4 rows 57 | 199, 16 rows 93 | 201;  of 256: 8 rows 103 | 374
+//   131071 keys, 8 rows 38 | 153, 32 rows 67 | 154
+//   32 sequences of up to 8192 keys, 8 rows 41 | 146, 16 rows 52 | 146, 32 rows 76 | 148
+//   the same, heads of 128: 4 rows 57 | 200, 16 rows 92 | 204;  of 256: 8 rows 104 | 374
 #include "attn_chunk.cuh"
 #include "attn_few.cuh"
 
@@ -55,8 +55,8 @@ int launch_few(AttnArgs a, cudaStream_t st) {
     const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
                                    : a.max_len;
     // A CTA's share is at least two units a warp, and a piece of a pair costs about three
-    // more (queries, first copies, join): 32 sequences with windows of 128 keys took 15.8 us
-    // without the pad and 13.4 with it, 64 of up to 8192 keys 116 and 101.
+    // more (queries, first copies, join): 32 sequences with windows of 128 keys take 27 us
+    // without the pad and 9.8 with it, 64 of up to 8192 keys 122 and 102.
     a.min_units = 2 * kFewWarps;
     a.pad_units = 3 * kFewWarps;
     const uint64_t units = keys / kFewUnit<DP> + 2 + a.pad_units;

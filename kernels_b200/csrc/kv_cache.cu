@@ -16,10 +16,11 @@
 // block it can touch whatever its start, so no prefix sum of block counts is
 // needed (a CTA past its sequence's blocks returns).
 //
-// Measured: reading 65521 tokens of 8 heads of 128 back in fp16 70.5 us, 5.7 TB/s; writing
-// them 84 us, 4.8 TB/s (instruction issue: rounding a code costs about seven instructions);
-// writing 7687 tokens of 8 heads of 64 and reading them back 14.1 us; one token of 64
-// sequences (8 heads of 128), written and its block read back, 7.8 us.
+// Measured: reading 65521 tokens of 8 heads of 128 back in fp16 71 us, 5.7 TB/s; writing
+// them 84 us, 4.8 TB/s (instruction issue, 67% of the slots: 13 warp instructions for 32 codes);
+// the same in fp32 157 and 168 us, 4.3 and 4.0 TB/s; writing 7687 tokens of 8 heads of 64 and
+// reading them back 14.0 us; one token of 64 sequences (8 heads of 128), written and its block
+// read back, 7.6 us.
 #include "kv_common.cuh"
 
 #include <algorithm>
@@ -410,7 +411,8 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     // Writing, a CTA a (head, K or V): 8 chunks of 8 elements a thread (what every thread does
     // once costs as much as two chunks), or 4 where that makes fewer than 128 threads.
     // 65521 tokens, blocks of 64, written and read back: 8 heads of 128 154 us so and 166 with
-    // 4 chunks; 8 heads of 64 76 with 4 chunks (128 threads) and 78 with 8.  Where most CTAs would be nearly empty and many, a warp each, eight to a CTA:
+    // 4 chunks; 8 heads of 64 76 with 4 chunks (128 threads) and 78 with 8.  Where most CTAs
+    // would be nearly empty and many, a warp each, eight to a CTA:
     //   one token of 64 sequences (8 heads of 128)      a chunk a lane 7.8 us, a CTA 10
     //   8 tokens of 256 sequences (8 heads of 64)       a warp 16.3 us, a CTA 22.0
     //   8 tokens of 64                                  a warp 10.3 us, a CTA 10.4
@@ -419,13 +421,16 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     const uint32_t most = std::min(range->max_tokens, a.bt) * a.cpt;   // chunks of an item
     DeviceInfo di;
     if (const int rc = current_device_info(&di)) return rc;
-    const bool sparse = 2 * (uint64_t)range->max_tokens <= a.bt && items * 2 * a.heads > 16ull * di.sm_count;
+    const bool sparse = 2 * (uint64_t)range->max_tokens <= a.bt &&
+                        items * 2 * a.heads > 16ull * di.sm_count;
     const Form form = !write                                ? kRead
                       : most <= 32                          ? kWriteOne
                       : most <= kWarpChunks && sparse       ? kWriteWarp
                                                             : kWriteCta;
-    const int whole = (int)(a.bt * a.cpt), fourth = (whole / 4 + 31) / 32 * 32, eighth = (whole / 8 + 31) / 32 * 32;
-    const int threads = form != kWriteCta ? 256 : std::min(512, std::max({64, eighth, std::min(fourth, 128)}));
+    const int whole = (int)(a.bt * a.cpt);
+    const int fourth = (whole / 4 + 31) / 32 * 32, eighth = (whole / 8 + 31) / 32 * 32;
+    const int threads = form != kWriteCta
+                            ? 256 : std::min(512, std::max({64, eighth, std::min(fourth, 128)}));
     const int chunks = (int)(a.bt * a.cpt + threads - 1) / threads;
     const uint32_t ny = form == kRead      ? 2 * ((a.heads + a.cta_heads - 1) / a.cta_heads)
                         : form == kWriteCta ? 2 * a.heads : (2 * a.heads + 7) / 8;

@@ -9,8 +9,10 @@
 // 16 bytes, d = (x - ref) scale log2(e), against a reference of its own that moves
 // only when a logit passes it by 2^64: no maximum is needed first.  So
 //   lse = scale*ref + ln L,  entropy = ln L - ln2 E / L      (L = sum e, E = sum e d)
-// and HBM bounds a long call (one exponential an element keeps the MUFU at about
-// 70% at that rate for 16-bit logits).
+// In a long call of 16-bit logits nothing is at its limit: the pass runs at 4.3 TB/s, about
+// 60% of the issue slots and of the MUFU (one exponential an element); four segments a row
+// are 2.3 rounds of the CTAs that fit.  fp32 logits are bound by HBM
+// (4096 rows of 128256, 5 alternatives: 5.7 TB/s).
 //
 // The top k come from the threads' own maxima, which the pass finds on the way: each
 // thread keeps its largest logit, the round of chunks where that is first, and the
@@ -21,9 +23,13 @@
 // index: keys are (value, index) pairs, all different.  Segments meet in the workspace,
 // and the row's last CTA joins them.
 //
-// Measured: 777 rows of 128256 in fp16 (199 MB), 5 alternatives: 52.3 us, 3.8 TB/s (46 us
-// without alternatives); one row of 201088, 20 alternatives: 9.3 us, without them 4.5;
-// 37 rows of 50021 in fp32, 8 alternatives: 9.1 us, without them 5.6.
+// Measured: 777 rows of 128256 in fp16 (199 MB), 5 alternatives: 52.8 us, 3.8 TB/s (46 us
+// without alternatives); one row of 201088, 20 alternatives: 9.1 us, without them 4.5;
+// 37 rows of 50021 in fp32, 8 alternatives: 9.0 us, without them 5.6.
+// Many alternatives of rows that one or two CTAs take (2368 rows or more: one) fall off:
+// a thread with two of them in different rounds lists all its chunks, more than kList holds,
+// and the row is read once for each alternative.  4096 rows of 128256 in fp32: 5 alternatives
+// 372 us, 20 3552, 32 11855; in fp16: 197, 218, 2982.
 #include "kv_common.cuh"
 
 #include <algorithm>
