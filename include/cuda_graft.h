@@ -549,6 +549,71 @@ int graft_kv_write(const GraftKVCache* cache, const GraftHeads* K, const GraftHe
 int graft_kv_read(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
                   const GraftKVRange* range, graft_stream_t stream);
 
+/* ------------------------------------------------------- rotary positions ---
+ * A head's first `dims` elements are pairs that turn by an angle proportional to
+ * the token's position p; the others stay as they are.  Pair i has the frequency
+ * f_i (radians a position), c = amplitude cos(p f_i), s = amplitude sin(p f_i):
+ *   (x, y) -> (x c - y s, y c + x s)
+ * GRAFT_ROPE_HALF: pair i is the elements i and i + dims/2;
+ * GRAFT_ROPE_INTERLEAVED: 2i and 2i + 1.
+ * inverse != 0 turns back (s negated), which is also the gradient's path: with the
+ * forward's amplitude, dx of dy.
+ * Frequencies are held as whole 2^-64ths of a turn, so that p f_i modulo a turn
+ * is exact for every int32 position. */
+enum { GRAFT_ROPE_HALF = 0, GRAFT_ROPE_INTERLEAVED = 1 };
+typedef struct {
+    const uint64_t* turns;   /* [dims/2], device memory (graft_rope_init)     */
+    uint32_t dims;           /* a multiple of 16 up to 256                    */
+    uint32_t layout;
+    float amplitude;         /* finite                                        */
+    uint32_t inverse;
+} GraftRope;
+
+/* Frequencies, b = base, i = 0 .. dims/2 - 1:
+ *   GRAFT_ROPE_PLAIN   g_i = b^(-2i/dims)
+ *   GRAFT_ROPE_LINEAR  g_i / factor
+ *   GRAFT_ROPE_YARN    g_i (1 - r_i) + g_i/factor r_i: r_i rises from 0 to 1 between the
+ *     pairs i that turn `high` and `low` times over orig_len positions,
+ *     i(t) = dims ln(orig_len / (2 pi t)) / (2 ln b), held within [0, dims - 1]
+ *   GRAFT_ROPE_BANDS   g_i s_i + g_i/factor (1 - s_i), s_i = (t_i - low) / (high - low)
+ *     held within [0, 1], t_i = orig_len g_i / (2 pi) the pair's turns over orig_len
+ * base > 0 (not 1 with YARN), factor > 0; YARN and BANDS: orig_len > 0, 0 < low < high. */
+enum { GRAFT_ROPE_PLAIN = 0, GRAFT_ROPE_LINEAR = 1, GRAFT_ROPE_YARN = 2, GRAFT_ROPE_BANDS = 3 };
+typedef struct {
+    uint32_t dims, scaling;
+    double base, factor, orig_len, low, high;
+} GraftRopeParams;
+
+/* Fills turns [P->dims/2] (device, 16-byte aligned), in 64 bits.  freqs (device,
+ * fp64 [dims/2], radians a position) takes the place of the formulas; or null. */
+int graft_rope_init(uint64_t* turns, const double* freqs, const GraftRopeParams* P,
+                    graft_stream_t stream);
+
+/* Turns `heads` heads of head_dim elements (a multiple of 16, at most 256) of each
+ * row t of x by positions[t] (int32, device; any value).  out: the same type and
+ * number of rows; the very same buffer and strides as x (in place), or one that
+ * shares no memory with it.  The products are fp32, rounded once.  16-bit types
+ * take the device's fast sine and cosine (2^-20 of the amplitude), fp32 the full ones. */
+int graft_rope(const GraftHeads* x, const GraftHeads* out, uint32_t heads, uint32_t head_dim,
+               const int32_t* positions, const GraftRope* rope, graft_stream_t stream);
+
+/* graft_kv_write with the keys turned on the way: a key is turned in fp32 and
+ * quantised without another rounding; values are written as they are.
+ * positions (int32 [K->tokens], device): of the rows of K; null: start[b] + i.
+ * q (with q_heads heads, K's type and rows), if not null, is turned into q_out
+ * (or in place, as for graft_rope) by the same positions, row by row of the range.
+ * rows and count (device; both or neither) write a part of the range's rows, in an
+ * order of their own -- the accepted tokens of a drafted tree to their final places:
+ * sequence b's tokens i = 0 .. count[b] - 1 <= n_b - 1 are the rows
+ * rows[cu_tokens[b] + i] of K and V, at positions start[b] + i of the sequence
+ * (the positions that keys are turned by: positions[row], or start[b] + i).  With
+ * them q must be null.  A row outside the buffer is reported as GRAFT_KV_EBOUNDS
+ * and written as zeros. */
+int graft_kv_write_rope(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                        const GraftKVRange* range, const GraftRope* rope, const int32_t* positions,
+                        const int32_t* rows, const int32_t* count, const GraftHeads* q,
+                        const GraftHeads* q_out, uint32_t q_heads, graft_stream_t stream);
+
 /* Device-side findings of the cache and attention kernels, or-ed together:
  * GRAFT_KV_EBLOCK: a block number outside the cache; GRAFT_KV_EBOUNDS: lengths
  * beyond max_tokens, max_len, the block table or a buffer; GRAFT_KV_EWAIT: a
@@ -593,6 +658,34 @@ int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHe
                    const GraftKVRange* range, const float* sinks, float* lse,
                    const GraftAttnParams* P, void* ws, size_t ws_bytes, graft_stream_t stream);
 
+/* ------------------------------------------- trees of drafted tokens -------
+ * The new tokens of a sequence may be a tree: its root, the newest token that is
+ * certain, and drafted ones, each after a parent.  In the cache they lie one after the
+ * other at start[b] .. start[b] + n_b - 1 like any new tokens; which of them a token sees
+ * is told by bits: bit j of row t of `mask` (int32 [tokens][mask_stride], bit j in word
+ * j / 32) says that token t sees its sequence's new token j.  A token sees the keys
+ * before start[b] as well: all, or with a window those above positions[t] - window.
+ *
+ * graft_draft_tree makes masks and positions of parents (int32 [tokens], indices within
+ * the sequence's new tokens; a parent comes before its children, anything else is no
+ * parent): token i sees itself and its ancestors, positions[t] = start + its depth,
+ * and with a window only what lies within it.  words: of a mask row,
+ * at least max_tokens / 32 rounded up (those behind are zeroed); positions may be null. */
+int graft_draft_tree(const int32_t* parents, const GraftKVRange* range, uint32_t tokens,
+                     uint32_t window, int32_t* mask, uint64_t mask_stride, uint32_t words,
+                     int32_t* positions, graft_stream_t stream);
+
+/* graft_attn_kv8 with masks: as described there, but for the keys that a token sees.
+ * mask: int32, 4-byte aligned, mask_stride words from row to row (max_tokens / 32 rounded up
+ * at least); bits beyond a sequence's tokens count for nothing.  positions (int32 [tokens],
+ * at least start[b]) must be given with a window, and is not read without one.  A token
+ * that sees no key gives zeros and lse -inf (its sink alone, if there are sinks). */
+int graft_attn_tree_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
+                        const GraftKVRange* range, const int32_t* mask, uint64_t mask_stride,
+                        const int32_t* positions, const float* sinks, float* lse,
+                        const GraftAttnParams* P, void* ws, size_t ws_bytes,
+                        graft_stream_t stream);
+
 /* ======================================================== log probabilities ===
  * From rows of logits (the lm_head's output), with z = scale * logit:
  *   lse          = log sum_v exp(z_v)
@@ -621,6 +714,49 @@ int graft_logprobs_init(void* ws, size_t ws_bytes, graft_stream_t stream);
 int graft_logprobs(const void* logits, const int32_t* targets, float* logprob, float* entropy,
                    float* top_logprob, int32_t* top_index, const GraftLogprobParams* P, void* ws,
                    size_t ws_bytes, graft_stream_t stream);
+
+/* ================================================ verifying drafted tokens ===
+ * Which drafted tokens stand, and the token after them.  Rows cu_tokens[b] ..
+ * cu_tokens[b+1] - 1 are the tokens of sequence b, its root first; parents as for
+ * graft_draft_tree (null: each token's parent is the one before it).  Row i of logits
+ * gives the target's distribution of what follows token i, p = softmax(scale logits),
+ * row i of draft the one that i's children were drawn from, q = softmax(draft_scale
+ * draft) (draft null: the children were chosen, not drawn, q = 1 for each).
+ * From the root on, with r = p and R = sum r, the children c of the last accepted
+ * token are asked in their order:
+ *   c is accepted if  uniform[c] q(tokens[c]) R < r(tokens[c]);
+ *   if not, r becomes max(r - R q, 0) (without draft: 0 at tokens[c]), R its sum.
+ * When no child is accepted, `next` is the smallest v with r(v) > 0 and
+ *   sum_{w <= v} r(w) > uniform_next[b] R
+ * (the last v with r(v) > 0 if rounding leaves none).  With uniform random numbers in
+ * [0, 1), accepted tokens and next are then distributed as if drawn from the target.
+ * If uniform and uniform_next are null, verification is greedy: a child is accepted
+ * if it is the row's largest logit (the first of equal ones), which is also what next is.
+ * Results: count[b], the accepted tokens with the root (0 for a sequence without
+ * tokens); path [tokens], the rows of these at cu_tokens[b] .., -1 behind; next[b].
+ * A logit of -inf is a token that cannot come.  Where the last row gives no
+ * distribution (a NaN, +inf, or nothing possible) next is -1; a child behind such a
+ * row, or with a token outside 0..vocab-1, is never accepted and changes nothing; nor does
+ * one behind such a row of draft.  If nothing is left of r, it is p again.
+ * Sums are fp32 for the first child of a token and fp64 from then on and for next. */
+typedef struct {
+    uint32_t n_seqs, tokens;      /* sequences, rows                           */
+    uint32_t max_tokens;          /* of a sequence, at most 1024               */
+    uint32_t vocab;
+    uint32_t dtype;               /* of logits and draft                       */
+    uint64_t row_stride, draft_stride;   /* elements from row to row (>= vocab) */
+    float scale, draft_scale;     /* 2^-100 to 2^100                           */
+} GraftVerifyParams;
+
+/* logits and draft aligned to their element.  ws: graft_verify_workspace bytes, 256-byte
+ * aligned, of any content, for calls of one stream at a time.  Lengths that do not fit
+ * (cu_tokens beyond tokens or max_tokens) give count 0 and next -1. */
+size_t graft_verify_workspace(const GraftVerifyParams* P);
+int graft_verify_drafts(const void* logits, const void* draft, const int32_t* tokens,
+                        const int32_t* parents, const int32_t* cu_tokens, const float* uniform,
+                        const float* uniform_next, int32_t* count, int32_t* path, int32_t* next,
+                        const GraftVerifyParams* P, void* ws, size_t ws_bytes,
+                        graft_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -19,7 +19,7 @@ import ctypes as C
 
 from ._lib import (AttnParams, ExpertParams, ExpertScratch, GemvParams, GraftError, Heads,
                    KVCacheDesc, KVRangeDesc, LogprobParams, MoEFormat, MoEParams, MoEScratch,
-                   VQParams, VQQuantParams, call, load)
+                   RopeDesc, RopeParams, VerifyParams, VQParams, VQQuantParams, call, load)
 
 __all__ = [
     "GemvParams", "VQParams", "MoEParams", "MoEFormat", "MoEScratch", "GraftError",
@@ -33,7 +33,8 @@ __all__ = [
     "MoEWorkspace", "moe_block", "moe_block_ex", "moe_format",
     "KVCache", "kv_range", "kv_write", "kv_read", "kv_device_errors", "AttnParams",
     "attn_params", "AttnWorkspace", "attn_kv8", "LogprobParams", "logprob_params",
-    "LogprobWorkspace", "logprobs",
+    "LogprobWorkspace", "logprobs", "RopeTable", "rope", "kv_write_rope", "draft_tree",
+    "attn_tree_kv8", "VerifyParams", "verify_params", "VerifyWorkspace", "verify_drafts",
 ]
 
 
@@ -470,6 +471,7 @@ class KVRange:
                                 max_len)
         # (a row may be a slice of a wider table: the library sees only its stride)
         self.blocks, self.max_len = block_table.shape[1] if n else 1 << 31, max_len
+        self.n_seqs, self.max_tokens = n, max_tokens
         self.ref = C.byref(self.desc)
 
 
@@ -558,6 +560,191 @@ def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorksp
         raise ValueError("the workspace is on another device than the tensors")
     call("graft_attn_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, sinks, lse, C.byref(P),
          ws.addr, ws.nbytes, _raw_stream(stream, dev))
+
+
+# -------------------------------------------------------- rotary positions --
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
+
+
+class RopeTable:
+    """Rotary positions of a head's first `dims` elements (graft_rope_init): layout
+    "half" or "interleaved"; scaling "plain", "linear" (factor), "yarn" or "bands"
+    (factor, orig_len, low, high).  freqs (fp64 [dims // 2], radians a position)
+    takes the place of the formulas.  amplitude multiplies sine and cosine."""
+
+    def __init__(self, dims: int, base: float = 10000.0, layout: str = "half",
+                 scaling: str = "plain", factor: float = 1.0, orig_len: float = 0.0,
+                 low: float = 1.0, high: float = 32.0, amplitude: float = 1.0, freqs=None,
+                 device="cuda"):
+        import torch
+        if layout not in _ROPE_LAYOUTS:
+            raise ValueError(f"unknown layout {layout!r}")
+        if scaling not in _ROPE_SCALINGS:
+            raise ValueError(f"unknown scaling {scaling!r}")
+        P = RopeParams(dims, _ROPE_SCALINGS[scaling], base, factor, orig_len, low, high)
+        if not 16 <= dims <= 256:      # (before anything is allocated)
+            raise ValueError(f"dims must be a multiple of 16 up to 256, not {dims}")
+        self.turns = torch.empty(dims // 2, dtype=torch.int64, device=device)
+        self.dev = self.turns.get_device()
+        f = _dense(freqs, torch.float64, (dims // 2,), self.dev)
+        call("graft_rope_init", _p(self.turns), f, C.byref(P), _raw_stream(None, self.dev))
+        self.dims = dims
+        self.desc = RopeDesc(_p(self.turns), dims, _ROPE_LAYOUTS[layout], amplitude, 0)
+        self.back = RopeDesc(_p(self.turns), dims, _ROPE_LAYOUTS[layout], amplitude, 1)
+        self.ref, self.back_ref = C.byref(self.desc), C.byref(self.back)
+
+
+def _on(t: RopeTable, dev: int):
+    if t.dev != dev:
+        raise ValueError("the rope table is on another device than the tensors")
+
+
+def rope(x, out, positions, table: RopeTable, inverse: bool = False, stream=None) -> None:
+    """x [tokens, heads, head_dim], any token and head strides, turned by positions
+    (int32 [tokens]) into out (or in place: out is x).  inverse turns back; that is the
+    gradient of x for that of out (graft_rope)."""
+    from torch import int32
+    if x.dim() != 3:
+        raise ValueError(f"expected a [tokens, heads, head_dim] tensor, not {tuple(x.shape)}")
+    n, h, d = x.shape
+    dev = x.get_device()
+    X, Y = _heads(x, h, d, dev), _heads(out, h, d, dev)
+    p = _dense(positions, int32, (n,), dev)
+    _on(table, dev)
+    call("graft_rope", C.byref(X), C.byref(Y), h, d, p, table.back_ref if inverse else table.ref,
+         _raw_stream(stream, dev))
+
+
+def kv_write_rope(cache: KVCache, K, V, rng: KVRange, table: RopeTable, positions=None, q=None,
+                  q_out=None, rows=None, count=None, stream=None) -> None:
+    """kv_write with the keys turned on the way, and the queries q [tokens, q_heads,
+    head_dim] into q_out beside.  rows (int32 [tokens]) and count (int32 [n_seqs]): which rows
+    of K and V each sequence's first tokens are (graft_kv_write_rope)."""
+    from torch import int32
+    h, d, dev = cache.heads, cache.dim, cache.dev
+    n = K.shape[0]
+    Kd, Vd = _heads(K, h, d, dev), _heads(V, h, d, dev)
+    Q = Qo = None
+    hq = 0
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out go together")
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError(f"expected a [tokens, q_heads, {d}] tensor, not {tuple(q.shape)}")
+        hq = q.shape[1]
+        Q, Qo = C.byref(_heads(q, hq, d, dev)), C.byref(_heads(q_out, hq, d, dev))
+    positions = _dense(positions, int32, (n,), dev)
+    rows, count = _dense(rows, int32, (n,), dev), _dense(count, int32, (rng.n_seqs,), dev)
+    _on(table, dev)
+    if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
+        _bad_range(cache, rng)
+    call("graft_kv_write_rope", cache.ref, C.byref(Kd), C.byref(Vd), rng.ref, table.ref, positions,
+         rows, count, Q, Qo, hq, _raw_stream(stream, dev))
+
+
+# ---------------------------------------------------- trees of drafted tokens --
+def draft_tree(parents, rng: KVRange, mask, positions=None, window: int = 0, stream=None) -> None:
+    """Masks (int32 [tokens, words]) and positions (int32 [tokens]) of trees of new
+    tokens from their parents (int32 [tokens], -1 for a root) (graft_draft_tree)."""
+    from torch import int32
+    if mask.dim() != 2 or mask.shape[0] != parents.shape[0]:
+        raise ValueError("mask must be [tokens, words]")
+    dev = parents.get_device()
+    n, words = mask.shape
+    par = _dense(parents, int32, (n,), dev)
+    m, stride = _mask(mask, n, dev)
+    pos = _dense(positions, int32, (n,), dev)
+    if rng.dev != dev:
+        raise ValueError("the range is on another device than the tensors")
+    call("graft_draft_tree", par, rng.ref, n, window, m, stride, words, pos, _raw_stream(stream, dev))
+
+
+def _mask(mask, n: int, dev: int):
+    if mask.dim() != 2 or mask.shape[0] != n:
+        raise ValueError(f"mask must be [{n}, words]")
+    _ints(mask, "mask")
+    if mask.get_device() != dev:
+        _elsewhere(mask, dev)
+    return mask.data_ptr(), mask.stride(0) if n > 1 else mask.shape[1]
+
+
+def attn_tree_kv8(cache: KVCache, q, out, rng: KVRange, mask, P: AttnParams, ws: AttnWorkspace,
+                  positions=None, sinks=None, lse=None, stream=None) -> None:
+    """attn_kv8 where the new tokens of a sequence see each other by the bits of mask
+    (int32 [tokens, words], draft_tree); positions (int32 [tokens]) are needed with a
+    window (graft_attn_tree_kv8)."""
+    from torch import float32, int32
+    d, hq, dev = cache.dim, P.q_heads, cache.dev
+    n = q.shape[0]
+    if mask.dim() == 2 and mask.shape[1] * 32 < rng.max_tokens:
+        raise ValueError(f"mask rows of {mask.shape[1]} words do not hold {rng.max_tokens} tokens")
+    m, stride = _mask(mask, n, dev)
+    positions = _dense(positions, int32, (n,), dev)
+    sinks, lse = _dense(sinks, float32, (hq,), dev), _dense(lse, float32, (n, hq), dev)
+    q, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
+    if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
+        _bad_range(cache, rng)
+    if ws.dev != dev:
+        raise ValueError("the workspace is on another device than the tensors")
+    call("graft_attn_tree_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, m, stride, positions,
+         sinks, lse, C.byref(P), ws.addr, ws.nbytes, _raw_stream(stream, dev))
+
+
+def verify_params(n_seqs: int, tokens: int, max_tokens: int, vocab: int, dtype, scale: float = 1.0,
+                  draft_scale: float = 1.0) -> VerifyParams:
+    """n_seqs trees of at most max_tokens tokens, `tokens` rows in all; dtype: of the logits."""
+    return VerifyParams(n_seqs, tokens, max_tokens, vocab, _dtype_code(dtype), vocab, vocab, scale,
+                        draft_scale)
+
+
+class VerifyWorkspace:
+    """The scratch of verify_drafts."""
+
+    def __init__(self, P: VerifyParams, device=None):
+        import torch
+        n = load().graft_verify_workspace(C.byref(P))
+        if n == 0:
+            raise GraftError("graft_verify_workspace", 1,
+                             load().graft_last_error_string().decode())
+        self.buffer = torch.empty(n + 256, dtype=torch.uint8, device=device or "cuda")
+        self.addr, self.dev = (self.buffer.data_ptr() + 255) & ~255, self.buffer.get_device()
+        self.nbytes = n
+
+
+def _rows(t, rows: int, vocab: int, code: int, dev: int):
+    """Address and row stride of rows of logits."""
+    if t.shape != (rows, vocab) or _dtype_code(t.dtype) != code:
+        raise ValueError("logits do not match the params")
+    if t.stride(1) != 1 and vocab > 1:
+        raise ValueError("a row of logits must be contiguous")
+    if t.get_device() != dev:
+        _elsewhere(t, dev)
+    return t.data_ptr(), t.stride(0) if rows > 1 else vocab
+
+
+def verify_drafts(logits, tokens, cu_tokens, count, path, next_token, P: VerifyParams,
+                  ws: VerifyWorkspace, draft=None, parents=None, uniform=None, uniform_next=None,
+                  stream=None) -> None:
+    """Which drafted tokens stand, and the token after them: count (int32 [n_seqs]),
+    path (int32 [tokens]) and next_token (int32 [n_seqs]) from the rows of logits
+    [tokens, vocab], the tokens (int32 [tokens], each tree's root first), cu_tokens
+    (int32 [n_seqs + 1]), parents (int32 [tokens], None: a chain), the draft's logits
+    and random numbers uniform (fp32 [tokens]) and uniform_next (fp32 [n_seqs]); without
+    these, greedily (graft_verify_drafts)."""
+    from torch import float32, int32
+    B, T, V = P.n_seqs, P.tokens, P.vocab
+    dev = logits.get_device()
+    z, zs = _rows(logits, T, V, P.dtype, dev)
+    d, ds = _rows(draft, T, V, P.dtype, dev) if draft is not None else (None, V)
+    args = (z, d, _dense(tokens, int32, (T,), dev), _dense(parents, int32, (T,), dev),
+            _dense(cu_tokens, int32, (B + 1,), dev), _dense(uniform, float32, (T,), dev),
+            _dense(uniform_next, float32, (B,), dev), _dense(count, int32, (B,), dev),
+            _dense(path, int32, (T,), dev), _dense(next_token, int32, (B,), dev))
+    Q = VerifyParams(B, T, P.max_tokens, V, P.dtype, zs, ds, P.scale, P.draft_scale)
+    if ws.dev != dev:
+        raise ValueError("the workspace is on another device than the tensors")
+    call("graft_verify_drafts", *args, C.byref(Q), ws.addr, ws.nbytes, _raw_stream(stream, dev))
 
 
 # ------------------------------------------------------ log probabilities --

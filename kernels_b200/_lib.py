@@ -97,6 +97,25 @@ class LogprobParams(C.Structure):
                 ("dtype", C.c_uint32), ("row_stride", C.c_uint64), ("scale", C.c_float)]
 
 
+class RopeParams(C.Structure):
+    """GraftRopeParams: where the frequencies of rotary positions come from."""
+    _fields_ = [("dims", C.c_uint32), ("scaling", C.c_uint32), ("base", C.c_double),
+                ("factor", C.c_double), ("orig_len", C.c_double), ("low", C.c_double),
+                ("high", C.c_double)]
+
+
+class RopeDesc(C.Structure):
+    """GraftRope: frequencies, layout and amplitude of rotary positions."""
+    _fields_ = [("turns", C.c_void_p), ("dims", C.c_uint32), ("layout", C.c_uint32),
+                ("amplitude", C.c_float), ("inverse", C.c_uint32)]
+
+
+class VerifyParams(C.Structure):
+    _fields_ = [("n_seqs", C.c_uint32), ("tokens", C.c_uint32), ("max_tokens", C.c_uint32),
+                ("vocab", C.c_uint32), ("dtype", C.c_uint32), ("row_stride", C.c_uint64),
+                ("draft_stride", C.c_uint64), ("scale", C.c_float), ("draft_scale", C.c_float)]
+
+
 P = C.c_void_p
 U32 = C.c_uint32
 U64 = C.c_uint64
@@ -174,6 +193,17 @@ SIGNATURES: dict[str, tuple] = {
     "graft_attn_kv8_init": (INT, [P, SIZE, P]),
     "graft_attn_kv8": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
                              C.POINTER(KVRangeDesc), P, P, C.POINTER(AttnParams), P, SIZE, P]),
+    "graft_rope_init": (INT, [P, P, C.POINTER(RopeParams), P]),
+    "graft_rope": (INT, [C.POINTER(Heads), C.POINTER(Heads), U32, U32, P, C.POINTER(RopeDesc), P]),
+    "graft_kv_write_rope": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+                                  C.POINTER(KVRangeDesc), C.POINTER(RopeDesc), P, P, P,
+                                  C.POINTER(Heads), C.POINTER(Heads), U32, P]),
+    "graft_draft_tree": (INT, [P, C.POINTER(KVRangeDesc), U32, U32, P, U64, U32, P, P]),
+    "graft_attn_tree_kv8": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+                                  C.POINTER(KVRangeDesc), P, U64, P, P, P, C.POINTER(AttnParams),
+                                  P, SIZE, P]),
+    "graft_verify_workspace": (SIZE, [C.POINTER(VerifyParams)]),
+    "graft_verify_drafts": (INT, [P, P, P, P, P, P, P, P, P, P, C.POINTER(VerifyParams), P, SIZE, P]),
     "graft_logprobs_workspace": (SIZE, [C.POINTER(LogprobParams)]),
     "graft_logprobs_init": (INT, [P, SIZE, P]),
     "graft_logprobs": (INT, [P, P, P, P, P, P, C.POINTER(LogprobParams), P, SIZE, P]),

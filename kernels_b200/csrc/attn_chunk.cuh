@@ -153,7 +153,7 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-template <int DP, int FMT>
+template <int DP, int FMT, bool TREE>   // TREE: the new tokens are a tree
 __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
     attn_chunk_kernel(const __grid_constant__ AttnArgs a, unsigned* err) {
     using C = Chunk<DP>;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
 
     // ---- keys of a row tile and of the row tiles before it
     auto open_tile = [&](Walk& w) {
-        const int i0 = w.rt * TT, i1 = min(w.s.n, i0 + TT);
+        const int i0 = TREE ? 0 : w.rt * TT, i1 = TREE ? w.s.n : min(w.s.n, i0 + TT);
         w.k0 = first_key(a, w.s.start + i0), w.k1 = w.s.start + i1;
         w.nk = w.k1 - w.k0 + a.pad_units;
     };
@@ -210,6 +210,8 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
         w.tiles = (w.s.n + TT - 1) / TT;
     };
     auto keys_before = [&](const Walk& w, int rt) {   // rt <= tiles
+        if constexpr (TREE)
+            return (long long)rt * (w.s.start + w.s.n - first_key(a, w.s.start) + a.pad_units);
         return tile_keys(w.s.start, w.s.n, TT, w.tiles, rt, (int)a.window, a.pad_units);
     };
     Split<long long> sp;
@@ -432,7 +434,9 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 if (lane == 0) mbar_arrive(smem_u32(&qfull[tile]));
             }
             // (rows without a token need no mask: nothing of theirs is kept)
-            const int p = on ? cw.s.start + tok : 1 << 30, lo = on ? first_key(a, p) : 0;
+            const int p = on ? cw.s.start + (TREE ? -1 : tok) : 1 << 30;   // (TREE: the last key that all see)
+            const int lo = !on ? 0 : TREE ? first_tree_key(a, cw.s, tok) : first_key(a, p);
+            const uint32_t* tree = TREE ? a.mask + (size_t)(cw.s.c0 + (on ? tok : 0)) * a.mask_stride : nullptr;
             float m = kNoMax, l = 0.f;   // reference, sum of the weights
             int raise = 0;               // of the reference, before the next unit
             // A reference beyond 2^20 (of any row of the warp): what is below is then worked out
@@ -454,6 +458,11 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                 for (int hh = 0; hh < C::HN; ++hh, ++hc) {   // its halves
                 const int b = C::HN == 1 ? hc & 1 : hh;
                 const uint32_t ts = ts0 + b * 64, tp = tp0 + b * C::P_STEP;
+                uint32_t see[2] = {~0u, ~0u};   // (TREE, a masked unit) the half's keys that the row sees
+                if (TREE && careful && on) {
+                    see[0] = seen32(tree, cw.s, lo, u * KT + 64 * hh);
+                    see[1] = seen32(tree, cw.s, lo, u * KT + 64 * hh + 32);
+                }
                 const float4* sc = scales[it % SC] + hh * 4;
                 wait(&sfull[tile][b], hc >> 1);
                 tc5_fence_after();
@@ -487,7 +496,10 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                             for (int e = 0; e < 16; ++e) {
                                 float y = __uint_as_float(v[16 * q + e]);
                                 const int col = 64 * hh + 32 * c + 16 * q + e;
-                                if (decltype(masked)::value) y = col >= c_lo && col <= c_hi ? y : -INFINITY;
+                                if (decltype(masked)::value) {
+                                    const bool in = TREE ? (see[c] >> (16 * q + e) & 1u) != 0 : col >= c_lo && col <= c_hi;
+                                    y = in ? y : -INFINITY;
+                                }
                                 x = fmaxf(x, y);
                             }
                             x = x == -INFINITY ? x : fmaf(x, f.x * cr, f.y);
@@ -526,8 +538,8 @@ __global__ void __launch_bounds__(Chunk<DP>::THREADS, 1)
                             unpair(decltype(masked)::value ? add2(t2, pair(-m, -m)) : t2, x, y);
                             if (decltype(masked)::value) {
                                 const int at = 64 * hh + col;
-                                x = at >= c_lo && at <= c_hi ? x : -INFINITY;
-                                y = at + 1 >= c_lo && at + 1 <= c_hi ? y : -INFINITY;
+                                x = (TREE ? (see[col / 32] >> (col % 32) & 1u) != 0 : at >= c_lo && at <= c_hi) ? x : -INFINITY;
+                                y = (TREE ? (see[col / 32] >> (col % 32 + 1) & 1u) != 0 : at + 1 >= c_lo && at + 1 <= c_hi) ? y : -INFINITY;
                             }
                             x = ex2(x), y = ex2(y);
                             sum = add2(sum, pair(x, y));

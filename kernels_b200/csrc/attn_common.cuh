@@ -26,6 +26,10 @@ struct AttnArgs {
     float* partials;      // two slots per CTA
     int min_units;        // smallest share of a CTA that is worth one
     int pad_units;        // units that a pair costs besides its own
+    // of trees of drafted tokens (TREE): which new tokens a token sees, and where it stands
+    const uint32_t* mask;     // [tokens][mask_stride]
+    uint64_t mask_stride;     // words
+    const int32_t* positions; // with a window
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -99,6 +103,34 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int b, unsigned* err)
 // First key that token i (position p) sees.
 __device__ __forceinline__ int first_key(const AttnArgs& a, int p) {
     return a.window && p >= (int)a.window ? p - (int)a.window + 1 : 0;
+}
+
+// .. in a tree, where all that is before the sequence's start is seen, or what its window leaves
+__device__ __forceinline__ int first_tree_key(const AttnArgs& a, const Seq& s, int tok) {
+    return a.window ? first_key(a, max(s.start, a.positions[s.c0 + tok])) : 0;
+}
+// Bits lo .. hi - 1 of 32, for any lo and hi.
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+    const uint32_t below = hi >= 32 ? ~0u : hi <= 0 ? 0u : (1u << hi) - 1u;
+    return lo <= 0 ? below : lo >= 32 ? 0u : below & ~((1u << lo) - 1u);
+}
+// Which of the 32 keys from `key` on a token of a tree sees: those in [lo, start) and those of its
+// sequence's n new tokens whose bits are set in its mask.
+__device__ __forceinline__ uint32_t seen32(const uint32_t* mask, const Seq& s, int lo, int key) {
+    uint32_t w = bit_range(lo - key, s.start - key);
+    const int at = key - s.start;   // the keys' place among the new tokens
+    if (at > -32 && at < s.n) {
+        uint32_t m;
+        if (at < 0) {
+            m = mask[0] << -at;
+        } else {
+            const int i = at >> 5;
+            m = mask[i] >> (at & 31);
+            if ((at & 31) && (i + 1) * 32 < s.n) m |= mask[i + 1] << (32 - (at & 31));
+        }
+        w |= m & bit_range(-at, s.n - at);
+    }
+    return w;
 }
 
 // ---- codes to fp16 pairs

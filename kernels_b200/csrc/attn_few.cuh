@@ -72,7 +72,8 @@ struct FewState {
     }
 };
 
-template <int DP, int NT, int FMT, bool FULL>   // FULL: head_dim == DP
+// FULL: head_dim == DP.  TREE: the new tokens are a tree (at most 32: a word of mask a row).
+template <int DP, int NT, int FMT, bool FULL, bool TREE>
 __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     attn_few_kernel(const __grid_constant__ AttnArgs a, unsigned* err) {
     constexpr int UK = kFewUnit<DP>, KT = UK / 16, NS = kFewRing<DP, NT>, W = kFewWarps;
@@ -235,7 +236,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     FewState<DP, NT> st;
     uint32_t qf[CH][NT][8];
     float cn[NT][2];    // scale log2(e) of the columns' rows
-    int pn[NT][2];      // positions of the columns' tokens
+    int pn[NT][2];      // positions of the columns' tokens (TREE: the first keys they see)
+    uint32_t seen[TREE ? NT : 1][2];   // and the new tokens
 
     // ---- two elements of a row of a finished pair, L relative to 2^M
     const int je = warp & 3, ce = (warp >> 2) & 1;   // the thread's accumulators: tile 4i + je, column ce
@@ -313,8 +315,15 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
             cn[n][0] = __shfl_sync(~0u, c, 8 * t);       // lane of row 2t (t = 0)
             cn[n][1] = __shfl_sync(~0u, c, 8 * t + 4);
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2)
-                pn[n][c2] = cw.s.start + (cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0);
+            for (int c2 = 0; c2 < 2; ++c2) {
+                const int tok = cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0;
+                if constexpr (TREE) {
+                    pn[n][c2] = first_tree_key(a, cw.s, tok);
+                    seen[n][c2] = a.mask[(size_t)(cw.s.c0 + tok) * a.mask_stride] & bit_range(0, cw.s.n);
+                } else {
+                    pn[n][c2] = cw.s.start + tok;
+                }
+            }
         }
     };
 
@@ -333,7 +342,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
             uint8_t* sl = ring + slot * kFewSlot<DP>;
             cp_async_wait<NS - 1>();
             __syncwarp();
-            const bool edge_unit = key0 < free_lo || key0 + UK - 1 > cw.s.start;
+            const bool edge_unit = TREE ? a.window || key0 + UK > cw.s.start
+                                        : key0 < free_lo || key0 + UK - 1 > cw.s.start;
             const int valid = len - key0;   // (at least 1)
             const float* sc = reinterpret_cast<const float*>(sl + 2 * UK * DP);
             if (FMT == GRAFT_KV_E4M3 && valid < UK) {
@@ -391,7 +401,13 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                         float x = fmaf(s[kt][n][e], ks * cn[n][e & 1], lv);
                         if (edge_unit) {
                             const int j = key0 + kt * 16 + g + (e & 2) * 4, p = pn[n][e & 1];
-                            const bool see = j <= p && (!a.window || j > p - (int)a.window);
+                            bool see;
+                            if constexpr (TREE) {
+                                const int i = j - cw.s.start;
+                                see = i < 0 ? j >= p : i < 32 && (seen[n][e & 1] >> i & 1u);
+                            } else {
+                                see = j <= p && (!a.window || j > p - (int)a.window);
+                            }
                             x = see ? x : -INFINITY;
                         }
                         s[kt][n][e] = x;

@@ -38,13 +38,13 @@ int error_word(int device, unsigned** out) {
 }
 
 // ---- few query rows
-template <int DP, int NT, int FMT, bool FULL>
+template <int DP, int NT, int FMT, bool FULL, bool TREE>
 int launch_few(AttnArgs a, cudaStream_t st) {
     DeviceInfo di;
     int rc = current_device_info(&di);
     if (rc) return rc;
     constexpr int smem = kFewSmem<DP, NT>;
-    const auto kern = attn_few_kernel<DP, NT, FMT, FULL>;
+    const auto kern = attn_few_kernel<DP, NT, FMT, FULL, TREE>;
     int per_sm = 1;
     if ((rc = ensure_smem((const void*)kern, smem)) ||
         (rc = occupancy((const void*)kern, kFewThreads, smem, &per_sm)))
@@ -68,23 +68,23 @@ int launch_few(AttnArgs a, cudaStream_t st) {
     const int grid = (int)std::min<uint64_t>(std::min(di.sm_count * per_sm, kAttnMaxGrid), want);
     return launch_pdl("attn_kv8", kern, dim3(grid), kFewThreads, smem, st, a, err);
 }
-template <int DP, int NT>
+template <int DP, int NT, bool TREE>
 int launch_few(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
     if (a.dim == DP)
-        return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, true>(a, st)
-                                    : launch_few<DP, NT, GRAFT_KV_E4M3, true>(a, st);
-    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, false>(a, st)
-                                : launch_few<DP, NT, GRAFT_KV_E4M3, false>(a, st);
+        return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, true, TREE>(a, st)
+                                    : launch_few<DP, NT, GRAFT_KV_E4M3, true, TREE>(a, st);
+    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, false, TREE>(a, st)
+                                : launch_few<DP, NT, GRAFT_KV_E4M3, false, TREE>(a, st);
 }
 
 // ---- many query rows
-template <int DP, int FMT>
+template <int DP, int FMT, bool TREE>
 int launch_chunk(AttnArgs a, cudaStream_t st) {
     using C = Chunk<DP>;
     DeviceInfo di;
     int rc = current_device_info(&di);
     if (rc) return rc;
-    const auto kern = attn_chunk_kernel<DP, FMT>;
+    const auto kern = attn_chunk_kernel<DP, FMT, TREE>;
     if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
     unsigned* err = nullptr;
     if ((rc = error_word(di.device, &err))) return rc;
@@ -102,10 +102,10 @@ int launch_chunk(AttnArgs a, cudaStream_t st) {
     const int grid = (int)std::min<uint64_t>(std::min(di.sm_count, kChunkMaxGrid), want);
     return launch_pdl("attn_kv8", kern, dim3(grid), C::THREADS, C::SMEM, st, a, err);
 }
-template <int DP>
+template <int DP, bool TREE>
 int launch_chunk(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
-    return fmt == GRAFT_KV_INT8 ? launch_chunk<DP, GRAFT_KV_INT8>(a, st)
-                                : launch_chunk<DP, GRAFT_KV_E4M3>(a, st);
+    return fmt == GRAFT_KV_INT8 ? launch_chunk<DP, GRAFT_KV_INT8, TREE>(a, st)
+                                : launch_chunk<DP, GRAFT_KV_E4M3, TREE>(a, st);
 }
 
 // Query rows that the few-row kernel takes for a head_dim (registers).
@@ -152,10 +152,30 @@ extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t str
     return GRAFT_OK;
 }
 
-extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
-                              const GraftKVRange* range, const float* sinks, float* lse,
-                              const GraftAttnParams* P, void* ws, size_t ws_bytes,
-                              graft_stream_t stream) {
+namespace {
+
+template <bool TREE>
+int launch_attn(const AttnArgs& a, uint32_t format, uint64_t rows, cudaStream_t stream) {
+    if (rows <= few_rows(a.dim)) {
+        if (a.dim <= 64)
+            return rows <= 8    ? launch_few<64, 1, TREE>(a, format, stream)
+                   : rows <= 16 ? launch_few<64, 2, TREE>(a, format, stream)
+                                : launch_few<64, 4, TREE>(a, format, stream);
+        if (a.dim <= 128)
+            return rows <= 8 ? launch_few<128, 1, TREE>(a, format, stream)
+                             : launch_few<128, 2, TREE>(a, format, stream);
+        return launch_few<256, 1, TREE>(a, format, stream);
+    }
+    return a.dim <= 64    ? launch_chunk<64, TREE>(a, format, stream)
+           : a.dim <= 128 ? launch_chunk<128, TREE>(a, format, stream)
+                          : launch_chunk<256, TREE>(a, format, stream);
+}
+
+// mask: of a tree of new tokens, or null
+int attend(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
+           const GraftKVRange* range, const int32_t* mask, uint64_t mask_stride,
+           const int32_t* positions, const float* sinks, float* lse, const GraftAttnParams* P,
+           void* ws, size_t ws_bytes, cudaStream_t stream) {
     int rc;
     if ((rc = check_attn(cache, range, P)) || (rc = kv_check_heads("q", q, cache->head_dim)) ||
         (rc = kv_check_heads("out", out, cache->head_dim)))
@@ -188,17 +208,35 @@ extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, co
     a.partials = (float*)((char*)ws + kAttnMaxGrid * 4);
     const uint64_t rows = (uint64_t)range->max_tokens * a.group;
     if (range->max_tokens == 0) return GRAFT_OK;
-    if (rows <= few_rows(a.dim)) {
-        if (a.dim <= 64)
-            return rows <= 8    ? launch_few<64, 1>(a, cache->format, stream)
-                   : rows <= 16 ? launch_few<64, 2>(a, cache->format, stream)
-                                : launch_few<64, 4>(a, cache->format, stream);
-        if (a.dim <= 128)
-            return rows <= 8 ? launch_few<128, 1>(a, cache->format, stream)
-                             : launch_few<128, 2>(a, cache->format, stream);
-        return launch_few<256, 1>(a, cache->format, stream);
+    a.mask = (const uint32_t*)mask, a.mask_stride = mask_stride, a.positions = positions;
+    return mask ? launch_attn<true>(a, cache->format, rows, stream)
+                : launch_attn<false>(a, cache->format, rows, stream);
+}
+
+}  // namespace
+
+extern "C" int graft_attn_kv8(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
+                              const GraftKVRange* range, const float* sinks, float* lse,
+                              const GraftAttnParams* P, void* ws, size_t ws_bytes,
+                              graft_stream_t stream) {
+    return attend(cache, q, out, range, nullptr, 0, nullptr, sinks, lse, P, ws, ws_bytes, stream);
+}
+
+extern "C" int graft_attn_tree_kv8(const GraftKVCache* cache, const GraftHeads* q,
+                                   const GraftHeads* out, const GraftKVRange* range,
+                                   const int32_t* mask, uint64_t mask_stride,
+                                   const int32_t* positions, const float* sinks, float* lse,
+                                   const GraftAttnParams* P, void* ws, size_t ws_bytes,
+                                   graft_stream_t stream) {
+    int rc;
+    if ((rc = check_attn(cache, range, P))) return rc;
+    if (range->n_seqs && range->max_tokens) {
+        GRAFT_REQUIRE(mask && aligned(mask, 4), "mask must be a 4-byte aligned buffer");
+        GRAFT_REQUIRE(mask_stride >= (range->max_tokens + 31ull) / 32 || (q && q->tokens <= 1),
+                      "mask_stride %llu does not hold max_tokens %u", (unsigned long long)mask_stride,
+                      range->max_tokens);
+        GRAFT_REQUIRE(P->window == 0 || (positions && aligned(positions, 4)),
+                      "positions must be a 4-byte aligned buffer when there is a window");
     }
-    return a.dim <= 64    ? launch_chunk<64>(a, cache->format, stream)
-           : a.dim <= 128 ? launch_chunk<128>(a, cache->format, stream)
-                          : launch_chunk<256>(a, cache->format, stream);
+    return attend(cache, q, out, range, mask, mask_stride, positions, sinks, lse, P, ws, ws_bytes, stream);
 }

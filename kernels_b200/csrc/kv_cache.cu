@@ -21,7 +21,7 @@
 // the same in fp32 157 and 168 us, 4.3 and 4.0 TB/s; writing 7687 tokens of 8 heads of 64 and
 // reading them back 14.0 us; one token of 64 sequences (8 heads of 128), written and its block
 // read back, 7.6 us.
-#include "kv_common.cuh"
+#include "rope.cuh"
 
 #include <algorithm>
 
@@ -47,6 +47,17 @@ struct KVArgs {
     uint32_t cta_heads;        // heads of a CTA (read)
     uint32_t wide;             // rows are 32-byte aligned (16-bit types; read)
 };
+// .. and of a write that turns the keys
+struct KVRopeArgs : KVArgs {
+    RopeArgs rope;
+    const int32_t *positions, *rows, *count;   // or null
+    const void* x_q;
+    void* y_q;
+    uint64_t tok_xq, head_xq, tok_yq, head_yq;
+    uint32_t q_heads, cta_q_heads;             // query heads, and those of a CTA
+    uint32_t kv_ny;                            // CTAs of an item for keys and values; then its queries'
+    uint32_t q_copy;                           // y_q is another buffer
+};
 
 // One item: `count` tokens of one sequence in one block.
 struct Item {
@@ -54,34 +65,38 @@ struct Item {
     int slot;               // first slot in it
     int row;                // row of the first token
     int count;
+    int pos;                // position of the first token
 };
 
 // The item of flat index x (false: none).  Every thread of the CTA calls it.  The
 // lengths of a sequence are read by the thread that looks at it, so that only one
 // round trip to memory comes before the rows' and the block number's.
-__device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it) {
-    __shared__ int sh_seq[4];   // sequence, its first row, one past its last, its start
+// counts: how many of each sequence's tokens are meant (null: all).
+__device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it,
+                                          const int32_t* counts = nullptr) {
+    __shared__ int sh_seq[5];   // sequence, its first row, one past its last, its start, its count
     const uint32_t bt = 1u << a.bt_log2;
     for (uint32_t s0 = 0;; s0 += blockDim.x) {
         const uint32_t s = s0 + threadIdx.x;
         bool here = false;   // x is one of its items: they start at or before x, the next one's after
         if (s < a.n_seqs) {
             const int c = a.cu[s], e = a.cu[s + 1], st = a.start[s];
+            const int some = counts ? counts[s] : e - c;
             // (a sequence of fewer than no tokens may have no items that would tell; the last
             // CTA looks at every sequence up to the last or to one that it finds too long)
             if (e < c) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
             here = (s == 0 || ((uint32_t)c >> a.bt_log2) + 2 * s <= x) &&
                    (s + 1 == a.n_seqs || ((uint32_t)e >> a.bt_log2) + 2 * (s + 1) > x);
-            if (here) sh_seq[0] = s, sh_seq[1] = c, sh_seq[2] = e, sh_seq[3] = st;
+            if (here) sh_seq[0] = s, sh_seq[1] = c, sh_seq[2] = e, sh_seq[3] = st, sh_seq[4] = some;
         }
         const int found = __syncthreads_count(here);
         if (found == 1) break;
         // (none, or with cu_tokens that do not rise several: nothing to do here)
         if (found > 1 || s0 + blockDim.x >= a.n_seqs) return false;
     }
-    const int b = sh_seq[0], c0 = sh_seq[1], n = sh_seq[2] - c0;
+    const int b = sh_seq[0], c0 = sh_seq[1], all = sh_seq[2] - c0, n = counts ? sh_seq[4] : all;
     const int64_t start = sh_seq[3];
-    if (c0 < 0 || n < 0 || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens ||
+    if (c0 < 0 || n < 0 || n > all || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.tokens ||
         start < 0 || (uint64_t)(start + n) > a.max_len) {
         if (threadIdx.x == 0) atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
         return false;
@@ -93,6 +108,7 @@ __device__ __forceinline__ bool find_item(const KVArgs& a, uint32_t x, Item& it)
     const int64_t lo = base > start ? base : start;
     it.slot = (int)(lo - base);
     it.row = c0 + (int)(lo - start);
+    it.pos = (int)lo;
     it.count = min((int)bt - it.slot, (int)(start + n - lo));
     it.block = a.table + (size_t)b * a.table_stride + (size_t)page;
     return true;
@@ -139,30 +155,44 @@ __device__ __forceinline__ uint32_t finite_codes(uint64_t ab, uint64_t cd) {
     }
 }
 
-template <int DT>
-struct Raw {
-    uint4 w[DT == GRAFT_F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ Raw<DT> load_raw(const void* base, uint64_t elem) {
-    Raw<DT> r;
-    const char* p = (const char*)base + elem * (DT == GRAFT_F32 ? 4 : 2);
-    r.w[0] = ld_stream(p);
-    if constexpr (DT == GRAFT_F32) r.w[1] = ld_stream(p + 16);
-    return r;
-}
-template <int DT>
-__device__ __forceinline__ void to_floats(const Raw<DT>& r, float (&f)[8]) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+// Eight elements as codes of scale s (inv: its reciprocal); odd: an infinity or a NaN may be among them.
+template <int FMT>
+__device__ __forceinline__ uint2 codes_of(const float (&f)[8], float s, uint64_t minus_s, uint64_t inv, bool odd) {
+    uint2 o = make_uint2(0u, 0u);
+    if (odd) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (DT == GRAFT_F32) {
-            f[2 * i] = __uint_as_float(w[2 * i]);
-            f[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
-        } else {
-            const float2 p = unpack2<DT>(w[i]);
-            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+        for (int e = 0; e < 4; ++e) {
+            o.x |= kv_code<FMT>(__fdiv_rn(f[e], s)) << (8 * e);
+            o.y |= kv_code<FMT>(__fdiv_rn(f[e + 4], s)) << (8 * e);
         }
+    } else {
+        uint64_t q[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = quotient2(pair(f[2 * e], f[2 * e + 1]), minus_s, inv);
+        o.x = finite_codes<FMT>(q[0], q[1]);
+        o.y = finite_codes<FMT>(q[2], q[3]);
+    }
+    return o;
+}
+
+// A block's earlier `bytes` codes, times ratio (the old scale by the grown one).
+template <int FMT>
+__device__ __forceinline__ void round_again(uint8_t* codes, int bytes, float ratio, int tid, int T) {
+    uint4* p = reinterpret_cast<uint4*>(codes);
+#pragma unroll 4
+    for (int c = tid; c < bytes / 16; c += T) {
+        uint4 w = p[c];
+        uint32_t* v = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float f[4];
+            kv_decode4<FMT>(v[q], f);
+            uint32_t o = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o |= kv_code<FMT>(f[e] * ratio) << (8 * e);
+            v[q] = o;
+        }
+        p[c] = w;
     }
 }
 
@@ -251,49 +281,154 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_kernel(const __grid
     if (tid == 0) *scale = s;
     const uint64_t inv = pair(__frcp_rn(s), __frcp_rn(s)), minus_s = pair(-s, -s);
 
-    if (it.slot && s > old) {   // the earlier tokens' codes, to the grown scale
-        const float ratio = __fdiv_rn(old, s);
-        uint4* p = reinterpret_cast<uint4*>(codes);
-        const int m = it.slot * (int)a.dim / 16;
-#pragma unroll 4
-        for (int c = tid; c < m; c += T) {
-            uint4 w = p[c];
-            uint32_t* v = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float f[4];
-                kv_decode4<FMT>(v[q], f);
-                uint32_t o = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o |= kv_code<FMT>(f[e] * ratio) << (8 * e);
-                v[q] = o;
-            }
-            p[c] = w;
-        }
-    }
+    // the earlier tokens' codes, to the grown scale
+    if (it.slot && s > old) round_again<FMT>(codes, it.slot * (int)a.dim, __fdiv_rn(old, s), tid, T);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int c = tid + i * T;
         if (c < n) {
             float f[8];
             to_floats<DT>(r[i], f);
-            uint2 o = make_uint2(0u, 0u);
-            if (odd) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o.x |= kv_code<FMT>(__fdiv_rn(f[e], s)) << (8 * e);
-                    o.y |= kv_code<FMT>(__fdiv_rn(f[e + 4], s)) << (8 * e);
-                }
-            } else {
-                uint64_t q[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[e] = quotient2(pair(f[2 * e], f[2 * e + 1]), minus_s, inv);
-                o.x = finite_codes<FMT>(q[0], q[1]);
-                o.y = finite_codes<FMT>(q[2], q[3]);
-            }
-            *reinterpret_cast<uint2*>(codes + (size_t)it.slot * a.dim + (size_t)c * kChunk) = o;
+            *reinterpret_cast<uint2*>(codes + (size_t)it.slot * a.dim + (size_t)c * kChunk) =
+                codes_of<FMT>(f, s, minus_s, inv, odd);
         }
     }
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// An item's queries: heads h0 .. of the CTA.  A thread takes a unit (16 elements) of a token for
+// several heads, with the same sines and cosines.
+template <int DT>
+__device__ __forceinline__ void turn_queries(const KVRopeArgs& a, const Item& it, int h0) {
+    const int units = a.dim / 16, per = it.count * units, T = blockDim.x;
+    const int heads = min(a.cta_q_heads, a.q_heads - h0);
+    const int G = max(1, min(heads, T / per));   // threads of a unit
+    for (int i = threadIdx.x; i < per * G; i += T) {
+        const int g = i / per, c = i - g * per, t = c / units, k = c - t * units;
+        const bool turned = k < a.rope.pairs;
+        if (!turned && !a.q_copy) continue;
+        const int row = it.row + t;
+        float cs[8], sn[8];
+        if (turned)
+            unit_turns<DT != GRAFT_F32>(a.rope, k, a.positions ? a.positions[row] : it.pos + t, cs, sn);
+        const int e0 = unit_chunk(a.rope, k, 0) * 8, e1 = unit_chunk(a.rope, k, 1) * 8;
+        constexpr int UN = DT == GRAFT_F32 ? 2 : 4;
+        for (int j0 = g; j0 < heads; j0 += UN * G) {
+            Raw<DT> p[UN], q[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (j0 + u * G < heads) {
+                    const uint64_t from = row * a.tok_xq + (h0 + j0 + u * G) * a.head_xq;
+                    p[u] = load_own<DT>(a.x_q, from + e0), q[u] = load_own<DT>(a.x_q, from + e1);
+                }
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (j0 + u * G < heads) {
+                    const uint64_t to = row * a.tok_yq + (h0 + j0 + u * G) * a.head_yq;
+                    if (turned) {
+                        float x[8], y[8];
+                        to_floats<DT>(p[u], x), to_floats<DT>(q[u], y);
+                        turn_unit(a.rope.half, cs, sn, x, y);
+                        p[u] = from_floats<DT>(x), q[u] = from_floats<DT>(y);
+                    }
+                    store_raw<DT>(a.y_q, to + e0, p[u]), store_raw<DT>(a.y_q, to + e1, q[u]);
+                }
+        }
+    }
+}
+
+// The same as kv_write_kernel with keys turned in fp32 before their maximum is taken.  A thread's
+// chunks come in twos, the halves of a unit (rope.cuh), so that it holds both elements of its pairs.
+// CTAs beyond those of keys and values turn the item's queries.
+template <int DT, int FMT, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_rope_kernel(const __grid_constant__ KVRopeArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ float red[16];
+    Item it;
+    if (!find_item(a, blockIdx.x, it, a.count)) return;
+    if (blockIdx.y >= a.kv_ny) {
+        turn_queries<DT>(a, it, (blockIdx.y - a.kv_ny) * a.cta_q_heads);
+        return;
+    }
+    const int block = *it.block;   // (not needed before the scale)
+    const int unit = WARP ? blockIdx.y * 8 + (threadIdx.x >> 5) : blockIdx.y;
+    if (WARP && unit >= 2 * (int)a.heads) return;
+    const int head = unit >> 1;
+    const bool is_v = unit & 1;
+    const void* x = is_v ? a.x_v : a.x_k;
+    const uint64_t ts = is_v ? a.tok_v : a.tok_k, hs = is_v ? a.head_v : a.head_k;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, T = WARP ? 32 : blockDim.x;
+    const int upr = (int)a.cpt / 2, n = it.count * upr;   // units of a row, of the item
+
+    float f[CH][8];
+    int chunk[CH];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; i += 2) {
+        const int w = tid + i / 2 * T;
+        chunk[i] = -1;
+        if (w < n) {
+            const int t = (w * a.cpt_magic) >> 20, k = w - t * upr;
+            int row = it.row + t;
+            if (a.rows) row = a.rows[row];
+            const bool turned = !is_v && k < a.rope.pairs;
+            const int c0 = turned ? unit_chunk(a.rope, k, 0) : 2 * k, c1 = turned ? unit_chunk(a.rope, k, 1) : 2 * k + 1;
+            chunk[i] = t * (int)a.cpt + c0, chunk[i + 1] = t * (int)a.cpt + c1;
+            if ((uint32_t)row < a.tokens) {
+                const uint64_t from = row * ts + head * hs;
+                to_floats<DT>(load_raw<DT>(x, from + c0 * kChunk), f[i]);
+                to_floats<DT>(load_raw<DT>(x, from + c1 * kChunk), f[i + 1]);
+                if (turned) {
+                    float cs[8], sn[8];
+                    unit_turns<DT != GRAFT_F32>(a.rope, k, a.positions ? a.positions[row] : it.pos + t, cs, sn);
+                    turn_unit(a.rope.half, cs, sn, f[i], f[i + 1]);
+                }
+            } else {
+                atomicOr(&g_kv_err, (unsigned)GRAFT_KV_EBOUNDS);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[i][e] = f[i + 1][e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = max_nan(amax, max_nan(fabsf(f[i][e]), fabsf(f[i + 1][e])));
+        }
+    }
+    if (!good_block(a, block)) return;
+    const size_t bh = (size_t)block * a.heads + head;
+    uint8_t* codes = (is_v ? a.v : a.k) + bh * a.bt * a.dim;
+    float* scale = (is_v ? a.v_scale : a.k_scale) + bh;
+    const float old = it.slot ? *scale : 0.f;
+    const bool odd = !(amax < INFINITY);
+    if (odd) {
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (chunk[i & ~1] >= 0)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fin_abs(f[i][e]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+    if constexpr (!WARP) {
+        if ((tid & 31) == 0) red[tid >> 5] = amax;
+        __syncthreads();
+        for (int w = 0; w < T / 32; ++w) amax = fmaxf(amax, red[w]);
+    }
+    const float s = fmaxf(fmaxf(__fdiv_rn(amax, kKVQmax<FMT>), kKVScaleFloor), old);
+    if constexpr (WARP) __syncwarp();   // (all lanes have read the old scale)
+    if (tid == 0) *scale = s;
+    const uint64_t inv = pair(__frcp_rn(s), __frcp_rn(s)), minus_s = pair(-s, -s);
+    if (it.slot && s > old) round_again<FMT>(codes, it.slot * (int)a.dim, __fdiv_rn(old, s), tid, T);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+        if (chunk[i & ~1] >= 0)
+            *reinterpret_cast<uint2*>(codes + (size_t)it.slot * a.dim + (size_t)chunk[i] * kChunk) =
+                codes_of<FMT>(f[i], s, minus_s, inv, odd);
 }
 
 constexpr int kReadThreads = 256, kReadUnroll = 4;   // (kReadThreads: also the launch's)
@@ -364,6 +499,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
 }
 
 using KVKernel = void (*)(const KVArgs);
+using KVRopeKernel = void (*)(const KVRopeArgs);
 enum Form { kRead, kWriteOne, kWriteWarp, kWriteCta };   // kWriteOne: a chunk a lane
 template <int DT, int FMT>
 KVKernel pick(Form form, int chunks) {
@@ -378,9 +514,22 @@ KVKernel pick(Form form, int chunks, uint32_t fmt) {
     return fmt == GRAFT_KV_INT8 ? pick<DT, GRAFT_KV_INT8>(form, chunks)
                                 : pick<DT, GRAFT_KV_E4M3>(form, chunks);
 }
+template <int DT, int FMT>
+KVRopeKernel pick_rope(Form form, int chunks) {
+    return form == kWriteOne    ? kv_write_rope_kernel<DT, FMT, 2, true>
+           : form == kWriteWarp ? kv_write_rope_kernel<DT, FMT, 8, true>
+           : chunks <= 4        ? kv_write_rope_kernel<DT, FMT, 4, false>
+                                : kv_write_rope_kernel<DT, FMT, 8, false>;
+}
+template <int DT>
+KVRopeKernel pick_rope(Form form, int chunks, uint32_t fmt) {
+    return fmt == GRAFT_KV_INT8 ? pick_rope<DT, GRAFT_KV_INT8>(form, chunks)
+                                : pick_rope<DT, GRAFT_KV_E4M3>(form, chunks);
+}
 
+// turned: a write that turns the keys (its fields beyond KVArgs), or null
 int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
-            const GraftKVRange* range, cudaStream_t st) {
+            const GraftKVRange* range, KVRopeArgs* turned, cudaStream_t st) {
     int rc;
     if ((rc = kv_check_cache(cache)) || (rc = kv_check_range(cache, range)) ||
         (rc = kv_check_heads("K", K, cache->head_dim)) ||
@@ -434,6 +583,26 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
     const int chunks = (int)(a.bt * a.cpt + threads - 1) / threads;
     const uint32_t ny = form == kRead      ? 2 * ((a.heads + a.cta_heads - 1) / a.cta_heads)
                         : form == kWriteCta ? 2 * a.heads : (2 * a.heads + 7) / 8;
+    if (turned) {
+        *static_cast<KVArgs*>(turned) = a;
+        KVRopeArgs& r = *turned;
+        const uint32_t upr = r.cpt / 2;
+        r.cpt_magic = ((1u << 20) + upr - 1) / upr;
+        r.kv_ny = ny;
+        // queries: about 16 units a thread
+        uint32_t q_ny = 0;
+        if (r.x_q) {
+            const uint64_t units = (uint64_t)std::min(range->max_tokens, a.bt) * (a.dim / 16) * r.q_heads;
+            q_ny = (uint32_t)std::min<uint64_t>(r.q_heads, std::max<uint64_t>(1, units / (16ull * threads)));
+            r.cta_q_heads = (r.q_heads + q_ny - 1) / q_ny;
+            q_ny = (r.q_heads + r.cta_q_heads - 1) / r.cta_q_heads;
+        }
+        GRAFT_REQUIRE(ny + q_ny <= 65535, "too many heads in one call");
+        const KVRopeKernel kern = K->dtype == GRAFT_F16    ? pick_rope<GRAFT_F16>(form, chunks, cache->format)
+                                  : K->dtype == GRAFT_BF16 ? pick_rope<GRAFT_BF16>(form, chunks, cache->format)
+                                                           : pick_rope<GRAFT_F32>(form, chunks, cache->format);
+        return launch_pdl("kv_write_rope", kern, dim3((unsigned)items, ny + q_ny), threads, 0, st, r);
+    }
     const KVKernel kern = K->dtype == GRAFT_F16    ? pick<GRAFT_F16>(form, chunks, cache->format)
                           : K->dtype == GRAFT_BF16 ? pick<GRAFT_BF16>(form, chunks, cache->format)
                                                    : pick<GRAFT_F32>(form, chunks, cache->format);
@@ -501,18 +670,49 @@ unsigned kv_cache_device_errors(bool clear) { return read_device_errors(g_kv_err
 
 extern "C" int graft_kv_write(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
                               const GraftKVRange* range, graft_stream_t stream) {
-    return kv_move(true, cache, K, V, range, stream);
+    return kv_move(true, cache, K, V, range, nullptr, stream);
+}
+
+extern "C" int graft_kv_write_rope(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
+                                   const GraftKVRange* range, const GraftRope* rope,
+                                   const int32_t* positions, const int32_t* rows, const int32_t* count,
+                                   const GraftHeads* q, const GraftHeads* q_out, uint32_t q_heads,
+                                   graft_stream_t stream) {
+    int rc;
+    if ((rc = kv_check_cache(cache)) || (rc = check_rope(rope, cache->head_dim))) return rc;
+    GRAFT_REQUIRE(aligned(positions, 4) && aligned(rows, 4) && aligned(count, 4),
+                  "positions, rows and count must be 4-byte aligned");
+    GRAFT_REQUIRE(!rows == !count, "rows and count go together");
+    GRAFT_REQUIRE(!q == !q_out, "q and q_out go together");
+    KVRopeArgs a = {};
+    a.rope = rope_args(rope);
+    a.positions = positions, a.rows = rows, a.count = count;
+    if (q) {
+        GRAFT_REQUIRE(!rows, "q cannot be turned together with rows and count");
+        GRAFT_REQUIRE(K, "K is null");
+        if ((rc = check_rope_rows(q, q_out, q_heads))) return rc;
+        GRAFT_REQUIRE(q->dtype == K->dtype && q->tokens == K->tokens,
+                      "q and K must have the same type and number of tokens");
+        if (q_heads) {
+            a.x_q = q->data, a.y_q = q_out->data;
+            a.tok_xq = q->token_stride, a.head_xq = q->head_stride;
+            a.tok_yq = q_out->token_stride, a.head_yq = q_out->head_stride;
+            a.q_heads = q_heads, a.q_copy = q->data != q_out->data;
+        }
+    }
+    return kv_move(true, cache, K, V, range, &a, stream);
 }
 
 extern "C" int graft_kv_read(const GraftKVCache* cache, const GraftHeads* K, const GraftHeads* V,
                              const GraftKVRange* range, graft_stream_t stream) {
-    return kv_move(false, cache, K, V, range, stream);
+    return kv_move(false, cache, K, V, range, nullptr, stream);
 }
 
 extern "C" int graft_kv_device_errors(uint32_t* bits, int clear) {
     clear_error();
     GRAFT_REQUIRE(bits, "bits pointer is null");
     GRAFT_CUDA(cudaDeviceSynchronize());
-    *bits = kv_cache_device_errors(clear != 0) | attn_device_errors(clear != 0);
+    *bits = kv_cache_device_errors(clear != 0) | attn_device_errors(clear != 0) |
+            tree_device_errors(clear != 0);
     return GRAFT_OK;
 }

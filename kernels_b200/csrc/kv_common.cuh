@@ -13,6 +13,7 @@ int kv_check_heads(const char* name, const GraftHeads* h, uint32_t dim);
 
 unsigned kv_cache_device_errors(bool clear);
 unsigned attn_device_errors(bool clear);
+unsigned tree_device_errors(bool clear);
 
 // Reads (and resets) one kernel file's device error word.
 template <typename Symbol>
