@@ -5,16 +5,17 @@
 //   child c accepted:  u_c q(x_c) R < r(x_c);   else  r <- max(r - R q, 0), R <- sum r
 //   next = smallest v with r(v) > 0 and  sum_{w <= v} r(w) > u R
 //
-// Two kernels.  The first reads the rows of tokens that have children (a leaf's row matters
-// only if it turns out to be the last) and leaves each segment's (reference, sum).  The
-// second gives a sequence a cluster of CTAs: whether a token's first child is accepted
-// follows from two logits and two sums, for all tokens at once, so the walk down the tree is
-// a few steps in shared memory; then the cluster goes over the last token's row (and the
-// draft's, where a child was rejected) in fp64: cumulative sums decide about `next`, and at 10^5
-// tokens an error of 2^-24 would move one draw in a hundred to a neighbour.
-#include "kv_common.cuh"
+// Three kernels.  The first reads the rows of tokens that have children (a leaf's row matters
+// only if it turns out to be the last) and leaves each segment's (reference, sum) in fp32.  The
+// second walks down the tree: whether a token's first child is accepted follows from two logits
+// and two sums, for all tokens at once.  Only where a token has several drawn children does it go
+// over whole rows, as a cluster of CTAs a sequence.  The third spreads the last token's row (and the
+// draft's, where a child was rejected) over the SMs, in fp64: cumulative sums decide about `next`,
+// and at 10^5 tokens an error of 2^-24 would move one draw in a hundred to a neighbour.
+#include "logits.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 using namespace graft;
@@ -67,9 +68,11 @@ __global__ void __launch_bounds__(kTreeThreads) draft_tree_kernel(const __grid_c
 // ------------------------------------------------------------------ verifying --
 constexpr int kMaxTree = 1024;       // tokens of a sequence
 constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
+constexpr int kUnroll = 4;           // chunks of a thread's round
 constexpr int kMaxSegs = 32, kMinSeg = 4096;
 constexpr int kRounds = 148 * 16;    // CTAs to aim at
-constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMaxCluster = 8;
+constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMaxCluster = 16;
+constexpr int kDrawThreads = 256, kDrawWarps = kDrawThreads / 32, kMaxDrawSegs = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct VerifyArgs {
@@ -82,57 +85,104 @@ struct VerifyArgs {
     float scale, draft_scale;
     int segs;
     uint64_t* parts;   // [draft: 2][rows][segs]: (reference, sum), or greedy the largest key
+    // between the walk and the draw
+    struct Record* records;   // [n_seqs]
+    unsigned* counters;       // [n_seqs], zeroed by the walk
+    int32_t* gone;            // [rows] rejected tokens of a sequence's last one, at its first row
+    double* mass;             // [rows] or the masses after so many rejections
+    double* sums;             // [n_seqs][draw_segs][kDrawWarps][4]
+    int draw_segs;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// fp32 in the order of unsigned integers, NaN above all (-0 = +0)
-__device__ __forceinline__ uint32_t order(float x) {
-    const uint32_t b = __float_as_uint(x + 0.f);
-    return x == x ? b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u) : 0xFFFFFFFFu;
-}
-constexpr uint32_t kOrderInf = 0xFF800000u, kOrderNone = 0x007FFFFFu;   // of +inf and -inf
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
-    return ((uint64_t)order(x) << 32) | (0xFFFFFFFFu - index);
-}
-__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+// What is to be drawn from: a row without the rejected tokens (kList), or with the rejections of
+// drawn children taken off (kOnce: one; kOften); greedy, the row's largest (kTop).
+enum Mode : int { kDone, kList, kOnce, kOften, kTop };
+struct Record {
+    int mode, row, k, from;   // row of logits; rejections, and those that left nothing
+    float ref, ref_q, near;   // references of the exponentials; Lp / Lq to 2^-20
+    double Lp, iq;            // kOften: the target's sum, and by the draft's
+};
 
-template <int DT>
-__device__ __forceinline__ float logit(const void* row, uint32_t i) {
-    if constexpr (DT == GRAFT_F32) return ((const float*)row)[i];
-    const uint16_t w = ((const uint16_t*)row)[i];
-    return DT == GRAFT_F16 ? h2f(w) : bf2f(w);
-}
+constexpr uint32_t kOrderInf = 0xFF800000u, kOrderNone = 0x007FFFFFu;   // order() of +inf and -inf
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 template <int DT>
 constexpr int kSize = DT == GRAFT_F32 ? 4 : 2;
 
-// Elements v .. v + 7 of a row; those from vocab on are -inf and are not read.
-template <int DT>
-__device__ __forceinline__ void load8(const void* row, uint32_t v, uint32_t vocab, float (&x)[8]) {
-    const char* p = (const char*)row + (uint64_t)v * kSize<DT>;
-    if (v + 8 <= vocab && ((uintptr_t)p & 15) == 0) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        if constexpr (DT == GRAFT_F32) {
-            const uint4 b = *reinterpret_cast<const uint4*>(p + 16);
-            x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z);
-            x[3] = __uint_as_float(a.w), x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y);
-            x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
-        } else {
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = unpack2<DT>(w[i]);
-                x[2 * i] = f.x, x[2 * i + 1] = f.y;
-            }
+// The largest logit so far and the first place that has it; a NaN stands above all.
+struct Best {
+    float x = -INFINITY;
+    uint32_t at = 0;
+    bool nan = false;
+    __device__ __forceinline__ void take(float y, uint32_t v) {
+        if (!(y <= x)) {
+            if (y != y) nan = true;
+            else x = y, at = v;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v + i < vocab ? logit<DT>(row, v + i) : -INFINITY;
     }
-}
+    __device__ __forceinline__ uint64_t key() const {
+        return nan ? ~0ull : x > -INFINITY ? key_of(x, at) : 0;
+    }
+};
+
+// Elements v .. v + 7 of a row, as they lie there; those outside 0..vocab-1 are -inf and are not read.
+template <int DT>
+struct Eight {
+    uint4 w[DT == GRAFT_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* row, int v, int vocab) {
+#pragma unroll
+        for (int i = 0; i < (DT == GRAFT_F32 ? 2 : 1); ++i) {
+            const int at = v + 4 * i;
+            const char* p = (const char*)row + (int64_t)at * kSize<DT>;
+            w[i] = at >= 0 && at + kPer<DT> <= vocab && ((uintptr_t)p & 15) == 0 ? ld_ro(p)
+                                                                                 : edge_chunk<DT>(row, at, vocab);
+        }
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        if constexpr (DT == GRAFT_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(reinterpret_cast<const uint32_t*>(w)[i]);
+        } else {
+            floats_of<DT>(w[0], x);
+        }
+    }
+};
+
+// exp(scale (x - ref)) in fp64, as 2^(t / 16): t split into a whole number n, of which n / 16 goes to
+// the exponent and n % 16 takes a power from a table (16 of them have a bank each), and f in
+// [-1/2, 1/2], for which 2^(f / 16) is its Chebyshev expansion on that interval up to degree 5 as a
+// polynomial (off by 5e-15).
+// Ten fp64 operations; the general exp costs about three times as many.  From 2^-1000 of
+// exp(scale ref) down, -inf included, it stays there: kNothing and less is nothing.  (Not for NaN.)
+constexpr int kPowers = 16;
+constexpr double kNothing = 0x1p-990;   // of a token, or a sum of tokens that have nothing
+__device__ __forceinline__ double or_none(double e) { return e > kNothing ? e : 0.0; }
+struct Expo {
+    uint32_t pow;        // 2^(i / 16), in shared memory
+    double c, off;
+    float lim;
+    __device__ __forceinline__ void set(const double* powers, float r, float scale) {
+        pow = smem_u32(powers);
+        c = (double)scale * (kPowers * 1.4426950408889634);
+        lim = fmaxf(__fsub_rd(r, (float)(1000.0 * kPowers / c)), -3.4028235e38f);
+        // where even the number below ref has nothing, a lower slope that says so: t stays exact
+        c = fmin(c, 1001.0 * kPowers / ((double)r - lim));
+        off = -(double)r * c;
+    }
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double whole = 6755399441055744.0;   // 1.5 2^52: adding it rounds to an integer
+        const double t = fma((double)fmaxf(x, lim), c, off), k = t + whole, f = t - (k - whole);
+        const int n = __double2loint(k);
+        double p = 1.2716121539285134e-09;
+        p = fma(p, f, 1.4676446000606026e-07);
+        p = fma(p, f, 1.3550807776365097e-05);
+        p = fma(p, f, 0.0009383847924836156);
+        p = fma(p, f, 0.04332169878499668);
+        p = fma(p, f, 1.0000000000000044);
+        double power;
+        asm("ld.shared.f64 %0, [%1];" : "=d"(power) : "r"(pow + (n & (kPowers - 1)) * 8));
+        return p * __hiloint2double(__double2hiint(power) + ((n & -kPowers) << 16), __double2loint(power));
+    }
+};
 
 // Whether row r is a token that has children (every thread of the CTA asks).
 __device__ __forceinline__ bool has_children(const VerifyArgs& a, int r) {
@@ -157,9 +207,11 @@ __device__ __forceinline__ bool has_children(const VerifyArgs& a, int r) {
     return __syncthreads_or(mine);
 }
 
-// A segment of a row: its largest logit and sum of exp(scale (z - it)), or the largest key.
+// A segment of a row: a reference and the sum of exp(scale (z - it)), or the largest key.  Each
+// thread has a reference of its own that moves only when a logit passes it by 2^64.
 template <int DT, bool GREEDY>
 __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a) {
+    constexpr int N = kPer<DT>, UN = kUnroll;
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float2 sh[kRowWarps];
@@ -170,32 +222,83 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
     const bool of_draft = blockIdx.y;
     const char* base = of_draft ? (const char*)a.draft + row * a.draft_stride * kSize<DT>
                                 : (const char*)a.logits + row * a.row_stride * kSize<DT>;
-    const float c = (of_draft ? a.draft_scale : a.scale) * kLog2e;
-    const uint32_t per = ((a.vocab + a.segs - 1) / a.segs + 7) / 8 * 8;
-    const uint32_t v0 = seg * per, v1 = min(a.vocab, v0 + per);
-    float m = -INFINITY, L = 0.f;
-    uint64_t key = 0;
-    for (uint32_t v = v0 + tid * 8; v < v1; v += kRowThreads * 8) {
-        float x[8];
-        load8<DT>(base, v, v1, x);
+    const int off = (int)(((uintptr_t)base & 15) / kSize<DT>);   // elements before the row in its first chunk
+    const int chunks = (int)(((uint64_t)off + a.vocab + N - 1) / N), per = (chunks + a.segs - 1) / a.segs;
+    const int c0 = min((int)seg * per, chunks), c1 = min(c0 + per, chunks);
+    // chunks that lie wholly in the row are [i0, i1)
+    const int i0 = c0 + (c0 == 0 && c1 > 0 && (off || (int)a.vocab < N));
+    const int i1 = max(i0, c1 - (c1 == chunks && (off + a.vocab) % N != 0));
+    const float c = (of_draft ? a.draft_scale : a.scale) * kLog2e, reach = 64.f / c;
+    float ref = 0.f, lim = -INFINITY, L[2] = {0.f, 0.f};
+    Best best;
+    auto take = [&](const uint4 (&v)[UN], int ch, int step) {   // chunks ch, ch + step, ..
         if constexpr (GREEDY) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) key = max64(key, v + i < v1 ? key_of(x[i], v + i) : 0);
-        } else {
-            float mx = x[0];
+            for (int u = 0; u < UN; ++u) {
+                float x[N];
+                floats_of<DT>(v[u], x);
 #pragma unroll
-            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-            if (mx > m) {
-                L *= m == -INFINITY ? 0.f : ex2((m - mx) * c);
-                m = mx;
+                for (int e = 0; e < N; ++e) best.take(x[e], (ch + u * step) * N - off + e);
             }
-            const float ref = m == -INFINITY ? 0.f : m;
+        } else {
+            float gm = chunk_max<DT>(v[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) L += ex2((x[i] - ref) * c);
+            for (int u = 1; u < UN; ++u) gm = fmaxf(gm, chunk_max<DT>(v[u]));
+            if (gm > lim) {
+                if (lim > -INFINITY) {
+                    const float f = ex2((ref - gm) * c);
+                    L[0] *= f, L[1] *= f;
+                }
+                ref = gm;
+                lim = __fadd_rd(gm, reach);   // (rounded up, it might let 2^128 through)
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    float d0, d1;
+                    if constexpr (DT == GRAFT_F32) {
+                        d0 = __uint_as_float(w[e]) - ref, d1 = __uint_as_float(w[e + 1]) - ref;
+                    } else {
+                        minus<DT>(w[e / 2], ref, d0, d1);
+                    }
+                    L[0] += ex2(d0 * c), L[1] += ex2(d1 * c);
+                }
+            }
         }
+    };
+    int ch = i0 + tid;
+    const char* from = base + ((int64_t)ch * N - off) * kSize<DT>;
+#pragma unroll 1
+    for (; ch + (UN - 1) * kRowThreads < i1; ch += UN * kRowThreads, from += UN * kRowThreads * 16) {
+        uint4 v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) v[u] = ld_stream(from + u * kRowThreads * 16);
+        take(v, ch, kRowThreads);
+    }
+    // what is left, and the row's edges (the first by thread 0, the last by thread 1), as rounds
+    // with empty chunks
+    const int edge = tid == 0 && i0 > c0 ? c0 : tid == 1 && i1 < c1 ? c1 - 1 : -1;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        if (part ? edge < 0 : ch >= i1) continue;
+        constexpr uint32_t none = DT == GRAFT_F32 ? 0xFF800000u : DT == GRAFT_F16 ? 0xFC00FC00u : 0xFF80FF80u;
+        uint4 v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            v[u] = make_uint4(none, none, none, none);
+            if (part) {
+                if (u == 0) v[u] = load_chunk<DT>(base, off, a.vocab, edge);
+            } else if (ch + u * kRowThreads < i1) {
+                v[u] = ld_stream(from + u * kRowThreads * 16);
+            }
+        }
+        take(v, part ? edge : ch, kRowThreads);
     }
     uint64_t* out = a.parts + ((uint64_t)of_draft * a.rows + row) * a.segs + seg;
     if constexpr (GREEDY) {
+        uint64_t key = best.key();
 #pragma unroll
         for (int o = 16; o; o >>= 1) key = max64(key, __shfl_xor_sync(~0u, key, o));
         if (lane == 0) sh_key[warp] = key;
@@ -205,21 +308,23 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
             *out = key;
         }
     } else {
-        auto join = [&](float m2, float L2) {
-            const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
-            L = (m == -INFINITY ? L : L * ex2((m - ref) * c)) + (m2 == -INFINITY ? L2 : L2 * ex2((m2 - ref) * c));
-            m = top;
-        };
+        // against the warp's largest reference, then the warps'
+        float m = lim == -INFINITY ? -INFINITY : ref, sum = L[0] + L[1], top = m;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float m2 = __shfl_xor_sync(~0u, m, o);
-            join(m2, __shfl_xor_sync(~0u, L, o));
-        }
-        if (lane == 0) sh[warp] = make_float2(m, L);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        sum = m == -INFINITY ? sum : sum * ex2((m - top) * c);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane == 0) sh[warp] = make_float2(top, sum);
         __syncthreads();
         if (tid == 0) {
-            for (int w = 1; w < kRowWarps; ++w) join(sh[w].x, sh[w].y);
-            *reinterpret_cast<float2*>(out) = make_float2(m, L);
+            m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, sh[w].x);
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w)
+                sum += sh[w].x == -INFINITY ? sh[w].y : sh[w].y * ex2((sh[w].x - m) * c);
+            *reinterpret_cast<float2*>(out) = make_float2(m, sum);
         }
     }
 }
@@ -240,6 +345,20 @@ __device__ __forceinline__ void store_remote(const void* at, uint32_t rank, uint
                  : "memory");
 }
 
+__device__ __forceinline__ double warp_sum64(double x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
+__device__ __forceinline__ double scan64(double x) {   // over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(~0u, x, o);
+        if ((int)(threadIdx.x & 31) >= o) x += y;
+    }
+    return x;
+}
+
 enum Flag : uint8_t { kRejected, kAccepted, kAsk, kIgnored };   // kAsk: the whole row decides
 
 struct Walk {
@@ -251,7 +370,10 @@ struct Walk {
     int16_t parent[kMaxTree], sibling[kMaxTree];   // sibling: the next one, or -1
     uint8_t flag[kMaxTree];
     bool again[kMaxTree];           // an earlier sibling has the same token
-    uint64_t part[2][kMaxCluster * kWalkWarps];
+    uint64_t part[2][2][kMaxCluster * kWalkWarps];   // the warps' sums
+    double pow[kPowers];
+    double u[kMaxTree];             // random numbers
+    float z[kMaxTree], zq[kMaxTree];   // logits of a token in its parent's rows
 };
 
 template <int DT, bool GREEDY>
@@ -261,27 +383,38 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = cluster_rank(), b = blockIdx.x / ctas, NW = ctas * kWalkWarps;
+    const int T = blockDim.x, W = T / 32;
+    const int rank = cluster_rank(), b = blockIdx.x / ctas, NW = ctas * W;
     const int c0 = a.cu[b], n = a.cu[b + 1] - c0;
     if (c0 < 0 || n <= 0 || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.rows) {
-        if (rank == 0 && tid == 0) a.count[b] = 0, a.next[b] = -1;
+        if (rank == 0 && tid == 0) a.count[b] = 0, a.next[b] = -1, a.records[b].mode = kDone;
         return;   // (the whole cluster)
     }
     const bool drawn = !GREEDY && a.draft;
-    const double scale = a.scale, scale_q = a.draft_scale;
     auto row_of = [&](int i) { return (const char*)a.logits + (uint64_t)(c0 + i) * a.row_stride * kSize<DT>; };
     auto draft_of = [&](int i) { return (const char*)a.draft + (uint64_t)(c0 + i) * a.draft_stride * kSize<DT>; };
     auto usable = [](float2 s) { return s.x < INFINITY && s.y > 0.f && s.y < INFINITY; };
 
-    // ---- the tree
-    for (int i = tid; i < n; i += kWalkThreads) {
-        const int p = i == 0 ? -1 : a.parents ? a.parents[c0 + i] : i - 1;
-        sh.parent[i] = p >= 0 && p < i ? p : -1;
-        sh.token[i] = a.tokens[c0 + i];
+    // ---- the tree, and each token's logits in its parent's rows
+    if (tid < kPowers) sh.pow[tid] = exp2(tid * (1.0 / kPowers));
+    if (tid == kPowers) sh.mass[0] = 1;   // (without draft, of no token: the root's)
+    for (int i = tid; i < n; i += T) {
+        int p = i == 0 ? -1 : a.parents ? a.parents[c0 + i] : i - 1;
+        p = p >= 0 && p < i ? p : -1;
+        const int x = a.tokens[c0 + i];
+        sh.parent[i] = p;
+        sh.token[i] = x;
         sh.first[i] = kMaxTree;
+        if constexpr (!GREEDY) {
+            sh.u[i] = a.uniform[c0 + i];
+            if (p >= 0 && (uint32_t)x < a.vocab) {
+                sh.z[i] = logit<DT>(row_of(p), x);
+                if (drawn) sh.zq[i] = logit<DT>(draft_of(p), x);
+            }
+        }
     }
     __syncthreads();
-    for (int i = 1 + tid; i < n; i += kWalkThreads) {
+    for (int i = 1 + tid; i < n; i += T) {
         const int p = sh.parent[i];
         if (p >= 0) atomicMin(&sh.first[p], i);
         int s = -1;
@@ -295,36 +428,36 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     }
     __syncthreads();
     // ---- sums of the rows of tokens with children, a warp a row
-    for (int i = warp; i < n; i += kWalkWarps)
-        if (sh.first[i] < kMaxTree) {
-            for (int which = 0; which < (drawn ? 2 : 1); ++which) {
-                const uint64_t* parts = a.parts + ((uint64_t)which * a.rows + c0 + i) * a.segs;
-                uint64_t v = lane < a.segs ? parts[lane] : 0;
-                if constexpr (GREEDY) {
+    const int sides = drawn ? 2 : 1;
+    for (int j = warp; j < n * sides; j += W) {
+        const int i = drawn ? j >> 1 : j, which = drawn ? j & 1 : 0;
+        if (sh.first[i] == kMaxTree) continue;
+        const uint64_t* parts = a.parts + ((uint64_t)which * a.rows + c0 + i) * a.segs;
+        uint64_t v = lane < a.segs ? parts[lane] : 0;
+        if constexpr (GREEDY) {
 #pragma unroll
-                    for (int o = 16; o; o >>= 1) v = max64(v, __shfl_xor_sync(~0u, v, o));
-                    if (lane == 0) {
-                        const uint32_t top = v >> 32;
-                        const bool ok = top > kOrderNone && top < kOrderInf;
-                        sh.stat[i] = make_float2(__int_as_float(ok ? (int)(0xFFFFFFFFu - (uint32_t)v) : -1), 0.f);
-                    }
-                } else {
-                    const float c = (which ? a.draft_scale : a.scale) * kLog2e;
-                    float m = lane < a.segs ? __uint_as_float((uint32_t)v) : -INFINITY;
-                    float L = lane < a.segs ? __uint_as_float((uint32_t)(v >> 32)) : 0.f;
-                    float top = m;
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-                    L = m == -INFINITY ? L : L * ex2((m - top) * c);
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
-                    if (lane == 0) (which ? sh.stat_q : sh.stat)[i] = make_float2(top, L);
-                }
+            for (int o = 16; o; o >>= 1) v = max64(v, __shfl_xor_sync(~0u, v, o));
+            if (lane == 0) {
+                const uint32_t top = v >> 32;
+                const bool ok = top > kOrderNone && top < kOrderInf;
+                sh.stat[i] = make_float2(__int_as_float(ok ? (int)(0xFFFFFFFFu - (uint32_t)v) : -1), 0.f);
             }
+        } else {
+            const float c = (which ? a.draft_scale : a.scale) * kLog2e;
+            float m = lane < a.segs ? __uint_as_float((uint32_t)v) : -INFINITY;
+            float L = lane < a.segs ? __uint_as_float((uint32_t)(v >> 32)) : 0.f;
+            float top = m;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+            L = m == -INFINITY ? L : L * ex2((m - top) * c);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(~0u, L, o);
+            if (lane == 0) (which ? sh.stat_q : sh.stat)[i] = make_float2(top, L);
         }
+    }
     __syncthreads();
     // ---- what each child's own chances say
-    for (int i = 1 + tid; i < n; i += kWalkThreads) {
+    for (int i = 1 + tid; i < n; i += T) {
         const int p = sh.parent[i], x = sh.token[i];
         uint8_t f = kIgnored;
         bool again = false;
@@ -334,12 +467,15 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 f = __float_as_int(sh.stat[p].x) == x ? kAccepted : kRejected;
             } else if (usable(sh.stat[p])) {
                 for (int e = sh.first[p]; e != i; e = sh.sibling[e]) again |= sh.token[e] == x;
-                chance = exp(((double)logit<DT>(row_of(p), x) - sh.stat[p].x) * scale) / sh.stat[p].y;
+                Expo ex;
+                ex.set(sh.pow, sh.stat[p].x, a.scale);
+                chance = or_none(ex(sh.z[i])) / sh.stat[p].y;
                 if (!drawn) {
                     f = kRejected;   // (decided below)
                 } else if (usable(sh.stat_q[p])) {
-                    const double q = exp(((double)logit<DT>(draft_of(p), x) - sh.stat_q[p].x) * scale_q) / sh.stat_q[p].y;
-                    f = sh.first[p] != i ? kAsk : (double)a.uniform[c0 + i] * q < chance ? kAccepted : kRejected;
+                    ex.set(sh.pow, sh.stat_q[p].x, a.draft_scale);
+                    const double q = ex(sh.zq[i]) / sh.stat_q[p].y;
+                    f = sh.first[p] != i ? kAsk : sh.u[i] * q < chance ? kAccepted : kRejected;
                 }
             }
         }
@@ -349,7 +485,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     if constexpr (!GREEDY) {
         if (!drawn) {
             // r is p without the earlier siblings' tokens
-            for (int i = 1 + tid; i < n; i += kWalkThreads)
+            for (int i = 1 + tid; i < n; i += T)
                 if (sh.flag[i] == kRejected && !sh.again[i]) {
                     double R = 1;
                     for (int e = sh.first[sh.parent[i]]; e != i; e = sh.sibling[e])
@@ -358,93 +494,93 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                     sh.mass[i] = R;
                 }
             __syncthreads();
-            for (int i = 1 + tid; i < n; i += kWalkThreads)
+            for (int i = 1 + tid; i < n; i += T)
                 if (sh.flag[i] == kRejected && !sh.again[i]) {
                     const double R = sh.mass[i];
-                    sh.flag[i] = R < 0x1p-10 ? kAsk : (double)a.uniform[c0 + i] * R < sh.chance[i] ? kAccepted : kRejected;
+                    sh.flag[i] = R < 0x1p-10 ? kAsk : sh.u[i] * R < sh.chance[i] ? kAccepted : kRejected;
                 }
             __syncthreads();
         }
     }
 
     // ---- passes of the cluster over a row: each warp a piece of whole steps of 256 tokens
-    const uint32_t piece = ((a.vocab + NW - 1) / NW + 255) / 256 * 256;
-    const uint64_t lo64 = (uint64_t)(rank * kWalkWarps + warp) * piece;
-    const uint32_t lo = (uint32_t)min(lo64, (uint64_t)a.vocab), hi = (uint32_t)min(lo64 + piece, (uint64_t)a.vocab);
     int turn = 0;
-    // every warp's value, at every CTA
-    auto spread = [&](uint64_t v) -> const uint64_t* {
-        uint64_t* to = sh.part[turn];
+    // every warp's values, at every CTA; value k of warp w at [k * kAll + w]
+    constexpr int kAll = kMaxCluster * kWalkWarps;
+    auto spread = [&](auto... v) -> const uint64_t* {
+        uint64_t* to = sh.part[turn][0];
         turn ^= 1;
-        if (lane < ctas) store_remote(to + rank * kWalkWarps + warp, lane, v);
+        int k = 0;
+        if (lane < ctas)
+            ((store_remote(to + k * kAll + rank * W + warp, lane, v), ++k), ...);
         cluster_sync();
         return to;
     };
-    auto warp_sum64 = [&](double x) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-        return x;
-    };
+    auto bits = [](double x) { return (uint64_t)__double_as_longlong(x); };
+    auto value = [](uint64_t x) { return __longlong_as_double((long long)x); };
     auto total = [&](const uint64_t* parts) {   // (the same order of sums in every thread)
         double s = 0;
-        for (int w = lane; w < NW; w += 32) s += __longlong_as_double(parts[w]);
+        for (int w = lane; w < NW; w += 32) s += value(parts[w]);
         return warp_sum64(s);
     };
 
-    // The last token's row: references, sums, rejections.
+    // The last token's row: exponentials, sums, rejections.
     int cur = 0, cnt = 1;
-    float ref = 0.f, ref_q = 0.f;
-    double Lp = 0, Lq = 0;
+    Expo ep, eq;
+    double Lp = 0, iq = 0;     // the target's sum; the draft's reciprocal sum, times Lp
     int m = 0, from = 0;       // rejections that count; those before `from` left nothing
-    bool summed = false;       // Lp and Lq are those of cur
-    // r of token v with target and draft exponentials ep and eq, after k rejections
-    auto left = [&](double ep, double eq, int k) {
-        double r = ep / Lp;
-        const double q = eq / Lq;
-        for (int i = from; i < k; ++i) r = fmax(r - sh.mass[i] * q, 0.0);
-        return r;
+    bool summed = false;       // Lp and iq are those of cur
+    // r, times Lp, of a token with exponentials x and y, after k rejections
+    auto left = [&](double x, double y, int k) {
+        const double q = y * iq;
+        for (int i = from; i < k; ++i) {
+            const double d = sh.mass[i] * q;
+            x = x > d ? x - d : 0.0;
+        }
+        return x;
     };
-    auto gone = [&](uint32_t v, int stop) {   // not drawn: the token of a rejected child before `stop`
+    auto gone = [&](int v, int stop) {   // not drawn: the token of a rejected child before `stop`
         for (int e = sh.first[cur]; e >= 0 && e < kMaxTree && e != stop; e = sh.sibling[e])
-            if (sh.flag[e] == kRejected && !sh.again[e] && sh.token[e] == (int)v) return true;
+            if (sh.flag[e] == kRejected && !sh.again[e] && sh.token[e] == v) return true;
         return false;
     };
-    // Sum over the warp's piece of what f makes of eight tokens of the row (and of the draft's).
+    // f of eight tokens at a time of the warp's piece of the row (and of the draft's)
+    int lo = 0, hi = 0;
     auto sweep = [&](bool both, auto f) {
-        const void *zp = row_of(cur), *zq = both ? draft_of(cur) : nullptr;
-        double s = 0;
-        for (uint32_t v = lo + lane * 8; v < hi; v += 256) {
+        const char *zp = row_of(cur), *zq = both ? draft_of(cur) : nullptr;
+        const int off = (int)(((uintptr_t)zp & 15) / kSize<DT>), V = (int)a.vocab;
+        const int64_t piece = (((int64_t)V + off + NW - 1) / NW + 255) / 256 * 256;
+        lo = (int)min((rank * W + warp) * piece - off, (int64_t)V);
+        hi = (int)min((int64_t)lo + piece, (int64_t)V);
+        for (int v = lo + lane * 8; v < hi; v += 256) {
+            Eight<DT> p, q;
+            p.load(zp, v, V);
+            if (both) q.load(zq, v, V);
             float x[8], y[8];
-            load8<DT>(zp, v, a.vocab, x);
-            if (both) load8<DT>(zq, v, a.vocab, y);
-            s += f(x, y, v);
+            p.floats(x);
+            if (both) q.floats(y);
+            f(x, y, v);
         }
-        return s;
     };
-    auto expo = [&](float x, float r, double sc) { return exp(((double)x - r) * sc); };
-    auto sums = [&]() {        // Lp (and Lq) in 64 bits
+    auto sums = [&]() {        // Lp and iq
         if (summed) return;
-        double sq = 0;
-        const double sp = sweep(true, [&](const float (&x)[8], const float (&y)[8], uint32_t) {
-            double s = 0;
+        double sp = 0, sq = 0;
+        sweep(true, [&](const float (&x)[8], const float (&y)[8], int) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += expo(x[i], ref, scale), sq += expo(y[i], ref_q, scale_q);
-            return s;
+            for (int i = 0; i < 8; ++i) sp += ep(x[i]), sq += eq(y[i]);
         });
-        const uint64_t* p = spread(__double_as_longlong(warp_sum64(sp)));
+        const uint64_t* p = spread(bits(warp_sum64(sp)), bits(warp_sum64(sq)));
         Lp = total(p);
-        p = spread(__double_as_longlong(warp_sum64(sq)));
-        Lq = total(p);
+        iq = Lp / total(p + kAll);
         summed = true;
     };
-    auto mass_of = [&](int k) {   // the warps' sums of r after k rejections
-        const double s = sweep(true, [&](const float (&x)[8], const float (&y)[8], uint32_t) {
-            double t = 0;
+    auto mass_of = [&](int k) {   // the warps' sums of r Lp after k rejections
+        double s = 0;
+        sweep(true, [&](const float (&x)[8], const float (&y)[8], int) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t += left(expo(x[i], ref, scale), expo(y[i], ref_q, scale_q), k);
-            return t;
+            for (int i = 0; i < 8; ++i) s += left(ep(x[i]), eq(y[i]), k);
         });
-        return spread(__double_as_longlong(warp_sum64(s)));
+        return spread(bits(warp_sum64(s)));
     };
     auto set_mass = [&](int k, double R) {   // (every thread has the same R)
         __syncthreads();
@@ -452,40 +588,38 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         __syncthreads();
     };
     auto without = [&](int stop) {   // the warps' sums of p's exponentials without rejected tokens
-        const double s = sweep(false, [&](const float (&x)[8], const float (&)[8], uint32_t v) {
-            double t = 0;
+        double s = 0;
+        sweep(false, [&](const float (&x)[8], const float (&)[8], int v) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t += m && gone(v + i, stop) ? 0.0 : expo(x[i], ref, scale);
-            return t;
+            for (int i = 0; i < 8; ++i) s += m && gone(v + i, stop) ? 0.0 : ep(x[i]);
         });
-        return spread(__double_as_longlong(warp_sum64(s)));
+        return spread(bits(warp_sum64(s)));
     };
 
     if (rank == 0)
-        for (int i = tid; i < n; i += kWalkThreads) a.path[c0 + i] = i ? -1 : c0;
+        for (int i = tid; i < n; i += T) a.path[c0 + i] = i ? -1 : c0;
     __syncthreads();
     for (;;) {   // (every thread of the cluster takes the same way)
         int c = sh.first[cur];
         m = from = 0, summed = false;
-        ref = sh.stat[cur].x, ref_q = sh.stat_q[cur].x;
-        if (drawn) set_mass(0, 1.0);
+        if constexpr (!GREEDY) {
+            ep.set(sh.pow, sh.stat[cur].x, a.scale);
+            if (drawn) eq.set(sh.pow, sh.stat_q[cur].x, a.draft_scale);
+        }
         int took = -1;
         if (c < kMaxTree)
             for (; c >= 0; c = sh.sibling[c]) {
                 uint8_t f = sh.flag[c];
                 if (f == kIgnored) continue;
                 if (f == kAsk) {
-                    const double u = a.uniform[c0 + c];
-                    const uint32_t x = sh.token[c];
+                    const double u = sh.u[c];
+                    const double e = or_none(ep(sh.z[c]));
                     if (drawn) {
                         sums();
-                        const double ep = expo(logit<DT>(row_of(cur), x), ref, scale);
-                        const double eq = expo(logit<DT>(draft_of(cur), x), ref_q, scale_q);
-                        f = u * (eq / Lq) * sh.mass[m] < left(ep, eq, m) ? kAccepted : kRejected;
+                        const double q = eq(sh.zq[c]);
+                        f = u * (q * iq) * sh.mass[m] < left(e, q, m) ? kAccepted : kRejected;
                     } else {
-                        double R = total(without(c));
-                        const double e = expo(logit<DT>(row_of(cur), x), ref, scale);
-                        f = u * R < e ? kAccepted : kRejected;
+                        f = u * total(without(c)) < e ? kAccepted : kRejected;
                         __syncthreads();
                         if (tid == 0) sh.flag[c] = f;
                         __syncthreads();
@@ -496,142 +630,389 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                     break;
                 }
                 ++m;
-                if (drawn) {
-                    // R is needed for the next child and for the draw; the last one's is found there
-                    if (sh.sibling[c] >= 0) {
-                        sums();
-                        double R = total(mass_of(m));
-                        if (!(R > 0)) from = m, R = 1;
-                        set_mass(m, R);
-                    }
+                // R is needed for the next child, who is asked with the whole row
+                if (drawn && sh.sibling[c] >= 0) {
+                    sums();
+                    double R = total(mass_of(m)) / Lp;
+                    if (!(R > kNothing)) from = m, R = 1;
+                    set_mass(m, R);
                 }
             }
         if (took < 0) break;
         cur = took;
         if (rank == 0 && tid == 0) a.path[c0 + cnt] = c0 + cur;
         ++cnt;
-        __syncthreads();   // (before masses and flags of the next token's children)
     }
     if (rank == 0 && tid == 0) a.count[b] = cnt;
 
-    // ---- next
-    const bool inner = sh.first[cur] < kMaxTree;
-    if constexpr (GREEDY) {
-        int best = __float_as_int(sh.stat[cur].x);
-        if (!inner) {
-            uint64_t key = 0;
-            for (uint32_t v = lo + lane * 8; v < hi; v += 256) {
-                float x[8];
-                load8<DT>(row_of(cur), v, a.vocab, x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) key = max64(key, v + i < a.vocab ? key_of(x[i], v + i) : 0);
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) key = max64(key, __shfl_xor_sync(~0u, key, o));
-            const uint64_t* p = spread(key);
-            key = 0;
-            for (int w = 0; w < NW; ++w) key = max64(key, p[w]);
-            const uint32_t top = key >> 32;
-            best = top > kOrderNone && top < kOrderInf ? (int)(0xFFFFFFFFu - (uint32_t)key) : -1;
-        }
-        if (rank == 0 && tid == 0) a.next[b] = best;
-    } else {
-        if (!inner) {   // a leaf's row has not been read yet
-            float top = -INFINITY;
-            for (uint32_t v = lo + lane * 8; v < hi; v += 256) {
-                float x[8];
-                load8<DT>(row_of(cur), v, a.vocab, x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);   // (a NaN shows in the sum)
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-            const uint64_t* p = spread(order(top));
-            uint64_t most = 0;
-            for (int w = 0; w < NW; ++w) most = max64(most, p[w]);
-            const uint32_t o = (uint32_t)most;
-            ref = __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-        }
-        const uint64_t* parts = nullptr;
-        double R = 0;
-        int k = drawn ? m : 0;
-        if (ref > -INFINITY && ref < INFINITY) {
-            if (k) {
-                sums();
-                parts = mass_of(k);
-                R = total(parts);
-                if (!(R > 0)) k = 0;   // nothing is left: p again
-            }
-            if (!k) {
-                parts = without(-1);
-                R = total(parts);
-                if (!(R > 0) && m) {
-                    m = 0;
-                    parts = without(-1);
-                    R = total(parts);
-                }
+    // ---- what `next` is drawn from
+    if (rank == 0) {
+        const bool inner = sh.first[cur] < kMaxTree;
+        if constexpr (!GREEDY) {
+            if (drawn) {
+                for (int i = tid; i < m && m > 1; i += T) a.mass[c0 + i] = sh.mass[i];
+            } else if (tid == 0 && inner) {
+                m = 0;
+                for (int e = sh.first[cur]; e >= 0; e = sh.sibling[e])
+                    if (sh.flag[e] == kRejected && !sh.again[e]) a.gone[c0 + m++] = sh.token[e];
             }
         }
-        if (!(R > 0 && R < INFINITY)) {
-            if (rank == 0 && tid == 0) a.next[b] = -1;
+        if (tid == 0) {
+            Record r = {kList, c0 + cur, m, from, 0.f, 0.f, 0.f, Lp, iq};
+            if constexpr (GREEDY) {
+                r.mode = inner ? kDone : kTop;
+                if (inner) a.next[b] = __float_as_int(sh.stat[cur].x);
+            } else if (inner && !usable(sh.stat[cur])) {
+                r.mode = kDone;
+                a.next[b] = -1;
+            } else if (drawn && m > from) {
+                r.mode = m == 1 ? kOnce : kOften;
+                r.ref = sh.stat[cur].x, r.ref_q = sh.stat_q[cur].x;
+                r.near = sh.stat[cur].y / sh.stat_q[cur].y;
+            } else if (drawn) {
+                r.k = 0;   // nothing was rejected, or nothing left: p
+            }
+            a.records[b] = r;
+            a.counters[b] = 0;
+        }
+    }
+    if (ctas > 1) cluster_sync();   // (no CTA ends while another's stores are on their way to it)
+}
+
+// ---- the draw
+// r's sums over pieces of the row, a warp a piece; the sequence's last CTA finds the token.
+template <int DT, bool GREEDY>
+__global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __grid_constant__ VerifyArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ int sh_gone[kMaxTree];
+    __shared__ double sh_mass[kMaxTree], sh_pow[kPowers];
+    __shared__ double sh_sum[2][kDrawWarps], sh_base;
+    __shared__ float sh_x[2][9 * kDrawThreads];
+    __shared__ int sh_at[kDrawWarps], sh_last, sh_owner;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.x / a.draw_segs, seg = blockIdx.x - b * a.draw_segs;
+    const Record rec = a.records[b];
+    if (rec.mode == kDone) return;
+    const int c0 = a.cu[b], V = (int)a.vocab, NW = a.draw_segs * kDrawWarps;
+    const char* zp = (const char*)a.logits + (uint64_t)rec.row * a.row_stride * kSize<DT>;
+    const char* zq = (const char*)a.draft + (uint64_t)rec.row * a.draft_stride * kSize<DT>;
+    const int off = (int)(((uintptr_t)zp & 15) / kSize<DT>);
+    const int64_t piece = (((int64_t)V + off + NW - 1) / NW + 255) / 256 * 256;
+    auto from_of = [&](int w) { return (int)min(w * piece - off, (int64_t)V); };
+    const int lo = from_of(seg * kDrawWarps + warp), hi = (int)min((int64_t)lo + piece, (int64_t)V);
+    double* mine = a.sums + ((uint64_t)b * NW + seg * kDrawWarps + warp) * 4;
+    const double* all = a.sums + (uint64_t)b * NW * 4;
+
+    if (tid < kPowers) sh_pow[tid] = exp2(tid * (1.0 / kPowers));
+    if (rec.mode == kList)
+        for (int i = tid; i < rec.k; i += kDrawThreads) sh_gone[i] = a.gone[c0 + i];
+    if (rec.mode == kOften)
+        for (int i = tid; i < rec.k; i += kDrawThreads) sh_mass[i] = a.mass[c0 + i];
+    __syncthreads();
+    Expo ep, eq;
+    ep.set(sh_pow, rec.ref, a.scale), eq.set(sh_pow, rec.ref_q, a.draft_scale);
+    double iq = rec.iq;
+    // r, times Lp, of drawn children's rejections
+    auto left = [&](double x, double y, int k) {
+        const double q = y * iq;
+        if (rec.mode == kOnce) return x > q ? x - q : 0.0;
+        for (int i = rec.from; i < k; ++i) {
+            const double d = sh_mass[i] * q;
+            x = x > d ? x - d : 0.0;
+        }
+        return x;
+    };
+    // which of the tokens v .. v + 7 are gone, as bits
+    auto gone8 = [&](int v, int k) {
+        uint32_t g = 0;
+        for (int i = 0; i < k; ++i) {
+            const uint32_t d = (uint32_t)(sh_gone[i] - v);
+            if (d < 8) g |= 1u << d;
+        }
+        return g;
+    };
+
+    // ---- the warp's piece, the next step's loads ahead
+    double s0 = 0, s1 = 0, s2 = 0, s3 = 0;
+    const bool both = rec.mode == kOnce || rec.mode == kOften;
+    float ref = -INFINITY, lim = -INFINITY, most = -INFINITY;   // kList
+    Best best;                                                  // kTop
+    Eight<DT> p, q;
+    auto load = [&](int v) {
+        p.load(zp, v, hi);
+        if (both) q.load(zq, v, hi);
+    };
+    if (lo < hi) load(lo + lane * 8);
+    for (int v0 = lo; v0 < hi; v0 += 256) {   // (the whole warp)
+        const int v = v0 + lane * 8;
+        float x[8], y[8];
+        p.floats(x);
+        if (both) q.floats(y);
+        if (v0 + 256 < hi) load(v + 256);
+        if constexpr (GREEDY) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) best.take(x[i], v + i);
+        } else if (rec.mode == kOnce) {
+            // s0 - less s1: r, s2 and s3: the whole of p and q.  r is ep - less eq where that is positive,
+            // less = Lp / Lq.  The first kernel's sums give that to 2^-20, which tells the tokens where r is
+            // positive but for some whose r is below 2^-20 of their p; with their sums, and the row's, one
+            // pass is enough.
+            const double near = rec.near;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double e = ep(x[i]), d = eq(y[i]);
+                if (e > near * d) s0 += e, s1 += d;
+                s2 += e, s3 += d;
+            }
+        } else if (rec.mode == kOften) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double e = ep(x[i]);
+                s0 += left(e, eq(y[i]), rec.k);
+                s2 += e;
+            }
         } else {
-            // ---- the warp whose piece the sum passes u R in, then the token
-            const double goal = (double)a.uniform_next[b] * R;
-            int owner = -1, last = 0;
-            double before = 0, base = 0;
-            for (int w = 0; w < NW; ++w) {
-                const double s = __longlong_as_double(parts[w]);
-                if (s > 0) last = w;
-                if (owner < 0 && s > 0 && before + s > goal) owner = w, base = before;
-                before += s;
+            // s0: what is left, s1: what is gone, against the reference s2 (the first steps' largest logit,
+            // or the largest of a later step that passes it by 2^500)
+            float top = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) top = max_nan(top, x[i]);
+            most = max_nan(most, top);
+            const float step = unorder(__reduce_max_sync(~0u, top == top ? order(top) : kOrderNone));
+            if (step > lim) {
+                const float was = ref;
+                ref = step, lim = step + (float)(500.0 / (1.4426950408889634 * a.scale));
+                ep.set(sh_pow, ref, a.scale);
+                const double f = was > -INFINITY ? ep(was) : 0.0;
+                s0 *= f, s1 *= f;
             }
-            const bool found = owner >= 0;
-            if (!found) owner = last;
-            if (owner == rank * kWalkWarps + warp) {
-                const void *zp = row_of(cur), *zq = k ? draft_of(cur) : nullptr;
-                int best = -1, final_one = -1;
-                for (uint32_t v0 = lo; v0 < hi && best < 0; v0 += 256) {
-                    const uint32_t v = v0 + lane * 8;
-                    double r[8], s = 0;
-                    float x[8], y[8];
+            if (ref == -INFINITY) continue;
+            const uint32_t g = rec.k ? gone8(v, rec.k) : 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) r[i] = 0;
-                    if (v < hi) {
-                        load8<DT>(zp, v, a.vocab, x);
-                        if (k) load8<DT>(zq, v, a.vocab, y);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const double ep = expo(x[i], ref, scale);
-                            r[i] = k ? left(ep, expo(y[i], ref_q, scale_q), k) : m && gone(v + i, -1) ? 0.0 : ep;
-                            s += r[i];
-                        }
-                    }
-                    double upto = s;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double t = __shfl_up_sync(~0u, upto, o);
-                        if (lane >= o) upto += t;
-                    }
-                    int mine = -1, tail = -1;
-                    double at = base + upto - s;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        at += r[i];
-                        if (r[i] > 0) {
-                            tail = v + i;
-                            if (mine < 0 && found && at > goal) mine = v + i;
-                        }
-                    }
-                    const unsigned hit = __ballot_sync(~0u, mine >= 0), some = __ballot_sync(~0u, tail >= 0);
-                    if (hit) best = __shfl_sync(~0u, mine, __ffs(hit) - 1);
-                    if (some) final_one = __shfl_sync(~0u, tail, 31 - __clz(some));
-                    base += __shfl_sync(~0u, upto, 31);
-                }
-                if (lane == 0) a.next[b] = best >= 0 ? best : final_one;
+            for (int i = 0; i < 8; ++i) {
+                const double e = ep(x[i]);
+                s0 += g >> i & 1 ? 0.0 : e;
+                if (rec.k) s1 += g >> i & 1 ? e : 0.0;
             }
         }
     }
-    cluster_sync();   // (no CTA ends while another's stores are on their way to it)
+    if constexpr (GREEDY) {
+        uint64_t key = best.key();
+#pragma unroll
+        for (int o = 16; o; o >>= 1) key = max64(key, __shfl_xor_sync(~0u, key, o));
+        s0 = __longlong_as_double((long long)key);
+    } else {
+        if (!(most < INFINITY)) s0 = NAN;   // (no distribution)
+        s0 = warp_sum64(s0), s1 = warp_sum64(s1);
+        if (rec.mode == kList) s2 = ref;
+        else s2 = warp_sum64(s2), s3 = warp_sum64(s3);
+    }
+    if (lane < 4) __stcg(mine + lane, lane == 0 ? s0 : lane == 1 ? s1 : lane == 2 ? s2 : s3);
+    __syncthreads();
+    if (tid == 0) {
+        unsigned was;   // release: the CTA's sums before its count; acquire: the others'
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(was) : "l"(a.counters + b) : "memory");
+        sh_last = was + 1 == (unsigned)a.draw_segs;
+    }
+    __syncthreads();
+    if (!sh_last) return;
+
+    // ---- the sequence's last CTA: a thread has up to `each` pieces' sums, one after the other
+    constexpr int kEach = kMaxDrawSegs * kDrawWarps / kDrawThreads;
+    const int each = (NW + kDrawThreads - 1) / kDrawThreads;
+    double2 in01[kEach], in23[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int w = tid * each + i;
+        const bool on = i < each && w < NW;
+        in01[i] = on ? __ldcg(reinterpret_cast<const double2*>(all + 4 * w)) : make_double2(0.0, 0.0);
+        in23[i] = on ? __ldcg(reinterpret_cast<const double2*>(all + 4 * w + 2)) : make_double2(0.0, 0.0);
+    }
+    if constexpr (GREEDY) {
+        uint64_t key = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) key = max64(key, (uint64_t)__double_as_longlong(in01[i].x));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) key = max64(key, __shfl_xor_sync(~0u, key, o));
+        if (lane == 0) sh_sum[0][warp] = __longlong_as_double((long long)key);
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < kDrawWarps; ++w) key = max64(key, (uint64_t)__double_as_longlong(sh_sum[0][w]));
+            const uint32_t top = key >> 32;
+            a.next[b] = top > kOrderNone && top < kOrderInf ? (int)(0xFFFFFFFFu - (uint32_t)key) : -1;
+        }
+        return;
+    }
+    auto sums_of = [&](double& x, double& y) {   // over the CTA
+        x = warp_sum64(x), y = warp_sum64(y);
+        __syncthreads();
+        if (lane == 0) sh_sum[0][warp] = x, sh_sum[1][warp] = y;
+        __syncthreads();
+        x = y = 0;
+#pragma unroll
+        for (int w = 0; w < kDrawWarps; ++w) x += sh_sum[0][w], y += sh_sum[1][w];
+    };
+    double S[kEach];
+    int k = rec.k;
+    double R = 0, full = 0;
+    if (rec.mode == kList) {
+        float top = -INFINITY;   // (the largest of the pieces' references)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (i < each && tid * each + i < NW) top = fmaxf(top, (float)in23[i].x);
+        const uint32_t o = __reduce_max_sync(~0u, order(top));
+        if (lane == 0) sh_at[warp] = (int)o;
+        __syncthreads();
+        uint32_t most_o = 0;
+#pragma unroll
+        for (int w = 0; w < kDrawWarps; ++w) most_o = max(most_o, (uint32_t)sh_at[w]);
+        top = unorder(most_o);
+        if (top > -INFINITY) {
+            ep.set(sh_pow, top, a.scale);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const double f = ep((float)in23[i].x);
+                S[i] = in01[i].x * f, in23[i].x = S[i] + in01[i].y * f;
+                R += S[i], full += in23[i].x;
+            }
+        }
+    } else {
+        double less = 0;
+        if (rec.mode == kOnce) {
+            double sq = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) less += in23[i].x, sq += in23[i].y;
+            sums_of(less, sq);
+            iq = less = less / sq;
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            S[i] = fma(-less, in01[i].y, in01[i].x);
+            R += S[i], full += in23[i].x;
+        }
+    }
+    sums_of(R, full);
+    if (!(R > kNothing)) {   // nothing is left: p again
+        k = 0, R = full;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) S[i] = in23[i].x;
+    }
+    if (!(R > kNothing && R < INFINITY)) {
+        if (tid == 0) a.next[b] = -1;
+        return;
+    }
+    // ---- the piece in which the sum passes u R (none, by rounding: the last that has any)
+    const double goal = (double)a.uniform_next[b] * R;
+    auto before_of = [&](double x, double& whole) {   // the sum of the threads before, and of all
+        const double upto = scan64(x);
+        __syncthreads();
+        if (lane == 31) sh_sum[0][warp] = upto;
+        __syncthreads();
+        double at = 0;
+        whole = 0;
+#pragma unroll
+        for (int w = 0; w < kDrawWarps; ++w) {
+            if (w < warp) at += sh_sum[0][w];
+            whole += sh_sum[0][w];
+        }
+        return at + (upto - x);
+    };
+    double mass = 0, whole;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mass += S[i];
+    if (tid == 0) sh_owner = 0x7FFFFFFF, sh_last = -1;
+    double at = before_of(mass, whole);
+    int owner = 0x7FFFFFFF, last = -1;
+    double base = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (S[i] > kNothing) {
+            last = tid * each + i;
+            if (owner == 0x7FFFFFFF && at + S[i] > goal) owner = last, base = at;
+        }
+        at += S[i];
+    }
+    if (owner != 0x7FFFFFFF) atomicMin(&sh_owner, owner);
+    if (last >= 0) atomicMax(&sh_last, last);
+    __syncthreads();
+    const bool found = sh_owner != 0x7FFFFFFF;
+    if (found && owner == sh_owner) sh_base = base;
+    __syncthreads();
+    base = found ? sh_base : 0;
+    owner = found ? sh_owner : sh_last;
+    // ---- the token: up to eight a thread, from shared memory (in loops of two: one CTA a sequence
+    // comes here, and its instructions come from far)
+    const int first = from_of(owner), end = (int)min((int64_t)first + piece, (int64_t)V);
+    const bool two = both && k;
+    const int per = min(8, (end - first + 2 * kDrawThreads - 1) / (2 * kDrawThreads) * 2);   // tokens of a thread
+    auto place = [](int i) { return i + (i >> 3); };
+    const double start = base;
+    int token = -1, tail = -1;
+#pragma unroll 1
+    for (int pass = found ? 0 : 1; pass < 2 && token < 0; ++pass) {   // (1: the last that has any)
+        base = start;
+#pragma unroll 1
+        for (int v0 = first; v0 < end && token < 0; v0 += per * kDrawThreads) {
+            float x[8], y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int v = v0 + i * kDrawThreads + tid;
+                const bool in = i < per && v >= 0 && v < end;
+                x[i] = in ? logit<DT>(zp, v) : -INFINITY;
+                y[i] = in && two ? logit<DT>(zq, v) : -INFINITY;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < per) {
+                    sh_x[0][place(i * kDrawThreads + tid)] = x[i];
+                    sh_x[1][place(i * kDrawThreads + tid)] = y[i];
+                }
+            __syncthreads();
+            const int v = v0 + per * tid;
+            const uint32_t g = !both && k ? gone8(v, k) : 0;
+            auto rest = [&](int i, double& r0, double& r1) {   // of tokens v + i and the next
+                const int at = per * tid + i;
+                r0 = ep(sh_x[0][place(at)]), r1 = ep(sh_x[0][place(at + 1)]);
+                if (two) r0 = left(r0, eq(sh_x[1][place(at)]), k), r1 = left(r1, eq(sh_x[1][place(at + 1)]), k);
+                r0 = g >> i & 1 ? 0.0 : r0, r1 = g >> i & 2 ? 0.0 : r1;
+            };
+            double s = 0;
+#pragma unroll 1
+            for (int i = 0; i < per; i += 2) {
+                double r0, r1;
+                rest(i, r0, r1);
+                s += r0 + r1;
+            }
+            double before = base + before_of(s, whole);
+            int here = pass ? -1 : 0x7FFFFFFF;
+            if (pass || before + s > goal) {
+#pragma unroll 1
+                for (int i = 0; i < per; i += 2) {
+                    double r[2];
+                    rest(i, r[0], r[1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        before += r[j];
+                        if (r[j] > kNothing) {
+                            if (pass) here = v + i + j;
+                            else if (before > goal) here = min(here, v + i + j);
+                        }
+                    }
+                }
+            }
+            here = pass ? __reduce_max_sync(~0u, here) : __reduce_min_sync(~0u, here);
+            if (lane == 0) sh_at[warp] = here;
+            __syncthreads();
+            for (int w = 0; w < kDrawWarps; ++w) here = pass ? max(here, sh_at[w]) : min(here, sh_at[w]);
+            if (pass) tail = max(tail, here);
+            else if (here != 0x7FFFFFFF) token = here;
+            base += whole;
+            __syncthreads();
+        }
+    }
+    if (tid == 0) a.next[b] = token >= 0 ? token : tail;
 }
 
 int check_verify(const GraftVerifyParams* P) {
@@ -658,36 +1039,87 @@ int segments(const GraftVerifyParams* P) {
     return (int)std::min<uint64_t>(std::min<uint64_t>(want, most), kMaxSegs);
 }
 
+// CTAs that go over a sequence's last row: two rounds of two an SM, none with less than 2048 tokens.
+int draw_segments(const GraftVerifyParams* P) {
+    const uint64_t seqs = P->n_seqs ? P->n_seqs : 1;
+    const uint64_t want = (148 * 4 + seqs - 1) / seqs, most = std::max<uint64_t>(1, P->vocab / 2048);
+    return (int)std::min<uint64_t>(std::min<uint64_t>(want, most), kMaxDrawSegs);
+}
+
+// The workspace's parts; its size.
+size_t carve(const GraftVerifyParams* P, char* ws, VerifyArgs* a) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char* p = ws + at;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    const size_t rows = P->tokens, seqs = P->n_seqs;
+    char* parts = take(2 * rows * segments(P) * 8);
+    char* records = take(seqs * sizeof(Record));
+    char* counters = take(seqs * 4);
+    char* gone = take(rows * 4);
+    char* mass = take(rows * 8);
+    char* sums = take(seqs * draw_segments(P) * kDrawWarps * 32);
+    if (a) {
+        a->parts = (uint64_t*)parts, a->records = (Record*)records, a->counters = (unsigned*)counters;
+        a->gone = (int32_t*)gone, a->mass = (double*)mass, a->sums = (double*)sums;
+    }
+    return std::max<size_t>(256, at);
+}
+
 template <int DT, bool GREEDY>
 int launch_verify(const VerifyArgs& a, cudaStream_t st) {
     int rc;
     if ((rc = launch_pdl("verify_drafts", verify_rows_kernel<DT, GREEDY>,
                          dim3(a.rows * (unsigned)a.segs, a.draft && !GREEDY ? 2 : 1), kRowThreads, 0, st, a)))
         return rc;
-    // CTAs of a cluster: up to eight, none with less than 4096 tokens
+    DeviceInfo di;
+    if ((rc = current_device_info(&di))) return rc;
+    // Whole rows are gone over during the walk where a token may have several drawn children: then a
+    // cluster a sequence (sixteen CTAs while all have an SM of their own), no CTA of it with less
+    // than 4096 tokens.
     int ctas = 1;
-    while (ctas < kMaxCluster && (uint64_t)ctas * 2 * 4096 <= a.vocab) ctas *= 2;
+    if (!GREEDY && a.draft && a.parents) {
+        const int most = (uint64_t)a.n_seqs * kMaxCluster <= (uint64_t)di.sm_count ? kMaxCluster : kMaxCluster / 2;
+        while (ctas < most && (uint64_t)ctas * 2 * 4096 <= a.vocab) ctas *= 2;
+    }
     const auto kern = verify_walk_kernel<DT, GREEDY>;
     if ((rc = ensure_smem((const void*)kern, sizeof(Walk)))) return rc;
+    static std::atomic<uint64_t> wide{0};   // devices where clusters of sixteen are allowed
+    const uint64_t bit = 1ull << (di.device & 63);
+    if (ctas > 8 && !(wide.load(std::memory_order_relaxed) & bit)) {
+        GRAFT_CUDA(cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        wide.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.n_seqs * ctas);
     cfg.blockDim = dim3(kWalkThreads);
     cfg.dynamicSmemBytes = sizeof(Walk);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    int attrs = 0;
+    if (ctas > 1) {
+        at[attrs].id = cudaLaunchAttributeClusterDimension;
+        at[attrs].val.clusterDim.x = ctas, at[attrs].val.clusterDim.y = 1, at[attrs].val.clusterDim.z = 1;
+        ++attrs;
+    }
+    if (pdl_enabled()) {
+        at[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[attrs].val.programmaticStreamSerializationAllowed = 1;
+        ++attrs;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = attrs;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, ctas);
     if (e != cudaSuccess) {
         cudaGetLastError();
         set_error("verify_drafts: launch failed: %s", cudaGetErrorString(e));
         return GRAFT_ECUDA;
     }
-    return check_launch("verify_drafts");
+    if ((rc = check_launch("verify_drafts"))) return rc;
+    return launch_pdl("verify_drafts", verify_draw_kernel<DT, GREEDY>, dim3(a.n_seqs * (unsigned)a.draw_segs),
+                      kDrawThreads, 0, st, a);
 }
 template <int DT>
 int launch_verify(const VerifyArgs& a, cudaStream_t st) {
@@ -724,7 +1156,7 @@ extern "C" int graft_draft_tree(const int32_t* parents, const GraftKVRange* rang
 
 extern "C" size_t graft_verify_workspace(const GraftVerifyParams* P) {
     if (check_verify(P)) return 0;
-    return std::max<size_t>(256, (size_t)2 * P->tokens * segments(P) * 8);
+    return carve(P, nullptr, nullptr);
 }
 
 extern "C" int graft_verify_drafts(const void* logits, const void* draft, const int32_t* tokens,
@@ -756,8 +1188,8 @@ extern "C" int graft_verify_drafts(const void* logits, const void* draft, const 
     a.row_stride = P->row_stride, a.draft_stride = P->draft_stride;
     a.n_seqs = P->n_seqs, a.rows = P->tokens, a.max_tokens = P->max_tokens, a.vocab = P->vocab;
     a.scale = P->scale, a.draft_scale = P->draft_scale;
-    a.segs = segments(P);
-    a.parts = (uint64_t*)ws;
+    a.segs = segments(P), a.draw_segs = draw_segments(P);
+    carve(P, (char*)ws, &a);
     return P->dtype == GRAFT_F16    ? launch_verify<GRAFT_F16>(a, stream)
            : P->dtype == GRAFT_BF16 ? launch_verify<GRAFT_BF16>(a, stream)
                                     : launch_verify<GRAFT_F32>(a, stream);
