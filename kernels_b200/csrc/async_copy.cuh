@@ -79,6 +79,10 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// The same, or zeros in place of the source, which is then not read.
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void* src, bool read) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0) : "memory");
+}
 // Arrives on `bar` once all of this thread's earlier cp.async copies have
 // landed (the arrival is pre-counted in the barrier's expected count).
 __device__ __forceinline__ void cp_async_mbar_arrive(uint32_t bar) {

@@ -11,105 +11,14 @@
 //   131071 keys, 8 rows 38 | 153, 32 rows 67 | 154
 //   32 sequences of up to 8192 keys, 8 rows 41 | 146, 16 rows 52 | 146, 32 rows 76 | 148
 //   the same, heads of 128: 4 rows 57 | 200, 16 rows 92 | 204;  of 256: 8 rows 104 | 374
-#include "attn_chunk.cuh"
-#include "attn_few.cuh"
+#include "attn_launch.cuh"
 
-#include <algorithm>
-#include <atomic>
 #include <cmath>
 
 using namespace graft;
 using namespace graft::dev;
 
 namespace {
-
-__device__ unsigned g_attn_err;
-
-// The error word's address on a device (asked for once).
-int error_word(int device, unsigned** out) {
-    static std::atomic<unsigned*> known[64];
-    unsigned* p = device < 64 ? known[device].load(std::memory_order_relaxed) : nullptr;
-    if (!p) {
-        GRAFT_CUDA(cudaGetSymbolAddress((void**)&p, g_attn_err));
-        if (device < 64) known[device].store(p, std::memory_order_relaxed);
-    }
-    *out = p;
-    return GRAFT_OK;
-}
-
-// ---- few query rows
-template <int DP, int NT, int FMT, bool FULL, bool TREE>
-int launch_few(AttnArgs a, cudaStream_t st) {
-    DeviceInfo di;
-    int rc = current_device_info(&di);
-    if (rc) return rc;
-    constexpr int smem = kFewSmem<DP, NT>;
-    const auto kern = attn_few_kernel<DP, NT, FMT, FULL, TREE>;
-    int per_sm = 1;
-    if ((rc = ensure_smem((const void*)kern, smem)) ||
-        (rc = occupancy((const void*)kern, kFewThreads, smem, &per_sm)))
-        return rc;
-    unsigned* err = nullptr;
-    if ((rc = error_word(di.device, &err))) return rc;
-    // no more CTAs than the longest possible range has pieces
-    const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
-                                   : a.max_len;
-    // A CTA's share is at least two units a warp, and a piece of a pair costs about three
-    // more (queries, first copies, join): 32 sequences with windows of 128 keys take 27 us
-    // without the pad and 9.8 with it, 64 of up to 8192 keys 122 and 102.
-    a.min_units = 2 * kFewWarps;
-    a.pad_units = 3 * kFewWarps;
-    const uint64_t units = keys / kFewUnit<DP> + 2 + a.pad_units;
-    const uint64_t pairs = (uint64_t)a.n_seqs * a.heads;
-    // (units and a piece's edge beyond them are counted in 31 bits)
-    GRAFT_REQUIRE(pairs * units < (1ull << 31) - a.pad_units - a.min_units,
-                  "max_len %u of %u sequences is too long", a.max_len, a.n_seqs);
-    const uint64_t want = std::max(2 * pairs, pairs * units / a.min_units + 1);
-    const int grid = (int)std::min<uint64_t>(std::min(di.sm_count * per_sm, kAttnMaxGrid), want);
-    return launch_pdl("attn_kv8", kern, dim3(grid), kFewThreads, smem, st, a, err);
-}
-template <int DP, int NT, bool TREE>
-int launch_few(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
-    if (a.dim == DP)
-        return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, true, TREE>(a, st)
-                                    : launch_few<DP, NT, GRAFT_KV_E4M3, true, TREE>(a, st);
-    return fmt == GRAFT_KV_INT8 ? launch_few<DP, NT, GRAFT_KV_INT8, false, TREE>(a, st)
-                                : launch_few<DP, NT, GRAFT_KV_E4M3, false, TREE>(a, st);
-}
-
-// ---- many query rows
-template <int DP, int FMT, bool TREE>
-int launch_chunk(AttnArgs a, cudaStream_t st) {
-    using C = Chunk<DP>;
-    DeviceInfo di;
-    int rc = current_device_info(&di);
-    if (rc) return rc;
-    const auto kern = attn_chunk_kernel<DP, FMT, TREE>;
-    if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
-    unsigned* err = nullptr;
-    if ((rc = error_word(di.device, &err))) return rc;
-    // a piece costs about as much besides its units as 3 units (queries in, output);
-    // the pad is counted in keys
-    a.min_units = 4;
-    a.pad_units = 3 * C::KT;
-    const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
-                                   : a.max_len;
-    const uint64_t units = keys / C::KT + 2;
-    const uint64_t pairs = ((uint64_t)a.tokens / (C::ROWS / a.group) + a.n_seqs) * a.heads;
-    GRAFT_REQUIRE(pairs < (1ull << 31) && (keys + a.pad_units) * a.heads < (1ull << 31),
-                  "%u tokens, max_len %u are too many for one call", a.tokens, a.max_len);
-    const uint64_t want = std::max(pairs, pairs * units / a.min_units + 1);
-    const int grid = (int)std::min<uint64_t>(std::min(di.sm_count, kChunkMaxGrid), want);
-    return launch_pdl("attn_kv8", kern, dim3(grid), C::THREADS, C::SMEM, st, a, err);
-}
-template <int DP, bool TREE>
-int launch_chunk(const AttnArgs& a, uint32_t fmt, cudaStream_t st) {
-    return fmt == GRAFT_KV_INT8 ? launch_chunk<DP, GRAFT_KV_INT8, TREE>(a, st)
-                                : launch_chunk<DP, GRAFT_KV_E4M3, TREE>(a, st);
-}
-
-// Query rows that the few-row kernel takes for a head_dim (registers).
-uint32_t few_rows(uint32_t dim) { return dim <= 64 ? 32 : dim <= 128 ? 16 : 8; }
 
 int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const GraftAttnParams* P) {
     int rc;
@@ -129,7 +38,9 @@ int check_attn(const GraftKVCache* cache, const GraftKVRange* range, const Graft
 }  // namespace
 
 namespace graft {
-unsigned attn_device_errors(bool clear) { return read_device_errors(g_attn_err, clear); }
+unsigned attn_device_errors(bool clear) {
+    return read_device_errors(g_attn_err, clear) | attn_tree_device_errors(clear);
+}
 }  // namespace graft
 
 extern "C" size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const GraftKVRange* range,
@@ -142,7 +53,9 @@ extern "C" size_t graft_attn_kv8_workspace(const GraftKVCache* cache, const Graf
                                       : d <= 128 ? kFewPartial<128, 2> : kFewPartial<256, 1>)
             : kChunkMaxGrid * (size_t)(d <= 64    ? Chunk<64>::PARTIAL
                                        : d <= 128 ? Chunk<128>::PARTIAL : Chunk<256>::PARTIAL);
-    return kAttnMaxGrid * 4 + 2 * 4 * floats;
+    // (trees take the same workspace, and may have their rows as columns)
+    const uint64_t rows = (uint64_t)range->max_tokens * (P->q_heads / cache->kv_heads);
+    return kAttnMaxGrid * 4 + 2 * 4 * std::max(floats, attn_tree_partials(d, rows));
 }
 
 extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t stream) {
@@ -153,23 +66,6 @@ extern "C" int graft_attn_kv8_init(void* ws, size_t ws_bytes, graft_stream_t str
 }
 
 namespace {
-
-template <bool TREE>
-int launch_attn(const AttnArgs& a, uint32_t format, uint64_t rows, cudaStream_t stream) {
-    if (rows <= few_rows(a.dim)) {
-        if (a.dim <= 64)
-            return rows <= 8    ? launch_few<64, 1, TREE>(a, format, stream)
-                   : rows <= 16 ? launch_few<64, 2, TREE>(a, format, stream)
-                                : launch_few<64, 4, TREE>(a, format, stream);
-        if (a.dim <= 128)
-            return rows <= 8 ? launch_few<128, 1, TREE>(a, format, stream)
-                             : launch_few<128, 2, TREE>(a, format, stream);
-        return launch_few<256, 1, TREE>(a, format, stream);
-    }
-    return a.dim <= 64    ? launch_chunk<64, TREE>(a, format, stream)
-           : a.dim <= 128 ? launch_chunk<128, TREE>(a, format, stream)
-                          : launch_chunk<256, TREE>(a, format, stream);
-}
 
 // mask: of a tree of new tokens, or null
 int attend(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out,
@@ -209,7 +105,7 @@ int attend(const GraftKVCache* cache, const GraftHeads* q, const GraftHeads* out
     const uint64_t rows = (uint64_t)range->max_tokens * a.group;
     if (range->max_tokens == 0) return GRAFT_OK;
     a.mask = (const uint32_t*)mask, a.mask_stride = mask_stride, a.positions = positions;
-    return mask ? launch_attn<true>(a, cache->format, rows, stream)
+    return mask ? launch_attn_tree(a, cache->format, rows, stream)
                 : launch_attn<false>(a, cache->format, rows, stream);
 }
 
