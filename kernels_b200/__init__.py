@@ -418,6 +418,28 @@ def _dense(t, dtype, shape, dev: int) -> int | None:
     return t.data_ptr()
 
 
+_TYPES: list = []
+
+
+def _types():
+    """int32 and float32 (torch is imported by whoever has tensors)."""
+    if not _TYPES:
+        import torch
+        _TYPES.extend((torch.int32, torch.float32))
+    return _TYPES
+
+
+def _vector(t, dtype, n: int, dev: int) -> int | None:
+    """The address of a contiguous tensor of n elements in one dimension; None for None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"expected a contiguous {dtype} {(n,)} tensor")
+    if t.get_device() != dev:
+        _elsewhere(t, dev)
+    return t.data_ptr()
+
+
 class KVCache:
     """A paged 8-bit key/value cache over the caller's tensors: k and v int8 or
     float8_e4m3fn [n_blocks, kv_heads, block_tokens, head_dim], k_scale and
@@ -604,14 +626,15 @@ def rope(x, out, positions, table: RopeTable, inverse: bool = False, stream=None
     """x [tokens, heads, head_dim], any token and head strides, turned by positions
     (int32 [tokens]) into out (or in place: out is x).  inverse turns back; that is the
     gradient of x for that of out (graft_rope)."""
-    from torch import int32
     if x.dim() != 3:
         raise ValueError(f"expected a [tokens, heads, head_dim] tensor, not {tuple(x.shape)}")
     n, h, d = x.shape
     dev = x.get_device()
-    X, Y = _heads(x, h, d, dev), _heads(out, h, d, dev)
-    p = _dense(positions, int32, (n,), dev)
-    _on(table, dev)
+    X = _heads(x, h, d, dev)
+    Y = X if out is x else _heads(out, h, d, dev)
+    p = _vector(positions, _types()[0], n, dev)
+    if table.dev != dev:
+        _on(table, dev)
     call("graft_rope", C.byref(X), C.byref(Y), h, d, p, table.back_ref if inverse else table.ref,
          _raw_stream(stream, dev))
 
@@ -621,9 +644,7 @@ def kv_write_rope(cache: KVCache, K, V, rng: KVRange, table: RopeTable, position
     """kv_write with the keys turned on the way, and the queries q [tokens, q_heads,
     head_dim] into q_out beside.  rows (int32 [tokens]) and count (int32 [n_seqs]): which rows
     of K and V each sequence's first tokens are (graft_kv_write_rope)."""
-    from torch import int32
     h, d, dev = cache.heads, cache.dim, cache.dev
-    n = K.shape[0]
     Kd, Vd = _heads(K, h, d, dev), _heads(V, h, d, dev)
     Q = Qo = None
     hq = 0
@@ -634,9 +655,12 @@ def kv_write_rope(cache: KVCache, K, V, rng: KVRange, table: RopeTable, position
             raise ValueError(f"expected a [tokens, q_heads, {d}] tensor, not {tuple(q.shape)}")
         hq = q.shape[1]
         Q, Qo = C.byref(_heads(q, hq, d, dev)), C.byref(_heads(q_out, hq, d, dev))
-    positions = _dense(positions, int32, (n,), dev)
-    rows, count = _dense(rows, int32, (n,), dev), _dense(count, int32, (rng.n_seqs,), dev)
-    _on(table, dev)
+    if positions is not None or rows is not None or count is not None:
+        int32, n = _types()[0], Kd.tokens
+        positions, rows = _vector(positions, int32, n, dev), _vector(rows, int32, n, dev)
+        count = _vector(count, int32, rng.n_seqs, dev)
+    if table.dev != dev:
+        _on(table, dev)
     if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
         _bad_range(cache, rng)
     call("graft_kv_write_rope", cache.ref, C.byref(Kd), C.byref(Vd), rng.ref, table.ref, positions,
@@ -647,26 +671,25 @@ def kv_write_rope(cache: KVCache, K, V, rng: KVRange, table: RopeTable, position
 def draft_tree(parents, rng: KVRange, mask, positions=None, window: int = 0, stream=None) -> None:
     """Masks (int32 [tokens, words]) and positions (int32 [tokens]) of trees of new
     tokens from their parents (int32 [tokens], -1 for a root) (graft_draft_tree)."""
-    from torch import int32
-    if mask.dim() != 2 or mask.shape[0] != parents.shape[0]:
-        raise ValueError("mask must be [tokens, words]")
-    dev = parents.get_device()
-    n, words = mask.shape
-    par = _dense(parents, int32, (n,), dev)
-    m, stride = _mask(mask, n, dev)
-    pos = _dense(positions, int32, (n,), dev)
+    n, dev = parents.shape[0], parents.get_device()
+    m, stride, words = _mask(mask, n, dev)
+    int32 = _types()[0]
+    par, pos = _vector(parents, int32, n, dev), _vector(positions, int32, n, dev)
     if rng.dev != dev:
         raise ValueError("the range is on another device than the tensors")
     call("graft_draft_tree", par, rng.ref, n, window, m, stride, words, pos, _raw_stream(stream, dev))
 
 
 def _mask(mask, n: int, dev: int):
-    if mask.dim() != 2 or mask.shape[0] != n:
+    """Address, row stride and words of a mask of n rows."""
+    shape, stride = mask.shape, mask.stride()
+    if len(shape) != 2 or shape[0] != n:
         raise ValueError(f"mask must be [{n}, words]")
-    _ints(mask, "mask")
+    if mask.dtype is not _types()[0] or (stride[1] != 1 and shape[1] > 1):
+        _ints(mask, "mask")
     if mask.get_device() != dev:
         _elsewhere(mask, dev)
-    return mask.data_ptr(), mask.stride(0) if n > 1 else mask.shape[1]
+    return mask.data_ptr(), stride[0] if n > 1 else shape[1], shape[1]
 
 
 def attn_tree_kv8(cache: KVCache, q, out, rng: KVRange, mask, P: AttnParams, ws: AttnWorkspace,
@@ -674,15 +697,15 @@ def attn_tree_kv8(cache: KVCache, q, out, rng: KVRange, mask, P: AttnParams, ws:
     """attn_kv8 where the new tokens of a sequence see each other by the bits of mask
     (int32 [tokens, words], draft_tree); positions (int32 [tokens]) are needed with a
     window (graft_attn_tree_kv8)."""
-    from torch import float32, int32
     d, hq, dev = cache.dim, P.q_heads, cache.dev
-    n = q.shape[0]
-    if mask.dim() == 2 and mask.shape[1] * 32 < rng.max_tokens:
-        raise ValueError(f"mask rows of {mask.shape[1]} words do not hold {rng.max_tokens} tokens")
-    m, stride = _mask(mask, n, dev)
-    positions = _dense(positions, int32, (n,), dev)
-    sinks, lse = _dense(sinks, float32, (hq,), dev), _dense(lse, float32, (n, hq), dev)
     q, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
+    n = q.tokens
+    m, stride, words = _mask(mask, n, dev)
+    if words * 32 < rng.max_tokens:
+        raise ValueError(f"mask rows of {words} words do not hold {rng.max_tokens} tokens")
+    int32, float32 = _types()
+    positions, sinks = _vector(positions, int32, n, dev), _vector(sinks, float32, hq, dev)
+    lse = _dense(lse, float32, (n, hq), dev)
     if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
         _bad_range(cache, rng)
     if ws.dev != dev:
@@ -716,11 +739,12 @@ def _rows(t, rows: int, vocab: int, code: int, dev: int):
     """Address and row stride of rows of logits."""
     if t.shape != (rows, vocab) or _dtype_code(t.dtype) != code:
         raise ValueError("logits do not match the params")
-    if t.stride(1) != 1 and vocab > 1:
+    stride = t.stride()
+    if stride[1] != 1 and vocab > 1:
         raise ValueError("a row of logits must be contiguous")
     if t.get_device() != dev:
         _elsewhere(t, dev)
-    return t.data_ptr(), t.stride(0) if rows > 1 else vocab
+    return t.data_ptr(), stride[0] if rows > 1 else vocab
 
 
 def verify_drafts(logits, tokens, cu_tokens, count, path, next_token, P: VerifyParams,
@@ -732,16 +756,16 @@ def verify_drafts(logits, tokens, cu_tokens, count, path, next_token, P: VerifyP
     (int32 [n_seqs + 1]), parents (int32 [tokens], None: a chain), the draft's logits
     and random numbers uniform (fp32 [tokens]) and uniform_next (fp32 [n_seqs]); without
     these, greedily (graft_verify_drafts)."""
-    from torch import float32, int32
-    B, T, V = P.n_seqs, P.tokens, P.vocab
+    int32, float32 = _types()
+    B, T, V, dtype = P.n_seqs, P.tokens, P.vocab, P.dtype
     dev = logits.get_device()
-    z, zs = _rows(logits, T, V, P.dtype, dev)
-    d, ds = _rows(draft, T, V, P.dtype, dev) if draft is not None else (None, V)
-    args = (z, d, _dense(tokens, int32, (T,), dev), _dense(parents, int32, (T,), dev),
-            _dense(cu_tokens, int32, (B + 1,), dev), _dense(uniform, float32, (T,), dev),
-            _dense(uniform_next, float32, (B,), dev), _dense(count, int32, (B,), dev),
-            _dense(path, int32, (T,), dev), _dense(next_token, int32, (B,), dev))
-    Q = VerifyParams(B, T, P.max_tokens, V, P.dtype, zs, ds, P.scale, P.draft_scale)
+    z, zs = _rows(logits, T, V, dtype, dev)
+    d, ds = _rows(draft, T, V, dtype, dev) if draft is not None else (None, V)
+    args = (z, d, _vector(tokens, int32, T, dev), _vector(parents, int32, T, dev),
+            _vector(cu_tokens, int32, B + 1, dev), _vector(uniform, float32, T, dev),
+            _vector(uniform_next, float32, B, dev), _vector(count, int32, B, dev),
+            _vector(path, int32, T, dev), _vector(next_token, int32, B, dev))
+    Q = VerifyParams(B, T, P.max_tokens, V, dtype, zs, ds, P.scale, P.draft_scale)
     if ws.dev != dev:
         raise ValueError("the workspace is on another device than the tensors")
     call("graft_verify_drafts", *args, C.byref(Q), ws.addr, ws.nbytes, _raw_stream(stream, dev))

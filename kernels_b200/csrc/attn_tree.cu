@@ -1,5 +1,5 @@
 // attn_tree.cu -- attention of trees of new tokens over the paged 8-bit key/value cache: the
-// kernels of attn_kv8.cu with masks of the new tokens, and one for 17 to 64 rows (attn_cols.cuh).
+// kernels of attn_kv8.cu with masks of the new tokens, and one for rows between (attn_cols.cuh).
 #include "attn_cols.cuh"
 #include "attn_launch.cuh"
 
@@ -17,8 +17,12 @@ int launch_cols(AttnArgs a, cudaStream_t st) {
     if ((rc = ensure_smem((const void*)kern, C::SMEM))) return rc;
     unsigned* err = nullptr;
     if ((rc = error_word(di.device, &err))) return rc;
-    a.min_units = 2;
-    a.pad_units = 3;
+    // A piece of a pair costs about as much as five units besides its own (queries, the first references,
+    // sums, the join): 32 requests of 8 tokens and up to 8191 keys, 4 query heads on a head of 128,
+    // take 134 us with a pad of three, 124 with five, 128 with eight.  Short calls want every SM: 7
+    // tokens after 777 keys 18.4 us with shares of one unit, 23 of two.
+    a.min_units = 1;
+    a.pad_units = 5;
     const uint64_t keys = a.window ? std::min<uint64_t>(a.max_len, (uint64_t)a.window + a.max_tokens)
                                    : a.max_len;
     const uint64_t units = keys / C::KT + 2 + a.pad_units;
@@ -38,19 +42,21 @@ int launch_cols(const AttnArgs& a, uint32_t fmt, uint64_t rows, cudaStream_t st)
                                 : launch_cols<DP, 64, GRAFT_KV_E4M3>(a, st);
 }
 
-// Rows of a tree from which on they are columns of the matrix unit (up to 64, head_dim up to 128).
-constexpr uint32_t kColsFrom = 8;
+// Rows as columns, from where the few-row kernel ends.  In us, few rows | columns | many rows (32
+// requests of up to 8191 keys; 8 heads): of 64 dims, 16 rows 65 | 99, 32 rows 97 | 104, 64 rows - | 117 | 155;
+// of 128 dims, 16 rows 111 | 127, 32 rows - | 124 | 238, 64 rows - | 148 | 241.
+bool as_columns(uint32_t dim, uint64_t rows) { return dim <= 128 && rows > few_rows(dim) && rows <= 64; }
 
 }  // namespace
 
 int launch_attn_tree(const AttnArgs& a, uint32_t format, uint64_t rows, cudaStream_t stream) {
-    if (a.dim <= 128 && rows > kColsFrom && rows <= 64)
+    if (as_columns(a.dim, rows))
         return a.dim <= 64 ? launch_cols<64>(a, format, rows, stream) : launch_cols<128>(a, format, rows, stream);
     return launch_attn<true>(a, format, rows, stream);
 }
 
 size_t attn_tree_partials(uint32_t dim, uint64_t rows) {
-    if (rows > 64 || dim > 128) return 0;
+    if (!as_columns(dim, rows)) return 0;
     return kChunkMaxGrid * (size_t)(dim <= 64 ? Cols<64>::PARTIAL : Cols<128>::PARTIAL);
 }
 

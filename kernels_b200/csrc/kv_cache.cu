@@ -344,9 +344,11 @@ __device__ __forceinline__ void turn_queries(const KVRopeArgs& a, const Item& it
 
 // The same as kv_write_kernel with keys turned in fp32 before their maximum is taken.  A thread's
 // chunks come in twos, the halves of a unit (rope.cuh), so that it holds both elements of its pairs.
-// CTAs beyond those of keys and values turn the item's queries.
+// CTAs beyond those of keys and values turn the item's queries.  (CTAs with 4 chunks a thread have 128
+// threads at most: the launch's rule.)
 template <int DT, int FMT, int CH, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_rope_kernel(const __grid_constant__ KVRopeArgs a) {
+__global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 128 : 512, WARP ? (CH == 2 ? 3 : 2) : CH == 4 ? 6 : 1)
+    kv_write_rope_kernel(const __grid_constant__ KVRopeArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float red[16];
