@@ -55,7 +55,7 @@ struct KVRopeArgs : KVArgs {
     void* y_q;
     uint64_t tok_xq, head_xq, tok_yq, head_yq;
     uint32_t q_heads, cta_q_heads;             // query heads, and those of a CTA
-    uint32_t kv_ny;                            // CTAs of an item for keys and values; then its queries'
+    uint32_t q_ny;                             // CTAs of an item for its queries, the first ones
     uint32_t q_copy;                           // y_q is another buffer
 };
 
@@ -344,7 +344,7 @@ __device__ __forceinline__ void turn_queries(const KVRopeArgs& a, const Item& it
 
 // The same as kv_write_kernel with keys turned in fp32 before their maximum is taken.  A thread's
 // chunks come in twos, the halves of a unit (rope.cuh), so that it holds both elements of its pairs.
-// CTAs beyond those of keys and values turn the item's queries.  (CTAs with 4 chunks a thread have 128
+// The first CTAs of an item turn its queries.  (CTAs with 4 chunks a thread have 128
 // threads at most: the launch's rule.)
 template <int DT, int FMT, int CH, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 128 : 512, WARP ? (CH == 2 ? 3 : 2) : CH == 4 ? 6 : 1)
@@ -354,12 +354,12 @@ __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 128 : 512, WARP ? (CH =
     __shared__ float red[16];
     Item it;
     if (!find_item(a, blockIdx.x, it, a.count)) return;
-    if (blockIdx.y >= a.kv_ny) {
-        turn_queries<DT>(a, it, (blockIdx.y - a.kv_ny) * a.cta_q_heads);
+    if (blockIdx.y < a.q_ny) {
+        turn_queries<DT>(a, it, blockIdx.y * a.cta_q_heads);
         return;
     }
     const int block = *it.block;   // (not needed before the scale)
-    const int unit = WARP ? blockIdx.y * 8 + (threadIdx.x >> 5) : blockIdx.y;
+    const int y = blockIdx.y - a.q_ny, unit = WARP ? y * 8 + (threadIdx.x >> 5) : y;
     if (WARP && unit >= 2 * (int)a.heads) return;
     const int head = unit >> 1;
     const bool is_v = unit & 1;
@@ -590,8 +590,7 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
         KVRopeArgs& r = *turned;
         const uint32_t upr = r.cpt / 2;
         r.cpt_magic = ((1u << 20) + upr - 1) / upr;
-        r.kv_ny = ny;
-        // queries: about 16 units a thread
+        // queries: about 16 units a thread; these CTAs first, for they take the longest
         uint32_t q_ny = 0;
         if (r.x_q) {
             const uint64_t units = (uint64_t)std::min(range->max_tokens, a.bt) * (a.dim / 16) * r.q_heads;
@@ -599,6 +598,7 @@ int kv_move(bool write, const GraftKVCache* cache, const GraftHeads* K, const Gr
             r.cta_q_heads = (r.q_heads + q_ny - 1) / q_ny;
             q_ny = (r.q_heads + r.cta_q_heads - 1) / r.cta_q_heads;
         }
+        r.q_ny = q_ny;
         GRAFT_REQUIRE(ny + q_ny <= 65535, "too many heads in one call");
         const KVRopeKernel kern = K->dtype == GRAFT_F16    ? pick_rope<GRAFT_F16>(form, chunks, cache->format)
                                   : K->dtype == GRAFT_BF16 ? pick_rope<GRAFT_BF16>(form, chunks, cache->format)
