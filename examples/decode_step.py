@@ -1,18 +1,23 @@
 """A prompt and decode steps of one gpt-oss-shaped layer on synthetic weights, all
 through the library: int4 products for q/k/v, the output projection and the
-lm_head, the 8-bit key/value cache, attention over it, the MoE block, and the
-log probabilities from which the next token is taken.
+lm_head, rotary positions on the way to the 8-bit key/value cache, attention over
+it, the MoE block, and the log probabilities from which the next token is taken.
 
     python examples/decode_step.py [--prompt 200] [--steps 8] [--hidden 2880]
         [--vocab 201088] [--experts 16] [--window 128] [--format int8|e4m3]
+        [--drafts 7 [--temperature 0.8]]
 
 Prints the prompt's mean log probability and each step's token, with its log
-probability, the distribution's entropy and the alternatives.  Norms, rotary
-positions and the embedding are a few PyTorch operations.
+probability, the distribution's entropy and the alternatives.  With --drafts, a
+step takes a tree of so many tokens (looked up: what followed the newest token
+before, and the likeliest alternatives) through the layer at once, verifies them, and
+writes the accepted ones to their places.  Norms and the embedding are a few PyTorch
+operations.
 """
 from __future__ import annotations
 
 import argparse
+import math
 import sys
 from pathlib import Path
 
@@ -30,16 +35,6 @@ def i32(x):
 def rms(x):
     x = x.float()
     return (x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-5)).half()
-
-
-def rotary(x, pos):
-    """x [tokens, heads, dim] turned by the tokens' positions (halves as pairs)."""
-    half = x.shape[-1] // 2
-    f = 150000.0 ** (-torch.arange(half, device=x.device) / half)
-    a = pos[:, None, None].float() * f
-    c, s = a.cos(), a.sin()
-    x1, x2 = x[..., :half].float(), x[..., half:].float()
-    return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), -1).half()
 
 
 class Layer:
@@ -67,6 +62,9 @@ class Layer:
         self.cache = kb.KVCache.empty(blocks, kv_heads, dim, block,
                                       torch.int8 if fmt == "int8" else torch.float8_e4m3fn)
         self.table = torch.randperm(blocks, device="cuda", generator=g).to(torch.int32)[None]
+        # base 150000, 4096 positions scaled by 32
+        self.rope = kb.RopeTable(dim, base=150000.0, scaling="yarn", factor=32.0, orig_len=4096.0,
+                                 amplitude=1.0 + 0.1 * math.log(32.0))
         self.P_attn = kb.attn_params(q_heads, torch.float16, scale=dim ** -0.5, window=window)
         self.max_len, self.len = max_len, 0
         self.plans = {}
@@ -87,39 +85,79 @@ class Layer:
             kb.gemm_int4_sb_f16(w["W"], w["SB"], x, Y[i:i + 16], x.shape[0], P)
         return Y
 
-    def attend(self, X, start, write=True):
-        """q/k/v of the tokens at positions start.., their keys and values into the
-        cache, attention over everything up to each."""
+    def qkv_of(self, X):
+        """Queries, keys and values, not turned yet."""
+        qkv = rms(self.product(self.qkv, self.P_qkv, rms(X)).view(X.shape[0], -1, self.dim))
+        return (qkv[:, :self.q_heads], qkv[:, self.q_heads:self.q_heads + self.kv_heads],
+                qkv[:, self.q_heads + self.kv_heads:])
+
+    def attend(self, X, start, write=True, tree=None):
+        """q/k/v of the tokens at positions start.., turned; their keys and values into
+        the cache, attention over everything up to each.  tree: the tokens are a tree
+        (mask, positions)."""
         n = X.shape[0]
-        qkv = self.product(self.qkv, self.P_qkv, rms(X)).view(n, -1, self.dim)
-        pos = torch.arange(start, start + n, device="cuda")
-        q = rotary(rms(qkv[:, :self.q_heads]), pos)
-        k = rotary(rms(qkv[:, self.q_heads:self.q_heads + self.kv_heads]), pos)
-        v = rms(qkv[:, self.q_heads + self.kv_heads:])
+        q, k, v = self.qkv_of(X)
         r = kb.kv_range(self.table, i32([start]), i32([0, n]), n, self.max_len)
+        turned, out = torch.empty_like(q), torch.empty_like(q)
+        pos = tree[1] if tree else torch.arange(start, start + n, dtype=torch.int32, device="cuda")
         if write:
-            kb.kv_write(self.cache, k, v, r)
-        out = torch.empty_like(q)
-        kb.attn_kv8(self.cache, q, out, r, self.P_attn, self.plan(n)[0], sinks=self.sinks)
+            kb.kv_write_rope(self.cache, k, v, r, self.rope, positions=pos, q=q, q_out=turned)
+        else:
+            kb.rope(q, turned, pos, self.rope)
+        if tree:
+            kb.attn_tree_kv8(self.cache, turned, out, r, tree[0], self.P_attn, self.plan(n)[0],
+                             positions=pos, sinks=self.sinks)
+            self.fresh = (k, v, pos, r)      # until it is known which of them stay
+        else:
+            kb.attn_kv8(self.cache, turned, out, r, self.P_attn, self.plan(n)[0], sinks=self.sinks)
         return out
 
-    def forward(self, tokens, targets):
-        """The tokens through the layer; log probabilities of `targets` after each."""
-        n = len(tokens)
-        X = self.embed[torch.as_tensor(tokens, device="cuda")]
-        a = self.attend(X, self.len)
-        self.len += n
-        X = X + rms(self.product(self.o, self.P_o, a.reshape(n, -1)))
+    def logits(self, tokens, tree=None):
+        """The tokens through the layer and the lm_head."""
+        X = self.embed[torch.as_tensor(tokens, device="cuda").long()]
+        a = self.attend(X, self.len, tree=tree)
+        X = X + rms(self.product(self.o, self.P_o, a.reshape(len(tokens), -1)))
         Y = torch.empty_like(X)
         for i, x in enumerate(rms(X)):
             kb.moe_block_ex(self.pool, self.R, x, Y[i], self.P_moe, self.fmt, self.ws_moe)
         X = X + rms(Y)
-        logits = self.product(self.head, self.P_head, rms(X))
+        return self.product(self.head, self.P_head, rms(X))
+
+    def forward(self, tokens, targets):
+        """The tokens through the layer; log probabilities of `targets` after each."""
+        n = len(tokens)
+        logits = self.logits(tokens)
+        self.len += n
         _, P, ws = self.plan(n)
         out = (torch.empty(n, device="cuda"), torch.empty(n, device="cuda"),
                torch.empty(n, 5, device="cuda"), torch.empty(n, 5, dtype=torch.int32, device="cuda"))
         kb.logprobs(logits, i32(targets), *out, P, ws)
         return out
+
+    def step(self, tokens, parents, temperature=0.0, generator=None):
+        """A tree of drafted tokens behind the newest one (tokens[0]): the accepted ones,
+        the token after them, and the rows of logits.  temperature 0: greedy."""
+        n = len(tokens)
+        words = -(-n // 32)
+        mask, pos = torch.empty(n, words, dtype=torch.int32, device="cuda"), i32([0] * n)
+        r = kb.kv_range(self.table, i32([self.len]), i32([0, n]), n, self.max_len)
+        par, tok, cu = i32(parents), i32(tokens), i32([0, n])
+        kb.draft_tree(par, r, mask, pos, window=self.P_attn.window)
+        logits = self.logits(tokens, tree=(mask, pos))
+        P = kb.verify_params(1, n, n, self.vocab, torch.float16,
+                             scale=1.0 / temperature if temperature else 1.0)
+        count, path, last = i32([0]), i32([0] * n), i32([0])
+        u = {}
+        if temperature:
+            u = dict(uniform=torch.rand(n, device="cuda", generator=generator),
+                     uniform_next=torch.rand(1, device="cuda", generator=generator))
+        kb.verify_drafts(logits, tok, cu, count, path, last, P, kb.VerifyWorkspace(P), parents=par, **u)
+        # the accepted tokens' keys and values, to the places that they have without the others
+        k, v, pos, r = self.fresh
+        kb.kv_write_rope(self.cache, k, v, r, self.rope, positions=pos, rows=path, count=count)
+        c = int(count)
+        self.len += c
+        return path[:c].tolist(), int(last), logits
 
 
 def generate(layer: Layer, prompt: list[int], steps: int):
@@ -134,6 +172,42 @@ def generate(layer: Layer, prompt: list[int], steps: int):
     return score, out
 
 
+def lookup(history: list[int], alternatives: list[int], drafts: int):
+    """A tree behind the newest token: what followed its last earlier occurrence, one after the
+    other, and the likeliest alternatives beside the first of these."""
+    tokens, parents = [history[-1]], [-1]
+    for at in range(len(history) - 2, -1, -1):
+        if history[at] == history[-1]:
+            for t in history[at + 1:at + 1 + max(1, drafts // 2)]:
+                parents.append(len(tokens) - 1)
+                tokens.append(t)
+            break
+    for t in alternatives:
+        if len(tokens) > drafts:
+            break
+        if t not in (x for x, p in zip(tokens, parents) if p == 0):
+            parents.append(0)
+            tokens.append(t)
+    return tokens, parents
+
+
+def speculate(layer: Layer, prompt: list[int], steps: int, drafts: int, temperature: float = 0.0,
+              seed: int = 0):
+    """The prompt in one chunk, then trees of drafted tokens: each step's accepted tokens and
+    the one drawn after them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    _, _, _, idx = layer.forward(prompt, prompt[1:] + [0])
+    history, alternatives = prompt + [int(idx[-1, 0])], idx[-1].tolist()
+    out = []
+    for _ in range(steps):
+        tokens, parents = lookup(history, alternatives, drafts)
+        rows, last, logits = layer.step(tokens, parents, temperature, g)
+        out.append(([tokens[r] for r in rows], last))
+        history += [tokens[r] for r in rows[1:]] + [last]
+        alternatives = logits[rows[-1]].topk(5).indices.tolist()
+    return out
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--prompt", type=int, default=200)
@@ -143,11 +217,17 @@ def main() -> None:
     ap.add_argument("--experts", type=int, default=16)
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--format", choices=["int8", "e4m3"], default="int8")
+    ap.add_argument("--drafts", type=int, default=0)
+    ap.add_argument("--temperature", type=float, default=0.0)
     a = ap.parse_args()
     layer = Layer(a.hidden, a.vocab, experts=a.experts, window=a.window, fmt=a.format,
-                  max_len=a.prompt + a.steps + 64)
+                  max_len=a.prompt + (a.steps + 1) * (a.drafts + 1) + 64)
     g = torch.Generator().manual_seed(1)
     prompt = torch.randint(0, a.vocab, (a.prompt,), generator=g).tolist()
+    if a.drafts:
+        for accepted, last in speculate(layer, prompt, a.steps, a.drafts, a.temperature):
+            print(f"accepted {accepted}, then {last}")
+        return
     score, out = generate(layer, prompt, a.steps)
     print(f"prompt: {a.prompt} tokens, mean log probability {score:.3f}")
     for tok, lp, ent, idx, top in out:

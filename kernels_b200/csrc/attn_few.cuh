@@ -93,6 +93,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     __shared__ int sh_scan[W];
     __shared__ float2 sh_ml[W][ROWS];
     __shared__ int sh_last;
+    // TREE: of a row, the first key and the new tokens that it sees (a copy a warp; only the units with
+    // a mask ask, and registers are short)
+    __shared__ uint2 sh_tree[TREE ? W : 1][ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = FULL ? DP : a.dim, H = a.heads;
     pdl_wait();
@@ -236,8 +239,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     FewState<DP, NT> st;
     uint32_t qf[CH][NT][8];
     float cn[NT][2];    // scale log2(e) of the columns' rows
-    int pn[NT][2];      // positions of the columns' tokens (TREE: the first keys they see)
-    uint32_t seen[TREE ? NT : 1][2];   // and the new tokens
+    int pn[NT][2];      // positions of the columns' tokens (not TREE)
 
     // ---- two elements of a row of a finished pair, L relative to 2^M
     const int je = warp & 3, ce = (warp >> 2) & 1;   // the thread's accumulators: tile 4i + je, column ce
@@ -315,15 +317,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
             cn[n][0] = __shfl_sync(~0u, c, 8 * t);       // lane of row 2t (t = 0)
             cn[n][1] = __shfl_sync(~0u, c, 8 * t + 4);
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2) {
-                const int tok = cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0;
-                if constexpr (TREE) {
-                    pn[n][c2] = first_tree_key(a, cw.s, tok);
-                    seen[n][c2] = a.mask[(size_t)(cw.s.c0 + tok) * a.mask_stride] & bit_range(0, cw.s.n);
-                } else {
-                    pn[n][c2] = cw.s.start + tok;
-                }
-            }
+            for (int c2 = 0; c2 < 2; ++c2)
+                pn[n][c2] = cw.s.start + (cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0);
+            if constexpr (TREE)
+                if (t == 0)
+                    sh_tree[warp][r] = make_uint2(first_tree_key(a, cw.s, tok),
+                                                  a.mask[(size_t)(cw.s.c0 + tok) * a.mask_stride] & bit_range(0, cw.s.n));
         }
     };
 
@@ -337,7 +336,10 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         const int first = first_key(a, cw.s.start);  // keys before it by none
 #pragma unroll 1
         for (int u = cw.lo + warp; u < cw.hi; u += W) {
-            if (u < cw.lo + W) load_queries();
+            if (u < cw.lo + W) {
+                load_queries();
+                if (TREE) __syncwarp();
+            }
             const int key0 = u * UK;
             uint8_t* sl = ring + slot * kFewSlot<DP>;
             cp_async_wait<NS - 1>();
@@ -400,12 +402,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                     for (int e = 0; e < 4; ++e) {
                         float x = fmaf(s[kt][n][e], ks * cn[n][e & 1], lv);
                         if (edge_unit) {
-                            const int j = key0 + kt * 16 + g + (e & 2) * 4, p = pn[n][e & 1];
+                            const int j = key0 + kt * 16 + g + (e & 2) * 4;
                             bool see;
                             if constexpr (TREE) {
+                                const uint2 of = sh_tree[warp][8 * n + 2 * t + (e & 1)];
                                 const int i = j - cw.s.start;
-                                see = i < 0 ? j >= p : i < 32 && (seen[n][e & 1] >> i & 1u);
+                                see = i < 0 ? j >= (int)of.x : i < 32 && (of.y >> i & 1u);
                             } else {
+                                const int p = pn[n][e & 1];
                                 see = j <= p && (!a.window || j > p - (int)a.window);
                             }
                             x = see ? x : -INFINITY;
