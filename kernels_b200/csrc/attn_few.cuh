@@ -93,9 +93,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     __shared__ int sh_scan[W];
     __shared__ float2 sh_ml[W][ROWS];
     __shared__ int sh_last;
-    // TREE: of a row, the first key and the new tokens that it sees (a copy a warp; only the units with
-    // a mask ask, and registers are short)
-    __shared__ uint2 sh_tree[TREE ? W : 1][ROWS];
+    // TREE: of a row, the first key and the new tokens that it sees, in registers or, where these are
+    // short, in shared memory (a copy a warp; only the units with a mask ask).  32 requests of up to
+    // 8191 keys, 8 heads of 64: 8 rows 42 us | 49, 16 rows 65 | 53, 32 rows 97 | 86.
+    constexpr bool ASIDE = TREE && NT > 1;
+    __shared__ uint2 sh_tree[ASIDE ? W : 1][ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = FULL ? DP : a.dim, H = a.heads;
     pdl_wait();
@@ -239,7 +241,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
     FewState<DP, NT> st;
     uint32_t qf[CH][NT][8];
     float cn[NT][2];    // scale log2(e) of the columns' rows
-    int pn[NT][2];      // positions of the columns' tokens (not TREE)
+    int pn[NT][2];      // positions of the columns' tokens (TREE: the first keys they see)
+    uint32_t seen[NT][2];   // TREE: and the new tokens
 
     // ---- two elements of a row of a finished pair, L relative to 2^M
     const int je = warp & 3, ce = (warp >> 2) & 1;   // the thread's accumulators: tile 4i + je, column ce
@@ -317,9 +320,16 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
             cn[n][0] = __shfl_sync(~0u, c, 8 * t);       // lane of row 2t (t = 0)
             cn[n][1] = __shfl_sync(~0u, c, 8 * t + 4);
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2)
-                pn[n][c2] = cw.s.start + (cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0);
-            if constexpr (TREE)
+            for (int c2 = 0; c2 < 2; ++c2) {
+                const int own = cw.s.n > 1 ? min(8 * n + 2 * t + c2, R - 1) / (int)a.group : 0;
+                if constexpr (TREE && !ASIDE) {
+                    pn[n][c2] = first_tree_key(a, cw.s, own);
+                    seen[n][c2] = a.mask[(size_t)(cw.s.c0 + own) * a.mask_stride] & bit_range(0, cw.s.n);
+                } else {
+                    pn[n][c2] = cw.s.start + own;
+                }
+            }
+            if constexpr (ASIDE)
                 if (t == 0)
                     sh_tree[warp][r] = make_uint2(first_tree_key(a, cw.s, tok),
                                                   a.mask[(size_t)(cw.s.c0 + tok) * a.mask_stride] & bit_range(0, cw.s.n));
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
         for (int u = cw.lo + warp; u < cw.hi; u += W) {
             if (u < cw.lo + W) {
                 load_queries();
-                if (TREE) __syncwarp();
+                if (ASIDE) __syncwarp();
             }
             const int key0 = u * UK;
             uint8_t* sl = ring + slot * kFewSlot<DP>;
@@ -405,7 +415,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewBig<DP, NT> ? 1 : 2)
                             const int j = key0 + kt * 16 + g + (e & 2) * 4;
                             bool see;
                             if constexpr (TREE) {
-                                const uint2 of = sh_tree[warp][8 * n + 2 * t + (e & 1)];
+                                uint2 of = make_uint2(pn[n][e & 1], seen[n][e & 1]);
+                                if constexpr (ASIDE) of = sh_tree[warp][8 * n + 2 * t + (e & 1)];
                                 const int i = j - cw.s.start;
                                 see = i < 0 ? j >= (int)of.x : i < 32 && (of.y >> i & 1u);
                             } else {

@@ -43,8 +43,8 @@ int launch_cols(const AttnArgs& a, uint32_t fmt, uint64_t rows, cudaStream_t st)
 }
 
 // Rows as columns, from where the few-row kernel ends.  In us, few rows | columns | many rows (32
-// requests of up to 8191 keys; 8 heads): of 64 dims, 16 rows 65 | 99, 32 rows 97 | 104, 64 rows - | 117 | 155;
-// of 128 dims, 16 rows 111 | 127, 32 rows - | 124 | 238, 64 rows - | 148 | 241.
+// requests of up to 8191 keys; 8 heads): of 64 dims, 16 rows 53 | 99, 32 rows 86 | 104, 64 rows - | 117 | 155;
+// of 128 dims, 16 rows 108 | 127, 32 rows - | 124 | 238, 64 rows - | 148 | 241.
 bool as_columns(uint32_t dim, uint64_t rows) { return dim <= 128 && rows > few_rows(dim) && rows <= 64; }
 
 }  // namespace
