@@ -16,8 +16,9 @@ no CPU fallback: if the library is missing, every call raises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
-from ._lib import (AttnParams, ExpertParams, ExpertScratch, GemvParams, GraftError, Heads,
+from ._lib import (AttnParams, ExpertParams, ExpertScratch, GemvParams, GraftError,
                    KVCacheDesc, KVRangeDesc, LogprobParams, MoEFormat, MoEParams, MoEScratch,
                    RopeDesc, RopeParams, VerifyParams, VQParams, VQQuantParams, call, load)
 
@@ -392,8 +393,12 @@ def _one_device(*tensors) -> int:
     return dev
 
 
-def _heads(t, heads: int, dim: int, dev: int) -> Heads:
-    """A [tokens, heads, dim] tensor with any token and head strides."""
+_pack_heads = struct.Struct("@QQQII").pack       # GraftHeads
+_pack_verify = struct.Struct("@5IQQff").pack      # GraftVerifyParams
+
+
+def _heads(t, heads: int, dim: int, dev: int) -> bytes:
+    """A [tokens, heads, dim] tensor with any token and head strides (GraftHeads)."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
         raise ValueError(f"expected a [tokens, {heads}, {dim}] tensor, not {tuple(shape)}")
@@ -403,8 +408,8 @@ def _heads(t, heads: int, dim: int, dev: int) -> Heads:
     if t.get_device() != dev:
         _elsewhere(t, dev)
     # (the stride of a single token or head is any number)
-    return Heads(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0,
-                 shape[0], code)
+    return _pack_heads(t.data_ptr(), stride[0] if shape[0] > 1 else 0,
+                       stride[1] if heads > 1 else 0, shape[0], code)
 
 
 def _dense(t, dtype, shape, dev: int) -> int | None:
@@ -517,7 +522,7 @@ def _kv_move(name: str, cache: KVCache, K, V, rng: KVRange, stream) -> None:
     K, V = _heads(K, h, d, dev), _heads(V, h, d, dev)
     if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
         _bad_range(cache, rng)
-    call(name, cache.ref, C.byref(K), C.byref(V), rng.ref, _raw_stream(stream, dev))
+    call(name, cache.ref, K, V, rng.ref, _raw_stream(stream, dev))
 
 
 def kv_write(cache: KVCache, K, V, rng: KVRange, stream=None) -> None:
@@ -580,7 +585,7 @@ def attn_kv8(cache: KVCache, q, out, rng: KVRange, P: AttnParams, ws: AttnWorksp
         _bad_range(cache, rng)
     if ws.dev != dev:
         raise ValueError("the workspace is on another device than the tensors")
-    call("graft_attn_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, sinks, lse, C.byref(P),
+    call("graft_attn_kv8", cache.ref, q, out, rng.ref, sinks, lse, C.byref(P),
          ws.addr, ws.nbytes, _raw_stream(stream, dev))
 
 
@@ -635,7 +640,7 @@ def rope(x, out, positions, table: RopeTable, inverse: bool = False, stream=None
     p = _vector(positions, _types()[0], n, dev)
     if table.dev != dev:
         _on(table, dev)
-    call("graft_rope", C.byref(X), C.byref(Y), h, d, p, table.back_ref if inverse else table.ref,
+    call("graft_rope", X, Y, h, d, p, table.back_ref if inverse else table.ref,
          _raw_stream(stream, dev))
 
 
@@ -654,16 +659,16 @@ def kv_write_rope(cache: KVCache, K, V, rng: KVRange, table: RopeTable, position
         if q.dim() != 3:
             raise ValueError(f"expected a [tokens, q_heads, {d}] tensor, not {tuple(q.shape)}")
         hq = q.shape[1]
-        Q, Qo = C.byref(_heads(q, hq, d, dev)), C.byref(_heads(q_out, hq, d, dev))
+        Q, Qo = _heads(q, hq, d, dev), _heads(q_out, hq, d, dev)
     if positions is not None or rows is not None or count is not None:
-        int32, n = _types()[0], Kd.tokens
+        int32, n = _types()[0], K.shape[0]
         positions, rows = _vector(positions, int32, n, dev), _vector(rows, int32, n, dev)
         count = _vector(count, int32, rng.n_seqs, dev)
     if table.dev != dev:
         _on(table, dev)
     if rng.dev != dev or rng.blocks * cache.block_tokens < rng.max_len:
         _bad_range(cache, rng)
-    call("graft_kv_write_rope", cache.ref, C.byref(Kd), C.byref(Vd), rng.ref, table.ref, positions,
+    call("graft_kv_write_rope", cache.ref, Kd, Vd, rng.ref, table.ref, positions,
          rows, count, Q, Qo, hq, _raw_stream(stream, dev))
 
 
@@ -698,8 +703,8 @@ def attn_tree_kv8(cache: KVCache, q, out, rng: KVRange, mask, P: AttnParams, ws:
     (int32 [tokens, words], draft_tree); positions (int32 [tokens]) are needed with a
     window (graft_attn_tree_kv8)."""
     d, hq, dev = cache.dim, P.q_heads, cache.dev
-    q, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
-    n = q.tokens
+    x, out = _heads(q, hq, d, dev), _heads(out, hq, d, dev)
+    n = q.shape[0]
     m, stride, words = _mask(mask, n, dev)
     if words * 32 < rng.max_tokens:
         raise ValueError(f"mask rows of {words} words do not hold {rng.max_tokens} tokens")
@@ -710,7 +715,7 @@ def attn_tree_kv8(cache: KVCache, q, out, rng: KVRange, mask, P: AttnParams, ws:
         _bad_range(cache, rng)
     if ws.dev != dev:
         raise ValueError("the workspace is on another device than the tensors")
-    call("graft_attn_tree_kv8", cache.ref, C.byref(q), C.byref(out), rng.ref, m, stride, positions,
+    call("graft_attn_tree_kv8", cache.ref, x, out, rng.ref, m, stride, positions,
          sinks, lse, C.byref(P), ws.addr, ws.nbytes, _raw_stream(stream, dev))
 
 
@@ -765,10 +770,10 @@ def verify_drafts(logits, tokens, cu_tokens, count, path, next_token, P: VerifyP
             _vector(cu_tokens, int32, B + 1, dev), _vector(uniform, float32, T, dev),
             _vector(uniform_next, float32, B, dev), _vector(count, int32, B, dev),
             _vector(path, int32, T, dev), _vector(next_token, int32, B, dev))
-    Q = VerifyParams(B, T, P.max_tokens, V, dtype, zs, ds, P.scale, P.draft_scale)
+    Q = _pack_verify(B, T, P.max_tokens, V, dtype, zs, ds, P.scale, P.draft_scale)
     if ws.dev != dev:
         raise ValueError("the workspace is on another device than the tensors")
-    call("graft_verify_drafts", *args, C.byref(Q), ws.addr, ws.nbytes, _raw_stream(stream, dev))
+    call("graft_verify_drafts", *args, Q, ws.addr, ws.nbytes, _raw_stream(stream, dev))
 
 
 # ------------------------------------------------------ log probabilities --

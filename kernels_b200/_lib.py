@@ -83,7 +83,8 @@ class KVRangeDesc(C.Structure):
 
 
 class Heads(C.Structure):
-    """GraftHeads: a strided [tokens][heads][head_dim] buffer."""
+    """GraftHeads: a strided [tokens][heads][head_dim] buffer (the wrappers pass the same 32
+    bytes packed, which costs the host a third)."""
     _fields_ = [("data", C.c_void_p), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64),
                 ("tokens", C.c_uint32), ("dtype", C.c_uint32)]
 
@@ -183,27 +184,27 @@ SIGNATURES: dict[str, tuple] = {
     "graft_gemm_int4_sharded": (INT, [P, P, P, P, P, U32, C.POINTER(GemvParams), P]),
     "graft_moe_block_ep": (INT, [P, P, P, P, P, C.POINTER(MoEParams), C.POINTER(MoEFormat),
                                  C.POINTER(MoEScratch), P]),
-    "graft_kv_write": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+    "graft_kv_write": (INT, [C.POINTER(KVCacheDesc), P, P,
                              C.POINTER(KVRangeDesc), P]),
-    "graft_kv_read": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+    "graft_kv_read": (INT, [C.POINTER(KVCacheDesc), P, P,
                             C.POINTER(KVRangeDesc), P]),
     "graft_kv_device_errors": (INT, [C.POINTER(U32), INT]),
     "graft_attn_kv8_workspace": (SIZE, [C.POINTER(KVCacheDesc), C.POINTER(KVRangeDesc),
                                         C.POINTER(AttnParams)]),
     "graft_attn_kv8_init": (INT, [P, SIZE, P]),
-    "graft_attn_kv8": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+    "graft_attn_kv8": (INT, [C.POINTER(KVCacheDesc), P, P,
                              C.POINTER(KVRangeDesc), P, P, C.POINTER(AttnParams), P, SIZE, P]),
     "graft_rope_init": (INT, [P, P, C.POINTER(RopeParams), P]),
-    "graft_rope": (INT, [C.POINTER(Heads), C.POINTER(Heads), U32, U32, P, C.POINTER(RopeDesc), P]),
-    "graft_kv_write_rope": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+    "graft_rope": (INT, [P, P, U32, U32, P, C.POINTER(RopeDesc), P]),
+    "graft_kv_write_rope": (INT, [C.POINTER(KVCacheDesc), P, P,
                                   C.POINTER(KVRangeDesc), C.POINTER(RopeDesc), P, P, P,
-                                  C.POINTER(Heads), C.POINTER(Heads), U32, P]),
+                                  P, P, U32, P]),
     "graft_draft_tree": (INT, [P, C.POINTER(KVRangeDesc), U32, U32, P, U64, U32, P, P]),
-    "graft_attn_tree_kv8": (INT, [C.POINTER(KVCacheDesc), C.POINTER(Heads), C.POINTER(Heads),
+    "graft_attn_tree_kv8": (INT, [C.POINTER(KVCacheDesc), P, P,
                                   C.POINTER(KVRangeDesc), P, U64, P, P, P, C.POINTER(AttnParams),
                                   P, SIZE, P]),
     "graft_verify_workspace": (SIZE, [C.POINTER(VerifyParams)]),
-    "graft_verify_drafts": (INT, [P, P, P, P, P, P, P, P, P, P, C.POINTER(VerifyParams), P, SIZE, P]),
+    "graft_verify_drafts": (INT, [P, P, P, P, P, P, P, P, P, P, P, P, SIZE, P]),
     "graft_logprobs_workspace": (SIZE, [C.POINTER(LogprobParams)]),
     "graft_logprobs_init": (INT, [P, SIZE, P]),
     "graft_logprobs": (INT, [P, P, P, P, P, P, C.POINTER(LogprobParams), P, SIZE, P]),
