@@ -742,7 +742,7 @@ int graft_logprobs(const void* logits, const int32_t* targets, float* logprob, f
 typedef struct {
     uint32_t n_seqs, tokens;      /* sequences, rows                           */
     uint32_t max_tokens;          /* of a sequence, at most 1024               */
-    uint32_t vocab;
+    uint32_t vocab;               /* 1 to 2^30                                 */
     uint32_t dtype;               /* of logits and draft                       */
     uint64_t row_stride, draft_stride;   /* elements from row to row (>= vocab) */
     float scale, draft_scale;     /* 2^-100 to 2^100                           */

@@ -347,8 +347,7 @@ __device__ __forceinline__ void turn_queries(const KVRopeArgs& a, const Item& it
 // The first CTAs of an item turn its queries: 7687 tokens (64 query heads on 8 of 64) turned, written and
 // read back 42 us, 46 with those CTAs last.  One token of 64 sequences and its block read back 9.7 us
 // (7.6 without turning).  Registers bound the first (24 warps an SM), latency the second.
-// (CTAs with 4 chunks a thread have 128
-// threads at most: the launch's rule.)
+// (CTAs with 4 chunks a thread have 128 threads at most: the launch's rule.)
 template <int DT, int FMT, int CH, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 128 : 512, WARP ? (CH == 2 ? 3 : 2) : CH == 4 ? 6 : 1)
     kv_write_rope_kernel(const __grid_constant__ KVRopeArgs a) {

@@ -107,7 +107,7 @@ def test_tree_attention_refuses(lib, match, args, p):
 
 
 @pytest.mark.parametrize("match,args,p", [
-    ("vocab", {}, dict(vocab=0)), ("max_tokens", {}, dict(max_tokens=1025)), ("element type", {}, dict(dtype=3)),
+    ("vocab", {}, dict(vocab=0)), ("vocab", {}, dict(vocab=(1 << 30) + 1)), ("max_tokens", {}, dict(max_tokens=1025)), ("element type", {}, dict(dtype=3)),
     ("row stride", {}, dict(row_stride=99)), ("row stride", {}, dict(draft_stride=99)),
     ("scales", {}, dict(scale=0.0)), ("scales", {}, dict(draft_scale=float("nan"))),
     ("tokens", {}, dict(tokens=1 << 27)), ("n_seqs", {}, dict(n_seqs=1 << 25)),

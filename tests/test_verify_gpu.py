@@ -132,6 +132,34 @@ def test_longest_trees(lib):
     check([1024], 40, "f32", 6, trees=False, drawn=False)
 
 
+@pytest.mark.parametrize("took", [None, 1, 400, 1022])
+@pytest.mark.parametrize("slope", [0.02, 0.6])
+def test_many_siblings(lib, slope, took):
+    """A root with 1023 children, the likeliest tokens first, that are rejected one after the
+    other (but one): what is left of p falls to e^-20 and e^-614."""
+    n, V = 1024, 20011
+    z = torch.full((n, V), -math.inf, device="cuda")
+    order = torch.from_numpy(np.random.default_rng(1).permutation(V)[:1200])
+    z[0, order.cuda()] = (-slope * torch.arange(1200.0)).cuda()
+    z[1:, :7] = 0.0
+    tokens = np.concatenate([[0], order[:n - 1].numpy()])
+    u = np.full(n, 0.9, np.float32)
+    if took:
+        u[took] = 0.001
+    cu, parents = [0, n], np.array([-1] + [0] * (n - 1))
+    last = np.array([0.3], np.float32)
+    want = expected(z, tokens, cu, parents, 1.0, None, 1.0, u, last)
+    assert min(want[3]) > 2.0 ** -18 and want[0] == [2 if took else 1]
+    assert call(z, tokens, cu, parents, uniform=u, last=last) == want[:3]
+
+
+def test_no_tokens(lib):
+    z = torch.zeros(0, 50, device="cuda")
+    for u in (None, []):
+        got = call(z, [], [0, 0, 0], None, uniform=u, last=None if u is None else [0.5, 0.5], longest=3)
+        assert got == ([0, 0], [], [-1, -1])
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("V", [3, 1000, 50021])
 def test_greedy(lib, V, dtype):
