@@ -193,3 +193,69 @@ def test_captured_masks(lib):
     kb.attn_tree_kv8(dev, q, want, r, m2, P, ws, positions=p2, sinks=args["sinks"], lse=wl)
     torch.cuda.synchronize()
     assert torch.equal(m2, mask) and torch.equal(want, out) and torch.equal(wl, lse)
+
+
+# (few rows in registers, in shared memory; rows as columns, one and both groups; many rows; 256 dims)
+FORMS = [([90, 40], [2, 2], 8, 2, 64), ([90, 40], [6, 3], 8, 2, 64), ([300, 40], [5, 8], 8, 2, 128),
+         ([300, 700], [16, 13], 8, 2, 64), ([300, 700], [30, 13], 8, 2, 64), ([90, 40], [7, 8], 4, 2, 256)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_bad_query_spoils_its_own_row_only(lib, form, dtype):
+    """The other rows' references may move with the spoilt row's, so both runs lie within run_case's
+    tolerance of the formula; codes times scales are at most 2 here, and so |o| and sum p |v|."""
+    dev, q, out, lse, r, P, ws, _ = run_case(*form, 16, "int8", dtype, 0, False, seed=9)
+    T = q.shape[0]
+    mask = torch.full((T, 1), -1, **I32)      # everything
+    good = torch.empty_like(out)
+    kb.attn_tree_kv8(dev, q, good, r, mask, P, ws)
+    D = q.shape[2]
+    d = (D + 8) * 2.0 ** -24 * float(q.float().abs().sum(2).max()) * 2 * D ** -0.5 + 2.0 ** -20
+    tol = 2 * (ROUND[dtype] * 2 * 1.01 + 2 * (2.0 ** -11 + 2 * d) + 1e-7)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        spoilt = q.clone()
+        spoilt[1, 3, 5] = bad
+        got = torch.empty_like(out)
+        kb.attn_tree_kv8(dev, spoilt, got, r, mask, P, ws)
+        others = torch.ones(T, q.shape[1], dtype=torch.bool, device="cuda")
+        others[1, 3] = False
+        a, b = got[others].float(), good[others].float()
+        assert (a - b).abs().max() <= tol
+        if bad != bad:
+            assert got[1, 3].isnan().all()
+    assert not any(kb.kv_device_errors().values())
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_strides_and_what_lies_around(lib, form):
+    """Queries in the middle of wider rows, masks with other words around them, and output that is
+    nobody's."""
+    dev, q, _, _, r, P, ws, _ = run_case(*form, 16, "e4m3", "f16", 0, False, seed=11)
+    T, Hq, D = q.shape
+    rng = np.random.default_rng(11)
+    wide = torch.full((T, Hq + 3, D + 16), float("nan"), device="cuda").half()
+    wide[:, 1:Hq + 1, 8:D + 8] = q
+    out = torch.full((T + 2, Hq + 1, D + 8), 7.0, device="cuda").half()
+    mask = torch.full((T, 5), -1, **I32)
+    mask[:, 2] = torch.from_numpy(rng.integers(0, 1 << 30, T).astype(np.int32)).cuda()
+    dense = torch.empty_like(q)
+    kb.attn_tree_kv8(dev, q, dense, r, mask[:, 2:3].contiguous(), P, ws)
+    kb.attn_tree_kv8(dev, wide[:, 1:Hq + 1, 8:D + 8], out[:T, :Hq, :D], r, mask[:, 2:3], P, ws)
+    assert torch.equal(out[:T, :Hq, :D], dense) and torch.isfinite(dense).all()
+    assert (out[T:] == 7).all() and (out[:, Hq:] == 7).all() and (out[:, :, D:] == 7).all()
+
+
+@pytest.mark.parametrize("new", [2, 5, 9])
+def test_more_sequences_than_threads(lib, new):
+    run_case([i % 37 for i in range(1100)], [new if i % 3 else 1 for i in range(1100)], 8, 1, 64, 16, "int8",
+             "f16", 0, False, seed=3)
+    run_case([i % 37 for i in range(500)], [0 if i % 5 else new for i in range(500)], 8, 1, 128, 16, "e4m3",
+             "bf16", 9, True, seed=3)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_sharp_and_flat_scores(lib, form):
+    for qscale in (0.0, 40.0):
+        run_case(*form, 32, "int8", "f16", 0, True, seed=13, qscale=qscale)
+        run_case(*form, 32, "e4m3", "bf16", 20, False, seed=13, qscale=qscale)
