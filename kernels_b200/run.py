@@ -10,8 +10,11 @@ the counterpart of the reference harness binaries' flags (int4gemv --M --K --G
     python -m kernels_b200.run vqquant --M 4096 --K 4096
     python -m kernels_b200.run expert [--copies 4]     # one gpt-oss expert (bf16 format)
     python -m kernels_b200.run attn [--ctx 131071] [--B 1] [--new 1] [--heads 64,8,64] [--e4m3]
+    python -m kernels_b200.run attn --tree --new 8     # .. the new tokens a tree
     python -m kernels_b200.run kvwrite|kvread [--ctx 65536] [--heads 64,8,64] [--e4m3]
+    python -m kernels_b200.run rope|kvwriterope [--ctx 65536] [--heads 64,8,64]
     python -m kernels_b200.run logprobs [--B 1] [--M 201088] [--top-k 20]   # B rows of M logits
+    python -m kernels_b200.run verify [--B 64] [--new 6] [--M 128256]   # B chains of drafted tokens
 
 Each iteration is one launch on a rotating weight copy, timed with CUDA events;
 use it for small profiler captures (a few launches, a few GB).  --graph N
@@ -28,7 +31,8 @@ import json
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["int4", "vq", "moe", "stream", "batch", "vqquant",
-                                       "expert", "attn", "kvwrite", "kvread", "logprobs"])
+                                       "expert", "attn", "kvwrite", "kvread", "rope", "kvwriterope",
+                                       "logprobs", "verify"])
     ap.add_argument("--M", type=int, default=4096)
     ap.add_argument("--K", type=int, default=4096)
     ap.add_argument("--G", type=int, default=64)
@@ -39,7 +43,9 @@ def main() -> None:
     ap.add_argument("--mbytes", type=int, default=1024)
     ap.add_argument("--B", type=int, default=8, help="batch: tokens per call")
     ap.add_argument("--ctx", type=int, default=131071, help="attn, kv*: tokens in the cache")
-    ap.add_argument("--new", type=int, default=1, help="attn: new tokens of each of B sequences")
+    ap.add_argument("--new", type=int, default=1,
+                    help="attn, verify: new tokens of each of B sequences")
+    ap.add_argument("--tree", action="store_true", help="attn: the new tokens are a tree")
     ap.add_argument("--heads", default="64,8,64", help="attn, kv*: query heads, kv heads, head_dim")
     ap.add_argument("--block", type=int, default=64, help="attn, kv*: tokens of a cache block")
     ap.add_argument("--window", type=int, default=0, help="attn: sliding window")
@@ -119,7 +125,7 @@ def main() -> None:
         nbytes = a.top_k * 3 * (2880 * 1440 + 2 * 2 * 2880 * 45) + a.experts * 2880 * 2 + 6 * 2880 \
             + 4 * a.top_k * 2880
         f = lambda i: kb.moe_block_ex(pool, R, xs_[i % 8], y, P, fmt, wsp)  # noqa
-    elif a.kernel in ("attn", "kvwrite", "kvread"):
+    elif a.kernel in ("attn", "kvwrite", "kvread", "rope", "kvwriterope"):
         Hq, H, D = (int(x) for x in a.heads.split(","))
         B = a.B if a.kernel == "attn" else 1
         per = -(-a.ctx // a.block)
@@ -129,6 +135,7 @@ def main() -> None:
         cache = kb.KVCache.empty(B * per, H, D, a.block,
                                  torch.float8_e4m3fn if a.e4m3 else torch.int8)
         x = torch.randn(a.ctx, H, D, device="cuda", generator=g).half()
+        turn = kb.RopeTable(D)
         for b in range(B):
             whole = kb.kv_range(table[b:b + 1], torch.zeros(1, **i32),
                                 torch.tensor([0, a.ctx], **i32), a.ctx, a.ctx)
@@ -141,10 +148,28 @@ def main() -> None:
             q = torch.randn(B * a.new, Hq, D, device="cuda", generator=g).half()
             o = torch.empty_like(q)
             nbytes = 2 * B * (min(a.ctx, a.window + a.new) if a.window else a.ctx) * H * D
-            f = lambda i: kb.attn_kv8(cache, q, o, rng, P, wsa)  # noqa
+            if a.tree:      # every token after one of those before it
+                tree = [max(0, i // 2 - 1) if i else -1 for i in range(a.new)]
+                parents = torch.tensor(tree, **i32).repeat(B)
+                mask = torch.empty(B * a.new, -(-a.new // 32), **i32)
+                pos = torch.empty(B * a.new, **i32)
+                kb.draft_tree(parents, rng, mask, pos, window=a.window)
+                f = lambda i: kb.attn_tree_kv8(cache, q, o, rng, mask, P, wsa,  # noqa
+                                               positions=pos)
+            else:
+                f = lambda i: kb.attn_kv8(cache, q, o, rng, P, wsa)  # noqa
         elif a.kernel == "kvwrite":
             nbytes = 6 * a.ctx * H * D
             f = lambda i: kb.kv_write(cache, x, x, whole)  # noqa
+        elif a.kernel in ("rope", "kvwriterope"):
+            q = torch.randn(a.ctx, Hq, D, device="cuda", generator=g).half()
+            o, pos = torch.empty_like(q), torch.arange(a.ctx, **i32)
+            nbytes = 4 * a.ctx * Hq * D
+            if a.kernel == "rope":
+                f = lambda i: kb.rope(q, o, pos, turn)  # noqa
+            else:
+                nbytes += 6 * a.ctx * H * D
+                f = lambda i: kb.kv_write_rope(cache, x, x, whole, turn, q=q, q_out=o)  # noqa
         else:
             k, v = torch.empty_like(x), torch.empty_like(x)
             nbytes = 6 * a.ctx * H * D
@@ -159,6 +184,17 @@ def main() -> None:
              torch.empty(a.B, a.top_k, dtype=torch.int32, device="cuda"))
         nbytes = 2 * a.B * a.M
         f = lambda i: kb.logprobs(z[i % a.copies], t, *o, P, wsl)  # noqa
+    elif a.kernel == "verify":
+        i32, T = dict(dtype=torch.int32, device="cuda"), a.B * a.new
+        z = torch.randn(T, a.M, device="cuda").mul_(3).half()
+        P = kb.verify_params(a.B, T, a.new, a.M, torch.float16)
+        wsv = kb.VerifyWorkspace(P)
+        t, cu = z.argmax(1).to(torch.int32).roll(1), torch.arange(a.B + 1, **i32) * a.new
+        o = [torch.empty(n, **i32) for n in (a.B, T, a.B)]
+        u = torch.rand(T, device="cuda"), torch.rand(a.B, device="cuda")
+        nbytes = 2 * T * a.M
+        f = lambda i: kb.verify_drafts(z, t, cu, *o, P, wsv, uniform=u[0],  # noqa
+                                       uniform_next=u[1])
     else:
         n = a.mbytes << 20
         bufs = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in range(a.copies)]
