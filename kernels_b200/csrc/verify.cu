@@ -395,13 +395,15 @@ template <int DT, bool GREEDY>
 __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     extern __shared__ __align__(16) uint8_t smem[];
     Walk& sh = *reinterpret_cast<Walk*>(smem);
-    pdl_wait();
-    pdl_launch_dependents();
+    // The first kernel starts this one only after its own wait, so what the caller gave is there; it is
+    // read from L2, while that kernel ends.  (Without a row there is no first kernel.)
+    if (a.rows == 0) pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int T = blockDim.x, W = T / 32;
     const int rank = cluster_rank(), b = blockIdx.x / ctas, NW = ctas * W;
-    const int c0 = a.cu[b], n = a.cu[b + 1] - c0;
+    const int c0 = __ldcg(a.cu + b), n = __ldcg(a.cu + b + 1) - c0;
     if (c0 < 0 || n <= 0 || n > (int)a.max_tokens || (uint64_t)c0 + (uint64_t)n > a.rows) {
+        pdl_wait();
         if (rank == 0 && tid == 0) a.count[b] = 0, a.next[b] = -1, a.records[b].mode = kDone;
         return;   // (the whole cluster)
     }
@@ -410,28 +412,27 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     auto draft_of = [&](int i) { return (const char*)a.draft + (uint64_t)(c0 + i) * a.draft_stride * kSize<DT>; };
     auto usable = [](float2 s) { return s.x < INFINITY && s.y > 0.f && s.y < INFINITY; };
 
-    // ---- the tree, and each token's logits in its parent's rows
+    // ---- the tree
     if (tid < kPowers) sh.pow[tid] = exp2(tid * (1.0 / kPowers));
     if (tid == kPowers) sh.mass[0] = 1;   // (without draft, of no token: the root's)
     for (int i = tid; i < n; i += T) {
-        int p = i == 0 ? -1 : a.parents ? a.parents[c0 + i] : i - 1;
+        int p = i == 0 ? -1 : a.parents ? __ldcg(a.parents + c0 + i) : i - 1;
         p = p >= 0 && p < i ? p : -1;
-        const int x = a.tokens[c0 + i];
         sh.parent[i] = p;
-        sh.token[i] = x;
+        sh.token[i] = __ldcg(a.tokens + c0 + i);
         sh.first[i] = kMaxTree;
-        if constexpr (!GREEDY) {
-            sh.u[i] = a.uniform[c0 + i];
-            if (p >= 0 && (uint32_t)x < a.vocab) {
-                sh.z[i] = logit<DT>(row_of(p), x);
-                if (drawn) sh.zq[i] = logit<DT>(draft_of(p), x);
-            }
-        }
+        if constexpr (!GREEDY) sh.u[i] = __ldcg(a.uniform + c0 + i);
     }
     __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
     for (int i = 1 + tid; i < n; i += T) {
-        const int p = sh.parent[i];
+        const int p = sh.parent[i], x = sh.token[i];
         if (p >= 0) atomicMin(&sh.first[p], i);
+        if (!GREEDY && p >= 0 && (uint32_t)x < a.vocab) {   // the token's logits in its parent's rows
+            sh.z[i] = logit<DT>(row_of(p), x);
+            if (drawn) sh.zq[i] = logit<DT>(draft_of(p), x);
+        }
         int s = -1;
         if (a.parents && p >= 0)
             for (int j = i + 1; j < n; ++j)
