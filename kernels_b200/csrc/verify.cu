@@ -13,9 +13,9 @@
 // draft's, where a child was rejected) over the SMs, in fp64: cumulative sums decide about `next`,
 // and at 10^5 tokens an error of 2^-24 would move one draw in a hundred to a neighbour.
 //
-// Measured: one tree of 6 tokens 18.4 us (three kernels' launches and joins); 64 of 6 76 us, 2.3 TB/s
+// Measured: one chain of 6 tokens 17.9 us (three kernels' launches and joins); 64 of 6 75 us, 2.3 TB/s
 // (the exponentials: the fp64 ones of the last rows, and a row is read again for its draw); 16
-// trees with drawn children 28.3 us.
+// trees with drawn children 27.5 us.
 #include "logits.cuh"
 
 #include <algorithm>
