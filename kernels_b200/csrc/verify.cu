@@ -352,6 +352,13 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The same in two halves, of which the second says that every CTA of the cluster runs.
+__device__ __forceinline__ void cluster_here() {
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_all_here() {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
 // Stores 64 bits at the same place of another CTA of the cluster.
 __device__ __forceinline__ void store_remote(const void* at, uint32_t rank, uint64_t v) {
     asm volatile("{\n\t.reg .b32 to;\n\tmapa.shared::cluster.u32 to, %0, %1;\n\t"
@@ -407,6 +414,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         if (rank == 0 && tid == 0) a.count[b] = 0, a.next[b] = -1, a.records[b].mode = kDone;
         return;   // (the whole cluster)
     }
+    if (ctas > 1) cluster_here();   // (waited for before the first store to another CTA)
     const bool drawn = !GREEDY && a.draft;
     auto row_of = [&](int i) { return (const char*)a.logits + (uint64_t)(c0 + i) * a.row_stride * kSize<DT>; };
     auto draft_of = [&](int i) { return (const char*)a.draft + (uint64_t)(c0 + i) * a.draft_stride * kSize<DT>; };
@@ -618,6 +626,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     if (rank == 0)
         for (int i = tid; i < n; i += T) a.path[c0 + i] = i ? -1 : c0;
     __syncthreads();
+    // another CTA's shared memory may be written once that CTA runs
+    if (ctas > 1) cluster_all_here();
     for (;;) {   // (every thread of the cluster takes the same way)
         int c = sh.first[cur];
         m = from = 0, summed = false;
