@@ -112,7 +112,8 @@ __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b
 template <int DT>
 constexpr int kSize = DT == GRAFT_F32 ? 4 : 2;
 
-// The largest logit so far and the first place that has it; a NaN stands above all.
+// The largest logit so far and the place that had it first of those taken, which are taken in their
+// order; a NaN stands above all.
 struct Best {
     float x = -INFINITY;
     uint32_t at = 0;
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
     const float c = (of_draft ? a.draft_scale : a.scale) * kLog2e, reach = 64.f / c;
     float ref = 0.f, lim = -INFINITY, L[2] = {0.f, 0.f};
     Best best;
+    uint64_t key = 0;   // of what `best` took before the edge
     auto take = [&](const uint4 (&v)[UN], int ch, int step) {   // chunks ch, ch + step, ..
         if constexpr (GREEDY) {
 #pragma unroll
@@ -287,6 +289,8 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
 #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
         if (part ? edge < 0 : ch >= i1) continue;
+        // (the first edge comes after what lies behind it: joined by its place, not by its turn)
+        if (GREEDY && part) key = best.key(), best = Best();
         constexpr uint32_t none = DT == GRAFT_F32 ? 0xFF800000u : DT == GRAFT_F16 ? 0xFC00FC00u : 0xFF80FF80u;
         uint4 v[UN];
 #pragma unroll
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
     }
     uint64_t* out = a.parts + ((uint64_t)of_draft * a.rows + row) * a.segs + seg;
     if constexpr (GREEDY) {
-        uint64_t key = best.key();
+        key = max64(key, best.key());
 #pragma unroll
         for (int o = 16; o; o >>= 1) key = max64(key, __shfl_xor_sync(~0u, key, o));
         if (lane == 0) sh_key[warp] = key;
