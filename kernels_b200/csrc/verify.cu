@@ -162,11 +162,11 @@ constexpr int kPowers = 16;
 constexpr double kNothing = 0x1p-990;   // of a token, or a sum of tokens that have nothing
 __device__ __forceinline__ double or_none(double e) { return e > kNothing ? e : 0.0; }
 struct Expo {
-    uint32_t pow;        // 2^(i / 16), in shared memory
-    double c, off;
-    float lim;
-    __device__ __forceinline__ void set(const double* powers, float r, float scale) {
-        pow = smem_u32(powers);
+    const double* pow;   // 2^(i / 16), in shared memory
+    double c = 0, off = 0;
+    float lim = 0;
+    __device__ __forceinline__ explicit Expo(const double* powers) : pow(powers) {}
+    __device__ __forceinline__ void set(float r, float scale) {
         c = (double)scale * (kPowers * 1.4426950408889634);
         lim = fmaxf(__fsub_rd(r, (float)(1000.0 * kPowers / c)), -3.4028235e38f);
         // where even the number below ref has nothing, a lower slope that says so: t stays exact
@@ -183,8 +183,7 @@ struct Expo {
         p = fma(p, f, 0.0009383847924836156);
         p = fma(p, f, 0.04332169878499668);
         p = fma(p, f, 1.0000000000000044);
-        double power;
-        asm("ld.shared.f64 %0, [%1];" : "=d"(power) : "r"(pow + (n & (kPowers - 1)) * 8));
+        const double power = pow[n & (kPowers - 1)];
         return p * __hiloint2double(__double2hiint(power) + ((n & -kPowers) << 16), __double2loint(power));
     }
 };
@@ -495,13 +494,13 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 f = __float_as_int(sh.stat[p].x) == x ? kAccepted : kRejected;
             } else if (usable(sh.stat[p])) {
                 for (int e = sh.first[p]; e != i; e = sh.sibling[e]) again |= sh.token[e] == x;
-                Expo ex;
-                ex.set(sh.pow, sh.stat[p].x, a.scale);
+                Expo ex(sh.pow);
+                ex.set(sh.stat[p].x, a.scale);
                 chance = or_none(ex(sh.z[i])) / sh.stat[p].y;
                 if (!drawn) {
                     f = kRejected;   // (decided below)
                 } else if (usable(sh.stat_q[p])) {
-                    ex.set(sh.pow, sh.stat_q[p].x, a.draft_scale);
+                    ex.set(sh.stat_q[p].x, a.draft_scale);
                     const double q = ex(sh.zq[i]) / sh.stat_q[p].y;
                     f = sh.first[p] != i ? kAsk : sh.u[i] * q < chance ? kAccepted : kRejected;
                 }
@@ -554,7 +553,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
 
     // The last token's row: exponentials, sums, rejections.
     int cur = 0, cnt = 1;
-    Expo ep, eq;
+    Expo ep(sh.pow), eq(sh.pow);
     double Lp = 0, iq = 0;     // the target's sum; the draft's reciprocal sum, times Lp
     int m = 0, from = 0;       // rejections that count; those before `from` left nothing
     bool summed = false;       // Lp and iq are those of cur
@@ -637,15 +636,15 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
         m = from = 0, summed = false;
         double swept = 0, rest = 0;   // what the row's last pass without rejected tokens gave; now left of it
         if constexpr (!GREEDY) {
-            ep.set(sh.pow, sh.stat[cur].x, a.scale);
-            if (drawn) eq.set(sh.pow, sh.stat_q[cur].x, a.draft_scale);
+            ep.set(sh.stat[cur].x, a.scale);
+            if (drawn) eq.set(sh.stat_q[cur].x, a.draft_scale);
         }
         int took = -1;
         if (c < kMaxTree)
             for (; c >= 0; c = sh.sibling[c]) {
                 uint8_t f = sh.flag[c];
                 if (f == kIgnored) continue;
-                if (f == kAsk) {
+                if (!GREEDY && f == kAsk) {
                     const double u = sh.u[c];
                     const double e = or_none(ep(sh.z[c]));
                     if (drawn) {
@@ -752,8 +751,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __gr
     if (rec.mode == kOften)
         for (int i = tid; i < rec.k; i += kDrawThreads) sh_mass[i] = a.mass[c0 + i];
     __syncthreads();
-    Expo ep, eq;
-    ep.set(sh_pow, rec.ref, a.scale), eq.set(sh_pow, rec.ref_q, a.draft_scale);
+    Expo ep(sh_pow), eq(sh_pow);
+    ep.set(rec.ref, a.scale), eq.set(rec.ref_q, a.draft_scale);
     double iq = rec.iq;
     // r, times Lp, of drawn children's rejections
     auto left = [&](double x, double y, int k) {
@@ -816,7 +815,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __gr
             if (step > lim) {
                 const float was = ref;
                 ref = step, lim = step + (float)(500.0 / (1.4426950408889634 * a.scale));
-                ep.set(sh_pow, ref, a.scale);
+                ep.set(ref, a.scale);
                 const double f = was > -INFINITY ? ep(was) : 0.0;
                 s0 *= f, s1 *= f;
             }
@@ -902,7 +901,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __gr
         for (int w = 0; w < kDrawWarps; ++w) most_o = max(most_o, (uint32_t)sh_at[w]);
         top = unorder(most_o);
         if (top > -INFINITY) {
-            ep.set(sh_pow, top, a.scale);
+            ep.set(top, a.scale);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const double f = ep((float)in23[i].x);

@@ -1,5 +1,7 @@
-"""CPU: in the kernels' source, no CTA of a cluster stores to another before a cluster-wide
-barrier has said that all of them run (which no run can show: they usually start together)."""
+"""CPU: what the kernels' source has to say and no run can show (a fault of this kind comes or stays
+away with how the compiler lays out the code, or with how CTAs start): no CTA of a cluster stores to
+another before a cluster-wide barrier has said that all of them run; assembly that reads memory is
+volatile; every exponential knows its table."""
 from __future__ import annotations
 
 import re
@@ -42,3 +44,16 @@ def test_only_the_walk_stores_to_other_ctas():
     inside = body("verify_walk_kernel")
     assert len(stores) == 2            # its definition and the one use
     assert stores[0] < walk < stores[1] < walk + SOURCE[walk:].index(inside) + len(inside)
+
+
+def test_assembly_that_loads_is_volatile():
+    """The compiler may run other assembly ahead of the branch that guards its address."""
+    for path in sorted((ROOT / "kernels_b200" / "csrc").glob("*.cu*")):
+        for m in re.finditer(r'\basm\s*\(\s*((?:"[^"]*"\s*(?://[^\n]*\n\s*)?)+)', path.read_text()):
+            assert not re.search(r"\b(ld|ldmatrix|ldu|atom|red)\.", m.group(1)), (path.name, m.group(1))
+
+
+def test_every_exponential_has_its_table():
+    """Of the kernels that never set it too: its address is read whatever the compiler makes of it."""
+    assert "explicit Expo(const double* powers)" in SOURCE
+    assert not re.search(r"\bExpo \w+\s*[;,]", SOURCE)
