@@ -156,26 +156,28 @@ struct Eight {
 // the exponent and n % 16 takes a power from a table (16 of them have a bank each), and f in
 // [-1/2, 1/2], for which 2^(f / 16) is its Chebyshev expansion on that interval up to degree 5 as a
 // polynomial (off by 5e-15).
-// Ten fp64 operations; the general exp costs about three times as many.  From 2^-1000 of
-// exp(scale ref) down, -inf included, it stays there: kNothing and less is nothing.  (Not for NaN.)
+// Ten fp64 operations; the general exp costs about three times as many.  From 2^-1023 of
+// exp(scale ref) down, -inf included, it is 0: however many tokens cannot come, their sum is
+// nothing.  (Not for NaN.)
 constexpr int kPowers = 16;
-constexpr double kNothing = 0x1p-990;   // of a token, or a sum of tokens that have nothing
-__device__ __forceinline__ double or_none(double e) { return e > kNothing ? e : 0.0; }
 struct Expo {
     const double* pow;   // 2^(i / 16), in shared memory
     double c = 0, off = 0;
-    float lim = 0;
     __device__ __forceinline__ explicit Expo(const double* powers) : pow(powers) {}
     __device__ __forceinline__ void set(float r, float scale) {
-        c = (double)scale * (kPowers * 1.4426950408889634);
-        lim = fmaxf(__fsub_rd(r, (float)(1000.0 * kPowers / c)), -3.4028235e38f);
-        // where even the number below ref has nothing, a lower slope that says so: t stays exact
-        c = fmin(c, 1001.0 * kPowers / ((double)r - lim));
+        // where the next number below r has nothing, a lower slope that says so: t stays exact
+        // (below the type's lowest there is none: the same step again)
+        const double step = fmin((double)r - (double)__fsub_rd(r, __int_as_float(1)), 0x1p104);
+        c = fmin((double)scale * (kPowers * 1.4426950408889634), 1025.0 * kPowers / step);
         off = -(double)r * c;
     }
     __device__ __forceinline__ double operator()(float x) const {
         constexpr double whole = 6755399441055744.0;   // 1.5 2^52: adding it rounds to an integer
-        const double t = fma((double)fmaxf(x, lim), c, off), k = t + whole, f = t - (k - whole);
+        // t at least -1023 16 (the upper half's bits 0xC0CFF800; those of numbers below are larger), which
+        // as an exponent is that of 0
+        double t = fma((double)x, c, off);
+        t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xC0CFF800u), __double2loint(t));
+        const double k = t + whole, f = t - (k - whole);
         const int n = __double2loint(k);
         double p = 1.2716121539285134e-09;
         p = fma(p, f, 1.4676446000606026e-07);
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 for (int e = sh.first[p]; e != i; e = sh.sibling[e]) again |= sh.token[e] == x;
                 Expo ex(sh.pow);
                 ex.set(sh.stat[p].x, a.scale);
-                chance = or_none(ex(sh.z[i])) / sh.stat[p].y;
+                chance = ex(sh.z[i]) / sh.stat[p].y;
                 if (!drawn) {
                     f = kRejected;   // (decided below)
                 } else if (usable(sh.stat_q[p])) {
@@ -646,7 +648,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 if (f == kIgnored) continue;
                 if (!GREEDY && f == kAsk) {
                     const double u = sh.u[c];
-                    const double e = or_none(ep(sh.z[c]));
+                    const double e = ep(sh.z[c]);
                     if (drawn) {
                         sums();
                         const double q = eq(sh.zq[c]);
@@ -675,7 +677,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                 if (drawn && sh.sibling[c] >= 0) {
                     sums();
                     double R = total(mass_of(m)) / Lp;
-                    if (!(R > kNothing)) from = m, R = 1;
+                    if (!(R > 0)) from = m, R = 1;
                     set_mass(m, R);
                 }
             }
@@ -925,126 +927,135 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __gr
         }
     }
     sums_of(R, full);
-    if (!(R > kNothing)) {   // nothing is left: p again
-        k = 0, R = full;
+    int token = -1;
+    // (once more with p, where nothing is left, or a rounding looked like something)
+    for (bool rest_of = R > 0;; rest_of = false) {
+        if (!rest_of) {
+            k = 0, R = full;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) S[i] = in23[i].x;
-    }
-    if (!(R > kNothing && R < INFINITY)) {
-        if (tid == 0) a.next[b] = -1;
-        return;
-    }
-    // ---- the piece in which the sum passes u R (none, by rounding: the last that has any)
-    const double goal = (double)a.uniform_next[b] * R;
-    auto before_of = [&](double x, double& whole) {   // the sum of the threads before, and of all
-        const double upto = scan64(x);
-        __syncthreads();
-        if (lane == 31) sh_sum[0][warp] = upto;
-        __syncthreads();
-        double at = 0;
-        whole = 0;
-#pragma unroll
-        for (int w = 0; w < kDrawWarps; ++w) {
-            if (w < warp) at += sh_sum[0][w];
-            whole += sh_sum[0][w];
+            for (int i = 0; i < kEach; ++i) S[i] = in23[i].x;
         }
-        return at + (upto - x);
-    };
-    double mass = 0, whole;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) mass += S[i];
-    if (tid == 0) sh_owner = 0x7FFFFFFF, sh_last = -1;
-    double at = before_of(mass, whole);
-    int owner = 0x7FFFFFFF, last = -1;
-    double base = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        if (S[i] > kNothing) {
-            last = tid * each + i;
-            if (owner == 0x7FFFFFFF && at + S[i] > goal) owner = last, base = at;
-        }
-        at += S[i];
-    }
-    if (owner != 0x7FFFFFFF) atomicMin(&sh_owner, owner);
-    if (last >= 0) atomicMax(&sh_last, last);
-    __syncthreads();
-    const bool found = sh_owner != 0x7FFFFFFF;
-    if (found && owner == sh_owner) sh_base = base;
-    __syncthreads();
-    base = found ? sh_base : 0;
-    owner = found ? sh_owner : sh_last;
-    // ---- the token: up to eight a thread, from shared memory (in loops of two: one CTA a sequence
-    // comes here, and its instructions come from far)
-    const int first = from_of(owner), end = (int)min((int64_t)first + piece, (int64_t)V);
-    const bool two = both && k;
-    const int per = min(8, (end - first + 2 * kDrawThreads - 1) / (2 * kDrawThreads) * 2);   // tokens of a thread
-    auto place = [](int i) { return i + (i >> 3); };
-    const double start = base;
-    int token = -1, tail = -1;
-#pragma unroll 1
-    for (int pass = found ? 0 : 1; pass < 2 && token < 0; ++pass) {   // (1: the last that has any)
-        base = start;
-#pragma unroll 1
-        for (int v0 = first; v0 < end && token < 0; v0 += per * kDrawThreads) {
-            float x[8], y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int v = v0 + i * kDrawThreads + tid;
-                const bool in = i < per && v >= 0 && v < end;
-                x[i] = in ? logit<DT>(zp, v) : -INFINITY;
-                y[i] = in && two ? logit<DT>(zq, v) : -INFINITY;
-            }
+        if (!(R > 0 && R < INFINITY)) break;
+        // ---- the piece in which the sum passes u R (none, by rounding: the last that has any)
+        const double goal = (double)a.uniform_next[b] * R;
+        auto before_of = [&](double x, double& whole) {   // the sum of the threads before, and of all
+            const double upto = scan64(x);
             __syncthreads();
+            if (lane == 31) sh_sum[0][warp] = upto;
+            __syncthreads();
+            double at = 0;
+            whole = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < per) {
-                    sh_x[0][place(i * kDrawThreads + tid)] = x[i];
-                    sh_x[1][place(i * kDrawThreads + tid)] = y[i];
+            for (int w = 0; w < kDrawWarps; ++w) {
+                if (w < warp) at += sh_sum[0][w];
+                whole += sh_sum[0][w];
+            }
+            return at + (upto - x);
+        };
+        double mass = 0, whole;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mass += S[i];
+        if (tid == 0) sh_owner = 0x7FFFFFFF, sh_last = -1;
+        double at = before_of(mass, whole);
+        int owner = 0x7FFFFFFF, last = -1;
+        double start = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (S[i] > 0) {
+                last = tid * each + i;
+                if (owner == 0x7FFFFFFF && at + S[i] > goal) owner = last, start = at;
+            }
+            at += S[i];
+        }
+        if (owner != 0x7FFFFFFF) atomicMin(&sh_owner, owner);
+        if (last >= 0) atomicMax(&sh_last, last);
+        __syncthreads();
+        const bool found = sh_owner != 0x7FFFFFFF;
+        if (found && owner == sh_owner) sh_base = start;
+        __syncthreads();
+        start = found ? sh_base : 0;
+        owner = found ? sh_owner : sh_last;
+        // ---- the token: up to eight a thread, from shared memory (in loops of two: one CTA a sequence
+        // comes here, and its instructions come from far).  Pass 0: the piece's first that passes u R; 1: its
+        // last that has any.  Sums and differences round, so that a piece may have a sum and no such token:
+        // then the first that has any of the pieces behind, or else the last of those before.
+        const bool two = both && k;
+        auto place = [](int i) { return i + (i >> 3); };
+        const int behind = found ? NW - 1 - owner : 0;
+#pragma unroll 1
+        for (int pass = found ? 0 : 1; token < 0; ++pass) {
+            const bool tail = pass == 1 || pass - 2 >= behind;
+            const int piece_of = pass < 2 ? owner : tail ? owner - 1 - (pass - 2 - behind) : owner + pass - 1;
+            if (piece_of < 0) break;
+            const double past = pass < 2 ? goal : -1;
+            const int first = from_of(piece_of), end = (int)min((int64_t)first + piece, (int64_t)V);
+            const int per = min(8, (end - first + 2 * kDrawThreads - 1) / (2 * kDrawThreads) * 2);   // tokens of a thread
+            double base = pass < 2 ? start : 0;
+            int late = -1;
+#pragma unroll 1
+            for (int v0 = first; v0 < end && token < 0; v0 += per * kDrawThreads) {
+                float x[8], y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int v = v0 + i * kDrawThreads + tid;
+                    const bool in = i < per && v >= 0 && v < end;
+                    x[i] = in ? logit<DT>(zp, v) : -INFINITY;
+                    y[i] = in && two ? logit<DT>(zq, v) : -INFINITY;
                 }
-            __syncthreads();
-            const int v = v0 + per * tid;
-            const uint32_t g = !both && k ? among(sh_gone, k, v) : 0;
-            auto rest = [&](int i, double& r0, double& r1) {   // of tokens v + i and the next
-                const int at = per * tid + i;
-                r0 = ep(sh_x[0][place(at)]), r1 = ep(sh_x[0][place(at + 1)]);
-                if (two) r0 = left(r0, eq(sh_x[1][place(at)]), k), r1 = left(r1, eq(sh_x[1][place(at + 1)]), k);
-                r0 = g >> i & 1 ? 0.0 : r0, r1 = g >> i & 2 ? 0.0 : r1;
-            };
-            double s = 0;
-#pragma unroll 1
-            for (int i = 0; i < per; i += 2) {
-                double r0, r1;
-                rest(i, r0, r1);
-                s += r0 + r1;
-            }
-            double before = base + before_of(s, whole);
-            int here = pass ? -1 : 0x7FFFFFFF;
-            if (pass || before + s > goal) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < per) {
+                        sh_x[0][place(i * kDrawThreads + tid)] = x[i];
+                        sh_x[1][place(i * kDrawThreads + tid)] = y[i];
+                    }
+                __syncthreads();
+                const int v = v0 + per * tid;
+                const uint32_t g = !both && k ? among(sh_gone, k, v) : 0;
+                auto rest = [&](int i, double& r0, double& r1) {   // of tokens v + i and the next
+                    const int at = per * tid + i;
+                    r0 = ep(sh_x[0][place(at)]), r1 = ep(sh_x[0][place(at + 1)]);
+                    if (two) r0 = left(r0, eq(sh_x[1][place(at)]), k), r1 = left(r1, eq(sh_x[1][place(at + 1)]), k);
+                    r0 = g >> i & 1 ? 0.0 : r0, r1 = g >> i & 2 ? 0.0 : r1;
+                };
+                double s = 0;
 #pragma unroll 1
                 for (int i = 0; i < per; i += 2) {
-                    double r[2];
-                    rest(i, r[0], r[1]);
+                    double r0, r1;
+                    rest(i, r0, r1);
+                    s += r0 + r1;
+                }
+                double before = base + before_of(s, whole);
+                int here = tail ? -1 : 0x7FFFFFFF;
+                if (tail || before + s > past) {
+#pragma unroll 1
+                    for (int i = 0; i < per; i += 2) {
+                        double r[2];
+                        rest(i, r[0], r[1]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        before += r[j];
-                        if (r[j] > kNothing) {
-                            if (pass) here = v + i + j;
-                            else if (before > goal) here = min(here, v + i + j);
+                        for (int j = 0; j < 2; ++j) {
+                            before += r[j];
+                            if (r[j] > 0) {
+                                if (tail) here = v + i + j;
+                                else if (before > past) here = min(here, v + i + j);
+                            }
                         }
                     }
                 }
+                here = tail ? __reduce_max_sync(~0u, here) : __reduce_min_sync(~0u, here);
+                if (lane == 0) sh_at[warp] = here;
+                __syncthreads();
+                for (int w = 0; w < kDrawWarps; ++w) here = tail ? max(here, sh_at[w]) : min(here, sh_at[w]);
+                if (tail) late = max(late, here);
+                else if (here != 0x7FFFFFFF) token = here;
+                base += whole;
+                __syncthreads();
             }
-            here = pass ? __reduce_max_sync(~0u, here) : __reduce_min_sync(~0u, here);
-            if (lane == 0) sh_at[warp] = here;
-            __syncthreads();
-            for (int w = 0; w < kDrawWarps; ++w) here = pass ? max(here, sh_at[w]) : min(here, sh_at[w]);
-            if (pass) tail = max(tail, here);
-            else if (here != 0x7FFFFFFF) token = here;
-            base += whole;
-            __syncthreads();
+            if (tail) token = late;
         }
+        if (token >= 0 || !rest_of) break;
     }
-    if (tid == 0) a.next[b] = token >= 0 ? token : tail;
+    if (tid == 0) a.next[b] = token;
 }
 
 int check_verify(const GraftVerifyParams* P) {

@@ -50,3 +50,63 @@ def test_greedy_ties_at_every_offset(lib, V, gap, dtype):
     tokens[1::2] = [t[-1] if len(t) > 1 else V + 1 for t in later]
     count, _, nxt = call(view, tokens, cu, None)
     assert count == [1] * n and nxt == first[0::2].tolist()
+
+
+def first_possible(kind, B, V, masked, dtype):
+    """B sequences, the same root's row: `masked` tokens that cannot come lie before all that can, but for
+    (kind "chosen") one among them, which is rejected.  Rejections leave the smallest token behind them
+    with something; the random number 0 has to find it."""
+    n = {"chosen": 2, "once": 2, "often": 4}[kind]
+    z = np.full(V, -np.inf, np.float32)
+    z[masked::997] = 0.0                             # few for the target, many for the draft, so that the
+    q = np.random.default_rng(V).normal(0, 1, V).astype(np.float32)   # target's sum is the smaller one
+    q[:masked] = -np.inf
+    drawn = np.argsort(-np.where(z == 0, -np.inf, q))[:n - 1]         # likely ones that cannot come
+    if kind == "chosen":
+        z[masked // 2] = 3.0
+        drawn = np.array([masked // 2])
+    u = np.full((B, n), 0.999, np.float32)
+    tokens = np.concatenate([[0], drawn])
+    parents = np.array([-1] + [0] * (n - 1)) if kind == "often" else None
+    rows = torch.from_numpy(np.stack([z] + [np.zeros(V, np.float32)] * (n - 1)))
+    rows = rows.to(DTYPES[dtype]).cuda().repeat(B, 1)
+    guess = None if kind == "chosen" else torch.from_numpy(q).to(DTYPES[dtype]).cuda().expand(n, V).repeat(B, 1)
+    cu = [n * b for b in range(B + 1)]
+    return rows, np.tile(tokens, B), cu, None if parents is None else np.tile(parents, B), guess, u.reshape(-1)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("B,V,masked", [(128, 128256, 8192), (128, 128256, 100001), (200, 33000, 20000)])
+@pytest.mark.parametrize("kind", ["chosen", "once", "often"])
+def test_masked_tokens_are_never_what_follows(lib, kind, B, V, masked, dtype):
+    """Thousands of tokens that cannot come are together still none: for the random number 0 `next` is the
+    first token that can."""
+    rows, tokens, cu, parents, guess, u = first_possible(kind, B, V, masked, dtype)
+    n = cu[1]
+    from draft_ref import verify
+    par = [-1] + [0] * (n - 1) if parents is not None else list(range(-1, n - 1))
+    path, nxt, _ = verify(f64(rows[:n]), tokens[:n], par, 1.0, None if guess is None else f64(guess[:n]),
+                          1.0, u[:n], 0.0)
+    assert path == [0] and nxt == masked
+    got = call(rows, tokens, cu, parents, draft=guess, uniform=u, last=np.zeros(B, np.float32))
+    assert got[0] == [1] * B and got[2] == [nxt] * B
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_lowest_finite_logits_are_tokens(lib, dtype):
+    """A row of the type's lowest value, as a mask leaves it, beside tokens that cannot come: only the former
+    can, each as often as the others."""
+    low, V = float(np.finfo(np.float16 if dtype == "f16" else np.float32).min), 1000
+    z = torch.full((40, V), float("-inf"))
+    z[:, 300:310] = low
+    z = z.to(DTYPES[dtype]).cuda()
+    last = (np.arange(40, dtype=np.float32) + 0.5) / 40
+    want = [300 + b // 4 for b in range(40)]
+    assert call(z, np.zeros(40, np.int64), list(range(41)), None, uniform=np.zeros(40, np.float32),
+                last=last)[2] == want
+    # .. also behind a child that was rejected, and whose token is one of them
+    z2 = z.repeat_interleave(2, 0)
+    got = call(z2, np.tile([0, 304], 40), [2 * b for b in range(41)], None,
+               uniform=np.tile(np.float32([0, 0.5]), 40), last=(np.arange(40, dtype=np.float32) + 0.5) / 40)
+    left = [t for t in range(300, 310) if t != 304]
+    assert got[0] == [1] * 40 and got[2] == [left[int(x * 9)] for x in last]
