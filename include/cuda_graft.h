@@ -738,7 +738,9 @@ int graft_logprobs(const void* logits, const int32_t* targets, float* logprob, f
  * distribution (a NaN, +inf, or nothing possible) next is -1; a child behind such a
  * row, or with a token outside 0..vocab-1, is never accepted and changes nothing; nor does
  * one behind such a row of draft.  If nothing is left of r, it is p again.
- * Sums are fp32 for the first child of a token and fp64 from then on and for next. */
+ * Decisions are those of fp64 sums: where a random number lies so near to a border that the
+ * fp32 sums that serve first (off by 2^-15 at most up to 200000 tokens of a vocabulary) might
+ * err, the whole row is summed again. */
 typedef struct {
     uint32_t n_seqs, tokens;      /* sequences, rows                           */
     uint32_t max_tokens;          /* of a sequence, at most 1024               */

@@ -8,8 +8,9 @@
 // Three kernels.  The first reads the rows of tokens that have children (a leaf's row matters
 // only if it turns out to be the last) and leaves each segment's (reference, sum) in fp32.  The
 // second walks down the tree: whether a token's first child is accepted follows from two logits
-// and two sums, for all tokens at once.  Only where a token has several drawn children does it go
-// over whole rows, as a cluster of CTAs a sequence.  The third spreads the last token's row (and the
+// and two sums, for all tokens at once, and so do looked-up siblings.  It goes over whole rows, in
+// fp64, where a random number lies so close to a border that the sums' errors might decide, and
+// where a token has several drawn children, as a cluster of CTAs a sequence.  The third spreads the last token's row (and the
 // draft's, where a child was rejected) over the SMs, in fp64: cumulative sums decide about `next`,
 // and at 10^5 tokens an error of 2^-24 would move one draw in a hundred to a neighbour.
 //
@@ -78,6 +79,14 @@ constexpr int kRounds = 148 * 16;    // CTAs to aim at
 constexpr int kWalkThreads = 512, kWalkWarps = kWalkThreads / 32, kMaxCluster = 16;
 constexpr int kDrawThreads = 256, kDrawWarps = kDrawThreads / 32, kMaxDrawSegs = 64;
 constexpr float kLog2e = 1.4426950408889634f;
+// The first kernel's sums are off by less than (kSumSteps + the rounds of a thread) 2^-24.  An exponent
+// t = (z - ref) c is off by 3.3 2^-24 of itself (c, difference, product), its power by ln 2 of that.  A
+// logit D octaves below the row's reference has powers of D + 2 kReach octaves together (its own, and
+// those that follow the reference, which it may pass by kReach), and the mean D over the powers is at
+// most log2 of the vocabulary, 30: 62 3.3 ln 2 < 143.  Powers: six roundings of 2^-22, 24.  Sums: 16 terms a
+// round, the rounds, joins of 2, 32, 4 and 32: 31 and the rounds.
+constexpr float kReach = 16.f;
+constexpr int kSumSteps = 200;
 
 struct VerifyArgs {
     const void *logits, *draft;
@@ -87,6 +96,7 @@ struct VerifyArgs {
     uint64_t row_stride, draft_stride;
     uint32_t n_seqs, rows, max_tokens, vocab;
     float scale, draft_scale;
+    double off;        // how far the first kernel's sums may be off, of themselves
     int segs;
     uint64_t* parts;   // [draft: 2][rows][segs]: (reference, sum), or greedy the largest key
     // between the walk and the draw
@@ -103,7 +113,7 @@ struct VerifyArgs {
 enum Mode : int { kDone, kList, kOnce, kOften, kTop };
 struct Record {
     int mode, row, k, from;   // row of logits; rejections, and those that left nothing
-    float ref, ref_q, near;   // references of the exponentials; Lp / Lq to 2^-20
+    float ref, ref_q, near;   // references of the exponentials; Lp / Lq by the first kernel's sums
     double Lp, iq;            // kOften: the target's sum, and by the draft's
 };
 
@@ -214,7 +224,7 @@ __device__ __forceinline__ bool has_children(const VerifyArgs& a, int r) {
 }
 
 // A segment of a row: a reference and the sum of exp(scale (z - it)), or the largest key.  Each
-// thread has a reference of its own that moves only when a logit passes it by 2^64.
+// thread has a reference of its own that moves only when a logit passes it by 2^kReach.
 template <int DT, bool GREEDY>
 __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_constant__ VerifyArgs a) {
     constexpr int N = kPer<DT>, UN = kUnroll;
@@ -234,7 +244,7 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
     // chunks that lie wholly in the row are [i0, i1)
     const int i0 = c0 + (c0 == 0 && c1 > 0 && (off || (int)a.vocab < N));
     const int i1 = max(i0, c1 - (c1 == chunks && (off + a.vocab) % N != 0));
-    const float c = (of_draft ? a.draft_scale : a.scale) * kLog2e, reach = 64.f / c;
+    const float c = (of_draft ? a.draft_scale : a.scale) * kLog2e, reach = kReach / c;
     float ref = 0.f, lim = -INFINITY, L[2] = {0.f, 0.f};
     Best best;
     uint64_t key = 0;   // of what `best` took before the edge
@@ -257,8 +267,9 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
                     L[0] *= f, L[1] *= f;
                 }
                 ref = gm;
-                lim = __fadd_rd(gm, reach);   // (rounded up, it might let 2^128 through)
+                lim = __fadd_rd(gm, reach);
             }
+            float now[2] = {0.f, 0.f};   // (a round's sums by themselves: their errors do not grow with the row)
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
                 const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
@@ -270,9 +281,10 @@ __global__ void __launch_bounds__(kRowThreads) verify_rows_kernel(const __grid_c
                     } else {
                         minus<DT>(w[e / 2], ref, d0, d1);
                     }
-                    L[0] += ex2(d0 * c), L[1] += ex2(d1 * c);
+                    now[0] += ex2(d0 * c), now[1] += ex2(d1 * c);
                 }
             }
+            L[0] += now[0], L[1] += now[1];
         }
     };
     int ch = i0 + tid;
@@ -503,8 +515,9 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                     f = kRejected;   // (decided below)
                 } else if (usable(sh.stat_q[p])) {
                     ex.set(sh.stat_q[p].x, a.draft_scale);
-                    const double q = ex(sh.zq[i]) / sh.stat_q[p].y;
-                    f = sh.first[p] != i ? kAsk : sh.u[i] * q < chance ? kAccepted : kRejected;
+                    const double uq = sh.u[i] * (ex(sh.zq[i]) / sh.stat_q[p].y);
+                    f = sh.first[p] != i || fabs(uq - chance) < a.off * (uq + chance) ? kAsk
+                        : uq < chance ? kAccepted : kRejected;
                 }
             }
         }
@@ -513,20 +526,20 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
     __syncthreads();
     if constexpr (!GREEDY) {
         if (!drawn) {
-            // r is p without the earlier siblings' tokens
+            // r is p without the earlier siblings' tokens: with L the row's sum and s that of their
+            // exponentials, u (L - s) < e decides, where L alone is uncertain
             for (int i = 1 + tid; i < n; i += T)
                 if (sh.flag[i] == kRejected && !sh.again[i]) {
                     double R = 1;
                     for (int e = sh.first[sh.parent[i]]; e != i; e = sh.sibling[e])
                         if (sh.flag[e] != kIgnored && !sh.again[e]) R -= sh.chance[e];
-                    // (where little is left of 1, the sums' own errors count: the row decides)
                     sh.mass[i] = R;
                 }
             __syncthreads();
             for (int i = 1 + tid; i < n; i += T)
                 if (sh.flag[i] == kRejected && !sh.again[i]) {
-                    const double R = sh.mass[i];
-                    sh.flag[i] = R < 0x1p-10 ? kAsk : sh.u[i] * R < sh.chance[i] ? kAccepted : kRejected;
+                    const double uR = sh.u[i] * sh.mass[i], e = sh.chance[i];
+                    sh.flag[i] = fabs(uR - e) < a.off * sh.u[i] ? kAsk : uR < e ? kAccepted : kRejected;
                 }
             __syncthreads();
         }
@@ -789,9 +802,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) verify_draw_kernel(const __gr
             for (int i = 0; i < 8; ++i) best.take(x[i], v + i);
         } else if (rec.mode == kOnce) {
             // s0 - less s1: r, s2 and s3: the whole of p and q.  r is ep - less eq where that is positive,
-            // less = Lp / Lq.  The first kernel's sums give that to 2^-20, which tells the tokens where r is
-            // positive but for some whose r is below 2^-20 of their p; with their sums, and the row's, one
-            // pass is enough.
+            // less = Lp / Lq.  The first kernel's sums give that to 2 off (2^-14 for half a million tokens at
+            // worst, 2^-20 as a rule), which tells the tokens where r is positive but for some whose r is below
+            // that share of their p; with their sums, and the row's, one pass is enough.
             const double near = rec.near;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -1233,6 +1246,8 @@ extern "C" int graft_verify_drafts(const void* logits, const void* draft, const 
     a.n_seqs = P->n_seqs, a.rows = P->tokens, a.max_tokens = P->max_tokens, a.vocab = P->vocab;
     a.scale = P->scale, a.draft_scale = P->draft_scale;
     a.segs = segments(P), a.draw_segs = draw_segments(P);
+    const uint64_t round = (uint64_t)kUnroll * kRowThreads * (16 / es);   // tokens of a CTA's round
+    a.off = (kSumSteps + (double)((a.vocab / a.segs + round - 1) / round + 2)) * 0x1p-24;
     carve(P, (char*)ws, &a);
     return P->dtype == GRAFT_F16    ? launch_verify<GRAFT_F16>(a, stream)
            : P->dtype == GRAFT_BF16 ? launch_verify<GRAFT_BF16>(a, stream)

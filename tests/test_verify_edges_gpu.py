@@ -110,3 +110,66 @@ def test_lowest_finite_logits_are_tokens(lib, dtype):
                uniform=np.tile(np.float32([0, 0.5]), 40), last=(np.arange(40, dtype=np.float32) + 0.5) / 40)
     left = [t for t in range(300, 310) if t != 304]
     assert got[0] == [1] * 40 and got[2] == [left[int(x * 9)] for x in last]
+
+
+def softmax_rows(z, scale):
+    z = z * np.float64(np.float32(scale))
+    e = np.exp(z - z.max(1, keepdims=True))
+    return e / e.sum(1, keepdims=True)
+
+
+# Random numbers lie 2^-9 to 2^-21 to either side of a border.  They are fp32, rounded to 2^-25 at
+# most where they are below 1/2 and a border of at least 1/8 moves them by 2^-22 of it; what side they
+# are on is worked out from the rounded ones, in fp64, whose sums are right to 2^-45 of the little that is left.
+SIDES = np.array([s * 2.0 ** -k for k in range(9, 22) for s in (-1, 1)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("V,top,scale", [(4099, 0.99, 1.3), (4099, 0.5, 0.7), (20011, 0.998, 1.0)])
+def test_second_children_near_their_border(lib, V, top, scale, dtype):
+    """A looked-up child that has most of the probability is rejected; whether the next is accepted against
+    what is left is decided as 64-bit sums do."""
+    rng = np.random.default_rng(V)
+    B = 26 * (40 if V < 9000 else 10)
+    z = torch.from_numpy(rng.normal(0, 1, (3 * B, V)).astype(np.float32)).to(DTYPES[dtype])
+    root = z[::3].double().numpy()
+    rest = np.log(np.exp(root * scale).sum(1))
+    root[:, 7] = (rest + np.log(top / (1 - top))) / scale      # p about `top`,
+    root[:, V - 9] = (rest + np.log(0.45)) / scale             # and a third of what is left without it
+    z[::3] = torch.from_numpy(root).to(z.dtype)
+    p = softmax_rows(f64(z[::3]), scale)
+    r, R = p[:, V - 9], p.sum(1) - p[:, 7]
+    u = np.full((B, 3), 0.9999, np.float32)
+    u[:, 2] = (r / R * (1 + np.resize(SIDES, B))).astype(np.float32)
+    assert (u[:, 1] > p[:, 7]).all() and (0.125 < u[:, 2]).all() and (u[:, 2] < 0.5).all()
+    want = (u[:, 2].astype(np.float64) * R < r)
+    assert 0.4 < want.mean() < 0.6
+    tokens, parents = np.tile([0, 7, V - 9], B), np.tile([-1, 0, 0], B)
+    count, path, _ = call(z.cuda(), tokens, [3 * b for b in range(B + 1)], parents, scale=scale,
+                          uniform=u.reshape(-1), last=np.full(B, 0.5, np.float32))
+    assert (np.array(count) == 1 + want).all()
+    assert (np.array(path).reshape(B, 3)[:, 1] == np.where(want, 3 * np.arange(B) + 2, -1)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("V,scale", [(4099, 1.3), (20011, 0.7)])
+def test_first_children_near_their_border(lib, V, scale, drawn, dtype):
+    """.. and so is a first child, of the draft's distribution or looked up."""
+    rng = np.random.default_rng(V + 1)
+    B = 26 * (40 if V < 9000 else 10)
+    z = torch.from_numpy(rng.normal(0, 2, (2 * B, V)).astype(np.float32)).to(DTYPES[dtype])
+    z[:, 5] = 4.0 + np.log(V) / scale
+    d = torch.from_numpy(rng.normal(0, 2, (2 * B, V)).astype(np.float32)).to(DTYPES[dtype])
+    d[:, 5] = 6.0 + np.log(V) / scale
+    p = softmax_rows(f64(z[::2]), scale)[:, 5]
+    q = softmax_rows(f64(d[::2]), scale)[:, 5] if drawn else np.ones(B)
+    u = np.full((B, 2), 0.5, np.float32)
+    u[:, 1] = (p / q * (1 + np.resize(SIDES, B))).astype(np.float32)
+    assert (0.125 < u[:, 1]).all() and (u[:, 1] < 1).all()     # (rounded by 2^-25: 2^-22 of 1/8)
+    want = u[:, 1].astype(np.float64) * q < p
+    assert 0.4 < want.mean() < 0.6
+    count, _, _ = call(z.cuda(), np.tile([0, 5], B), [2 * b for b in range(B + 1)], None, scale=scale,
+                       draft=d.cuda() if drawn else None, draft_scale=scale, uniform=u.reshape(-1),
+                       last=np.full(B, 0.5, np.float32))
+    assert (np.array(count) == 1 + want).all()
