@@ -126,7 +126,8 @@ extern "C" int graft_attn_tree_kv8(const GraftKVCache* cache, const GraftHeads* 
                                    graft_stream_t stream) {
     int rc;
     if ((rc = check_attn(cache, range, P))) return rc;
-    if (range->n_seqs && range->max_tokens) {
+    // (a step without new tokens may have no mask: empty buffers have no address)
+    if (range->n_seqs && range->max_tokens && !(q && q->tokens == 0)) {
         GRAFT_REQUIRE(mask && aligned(mask, 4), "mask must be a 4-byte aligned buffer");
         GRAFT_REQUIRE(mask_stride >= (range->max_tokens + 31ull) / 32 || (q && q->tokens <= 1),
                       "mask_stride %llu does not hold max_tokens %u", (unsigned long long)mask_stride,
