@@ -574,7 +574,9 @@ typedef struct {
  *   GRAFT_ROPE_LINEAR  g_i / factor
  *   GRAFT_ROPE_YARN    g_i (1 - r_i) + g_i/factor r_i: r_i rises from 0 to 1 between the
  *     pairs i that turn `high` and `low` times over orig_len positions,
- *     i(t) = dims ln(orig_len / (2 pi t)) / (2 ln b), held within [0, dims - 1]
+ *     i(t) = dims ln(orig_len / (2 pi t)) / (2 ln b), held within [0, dims - 1].  Neither end is
+ *     rounded to a whole pair; where a model's frequencies were made with ends rounded down
+ *     and up (common, and often the default), give them as freqs
  *   GRAFT_ROPE_BANDS   g_i s_i + g_i/factor (1 - s_i), s_i = (t_i - low) / (high - low)
  *     held within [0, 1], t_i = orig_len g_i / (2 pi) the pair's turns over orig_len
  * base > 0 (not 1 with YARN), factor > 0; YARN and BANDS: orig_len > 0, 0 < low < high. */

@@ -597,8 +597,8 @@ _ROPE_SCALINGS = {"plain": 0, "linear": 1, "yarn": 2, "bands": 3}
 class RopeTable:
     """Rotary positions of a head's first `dims` elements (graft_rope_init): layout
     "half" or "interleaved"; scaling "plain", "linear" (factor), "yarn" or "bands"
-    (factor, orig_len, low, high).  freqs (fp64 [dims // 2], radians a position)
-    takes the place of the formulas.  amplitude multiplies sine and cosine."""
+    (factor, orig_len, low, high; the ramp's ends are not rounded to whole pairs).  freqs
+    (fp64 [dims // 2], radians a position) takes the place of the formulas.  amplitude multiplies sine and cosine."""
 
     def __init__(self, dims: int, base: float = 10000.0, layout: str = "half",
                  scaling: str = "plain", factor: float = 1.0, orig_len: float = 0.0,

@@ -29,7 +29,7 @@
 // Short calls are a chain of latencies: 517 keys 7.5 us, 32 sequences with a window of 128 and
 // two tokens each 9.8 us.  17 to 32 rows take one CTA an SM (registers), whose 8 warps hide
 // little: 32 sequences of up to 8192 keys 76 us, with 8 rows 41.
-// Spills: instances for 16 rows of 64 dims 56 to 104 bytes, for 8 rows 28 to 40.
+// Spills: instances for 16 rows of 64 dims 56 to 104 bytes (of trees 20 to 44), for 8 rows 28 to 40.
 #pragma once
 #include "attn_common.cuh"
 

@@ -10,13 +10,17 @@
 // second walks down the tree: whether a token's first child is accepted follows from two logits
 // and two sums, for all tokens at once, and so do looked-up siblings.  It goes over whole rows, in
 // fp64, where a random number lies so close to a border that the sums' errors might decide, and
-// where a token has several drawn children, as a cluster of CTAs a sequence.  The third spreads the last token's row (and the
-// draft's, where a child was rejected) over the SMs, in fp64: cumulative sums decide about `next`,
-// and at 10^5 tokens an error of 2^-24 would move one draw in a hundred to a neighbour.
+// where a token has several drawn children, as a cluster of CTAs a sequence.  The third spreads the
+// last token's row (and the draft's, where a child was rejected) over the SMs, in fp64: cumulative
+// sums decide about `next`, and at 10^5 tokens an error of 2^-24 would move one draw in a hundred to
+// a neighbour.
 //
-// Measured: one chain of 6 tokens 17.9 us (three kernels' launches and joins); 64 of 6 75 us, 2.3 TB/s
-// (the exponentials: the fp64 ones of the last rows, and a row is read again for its draw); 16
-// trees with drawn children 27.5 us.
+// Measured (replayed): one chain of 6 tokens over 201088 17.6 us (three kernels' launches and joins),
+// 10 greedily; 64 of 6 over 128256 73 us, 2.4 TB/s (the exponentials: the fp64 ones of the last rows,
+// and a row is read again for its draw), 39 greedily, 82 with the draft's rows at another place in
+// their 16 bytes than the target's; 16 looked-up trees of 1 to 31 over 50021 in fp32 27 us; trees of
+// drawn children over 128256, 16 of 16 85 us, 64 of 64 368.  A random number next to a border, one
+// sequence: 36 us more over 128256, 55 over 201088.
 #include "logits.cuh"
 
 #include <algorithm>
@@ -668,7 +672,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
                         f = u * (q * iq) * sh.mass[m] < left(e, q, m) ? kAccepted : kRejected;
                     } else if (e > 0) {
                         // while the differences keep 2^-10 of the sum they are exact to 2^-42 (511 children,
-                        // all rejected, over 128256: 0.51 ms; with a pass for each 1950)
+                        // all rejected, over 128256: 0.2 to 0.5 ms; with a pass for each 1950 ms)
                         if (!(rest > swept * 0x1p-10)) rest = swept = without(c);
                         f = u * rest < e ? kAccepted : kRejected;
                         rest -= e;
