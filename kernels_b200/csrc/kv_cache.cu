@@ -295,12 +295,6 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) kv_write_kernel(const __grid
     }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
-
 // An item's queries: heads h0 .. of the CTA.  A thread takes a unit (16 elements) of a token for
 // several heads, with the same sines and cosines.
 template <int DT>

@@ -112,6 +112,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // Pairs of fp32 numbers (sm_100's two-wide operations).
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;

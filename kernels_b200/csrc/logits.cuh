@@ -11,11 +11,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 // fp32 in the order of unsigned integers (finite and infinite; -0 = +0)
 __device__ __forceinline__ uint32_t order(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);

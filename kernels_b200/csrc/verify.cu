@@ -1092,7 +1092,8 @@ int check_verify(const GraftVerifyParams* P) {
     return GRAFT_OK;
 }
 
-// Segments of a row: enough CTAs for several rounds over the SMs, none shorter than kMinSeg.
+// Segments of a row: enough CTAs for several rounds over the SMs (counted as 148, for the workspace is
+// sized before there is a device), none shorter than kMinSeg.
 int segments(const GraftVerifyParams* P) {
     const uint64_t rows = P->tokens ? P->tokens : 1;
     const uint64_t want = (kRounds + rows - 1) / rows, most = std::max<uint64_t>(1, P->vocab / kMinSeg);
